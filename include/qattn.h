@@ -53,7 +53,8 @@ extern "C" {
  * 7: qattn_run_update no longer waits for the device (two work-list images per run);
  *    qattn_debug_fail_allocs
  * 8: qattn_debug_run_timeline
- * 9: qattn_buffer_read_after, qattn_event_synchronize */
+ * 9: qattn_buffer_read_after, qattn_event_synchronize; added since without a change to what was
+ *    there: qattn_rope, qattn_kv_*, qattn_shared_* */
 #define QATTN_ABI_VERSION 9
 
 #define QATTN_Q_HEADS 16
@@ -313,6 +314,94 @@ int qattn_q4_matmul(qattn_ctx* ctx, const void* x, int64_t ldx, int32_t M, int32
  * multiple of 64; ldy >= n_inter; the other rules of qattn_q4_matmul with N = 2 n_inter. */
 int qattn_q4_matmul_swiglu(qattn_ctx* ctx, const void* x, int64_t ldx, int32_t M, int32_t K, const void* w,
                            int64_t w_bytes, int32_t n_inter, void* y, int64_t ldy, qattn_stream_t stream);
+
+/* ---- requests behind one shared prefix: rotary positions, a paged K/V cache, attention over it --- */
+/* No counterpart in the reference, which recomputes an instruction's tokens with every request.  A
+ * prefix is run once and its K and V kept (qattn_kv_write); a batch of requests then rotates its q and
+ * k to positions that follow the prefix (qattn_rope) and attends to the cached prefix and its own keys
+ * (qattn_shared_run_*).  Storage is fp16 or bf16 (enum qattn_dtype), arithmetic f32. */
+enum qattn_dtype { QATTN_DTYPE_F16 = 0, QATTN_DTYPE_BF16 = 1 };
+#define QATTN_MAX_ROPE_DIM 512
+
+enum qattn_rope_layout {
+  QATTN_ROPE_HALF = 0,       /* pair i: elements i and i + rotary_dim / 2 */
+  QATTN_ROPE_INTERLEAVED = 1 /* pair i: elements 2 i and 2 i + 1 */
+};
+enum qattn_rope_scaling {
+  QATTN_ROPE_PLAIN = 0,  /* f_i = theta^(-2 i / rotary_dim) radians per position */
+  QATTN_ROPE_LINEAR = 1, /* f_i / factor: position interpolation */
+  QATTN_ROPE_YARN = 2    /* the YaRN paper's "NTK by parts": f_i (1 - r_i) + r_i f_i / factor, with r_i a
+                          * ramp from 0 to 1 over the pairs between the one that turns beta_fast times in
+                          * original_context positions (rounded down, >= 0) and the one that turns
+                          * beta_slow times (rounded up, < rotary_dim) */
+};
+/* The head vectors of one tensor: head h of token t at element t*x_row_stride + h*head_dim of x, its
+ * result likewise in out.  out may be x with the same stride (in place); they may not overlap
+ * otherwise.  Any stride >= heads*head_dim and any 2-byte aligned address; 16-byte aligned ones with
+ * strides of multiples of 8 elements run faster. */
+typedef struct qattn_rope_block {
+  const void* x;
+  void* out;
+  int64_t x_row_stride, out_row_stride;
+  int32_t heads;
+} qattn_rope_block;
+typedef struct qattn_rope_desc {
+  qattn_rope_block q, k;    /* rotated alike in one launch; k.heads 0: no k */
+  const int32_t* positions; /* device [tokens]: any value, in any order */
+  int64_t tokens;           /* below 2^24 */
+  int32_t dtype;            /* enum qattn_dtype */
+  int32_t head_dim;         /* up to QATTN_MAX_ROPE_DIM */
+  int32_t rotary_dim;       /* even, 2 .. head_dim: the first elements of a head; the others pass through */
+  int32_t layout, scaling;  /* enum qattn_rope_layout, enum qattn_rope_scaling */
+  int32_t inverse;          /* nonzero: the rotation by the negative angle, which undoes the rotation (with
+                             * a magnitude of 1) and maps the output's gradient to the input's */
+  double theta;
+  double factor;            /* LINEAR, YARN: > 0 */
+  double original_context, beta_fast, beta_slow; /* YARN: > 0, beta_fast > beta_slow */
+  double magnitude;         /* cos and sin are multiplied by it; 0: 1, for YARN 0.1 ln(factor) + 1 */
+} qattn_rope_desc;
+/* out_a = x_a cos - x_b sin, out_b = x_b cos + x_a sin for each pair (a, b), angle = position * f_i,
+ * in f32 with the angle reduced in f64, rounded once.  Enqueued on `stream` (NULL: the context
+ * stream); allocates nothing, waits for nothing. */
+int qattn_rope(qattn_ctx* ctx, const qattn_rope_desc* desc, qattn_stream_t stream);
+
+enum qattn_kv_format {
+  QATTN_KV_16BIT = 0, /* elements of `dtype` as they are */
+  /* One byte an element and one f32 scale per (slot, KV head), for K and V each; the value is
+   * code * scale.  amax is the vector's largest finite magnitude; vectors with amax < 2^-100 are stored
+   * as zeros with scale 1. */
+  QATTN_KV_E4M3 = 1,  /* OCP e4m3 code of x / scale, scale the least power of two with amax <= 448 scale;
+                       * infinities become +-448 scale, NaN the NaN code; no code whose value is past
+                       * the largest of `dtype` (240 takes the place of 256 and more at scale 2^8 for
+                       * fp16, 2^120 for bf16) */
+  QATTN_KV_INT8 = 2   /* rint(x * (127 / amax)) in [-127, 127], scale = amax / 127; infinities become
+                       * +-127, NaN 0 */
+};
+/* A paged cache in the caller's device memory: slot s is row s % page_size of page s / page_size;
+ * codes [pages][kv_heads][page_size][head_dim], scales [pages][kv_heads][page_size].  Device
+ * pointers 16-byte aligned; page_size a power of two in [16, 4096]; head_dim 64 or 128. */
+typedef struct qattn_kv_cache {
+  void* k;
+  void* v;
+  float* k_scale; /* E4M3, INT8 (not read for 16BIT) */
+  float* v_scale;
+  int32_t pages, page_size, kv_heads, head_dim;
+  int32_t dtype;  /* enum qattn_dtype: of the rows written and read */
+  int32_t format; /* enum qattn_kv_format */
+} qattn_kv_cache;
+/* Writes K and V rows into the cache: token t's head h, at element t*k_row_stride + h*head_dim of k
+ * (likewise v), goes to slot slots[t], a device array of `tokens` int64; a slot outside
+ * [0, pages*page_size) writes nothing (padding), and no slot may be named twice in a call.  Rows 16-byte
+ * aligned, strides multiples of 8 elements, >= kv_heads*head_dim; tokens below 2^24 and
+ * tokens*kv_heads*head_dim below 2^35.  Enqueued on `stream`; allocates
+ * nothing. */
+int qattn_kv_write(qattn_ctx* ctx, const qattn_kv_cache* cache, const void* k, int64_t k_row_stride,
+                   const void* v, int64_t v_row_stride, const int64_t* slots, int64_t tokens,
+                   qattn_stream_t stream);
+/* Reads slots back into rows: element = code * scale rounded to `dtype`; a slot outside the cache
+ * gives a row of zeros.  Otherwise as qattn_kv_write (slots may repeat). */
+int qattn_kv_read(qattn_ctx* ctx, const qattn_kv_cache* cache, const int64_t* slots, int64_t tokens,
+                  void* k, int64_t k_row_stride, void* v, int64_t v_row_stride, qattn_stream_t stream);
 
 /* ---- consumer: last-token pool + L2 norm  (replaces LastTokenPoolKernel, ops.ts:347-379) --- */
 /* For each sequence i < nseq: out[i*out_row_stride + d] = f32(x[r*row_stride + d]) * s for

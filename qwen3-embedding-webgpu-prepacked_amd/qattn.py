@@ -21,6 +21,10 @@ OK, EINVAL, EHIP, ENOMEM, ENODEV = 0, -1, -2, -3, -4
 MASK_CAUSAL, MASK_PREFIX_LOCAL = 0, 1
 FLAG_BATCH_INVARIANT = 1  # qattn_run_flags
 HQ, HKV, HD = 16, 8, 128
+F16, BF16 = 0, 1  # qattn_dtype
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1  # qattn_rope_layout
+ROPE_PLAIN, ROPE_LINEAR, ROPE_YARN = 0, 1, 2  # qattn_rope_scaling
+KV_16BIT, KV_E4M3, KV_INT8 = 0, 1, 2  # qattn_kv_format
 
 
 class QattnError(RuntimeError):
@@ -83,6 +87,38 @@ class ModelDesc(ctypes.Structure):
         ("eps", ctypes.c_double), ("rope_theta", ctypes.c_double),
         ("mask", ctypes.c_int32), ("prefix", ctypes.c_int32), ("window", ctypes.c_int32),
         ("flags", ctypes.c_int32),
+    ]
+
+
+class RopeBlock(ctypes.Structure):
+    """qattn_rope_block."""
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("out", ctypes.c_void_p),
+        ("x_row_stride", ctypes.c_int64), ("out_row_stride", ctypes.c_int64),
+        ("heads", ctypes.c_int32),
+    ]
+
+
+class RopeDesc(ctypes.Structure):
+    """qattn_rope_desc."""
+    _fields_ = [
+        ("q", RopeBlock), ("k", RopeBlock),
+        ("positions", ctypes.c_void_p), ("tokens", ctypes.c_int64),
+        ("dtype", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("rotary_dim", ctypes.c_int32),
+        ("layout", ctypes.c_int32), ("scaling", ctypes.c_int32), ("inverse", ctypes.c_int32),
+        ("theta", ctypes.c_double), ("factor", ctypes.c_double), ("original_context", ctypes.c_double),
+        ("beta_fast", ctypes.c_double), ("beta_slow", ctypes.c_double), ("magnitude", ctypes.c_double),
+    ]
+
+
+class KvCache(ctypes.Structure):
+    """qattn_kv_cache: a paged K/V cache in the caller's device memory."""
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+        ("pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32), ("format", ctypes.c_int32),
     ]
 
 
@@ -154,6 +190,9 @@ def lib():
         "qattn_embed_q6k": (ctypes.c_int, [vp, vp, i64, vp, i64, i32, vp, i64, vp]),
         "qattn_rmsnorm": (ctypes.c_int, [vp, vp, i64, vp, i64, vp, vp, i64, i64, i32, ctypes.c_double, vp]),
         "qattn_swiglu": (ctypes.c_int, [vp, vp, i64, vp, i64, i64, i32, vp]),
+        "qattn_rope": (ctypes.c_int, [vp, ctypes.POINTER(RopeDesc), vp]),
+        "qattn_kv_write": (ctypes.c_int, [vp, ctypes.POINTER(KvCache), vp, i64, vp, i64, vp, i64, vp]),
+        "qattn_kv_read": (ctypes.c_int, [vp, ctypes.POINTER(KvCache), vp, i64, vp, i64, vp, i64, vp]),
         "qattn_model_create": (ctypes.c_int, [vp, ctypes.POINTER(ModelDesc), pvp]),
         "qattn_model_destroy": (None, [vp]),
         "qattn_model_plan_create": (ctypes.c_int, [vp, i32, i32, pvp]),
@@ -189,6 +228,32 @@ def make_desc(q, k, v, o, cu_seqlens, mask=MASK_PREFIX_LOCAL, prefix=176, window
                 cu.ctypes.data, len(cu) - 1, mask, prefix, window, o_last, flags)
     d._cu = cu
     return d
+
+
+def make_rope_desc(positions, tokens, q, k=None, head_dim=HD, rotary_dim=None, layout=ROPE_HALF, dtype=F16,
+                   q_row_stride=None, k_row_stride=None, q_out_row_stride=None, k_out_row_stride=None, theta=1e6,
+                   scaling=ROPE_PLAIN, factor=1.0, original_context=32768, beta_fast=32.0, beta_slow=1.0,
+                   magnitude=0.0, inverse=False):
+    """Build a qattn_rope_desc.  q and k are (x, out, heads) with device addresses (out = x: in
+    place); row strides default to heads * head_dim.  positions: device int32 [tokens]."""
+    def block(part, stride, out_stride):
+        if part is None:
+            return RopeBlock()
+        x, out, heads = part
+        stride = heads * head_dim if stride is None else stride
+        if out_stride is None:
+            out_stride = stride if x == out else heads * head_dim
+        return RopeBlock(x, out, stride, out_stride, heads)
+    return RopeDesc(block(q, q_row_stride, q_out_row_stride), block(k, k_row_stride, k_out_row_stride), positions,
+                    tokens, dtype, head_dim, head_dim if rotary_dim is None else rotary_dim, layout, scaling,
+                    1 if inverse else 0, theta, factor, original_context, beta_fast, beta_slow, magnitude)
+
+
+def make_kv_cache(k, v, pages, page_size, kv_heads=HKV, head_dim=HD, dtype=F16, format=KV_16BIT, k_scale=None,
+                  v_scale=None):
+    """Build a qattn_kv_cache over device addresses: codes [pages, kv_heads, page_size, head_dim],
+    scales f32 [pages, kv_heads, page_size]."""
+    return KvCache(k, v, k_scale, v_scale, pages, page_size, kv_heads, head_dim, dtype, format)
 
 
 def plan_slots(desc, max_slots=0):
@@ -471,6 +536,25 @@ class Context:
                                   2 * width if gate_up_row_stride is None else gate_up_row_stride, out_ptr,
                                   width if out_row_stride is None else out_row_stride, rows, width, stream),
                self.handle)
+
+    def rope(self, desc, stream=None):
+        """Rotary positions of one launch's q and k (qattn_rope; desc from make_rope_desc)."""
+        _check(lib().qattn_rope(self.handle, ctypes.byref(desc), stream), self.handle)
+
+    def kv_write(self, cache, k_ptr, v_ptr, slots_ptr, tokens, k_row_stride=None, v_row_stride=None, stream=None):
+        """K and V rows into cache slots (qattn_kv_write); slots: device int64 [tokens]."""
+        width = cache.kv_heads * cache.head_dim
+        _check(lib().qattn_kv_write(self.handle, ctypes.byref(cache), k_ptr,
+                                    width if k_row_stride is None else k_row_stride, v_ptr,
+                                    width if v_row_stride is None else v_row_stride, slots_ptr, tokens, stream),
+               self.handle)
+
+    def kv_read(self, cache, slots_ptr, tokens, k_ptr, v_ptr, k_row_stride=None, v_row_stride=None, stream=None):
+        """Cache slots into K and V rows (qattn_kv_read)."""
+        width = cache.kv_heads * cache.head_dim
+        _check(lib().qattn_kv_read(self.handle, ctypes.byref(cache), slots_ptr, tokens, k_ptr,
+                                   width if k_row_stride is None else k_row_stride, v_ptr,
+                                   width if v_row_stride is None else v_row_stride, stream), self.handle)
 
     def model(self, token_embd, output_norm, layers, eps=1e-6, rope_theta=1e6, mask=MASK_PREFIX_LOCAL,
               prefix=176, window=432, flags=0):
