@@ -403,6 +403,75 @@ int qattn_kv_write(qattn_ctx* ctx, const qattn_kv_cache* cache, const void* k, i
 int qattn_kv_read(qattn_ctx* ctx, const qattn_kv_cache* cache, const int64_t* slots, int64_t tokens,
                   void* k, int64_t k_row_stride, void* v, int64_t v_row_stride, qattn_stream_t stream);
 
+typedef struct qattn_shared_run qattn_shared_run;
+/* Attention of a batch of sequences behind one shared prefix.  The keys of sequence i are the prefix's
+ * prefix_len keys at positions 0 .. prefix_len-1, then its own own_len[i] keys; its m = cu_q[i+1] -
+ * cu_q[i] queries are the last m of those positions (a prompt: m = own_len[i]; a step: m = 1).  Query
+ * head h reads KV head h / (q_heads / kv_heads).  A query sees the keys at its position and before it,
+ * under QATTN_MASK_PREFIX_LOCAL those of positions < prefix or > its own - window.  One that sees none
+ * (at a position below 0: m beyond the keys; an empty mask) gives zeros, and a key that a query does
+ * not see adds nothing to it, whatever it holds. */
+typedef struct qattn_shared_desc {
+  const void* q; /* head h of packed query t at element t*q_row_stride + h*head_dim; o likewise */
+  void* o;
+  int64_t q_row_stride, o_row_stride;
+  int32_t q_heads;          /* a multiple of cache.kv_heads, up to 64 of them to a KV head */
+  qattn_kv_cache cache;     /* kv_heads, head_dim and dtype always; the rest if pages are read */
+  const int32_t* prefix_pages; /* host: ceil(prefix_len / page_size) page numbers; copied */
+  int32_t prefix_len;       /* may be 0 */
+  const int32_t* cu_q;      /* host: nseq+1 non-decreasing offsets of the packed queries, from 0; copied */
+  int32_t nseq;
+  const int32_t* own_len;   /* host [nseq], each >= 0; copied */
+  const int32_t* own_pages; /* host: ceil(own_len[i] / page_size) page numbers of each sequence in turn;
+                             * copied.  NULL: the own keys are rows of k and v, packed in turn */
+  const void* k;            /* own keys as rows of `dtype`, 16 bit */
+  const void* v;
+  int64_t k_row_stride, v_row_stride;
+  int32_t mask, prefix, window; /* enum qattn_mask_kind; PREFIX_LOCAL: >= 0, both may be 0 */
+  double scale;             /* of the scores; 0: 1/sqrt(head_dim) */
+} qattn_shared_desc;
+/* Tensors 16-byte aligned, strides multiples of 8 elements up to 2^24 and at least the heads' width;
+ * page numbers in [0, pages); positions below 2^30; at most 2^22 rows (queries * q_heads / kv_heads).
+ * The run plans the launch on the host, as qattn_run_create does: rows (query, head of the group) of
+ * all sequences are stacked, so that a tile of prefix keys is read once for up to 128 rows; long key
+ * ranges of few rows are spread over workgroups and their partial results merged by a second launch. */
+int qattn_shared_run_create(qattn_ctx* ctx, const qattn_shared_desc* desc, qattn_shared_run** out);
+/* Enqueues the launch.  Launches of one run must not overlap on the device: they share its workspace.
+ * Allocates and waits for nothing, so it can be captured; a captured launch stays valid until the run is
+ * updated, rebound or destroyed. */
+int qattn_shared_run_encode(qattn_shared_run* run, qattn_stream_t stream);
+/* New lengths and pages (a step later, the next batch); the tensors hold as many rows as it names.
+ * Works as qattn_run_update: two plan images, waits only for this run's launches that read the older
+ * one, and on failure the run keeps its plan. */
+int qattn_shared_run_update(qattn_shared_run* run, const int32_t* prefix_pages, int32_t prefix_len,
+                            const int32_t* cu_q, int32_t nseq, const int32_t* own_len, const int32_t* own_pages);
+/* Other tensors of the same strides, and another cache of the same geometry (the layers of a model):
+ * k and v for runs whose own keys are rows. */
+int qattn_shared_run_rebind(qattn_shared_run* run, const void* q, void* o, const qattn_kv_cache* cache,
+                            const void* k, const void* v);
+void qattn_shared_run_destroy(qattn_shared_run* run);
+
+typedef struct qattn_shared_info {
+  int64_t tokens;        /* queries */
+  int64_t keys;          /* prefix_len + the sum of own_len */
+  int64_t pairs;         /* (query, key) pairs that are seen */
+  int64_t flops;         /* 4 * head_dim * q_heads * pairs */
+  int32_t items;         /* workgroups per KV head */
+  int32_t merged_rows;   /* rows per KV head that the second launch merges */
+  int64_t partial_rows;  /* rows per KV head of partial results */
+} qattn_shared_info;
+int qattn_shared_run_get_info(const qattn_shared_run* run, qattn_shared_info* info);
+/* Host-only planning (no device; 256 compute units): the plan as int32 words, the counts first:
+ * {items, segments, merged rows, tokens, page numbers, 0, 0, 0}, then per item {first row, rows, first
+ * segment, end segment, first partial row or -1, key tiles, kind (0: 128-row blocks over 64-key tiles,
+ * 1: 16-row blocks over 32-key tiles), least query position, greatest, 0, 0, 0}, per segment {source
+ * (0 prefix pages, 1 own pages, 2 own rows), first page number or first row, keys, position of key 0,
+ * first tile, end tile, first row, end row}, per merged row {row, then for up to two groups of partial
+ * results: first partial row, count, distance between them, and 0}, per token its position, and the
+ * page numbers.  words NULL: only *count. */
+int qattn_shared_plan_describe(const qattn_shared_desc* desc, int32_t* words, int64_t capacity, int64_t* count,
+                               qattn_shared_info* info);
+
 /* ---- consumer: last-token pool + L2 norm  (replaces LastTokenPoolKernel, ops.ts:347-379) --- */
 /* For each sequence i < nseq: out[i*out_row_stride + d] = f32(x[r*row_stride + d]) * s for
  * d < width, r = cu_seqlens[i+1]-1 (the reference's row b*S + lengths[b]-1 of its padded layout,

@@ -1,16 +1,31 @@
 // shared_api.hip -- entry points of the operators behind one shared prefix: rotary positions, the paged
-// K/V cache.
+// K/V cache, and the attention over it.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <cmath>
+#include <cstring>
+#include <new>
+#include <vector>
 
 #include "context.h"
-#include "shared_api.h"
+#include "shared_attn.h"
 #include "shared_ops.h"
 
-namespace qattn {
+using namespace qattn;
 
+namespace {
+
+constexpr int32_t kMaxKvHeads = 256;
+constexpr int32_t kMaxRopeHeads = 4096;
+// Of a row-wise launch, whose grid has to stay below 2^32 threads.
+constexpr int64_t kMaxRowTokens = ((int64_t)1 << 24) - 1;
+constexpr int64_t kMaxRowValues = ((int64_t)1 << 35) - 1;  // tokens * kv_heads * head_dim: eight to a thread
+constexpr int64_t kMaxSharedRows = (int64_t)1 << 22;       // queries * heads of a group
+constexpr int64_t kMaxSharedStride = (int64_t)1 << 24;     // elements: 16 rows of it within a 32-bit offset
+constexpr int64_t kMaxSharedGroups = (int64_t)1 << 23;     // workgroups of a launch
+
+// Geometry, and with needs_pages the tensors, of a cache.
 int check_kv_cache(qattn_ctx* ctx, const qattn_kv_cache* c, bool needs_pages) {
   if (!c) return fail(ctx, QATTN_EINVAL, "cache is NULL");
   if (c->dtype != QATTN_DTYPE_F16 && c->dtype != QATTN_DTYPE_BF16) return fail(ctx, QATTN_EINVAL, "unknown dtype %d", c->dtype);
@@ -27,12 +42,6 @@ int check_kv_cache(qattn_ctx* ctx, const qattn_kv_cache* c, bool needs_pages) {
     return fail(ctx, QATTN_EINVAL, "cache k_scale/v_scale NULL or not 16-byte aligned");
   return QATTN_OK;
 }
-
-}  // namespace qattn
-
-using namespace qattn;
-
-namespace {
 
 int check_rope_block(qattn_ctx* ctx, const char* name, const qattn_rope_block& b, int32_t head_dim) {
   if (!b.x || !b.out) return fail(ctx, QATTN_EINVAL, "%s: x/out is NULL", name);
@@ -165,6 +174,340 @@ int qattn_kv_read(qattn_ctx* ctx, const qattn_kv_cache* cache, const int64_t* sl
   if (rc || !tokens) return rc;
   DeviceGuard g(ctx->device);
   HIP_TRY(ctx, launch_kv_read(a, pick_stream(ctx, stream)));
+  return QATTN_OK;
+}
+
+}  // extern "C"
+
+// ---- attention behind one shared prefix ---------------------------------------------------------------
+
+// Two plan images, as a qattn_run keeps them: the installed plan lives in image `cur`; an update waits for
+// the launches that last read the other one (events recorded on their streams when it was retired),
+// fills it and switches.
+struct qattn_shared_run {
+  qattn_ctx* ctx = nullptr;
+  qattn_shared_desc desc{};  // without its host arrays
+  SharedParams params{};
+  void* image[2] = {nullptr, nullptr};
+  size_t image_bytes[2] = {0, 0};
+  std::vector<hipStream_t> streams[2];
+  std::vector<hipEvent_t> fences[2];
+  int cur = -1;
+  void* partials = nullptr;
+  size_t partial_bytes = 0;
+  qattn_shared_info info{};
+};
+
+namespace {
+
+int check_shared_tensors(qattn_ctx* ctx, const qattn_shared_desc* d, bool needs_pages, bool needs_rows) {
+  int rc = check_kv_cache(ctx, &d->cache, needs_pages);
+  if (rc) return rc;
+  const int64_t group = d->q_heads / d->cache.kv_heads;
+  if (d->q_heads < 1 || d->q_heads % d->cache.kv_heads || group > 64)
+    return fail(ctx, QATTN_EINVAL, "q_heads %d: a multiple of kv_heads %d, up to 64 times", d->q_heads, d->cache.kv_heads);
+  const auto bad_stride = [](int64_t stride, int64_t width) { return stride < width || stride % 8 || stride > kMaxSharedStride; };
+  if (!d->q || !d->o || !aligned16(d->q) || !aligned16(d->o)) return fail(ctx, QATTN_EINVAL, "q/o NULL or not 16-byte aligned");
+  const int64_t q_width = (int64_t)d->q_heads * d->cache.head_dim, kv_width = (int64_t)d->cache.kv_heads * d->cache.head_dim;
+  if (bad_stride(d->q_row_stride, q_width) || bad_stride(d->o_row_stride, q_width))
+    return fail(ctx, QATTN_EINVAL, "row strides (q %lld, o %lld): q_heads*head_dim = %lld .. 2^24, multiples of 8",
+                (long long)d->q_row_stride, (long long)d->o_row_stride, (long long)q_width);
+  if (!needs_rows) return QATTN_OK;
+  if (!d->k || !d->v || !aligned16(d->k) || !aligned16(d->v)) return fail(ctx, QATTN_EINVAL, "k/v NULL or not 16-byte aligned");
+  if (bad_stride(d->k_row_stride, kv_width) || bad_stride(d->v_row_stride, kv_width))
+    return fail(ctx, QATTN_EINVAL, "row strides (k %lld, v %lld): kv_heads*head_dim = %lld .. 2^24, multiples of 8",
+                (long long)d->k_row_stride, (long long)d->v_row_stride, (long long)kv_width);
+  return QATTN_OK;
+}
+
+int check_shared(qattn_ctx* ctx, const qattn_shared_desc* d) {
+  if (!d) return fail(ctx, QATTN_EINVAL, "desc is NULL");
+  int rc = validate_cu(ctx, d->cu_q, d->nseq);
+  if (rc) return rc;
+  if (!d->own_len) return fail(ctx, QATTN_EINVAL, "own_len is NULL");
+  if (d->prefix_len < 0 || d->prefix_len >= kMaxPosition) return fail(ctx, QATTN_EINVAL, "prefix_len %d outside [0, 2^30)", d->prefix_len);
+  int64_t own = 0;
+  for (int32_t i = 0; i < d->nseq; ++i) {
+    if (d->own_len[i] < 0 || (int64_t)d->prefix_len + d->own_len[i] >= kMaxPosition)
+      return fail(ctx, QATTN_EINVAL, "own_len[%d] = %d: >= 0, positions below 2^30", i, d->own_len[i]);
+    own += d->own_len[i];
+  }
+  if (own >= ((int64_t)1 << 31)) return fail(ctx, QATTN_EINVAL, "too many own keys (%lld)", (long long)own);
+  rc = check_shared_tensors(ctx, d, d->prefix_len > 0 || (d->own_pages && own), !d->own_pages && own);
+  if (rc) return rc;
+  if (d->mask != QATTN_MASK_CAUSAL && d->mask != QATTN_MASK_PREFIX_LOCAL) return fail(ctx, QATTN_EINVAL, "unknown mask kind %d", d->mask);
+  if (d->mask == QATTN_MASK_PREFIX_LOCAL && (d->prefix < 0 || d->window < 0))
+    return fail(ctx, QATTN_EINVAL, "prefix (%d) and window (%d) must be >= 0", d->prefix, d->window);
+  if (!(d->scale >= 0.0) || !(d->scale < 1e30)) return fail(ctx, QATTN_EINVAL, "scale must be >= 0 and finite");
+  if (d->cu_q[d->nseq] * (int64_t)(d->q_heads / d->cache.kv_heads) > kMaxSharedRows)
+    return fail(ctx, QATTN_EINVAL, "%d queries: queries * q_heads / kv_heads up to 2^22", d->cu_q[d->nseq]);
+  const int32_t size = d->cache.page_size;
+  const auto check_pages = [&](const char* name, const int32_t* pages, int64_t n) -> int {
+    if (n && !pages) return fail(ctx, QATTN_EINVAL, "%s is NULL", name);
+    for (int64_t i = 0; i < n; ++i)
+      if (pages[i] < 0 || pages[i] >= d->cache.pages)
+        return fail(ctx, QATTN_EINVAL, "%s[%lld] = %d outside [0, %d)", name, (long long)i, pages[i], d->cache.pages);
+    return QATTN_OK;
+  };
+  if (d->prefix_len) rc = check_pages("prefix_pages", d->prefix_pages, (d->prefix_len + (int64_t)size - 1) / size);
+  if (rc || !d->own_pages || !own) return rc;
+  int64_t n = 0;
+  for (int32_t i = 0; i < d->nseq; ++i) n += (d->own_len[i] + (int64_t)size - 1) / size;
+  return check_pages("own_pages", d->own_pages, n);
+}
+
+// Plans a checked description; refuses what no launch could hold.
+int make_shared_plan(qattn_ctx* ctx, const qattn_shared_desc& d, int compute_units, SharedPlan* plan) {
+  plan_shared(d, compute_units, plan);
+  const int64_t heads = d.cache.kv_heads;
+  if ((int64_t)plan->items.size() * heads > kMaxSharedGroups || ((int64_t)plan->merges.size() * heads + 3) / 4 > kMaxSharedGroups ||
+      plan->partial_rows >= ((int64_t)1 << 31))
+    return fail(ctx, QATTN_EINVAL, "too many rows for one launch (%zu items, %zu merged rows, %lld KV heads)", plan->items.size(),
+                plan->merges.size(), (long long)heads);
+  return QATTN_OK;
+}
+
+void bind_shared(SharedParams* p, const qattn_shared_desc& d) {
+  p->q = static_cast<const uint16_t*>(d.q);
+  p->o = static_cast<uint16_t*>(d.o);
+  p->cache[0] = static_cast<const char*>(d.cache.k);
+  p->cache[1] = static_cast<const char*>(d.cache.v);
+  p->cache_scale[0] = d.cache.k_scale;
+  p->cache_scale[1] = d.cache.v_scale;
+  p->rows[0] = static_cast<const uint16_t*>(d.k);
+  p->rows[1] = static_cast<const uint16_t*>(d.v);
+}
+
+int retire_shared(qattn_shared_run* run, int i) {
+  for (hipStream_t s : run->streams[i]) {
+    hipEvent_t ev = nullptr;
+    HIP_TRY(run->ctx, hipEventCreateWithFlags(&ev, hipEventDisableTiming));
+    const hipError_t e = hipEventRecord(ev, s);
+    if (e != hipSuccess) {
+      (void)hipEventDestroy(ev);
+      return fail(run->ctx, QATTN_EHIP, "hipEventRecord: %s", hipGetErrorString(e));
+    }
+    run->fences[i].push_back(ev);
+  }
+  run->streams[i].clear();
+  return QATTN_OK;
+}
+
+int wait_shared(qattn_shared_run* run, int i) {
+  auto& f = run->fences[i];
+  while (!f.empty()) {
+    HIP_TRY(run->ctx, hipEventSynchronize(f.back()));
+    (void)hipEventDestroy(f.back());
+    f.pop_back();
+  }
+  return QATTN_OK;
+}
+
+// Plans `d` into the run's other image and switches to it; on failure the installed plan stays.
+int install_shared_plan(qattn_shared_run* run, const qattn_shared_desc& d) {
+  qattn_ctx* ctx = run->ctx;
+  SharedPlan plan;
+  int rc = make_shared_plan(ctx, d, std::max(1, ctx->cu_count), &plan);
+  if (rc) return rc;
+  std::vector<char> host;
+  const auto put = [&](const void* data, size_t bytes) {
+    const size_t at = (host.size() + 63) / 64 * 64;
+    host.resize(at + bytes);
+    if (bytes) std::memcpy(host.data() + at, data, bytes);
+    return at;
+  };
+  const size_t items = put(plan.items.data(), plan.items.size() * sizeof(SharedItem));
+  const size_t segs = put(plan.segs.data(), plan.segs.size() * sizeof(SharedSeg));
+  const size_t merges = put(plan.merges.data(), plan.merges.size() * sizeof(SharedMerge));
+  const size_t positions = put(plan.positions.data(), plan.positions.size() * sizeof(int32_t));
+  const size_t pages = put(plan.pages.data(), plan.pages.size() * sizeof(int32_t));
+  DeviceGuard g(ctx->device);
+  const int next = run->cur < 0 ? 0 : run->cur ^ 1;
+  if (run->cur >= 0 && (rc = retire_shared(run, run->cur))) return rc;
+  if ((rc = wait_shared(run, next))) return rc;
+  if (host.size() > run->image_bytes[next]) {
+    void* grown = nullptr;
+    const size_t bytes = host.size() + host.size() / 4;  // room for a few steps
+    const hipError_t e = hipMalloc(&grown, bytes);
+    if (e != hipSuccess) return fail(ctx, QATTN_ENOMEM, "hipMalloc(plan, %zu): %s", bytes, hipGetErrorString(e));
+    if (run->image[next]) (void)hipFree(run->image[next]);
+    run->image[next] = grown;
+    run->image_bytes[next] = bytes;
+  }
+  const size_t values = (size_t)plan.partial_rows * d.cache.kv_heads;
+  const size_t part_bytes = values * (d.cache.head_dim * sizeof(float) + sizeof(float2));
+  if (part_bytes > run->partial_bytes) {
+    // Launches of the installed plan may still use the workspace.
+    if (run->cur >= 0 && (rc = wait_shared(run, run->cur))) return rc;
+    void* grown = nullptr;
+    const size_t bytes = part_bytes + part_bytes / 4;
+    const hipError_t e = hipMalloc(&grown, bytes);
+    if (e != hipSuccess) return fail(ctx, QATTN_ENOMEM, "hipMalloc(workspace, %zu): %s", bytes, hipGetErrorString(e));
+    if (run->partials) (void)hipFree(run->partials);
+    run->partials = grown;
+    run->partial_bytes = bytes;
+    // The installed plan keeps working, should the upload below fail: its rows fit the larger workspace.
+    run->params.part_o = static_cast<float*>(grown);
+    run->params.part_ml = reinterpret_cast<float2*>(run->params.part_o + (size_t)run->info.partial_rows * d.cache.kv_heads * d.cache.head_dim);
+  }
+  if (!host.empty()) HIP_TRY(ctx, hipMemcpy(run->image[next], host.data(), host.size(), hipMemcpyHostToDevice));
+  SharedParams p{};
+  bind_shared(&p, d);
+  p.q_stride = d.q_row_stride;
+  p.o_stride = d.o_row_stride;
+  p.row_stride[0] = d.k_row_stride;
+  p.row_stride[1] = d.v_row_stride;
+  const char* image = static_cast<const char*>(run->image[next]);
+  p.items = reinterpret_cast<const SharedItem*>(image + items);
+  p.segs = reinterpret_cast<const SharedSeg*>(image + segs);
+  p.merges = reinterpret_cast<const SharedMerge*>(image + merges);
+  p.positions = reinterpret_cast<const int32_t*>(image + positions);
+  p.pages = reinterpret_cast<const int32_t*>(image + pages);
+  p.part_o = static_cast<float*>(run->partials);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + values * d.cache.head_dim);
+  p.n_items = (int32_t)plan.items.size();
+  p.n_merges = (int32_t)plan.merges.size();
+  p.kv_heads = d.cache.kv_heads;
+  p.group = d.q_heads / d.cache.kv_heads;
+  while ((1 << p.page_shift) < d.cache.page_size) ++p.page_shift;
+  p.mask = d.mask;
+  p.prefix = d.prefix;
+  p.window = std::min(d.window, kMaxPosition);
+  p.scale_log2 = (float)((d.scale > 0.0 ? d.scale : 1.0 / std::sqrt((double)d.cache.head_dim)) * 1.4426950408889634);
+  run->params = p;
+  run->info = plan.info;
+  run->desc = d;
+  run->desc.prefix_pages = run->desc.cu_q = run->desc.own_len = nullptr;
+  if (d.own_pages) run->desc.own_pages = reinterpret_cast<const int32_t*>(run);  // only whether there are any
+  run->cur = next;
+  return QATTN_OK;
+}
+
+int install_shared(qattn_shared_run* run, const qattn_shared_desc& d) {
+  try {
+    return install_shared_plan(run, d);
+  } catch (const std::bad_alloc&) {
+    return fail(run->ctx, QATTN_ENOMEM, "out of host memory for the plan");
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int qattn_shared_run_create(qattn_ctx* ctx, const qattn_shared_desc* desc, qattn_shared_run** out) {
+  if (!ctx || !out) return fail(ctx, QATTN_EINVAL, "ctx/out is NULL");
+  *out = nullptr;
+  int rc = check_shared(ctx, desc);
+  if (rc) return rc;
+  auto* run = new (std::nothrow) qattn_shared_run();
+  if (!run) return fail(ctx, QATTN_ENOMEM, "out of host memory");
+  run->ctx = ctx;
+  rc = install_shared(run, *desc);
+  if (rc) {
+    qattn_shared_run_destroy(run);
+    return rc;
+  }
+  *out = run;
+  return QATTN_OK;
+}
+
+int qattn_shared_run_encode(qattn_shared_run* run, qattn_stream_t stream) {
+  if (!run) return fail(nullptr, QATTN_EINVAL, "run is NULL");
+  DeviceGuard g(run->ctx->device);
+  const hipStream_t s = pick_stream(run->ctx, stream);
+  auto& used = run->streams[run->cur];
+  if (std::find(used.begin(), used.end(), s) == used.end()) used.push_back(s);
+  HIP_TRY(run->ctx, launch_shared_attn(run->params, run->desc.cache.dtype, run->desc.cache.format, run->desc.cache.head_dim, s));
+  return QATTN_OK;
+}
+
+int qattn_shared_run_update(qattn_shared_run* run, const int32_t* prefix_pages, int32_t prefix_len, const int32_t* cu_q,
+                            int32_t nseq, const int32_t* own_len, const int32_t* own_pages) {
+  if (!run) return fail(nullptr, QATTN_EINVAL, "run is NULL");
+  if ((own_pages != nullptr) != (run->desc.own_pages != nullptr))
+    return fail(run->ctx, QATTN_EINVAL, "own_pages must be given as when the run was created");
+  qattn_shared_desc d = run->desc;
+  d.prefix_pages = prefix_pages;
+  d.prefix_len = prefix_len;
+  d.cu_q = cu_q;
+  d.nseq = nseq;
+  d.own_len = own_len;
+  d.own_pages = own_pages;
+  const int rc = check_shared(run->ctx, &d);
+  return rc ? rc : install_shared(run, d);
+}
+
+int qattn_shared_run_rebind(qattn_shared_run* run, const void* q, void* o, const qattn_kv_cache* cache, const void* k,
+                            const void* v) {
+  if (!run) return fail(nullptr, QATTN_EINVAL, "run is NULL");
+  if (!cache) return fail(run->ctx, QATTN_EINVAL, "cache is NULL");
+  qattn_shared_desc d = run->desc;
+  const qattn_kv_cache& c = d.cache;
+  if (cache->pages != c.pages || cache->page_size != c.page_size || cache->kv_heads != c.kv_heads || cache->head_dim != c.head_dim ||
+      cache->dtype != c.dtype || cache->format != c.format)
+    return fail(run->ctx, QATTN_EINVAL, "the cache has another geometry than the run's");
+  d.q = q;
+  d.o = o;
+  d.cache = *cache;
+  d.k = k;
+  d.v = v;
+  const int rc = check_shared_tensors(run->ctx, &d, run->desc.cache.k != nullptr, run->desc.k != nullptr);
+  if (rc) return rc;
+  bind_shared(&run->params, d);
+  run->desc = d;
+  return QATTN_OK;
+}
+
+void qattn_shared_run_destroy(qattn_shared_run* run) {
+  if (!run) return;
+  DeviceGuard g(run->ctx->device);
+  for (int i = 0; i < 2; ++i) {
+    if (retire_shared(run, i) != QATTN_OK)
+      for (hipStream_t s : run->streams[i]) (void)hipStreamSynchronize(s);
+    (void)wait_shared(run, i);
+  }
+  for (void* image : run->image)
+    if (image) (void)hipFree(image);
+  if (run->partials) (void)hipFree(run->partials);
+  delete run;
+}
+
+int qattn_shared_run_get_info(const qattn_shared_run* run, qattn_shared_info* info) {
+  if (!run || !info) return fail(nullptr, QATTN_EINVAL, "NULL argument");
+  *info = run->info;
+  return QATTN_OK;
+}
+
+int qattn_shared_plan_describe(const qattn_shared_desc* desc, int32_t* words, int64_t capacity, int64_t* count,
+                               qattn_shared_info* info) {
+  if (!count) return fail(nullptr, QATTN_EINVAL, "count is NULL");
+  int rc = check_shared(nullptr, desc);
+  if (rc) return rc;
+  SharedPlan plan;
+  try {
+    rc = make_shared_plan(nullptr, *desc, 256, &plan);
+  } catch (const std::bad_alloc&) {
+    rc = fail(nullptr, QATTN_ENOMEM, "out of host memory for the plan");
+  }
+  if (rc) return rc;
+  const int32_t head[8] = {(int32_t)plan.items.size(), (int32_t)plan.segs.size(), (int32_t)plan.merges.size(),
+                           (int32_t)plan.positions.size(), (int32_t)plan.pages.size(), 0, 0, 0};
+  *count = 8 + (int64_t)plan.items.size() * 12 + (int64_t)plan.segs.size() * 8 + (int64_t)plan.merges.size() * 8 +
+           (int64_t)plan.positions.size() + (int64_t)plan.pages.size();
+  if (info) *info = plan.info;
+  if (!words) return QATTN_OK;
+  if (capacity < *count) return fail(nullptr, QATTN_EINVAL, "capacity %lld < %lld words", (long long)capacity, (long long)*count);
+  const auto put = [&](const void* data, size_t bytes) {
+    if (bytes) std::memcpy(words, data, bytes);
+    words += bytes / sizeof(int32_t);
+  };
+  put(head, sizeof(head));
+  put(plan.items.data(), plan.items.size() * sizeof(SharedItem));
+  put(plan.segs.data(), plan.segs.size() * sizeof(SharedSeg));
+  put(plan.merges.data(), plan.merges.size() * sizeof(SharedMerge));
+  put(plan.positions.data(), plan.positions.size() * sizeof(int32_t));
+  put(plan.pages.data(), plan.pages.size() * sizeof(int32_t));
   return QATTN_OK;
 }
 

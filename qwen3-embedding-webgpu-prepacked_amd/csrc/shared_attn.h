@@ -1,0 +1,78 @@
+// shared_attn.h -- work items and launch arguments of the attention behind one shared prefix
+// (shared_attn.hip), filled by its host planner (shared_plan.cpp).
+//
+// Row r of the launch is head r % group of query r / group, the same for every KV head.  A plan is made
+// for one KV head; workgroup b runs item b / kv_heads for KV head b % kv_heads.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <vector>
+
+#include "../../include/qattn.h"
+
+namespace qattn {
+
+constexpr int kSharedThreads = 256;
+constexpr int kTallRows = 128, kTallKeys = 64;  // 4 wavefronts x 32 rows share a tile of 64 keys
+constexpr int kFlatRows = 16, kFlatKeys = 32;   // 4 wavefronts x the same 16 rows, a tile of 32 keys each
+constexpr int32_t kMaxPosition = 1 << 30;
+
+enum SharedSource { kPrefixPages = 0, kOwnPages = 1, kOwnRows = 2 };
+enum SharedKind { kTall = 0, kFlat = 1 };
+
+// Rows row0 .. row0 + rows - 1 over the tiles of segments seg_begin .. seg_end - 1.  Results go to the output
+// (part < 0) or, unnormalised, to partial rows part, part + 1, ...
+struct SharedItem {
+  int32_t row0, rows, seg_begin, seg_end, part, tiles, kind;
+  int32_t least, greatest;  // query positions among the rows
+  int32_t pad[3];
+};
+// Tiles tile_begin .. tile_end - 1 (of the item kind's size) of `keys` keys, seen by rows row_begin ..
+// row_end - 1 only.  base: the source's first page number (an index into the plan's list) or row.
+struct SharedSeg {
+  int32_t source, base, keys, position, tile_begin, tile_end, row_begin, row_end;
+};
+// A row whose results are merged: `count` partial rows from `first` on, `step` apart, in two groups.
+struct SharedMerge {
+  int32_t row;
+  struct Group {
+    int32_t first, count, step;
+  } group[2];
+  int32_t pad;
+};
+static_assert(sizeof(SharedItem) == 48 && sizeof(SharedSeg) == 32 && sizeof(SharedMerge) == 32, "plan words");
+
+struct SharedPlan {
+  std::vector<SharedItem> items;
+  std::vector<SharedSeg> segs;
+  std::vector<SharedMerge> merges;
+  std::vector<int32_t> positions;  // of each query
+  std::vector<int32_t> pages;
+  int64_t partial_rows = 0;
+  qattn_shared_info info{};
+};
+// `d`: validated.  compute_units: of the device.
+void plan_shared(const qattn_shared_desc& d, int compute_units, SharedPlan* plan);
+
+struct SharedParams {
+  const uint16_t* q;
+  uint16_t* o;
+  const char* cache[2];         // codes of K, V
+  const float* cache_scale[2];
+  const uint16_t* rows[2];      // own K, V rows
+  int64_t q_stride, o_stride, row_stride[2];
+  const SharedItem* items;
+  const SharedSeg* segs;
+  const SharedMerge* merges;
+  const int32_t* positions;
+  const int32_t* pages;
+  float* part_o;                // [partial row][kv_heads][head_dim]
+  float2* part_ml;              // [partial row][kv_heads]: the row's reference (log2) and sum
+  int32_t n_items, n_merges, kv_heads, group, page_shift;
+  int32_t mask, prefix, window;
+  float scale_log2;
+};
+hipError_t launch_shared_attn(const SharedParams& p, int dtype, int format, int head_dim, hipStream_t stream);
+
+}  // namespace qattn

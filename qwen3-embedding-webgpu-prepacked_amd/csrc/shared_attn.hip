@@ -1,0 +1,771 @@
+// shared_attn.hip -- attention of a batch of sequences behind one shared prefix (qattn_shared_run_*).
+//
+// o[r] = sum_j p_rj v_j / sum_j p_rj, p_rj = 2^(c q_r . k_j - m_r), over the keys that row r sees: the
+// prefix's, read from a paged cache that may hold 8-bit codes, and its sequence's own.  Rows of all
+// sequences are stacked (row = query * group + head of the group), so one tile of prefix keys serves 128
+// rows, whatever sequences they belong to.  Two kinds of item share a launch:
+//   tall  128 rows, 32 to a wavefront, over 64-key tiles that the four wavefronts share in LDS;
+//         S^T = K Q^T and O^T = V^T P^T on 32x32x16 MFMAs, a query row to a lane.  Codes become 16-bit
+//         elements once, on their way into LDS.  Bound by the matrix cores, the softmax's exponentials
+//         and LDS reads.
+//   flat  16 rows over 32-key tiles, every fourth tile to a wavefront, which keeps its own sum; K goes from
+//         memory straight into the MFMA operand, V through the wavefront's own 8 KiB of LDS for the
+//         transposed read; the four sums are joined at the end.  Bound by the cache's bytes.
+// An item whose rows have keys elsewhere too (other chunks, other items) leaves its unnormalised f32
+// sums, the row's reference m and its sum of p; shared_merge_kernel joins them.
+//
+// A row's reference moves only when a tile's maximum exceeds it by kLazy (in log2): p then stays below
+// 2^kLazy, far inside fp16, and most tiles rescale nothing.  p is rounded to the storage type for the PV
+// product, which moves each weight by at most half a step of that type; l sums the unrounded p in f32.
+#include "shared_attn.h"
+
+#include "elem.h"
+
+namespace qattn {
+
+namespace {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16x __attribute__((ext_vector_type(16)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s4 lds_s4;
+typedef __attribute__((address_space(4))) const int32_t const_i32;
+
+constexpr float kLazy = 8.f;
+constexpr float kNone = -INFINITY;
+
+template <bool BF16>
+__device__ inline f16x mfma32(u32x4 a, u32x4 b, f16x c) {
+  typedef typename Elem<BF16>::T8 T8;
+  if constexpr (BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(T8, a), __builtin_bit_cast(T8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(T8, a), __builtin_bit_cast(T8, b), c, 0, 0, 0);
+}
+template <bool BF16>
+__device__ inline f4 mfma16(u32x4 a, u32x4 b, f4 c) {
+  typedef typename Elem<BF16>::T8 T8;
+  if constexpr (BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(T8, a), __builtin_bit_cast(T8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(T8, a), __builtin_bit_cast(T8, b), c, 0, 0, 0);
+}
+
+// Raw buffer over `bytes` bytes: loads past its end give zeros.
+__device__ inline __amdgpu_buffer_rsrc_t buffer(const void* base, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00020000);
+}
+__device__ inline u32x4 load16(__amdgpu_buffer_rsrc_t rs, uint32_t offset) {
+  return __builtin_amdgcn_raw_buffer_load_b128(rs, offset, 0, 0);
+}
+
+// Combined with the other half-wavefront (lane ^ 32), and with the other 16-lane rows (lane ^ 16, ^ 32).
+__device__ inline float half_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ inline float half_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ inline float rows_max(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return half_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ inline float rows_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return half_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+__device__ inline int wave_min(int x) {
+  for (int d = 32; d; d >>= 1) x = min(x, __shfl_xor(x, d));
+  return __builtin_amdgcn_readfirstlane(x);
+}
+__device__ inline int wave_max(int x) {
+  for (int d = 32; d; d >>= 1) x = max(x, __shfl_xor(x, d));
+  return __builtin_amdgcn_readfirstlane(x);
+}
+
+__device__ inline SharedItem item_at(const SharedParams& p, int i) {
+  const const_i32* w = (const const_i32*)(p.items + i);
+  return SharedItem{w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7], w[8], {0, 0, 0}};
+}
+
+// The tiles of an item one after another, through its segments.
+struct Cursor {
+  const const_i32* words;
+  int tile;
+  SharedSeg seg;
+  __device__ Cursor(const SharedParams& p, int first) : words((const const_i32*)(p.segs + first)) {
+    read();
+    tile = seg.tile_begin;
+  }
+  __device__ void read() {
+    seg = SharedSeg{words[0], words[1], words[2], words[3], words[4], words[5], words[6], words[7]};
+  }
+  // `n` tiles on; the item has that many.
+  __device__ void advance(int n) {
+    tile += n;
+    while (tile >= seg.tile_end) {
+      const int over = tile - seg.tile_end;
+      words += 8;
+      read();
+      tile = seg.tile_begin + over;
+    }
+  }
+};
+
+// Where the rows of an aligned group of keys (within one page: groups are of 16 keys at most) lie.
+struct Group {
+  const char* base[2];   // key `first`'s row of K, V for this KV head
+  const float* scale[2];
+  int count;             // keys of the group that exist
+  uint32_t stride;       // bytes between rows
+};
+template <int FORMAT, int DIM>
+__device__ inline Group group_at(const SharedParams& p, const SharedSeg& s, int first, int size, int kvh) {
+  Group g;
+  g.count = min(max(s.keys - first, 0), size);
+  if (s.source == kOwnRows) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      g.base[i] = reinterpret_cast<const char*>(p.rows[i] + ((int64_t)s.base + first) * p.row_stride[i] + kvh * DIM);
+      g.scale[i] = nullptr;
+    }
+  } else {
+    constexpr int kRow = FORMAT == QATTN_KV_16BIT ? 2 * DIM : DIM;
+    const int in_page = first & ((1 << p.page_shift) - 1);
+    const int page = ((const const_i32*)p.pages)[s.base + (min(first, s.keys - 1) >> p.page_shift)];
+    const int64_t row = (((int64_t)page * p.kv_heads + kvh) << p.page_shift) + in_page;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      g.base[i] = p.cache[i] + row * kRow;
+      g.scale[i] = p.cache_scale[i] + row;
+    }
+  }
+  return g;
+}
+
+// 16 codes as two 16-byte chunks of 16-bit elements.
+template <bool BF16, int FORMAT>
+__device__ inline void expand(u32x4 codes, float scale, u32x4 (&out)[2]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const u32x2 y = FORMAT == QATTN_KV_E4M3 ? e4m3_elems<BF16>(codes[e], scale) : int8_elems<BF16>(codes[e], scale);
+    out[e >> 1][2 * (e & 1)] = y[0];
+    out[e >> 1][2 * (e & 1) + 1] = y[1];
+  }
+}
+
+// ---- values that a row must not see ----------------------------------------------------------------
+// A masked key's p is 0, but 0 times an infinity or NaN is NaN.  In tiles that some row of the item sees
+// only part of, such elements of V are replaced by 0 on their way into LDS, and where there were any,
+// the rows that do see the key get them added afterwards (p times an infinity is that infinity).
+template <bool BF16>
+__device__ inline bool drop_nonfinite(u32x4& chunk) {
+  constexpr uint32_t kExp = Elem<BF16>::kExponent;
+  bool any = false;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const bool low = (chunk[e] & kExp) == kExp, high = ((chunk[e] >> 16) & kExp) == kExp;
+    any |= low | high;
+    chunk[e] &= (low ? 0xFFFF0000u : 0xFFFFFFFFu) & (high ? 0x0000FFFFu : 0xFFFFFFFFu);
+  }
+  return any;
+}
+// Elements d .. d + 3 of key `key`'s V.
+template <bool BF16, int FORMAT, int DIM>
+__device__ inline f4 value_at(const SharedParams& p, const SharedSeg& s, int key, int kvh, int d) {
+  const Group g = group_at<FORMAT, DIM>(p, s, key, 1, kvh);
+  u32x2 x;
+  if (FORMAT == QATTN_KV_16BIT || s.source == kOwnRows) {
+    x = *reinterpret_cast<const u32x2*>(g.base[1] + 2 * d);
+  } else {
+    const uint32_t codes = *reinterpret_cast<const uint32_t*>(g.base[1] + d);
+    x = FORMAT == QATTN_KV_E4M3 ? e4m3_elems<BF16>(codes, *g.scale[1]) : int8_elems<BF16>(codes, *g.scale[1]);
+  }
+  return f4{widen<BF16, 0>(x[0]), widen<BF16, 1>(x[0]), widen<BF16, 0>(x[1]), widen<BF16, 1>(x[1])};
+}
+__device__ inline float nonfinite(float v, bool seen) { return seen && !(fabsf(v) < INFINITY) ? v : 0.f; }
+
+// Does every row of [row_begin, row_end) with positions in [least, greatest] see every existing key of the
+// `size` keys from `first` on?
+__device__ inline bool all_seen(const SharedParams& p, const SharedSeg& s, int first, int size, int row_begin, int row_end,
+                                int least, int greatest) {
+  const int from = s.position + first, to = s.position + min(s.keys, first + size) - 1;
+  return s.row_begin <= row_begin && s.row_end >= row_end && to <= least &&
+         (p.mask == QATTN_MASK_CAUSAL || to < p.prefix || from > greatest - p.window);
+}
+
+// ---- tall items -----------------------------------------------------------------------------------
+
+template <bool BF16, int FORMAT, int DIM>
+struct Tall {
+  static constexpr int kRow = 2 * DIM;                  // bytes of a row in LDS
+  static constexpr int kTile = kTallKeys * kRow;        // of K or V
+  static constexpr int kLds = 4 * kTile;                // K and V, double buffered
+  // 16-byte chunks of a row in memory, rows of a wavefront's load, loads per tile: of 16-bit rows, codes.
+  static constexpr int kChunks16 = kRow / 16, kRows16 = 64 / kChunks16, kLoads16 = kTallKeys / (4 * kRows16);
+  static constexpr int kChunks8 = DIM / 16, kRows8 = 64 / kChunks8, kLoads8 = kTallKeys / (4 * kRows8);
+  static constexpr bool kCodes = FORMAT != QATTN_KV_16BIT;
+
+  // 16-byte chunk c of row r, swizzled so that 16 rows' reads of one chunk (K) and the transposed reads
+  // of four rows by four chunks (V) cover all 64 banks.
+  __device__ static uint32_t k_at(int r, int c) { return r * kRow + ((c ^ (DIM == 128 ? r & 15 : (r >> 1) & 7)) << 4); }
+  __device__ static uint32_t v_at(int r, int c) { return r * kRow + ((c ^ (DIM == 128 ? (r & 3) << 2 : (r & 2) << 1)) << 4); }
+
+  u32x4 raw[2][kLoads16];
+  float scale[2][kCodes ? kLoads8 : 1];
+
+  // Key tile `tile` into registers.
+  __device__ void load(const SharedParams& p, const SharedSeg& s, int tile, int kvh, int wave, int lane) {
+    if (!kCodes || s.source == kOwnRows) {
+#pragma unroll
+      for (int j = 0; j < kLoads16; ++j) {
+        const Group g = group_at<FORMAT, DIM>(p, s, tile * kTallKeys + (j * 4 + wave) * kRows16, kRows16, kvh);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t stride = s.source == kOwnRows ? (uint32_t)p.row_stride[i] * 2 : kRow;
+          raw[i][j] = load16(buffer(g.base[i], g.count ? (g.count - 1) * stride + kRow : 0),
+                             (lane / kChunks16) * stride + (lane % kChunks16) * 16);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kLoads8; ++j) {
+        const Group g = group_at<FORMAT, DIM>(p, s, tile * kTallKeys + (j * 4 + wave) * kRows8, kRows8, kvh);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          raw[i][j] = load16(buffer(g.base[i], g.count * DIM), lane * 16);
+          scale[i][kCodes ? j : 0] = __uint_as_float(
+              __builtin_amdgcn_raw_buffer_load_b32(buffer(g.scale[i], g.count * 4), (lane / kChunks8) * 4, 0, 0));
+        }
+      }
+    }
+  }
+
+  // The loaded tile into LDS as 16-bit elements.  partly: some row sees only part of it; returns whether
+  // this wavefront's V had infinities or NaN then.
+  __device__ bool store(char* k, char* v, const SharedSeg& s, int wave, int lane, bool partly) {
+    bool any = false;
+    if (!kCodes || s.source == kOwnRows) {
+#pragma unroll
+      for (int j = 0; j < kLoads16; ++j) {
+        const int r = (j * 4 + wave) * kRows16 + lane / kChunks16, c = lane % kChunks16;
+        *reinterpret_cast<u32x4*>(k + k_at(r, c)) = raw[0][j];
+        u32x4 x = raw[1][j];
+        if (partly) any |= drop_nonfinite<BF16>(x);
+        *reinterpret_cast<u32x4*>(v + v_at(r, c)) = x;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kLoads8; ++j) {
+        const int r = (j * 4 + wave) * kRows8 + lane / kChunks8, c = 2 * (lane % kChunks8);
+        u32x4 x[2];
+        expand<BF16, FORMAT>(raw[0][j], scale[0][kCodes ? j : 0], x);
+        *reinterpret_cast<u32x4*>(k + k_at(r, c)) = x[0];
+        *reinterpret_cast<u32x4*>(k + k_at(r, c + 1)) = x[1];
+        expand<BF16, FORMAT>(raw[1][j], scale[1][kCodes ? j : 0], x);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (partly) any |= drop_nonfinite<BF16>(x[h]);
+          *reinterpret_cast<u32x4*>(v + v_at(r, c + h)) = x[h];
+        }
+      }
+    }
+    return partly && __any(any);
+  }
+};
+
+// Offset of accumulator element r (0 .. 31 over the two 32-key blocks) from the tile's first key + 4 hl.
+__device__ constexpr int key_off(int r) { return 32 * (r >> 4) + 8 * ((r & 15) >> 2) + (r & 3); }
+
+template <bool BF16, int FORMAT, int DIM>
+__device__ inline void tall_item(const SharedParams& p, const SharedItem& it, int kvh, char* lds, uint32_t* flags) {
+  typedef Tall<BF16, FORMAT, DIM> T;
+  constexpr int kBlocks = DIM / 32, kSteps = DIM / 16;
+  const int lane = threadIdx.x & 63, lq = lane & 31, hl = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int end_row = it.row0 + it.rows, wave_row = it.row0 + 32 * wave;
+  const int wave_end = min(end_row, wave_row + 32);
+  const int row = wave_row + lq;
+  const bool exists = row < end_row;
+  const int token = exists ? row / p.group : 0;
+  const int head = kvh * p.group + row - token * p.group;
+  const int at = exists ? p.positions[token] : -1;
+  const int least = wave_min(exists ? at : kMaxPosition), greatest = wave_max(at);
+  const bool local = p.mask != QATTN_MASK_CAUSAL;
+
+  // Q (B operand of S^T = K Q^T): this lane's row, dims 16 st + 8 hl .. + 7 at step st.
+  u32x4 q[kSteps];
+  {
+    const uint16_t* src = p.q + (int64_t)token * p.q_stride + head * DIM + 8 * hl;
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st) q[st] = exists ? *reinterpret_cast<const u32x4*>(src + 16 * st) : u32x4{};
+  }
+
+  f16x o[kBlocks];
+#pragma unroll
+  for (int db = 0; db < kBlocks; ++db) o[db] = f16x{};
+  float m = kNone, l = 0.f;
+
+  // LDS read addresses.  K: rows lq, lq + 32.  V^T through the transposing read: in each 16-lane group G
+  // lane a reads 4 elements of key 4 (G >> 1) + (a >> 2) (+ 16 t, + 8) at dims 32 db + 16 (G & 1) + 4 (a & 3)
+  // and receives those keys' elements of dim 32 db + 16 (G & 1) + a.
+  uint32_t v_read[kBlocks];
+  {
+    const int a = lane & 15, G = lane >> 4, r = 4 * (G >> 1) + (a >> 2);
+#pragma unroll
+    for (int db = 0; db < kBlocks; ++db) v_read[db] = T::v_at(r, 4 * db + 2 * (G & 1) + ((a & 3) >> 1)) + ((a & 1) << 3);
+  }
+
+  Cursor ahead(p, it.seg_begin), now = ahead;
+  T tile;
+  const auto partly = [&](const Cursor& c) {
+    return !all_seen(p, c.seg, c.tile * kTallKeys, kTallKeys, it.row0, end_row, it.least, it.greatest);
+  };
+  const auto put = [&](int buf) {
+    const bool part = partly(ahead);
+    const bool any = tile.store(lds + buf * 2 * T::kTile, lds + buf * 2 * T::kTile + T::kTile, ahead.seg, wave, lane, part);
+    if (part && lane == 0) flags[4 * buf + wave] = any;
+  };
+
+  tile.load(p, ahead.seg, ahead.tile, kvh, wave, lane);
+  put(0);
+  if (it.tiles > 1) {
+    ahead.advance(1);
+    tile.load(p, ahead.seg, ahead.tile, kvh, wave, lane);
+  }
+  for (int t = 0; t < it.tiles; ++t) {
+    // The tile is in LDS, and every wavefront is done with the other buffer.
+    __syncthreads();
+    if (t + 1 < it.tiles) {
+      put((t + 1) & 1);
+      if (t + 2 < it.tiles) {
+        ahead.advance(1);
+        tile.load(p, ahead.seg, ahead.tile, kvh, wave, lane);
+      }
+    }
+    const SharedSeg& s = now.seg;
+    const int first = now.tile * kTallKeys, from = s.position + first;
+    if (s.row_begin < wave_end && s.row_end > wave_row && from <= greatest) {
+      const char* k = lds + (t & 1) * 2 * T::kTile;
+      const char* v = k + T::kTile;
+      f16x sc[2] = {};
+#pragma unroll
+      for (int st = 0; st < kSteps; ++st)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          sc[h] = mfma32<BF16>(*reinterpret_cast<const u32x4*>(k + T::k_at(lq + 32 * h, 2 * st + hl)), q[st], sc[h]);
+      const bool mine = row >= s.row_begin && row < s.row_end;
+      const int limit = min(mine ? at : -1, s.position + s.keys - 1);
+      if (first + kTallKeys > s.keys ||
+          !all_seen(p, s, first, kTallKeys, wave_row, wave_end, least, greatest)) {
+        // Offsets from this lane's first key: the last one seen, and where the prefix and the window leave a gap.
+        const int base = from + 4 * hl, last = limit - base;
+        const int gap = local ? p.prefix - base : kMaxPosition, window = (mine ? at : -1) - p.window - base;
+#pragma unroll
+        for (int r = 0; r < 32; ++r) {
+          const int off = key_off(r);
+          const bool hidden = (int)(off > last) | ((int)(off >= gap) & (int)(off <= window));
+          sc[r >> 4][r & 15] = hidden ? kNone : sc[r >> 4][r & 15];
+        }
+      }
+      float top = fmaxf(fmaxf(sc[0][0], sc[0][1]), sc[0][2]);
+#pragma unroll
+      for (int r = 3; r < 31; r += 2) top = fmaxf(fmaxf(top, sc[r >> 4][r & 15]), sc[(r + 1) >> 4][(r + 1) & 15]);
+      top = half_max(fmaxf(top, sc[1][15])) * p.scale_log2;
+      if (__any(top > m + kLazy || (m == kNone && top > kNone))) {
+        const float next = top > m + kLazy || m == kNone ? fmaxf(top, m) : m;
+        const float keep = m == next ? 1.f : __builtin_amdgcn_exp2f(m - next);
+#pragma unroll
+        for (int db = 0; db < kBlocks; ++db) o[db] *= keep;
+        l *= keep;
+        m = next;
+      }
+      const float ref = m == kNone ? 0.f : m;
+      u32x4 pf[4];
+#pragma unroll
+      for (int r = 0; r < 32; r += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[r >> 4][r & 15], p.scale_log2, -ref));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[r >> 4][(r & 15) + 1], p.scale_log2, -ref));
+        l += p0 + p1;
+        pf[r >> 3][(r & 7) >> 1] = narrow2<BF16>(p0, p1);
+      }
+#pragma unroll
+      for (int st = 0; st < 4; ++st)
+#pragma unroll
+        for (int db = 0; db < kBlocks; ++db) {
+          const char* src = v + v_read[db] + st * 16 * T::kRow;
+          const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)src));
+          const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(src + 8 * T::kRow)));
+          o[db] = mfma32<BF16>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pf[st], o[db]);
+        }
+      if (partly(now)) {
+        const uint32_t* f = flags + 4 * (t & 1);
+        if (__builtin_amdgcn_readfirstlane(f[0] | f[1] | f[2] | f[3])) {
+          for (int key = first; key < min(s.keys, first + kTallKeys); ++key) {
+            const int pos = s.position + key;
+            const bool seen = pos <= limit && (!local || pos < p.prefix || pos > (mine ? at : -1) - p.window);
+#pragma unroll
+            for (int db = 0; db < kBlocks; ++db)
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {
+                const f4 x = value_at<BF16, FORMAT, DIM>(p, s, key, kvh, 32 * db + 8 * g + 4 * hl);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[db][4 * g + e] += nonfinite(x[e], seen);
+              }
+          }
+        }
+      }
+    }
+    if (t + 1 < it.tiles) now.advance(1);
+  }
+
+  // O^T: this lane holds dims 32 db + 8 g + 4 hl .. + 3 of its row.
+  l = half_sum(l);
+  if (it.part < 0) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;  // a NaN stays one
+    uint16_t* dst = p.o + (int64_t)token * p.o_stride + head * DIM + 8 * hl;
+#pragma unroll
+    for (int db = 0; db < kBlocks; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; g += 2) {
+        const f16x& x = o[db];
+        const int a = 4 * g, b = 4 * g + 4;
+        const auto r0 = __builtin_amdgcn_permlane32_swap(narrow2<BF16>(x[a] * inv, x[a + 1] * inv),
+                                                         narrow2<BF16>(x[b] * inv, x[b + 1] * inv), false, false);
+        const auto r1 = __builtin_amdgcn_permlane32_swap(narrow2<BF16>(x[a + 2] * inv, x[a + 3] * inv),
+                                                         narrow2<BF16>(x[b + 2] * inv, x[b + 3] * inv), false, false);
+        if (exists) *reinterpret_cast<u32x4*>(dst + 32 * db + 8 * g) = u32x4{r0[0], r1[0], r0[1], r1[1]};
+      }
+  } else if (exists) {
+    const int64_t part = ((int64_t)it.part + row - it.row0) * p.kv_heads + kvh;
+    float* dst = p.part_o + part * DIM + 4 * hl;
+#pragma unroll
+    for (int db = 0; db < kBlocks; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f4*>(dst + 32 * db + 8 * g) = f4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
+    if (hl == 0) p.part_ml[part] = float2{m, l};
+  }
+}
+
+// ---- flat items -----------------------------------------------------------------------------------
+
+template <bool BF16, int FORMAT, int DIM>
+struct Flat {
+  static constexpr int kRow = 2 * DIM;
+  static constexpr int kLds = 4 * kFlatKeys * kRow;  // each wavefront's V tile, later its 16 rows of O in f32
+  static constexpr int kSteps = DIM / 32;            // K: two 16-byte loads of codes, four of 16-bit elements per 128 dims
+  static constexpr int kChunks16 = kRow / 16, kRows16 = 64 / kChunks16, kLoads16 = 16 / kRows16;
+  static constexpr int kChunks8 = DIM / 16, kRows8 = 64 / kChunks8, kLoads8 = 16 / kRows8;
+  static constexpr bool kCodes = FORMAT != QATTN_KV_16BIT;
+  static_assert(kLds >= 4 * kFlatRows * DIM * 4, "O of four wavefronts");
+
+  // Eight rows by two chunks cover all 64 banks.
+  __device__ static uint32_t v_at(int r, int c) { return r * kRow + ((c ^ (DIM == 128 ? (r & 7) << 1 : (r & 6))) << 4); }
+
+  // Per 16-key group: K's operand chunks (key lane & 15, dims 64 h + 16 (lane >> 4) + 8 half at step 2 h +
+  // half) and V's rows as they lie.
+  u32x4 k[2][kSteps], v[2][kLoads16];
+  float ks[2], vs[2][kCodes ? kLoads8 : 1];
+
+  __device__ void load(const SharedParams& p, const SharedSeg& s, int tile, int kvh, int lane) {
+    const int key = lane & 15, c = lane >> 4;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const Group g = group_at<FORMAT, DIM>(p, s, tile * kFlatKeys + 16 * b, 16, kvh);
+      if (!kCodes || s.source == kOwnRows) {
+        uint32_t stride[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) stride[i] = s.source == kOwnRows ? (uint32_t)p.row_stride[i] * 2 : kRow;
+        const auto bk = buffer(g.base[0], g.count ? (g.count - 1) * stride[0] + kRow : 0);
+        const auto bv = buffer(g.base[1], g.count ? (g.count - 1) * stride[1] + kRow : 0);
+#pragma unroll
+        for (int st = 0; st < kSteps; ++st) k[b][st] = load16(bk, key * stride[0] + 128 * (st >> 1) + 32 * c + 16 * (st & 1));
+#pragma unroll
+        for (int j = 0; j < kLoads16; ++j)
+          v[b][j] = load16(bv, (j * kRows16 + lane / kChunks16) * stride[1] + (lane % kChunks16) * 16);
+      } else {
+        const auto bk = buffer(g.base[0], g.count * DIM), bv = buffer(g.base[1], g.count * DIM);
+        const auto sk = buffer(g.scale[0], g.count * 4), sv = buffer(g.scale[1], g.count * 4);
+#pragma unroll
+        for (int h = 0; h < DIM / 64; ++h) k[b][h] = load16(bk, key * DIM + 64 * h + 16 * c);
+        ks[b] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(sk, key * 4, 0, 0));
+#pragma unroll
+        for (int j = 0; j < kLoads8; ++j) {
+          v[b][j] = load16(bv, j * 1024 + lane * 16);
+          vs[b][kCodes ? j : 0] =
+              __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(sv, (j * kRows8 + lane / kChunks8) * 4, 0, 0));
+        }
+      }
+    }
+  }
+  // The K operands of group b at every step.
+  __device__ void operands(int b, const SharedSeg& s, u32x4 (&out)[kSteps]) const {
+    if (!kCodes || s.source == kOwnRows) {
+#pragma unroll
+      for (int st = 0; st < kSteps; ++st) out[st] = k[b][st];
+    } else {
+#pragma unroll
+      for (int h = 0; h < DIM / 64; ++h) {
+        u32x4 x[2];
+        expand<BF16, FORMAT>(k[b][h], ks[b], x);
+        out[2 * h] = x[0];
+        out[2 * h + 1] = x[1];
+      }
+    }
+  }
+  __device__ bool store(char* lds, const SharedSeg& s, int lane, bool partly) const {
+    bool any = false;
+    const auto put = [&](int r, int c, u32x4 x) {
+      if (partly) any |= drop_nonfinite<BF16>(x);
+      *reinterpret_cast<u32x4*>(lds + v_at(r, c)) = x;
+    };
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      if (!kCodes || s.source == kOwnRows) {
+#pragma unroll
+        for (int j = 0; j < kLoads16; ++j) put(16 * b + j * kRows16 + lane / kChunks16, lane % kChunks16, v[b][j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kLoads8; ++j) {
+          const int r = 16 * b + j * kRows8 + lane / kChunks8, c = 2 * (lane % kChunks8);
+          u32x4 x[2];
+          expand<BF16, FORMAT>(v[b][j], vs[b][kCodes ? j : 0], x);
+          put(r, c, x[0]);
+          put(r, c + 1, x[1]);
+        }
+      }
+    }
+    return partly && __any(any);
+  }
+};
+
+template <bool BF16, int FORMAT, int DIM>
+__device__ inline void flat_item(const SharedParams& p, const SharedItem& it, int kvh, char* lds_all, float2* stats) {
+  typedef Flat<BF16, FORMAT, DIM> T;
+  constexpr int kBlocks = DIM / 16;
+  const int lane = threadIdx.x & 63, n = lane & 15, c = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  char* lds = lds_all + wave * (T::kLds / 4);
+  const int end_row = it.row0 + it.rows, row = it.row0 + n;
+  const bool exists = row < end_row;
+  const int token = exists ? row / p.group : 0;
+  const int at = exists ? p.positions[token] : -1;
+  const bool local = p.mask != QATTN_MASK_CAUSAL;
+
+  // Q (B operand): this lane's row, the dims of K's chunks.
+  u32x4 q[T::kSteps];
+  {
+    const int head = kvh * p.group + row - token * p.group;
+    const uint16_t* src = p.q + (int64_t)token * p.q_stride + head * DIM + 16 * c;
+#pragma unroll
+    for (int st = 0; st < T::kSteps; ++st)
+      q[st] = exists ? *reinterpret_cast<const u32x4*>(src + 64 * (st >> 1) + 8 * (st & 1)) : u32x4{};
+  }
+  f4 o[kBlocks];
+#pragma unroll
+  for (int db = 0; db < kBlocks; ++db) o[db] = f4{};
+  float m = kNone, l = 0.f;
+  // V^T: the 16 lanes of group c read keys 4 c .. 4 c + 3 (and 16 more) by the 16 dims of a block.
+  const int vr = 4 * c + (n >> 2);
+
+  if (wave < it.tiles) {
+    Cursor now(p, it.seg_begin);
+    now.advance(wave);
+    T tile;
+    tile.load(p, now.seg, now.tile, kvh, lane);
+    for (int t = wave; t < it.tiles; t += 4) {
+      const SharedSeg s = now.seg;
+      const int first = now.tile * kFlatKeys, from = s.position + first;
+      f4 sc[2] = {};
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        u32x4 a[T::kSteps];
+        tile.operands(b, s, a);
+#pragma unroll
+        for (int st = 0; st < T::kSteps; ++st) sc[b] = mfma16<BF16>(a[st], q[st], sc[b]);
+      }
+      const bool part = !all_seen(p, s, first, kFlatKeys, it.row0, end_row, it.least, it.greatest);
+      const bool poisoned = tile.store(lds, s, lane, part);
+      if (t + 4 < it.tiles) {
+        now.advance(4);
+        tile.load(p, now.seg, now.tile, kvh, lane);
+      }
+      const bool mine = row >= s.row_begin && row < s.row_end;
+      const int limit = min(mine ? at : -1, s.position + s.keys - 1);
+      const int window_from = (mine ? at : -1) - p.window;
+      if (part || first + kFlatKeys > s.keys) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const int pos = from + 16 * (r >> 2) + 4 * c + (r & 3);
+          const bool hidden = (int)(pos > limit) | ((int)local & (int)(pos >= p.prefix) & (int)(pos <= window_from));
+          sc[r >> 2][r & 3] = hidden ? kNone : sc[r >> 2][r & 3];
+        }
+      }
+      float top = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
+                        fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+      top = rows_max(top) * p.scale_log2;
+      if (__any(top > m + kLazy || (m == kNone && top > kNone))) {
+        const float next = top > m + kLazy || m == kNone ? fmaxf(top, m) : m;
+        const float keep = m == next ? 1.f : __builtin_amdgcn_exp2f(m - next);
+#pragma unroll
+        for (int db = 0; db < kBlocks; ++db) o[db] *= keep;
+        l *= keep;
+        m = next;
+      }
+      const float ref = m == kNone ? 0.f : m;
+      u32x4 pf;
+#pragma unroll
+      for (int r = 0; r < 8; r += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[r >> 2][r & 3], p.scale_log2, -ref));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[r >> 2][(r & 3) + 1], p.scale_log2, -ref));
+        l += p0 + p1;
+        pf[r >> 1] = narrow2<BF16>(p0, p1);
+      }
+#pragma unroll
+      for (int db = 0; db < kBlocks; ++db) {
+        const char* src = lds + T::v_at(vr, 2 * db + ((n & 3) >> 1)) + ((n & 1) << 3);
+        const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)src));
+        const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(src + 16 * T::kRow)));
+        o[db] = mfma16<BF16>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pf, o[db]);
+      }
+      if (poisoned) {
+        for (int key = first; key < min(s.keys, first + kFlatKeys); ++key) {
+          const int pos = s.position + key;
+          const bool seen = pos <= limit && (!local || pos < p.prefix || pos > window_from);
+#pragma unroll
+          for (int db = 0; db < kBlocks; ++db) {
+            const f4 x = value_at<BF16, FORMAT, DIM>(p, s, key, kvh, 16 * db + 4 * c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[db][e] += nonfinite(x[e], seen);
+          }
+        }
+      }
+    }
+  }
+
+  // The four wavefronts' sums: lane (n, c) holds dims 16 db + 4 c .. + 3 of row n.
+  l = rows_sum(l);
+  float* own = reinterpret_cast<float*>(lds);
+#pragma unroll
+  for (int db = 0; db < kBlocks; ++db) *reinterpret_cast<f4*>(own + n * DIM + 16 * db + 4 * c) = o[db];
+  if (c == 0) stats[16 * wave + n] = float2{m, l};
+  __syncthreads();
+  const int r = threadIdx.x >> 4, d = (threadIdx.x & 15) * (DIM / 16);
+  if (it.row0 + r >= end_row) return;
+  float2 st[4];
+  float top = kNone, sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    st[w] = stats[16 * w + r];
+    top = fmaxf(top, st[w].x);
+  }
+  float x[DIM / 16] = {};
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float f = __builtin_amdgcn_exp2f(st[w].x - (top == kNone ? 0.f : top));
+    sum += f * st[w].y;
+    const float* src = reinterpret_cast<const float*>(lds_all + w * (T::kLds / 4)) + r * DIM + d;
+#pragma unroll
+    for (int e = 0; e < DIM / 16; ++e) x[e] += f * src[e];
+  }
+  const int out_row = it.row0 + r, out_token = out_row / p.group;
+  if (it.part < 0) {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(p.o + (int64_t)out_token * p.o_stride +
+                                                (kvh * p.group + out_row - out_token * p.group) * DIM + d);
+#pragma unroll
+    for (int e = 0; e < DIM / 16; e += 2) dst[e / 2] = narrow2<BF16>(x[e] * inv, x[e + 1] * inv);
+  } else {
+    const int64_t part = ((int64_t)it.part + r) * p.kv_heads + kvh;
+#pragma unroll
+    for (int e = 0; e < DIM / 16; ++e) p.part_o[part * DIM + d + e] = x[e];
+    if (d == 0) p.part_ml[part] = float2{top, sum};
+  }
+}
+
+template <bool BF16, int FORMAT, int DIM>
+__global__ __launch_bounds__(kSharedThreads, 2) void shared_attn_kernel(SharedParams p) {
+  __shared__ __attribute__((aligned(1024))) char lds[Tall<BF16, FORMAT, DIM>::kLds];
+  __shared__ __attribute__((aligned(16))) float2 stats[4 * kFlatRows];
+  const int kvh = (int)(blockIdx.x % (uint32_t)p.kv_heads);
+  const SharedItem it = item_at(p, (int)(blockIdx.x / (uint32_t)p.kv_heads));
+  if (it.kind == kTall)
+    tall_item<BF16, FORMAT, DIM>(p, it, kvh, lds, reinterpret_cast<uint32_t*>(stats));
+  else
+    flat_item<BF16, FORMAT, DIM>(p, it, kvh, lds, stats);
+}
+
+// One wavefront per merged row and KV head: sum over its partial rows of 2^(m_i - max m) times the row's
+// sums; a partial row that saw no key has m = -inf and weighs 0.  Without partial rows: zeros.
+template <bool BF16, int DIM>
+__global__ __launch_bounds__(kSharedThreads) void shared_merge_kernel(SharedParams p) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int64_t index = (int64_t)blockIdx.x * 4 + wave;
+  if (index >= (int64_t)p.n_merges * p.kv_heads) return;
+  const int kvh = (int)(index % p.kv_heads);
+  const SharedMerge e = p.merges[index / p.kv_heads];
+  const int count = e.group[0].count + e.group[1].count;
+  const auto part_at = [&](int i) {
+    const int g = i >= e.group[0].count;
+    const SharedMerge::Group& of = e.group[g];
+    return ((int64_t)of.first + (int64_t)(g ? i - e.group[0].count : i) * of.step) * p.kv_heads + kvh;
+  };
+  float top = kNone;
+  for (int i = lane; i < count; i += 64) top = fmaxf(top, p.part_ml[part_at(i)].x);
+  for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+  const float ref = top == kNone ? 0.f : top;
+  constexpr int kDims = DIM / 64;
+  float sum = 0.f, x[kDims] = {};
+  for (int i = 0; i < count; ++i) {
+    const int64_t part = part_at(i);
+    const float2 ml = p.part_ml[part];
+    const float f = __builtin_amdgcn_exp2f(ml.x - ref);
+    sum += f * ml.y;
+#pragma unroll
+    for (int k = 0; k < kDims; ++k) x[k] += f * p.part_o[part * DIM + kDims * lane + k];
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int token = e.row / p.group;
+  uint16_t* dst = p.o + (int64_t)token * p.o_stride + (kvh * p.group + e.row - token * p.group) * DIM + kDims * lane;
+  if constexpr (kDims == 2)
+    *reinterpret_cast<uint32_t*>(dst) = narrow2<BF16>(x[0] * inv, x[1] * inv);
+  else
+    *dst = (uint16_t)narrow2<BF16>(x[0] * inv, 0.f);
+}
+
+template <bool BF16, int FORMAT, int DIM>
+void launch_attn(const SharedParams& p, hipStream_t stream) {
+  hipLaunchKernelGGL((shared_attn_kernel<BF16, FORMAT, DIM>), dim3((unsigned)p.n_items * p.kv_heads), dim3(kSharedThreads),
+                     0, stream, p);
+}
+template <bool BF16, int DIM>
+hipError_t launch(const SharedParams& p, int format, hipStream_t stream) {
+  if (p.n_items > 0) {
+    switch (format) {
+      case QATTN_KV_16BIT: launch_attn<BF16, QATTN_KV_16BIT, DIM>(p, stream); break;
+      case QATTN_KV_E4M3: launch_attn<BF16, QATTN_KV_E4M3, DIM>(p, stream); break;
+      default: launch_attn<BF16, QATTN_KV_INT8, DIM>(p, stream);
+    }
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  if (p.n_merges > 0) {
+    const int64_t waves = (int64_t)p.n_merges * p.kv_heads;
+    hipLaunchKernelGGL((shared_merge_kernel<BF16, DIM>), dim3((unsigned)((waves + 3) / 4)), dim3(kSharedThreads), 0, stream, p);
+    return hipGetLastError();
+  }
+  return hipSuccess;
+}
+
+}  // namespace
+
+hipError_t launch_shared_attn(const SharedParams& p, int dtype, int format, int head_dim, hipStream_t stream) {
+  if (dtype == QATTN_DTYPE_BF16)
+    return head_dim == 64 ? launch<true, 64>(p, format, stream) : launch<true, 128>(p, format, stream);
+  return head_dim == 64 ? launch<false, 64>(p, format, stream) : launch<false, 128>(p, format, stream);
+}
+
+}  // namespace qattn

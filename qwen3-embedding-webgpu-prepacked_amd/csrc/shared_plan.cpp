@@ -1,0 +1,345 @@
+// shared_plan.cpp -- host planner of the attention behind one shared prefix.
+//
+// Row blocks.  The rows of all sequences are stacked and cut into blocks of 128, so that short sequences
+// fill a block together and a tile of prefix keys is read once for all its rows.  A block also visits
+// the own keys of its sequences, one segment each, in which only their rows see anything.  Sequences
+// of up to 16 rows (single tokens) would waste most of a block on their own keys: those go to items of
+// 16 rows whose four wavefronts take a tile of keys each, and so do the prefix's if the launch has no
+// more rows than that.
+//
+// Cuts.  Items are cut along their keys where that shortens the launch: the planner compares the time at
+// which the last of the GPU's slots ends, for a range of chunk sizes, by a cost model in units of one
+// 64-key tile of a full block.
+#include <algorithm>
+#include <cmath>
+#include <queue>
+
+#include "shared_attn.h"
+
+namespace qattn {
+
+namespace {
+
+// Costs in units of a block's 64-key tile, from measured launches: an item's start and end, a round of four
+// 32-key tiles of a flat item, and the second launch.
+constexpr double kTallItem = 1.5, kFlatItem = 1.0, kFlatRound = 0.4, kPartial = 0.5, kMergeLaunch = 2.0;
+constexpr int kMostSimulated = 16384;
+
+struct Sequence {
+  int32_t first, queries, keys;  // first query; own keys
+  int32_t base, source;
+};
+
+struct Draft {
+  SharedItem item;
+  std::vector<SharedSeg> segs;
+  bool merged = false;  // its rows have partial results elsewhere too
+  int chunks = 1, first_part = 0;
+  double cost(int tiles) const {
+    return item.kind == kTall ? kTallItem + tiles : kFlatItem + kFlatRound * ((tiles + 3) / 4);
+  }
+};
+
+class Planner {
+ public:
+  Planner(const qattn_shared_desc& d, int compute_units, SharedPlan* plan)
+      : d_(d), plan_(plan), group_(d.q_heads / d.cache.kv_heads),
+        slots_(std::max(1, 2 * compute_units / d.cache.kv_heads)) {}
+
+  void run() {
+    read();
+    draft();
+    cut();
+    emit();
+  }
+
+ private:
+  bool local() const { return d_.mask == QATTN_MASK_PREFIX_LOCAL; }
+  int64_t window() const { return std::min<int64_t>(d_.window, kMaxPosition); }
+
+  void read() {
+    int32_t first_row = 0;
+    size_t page = 0;
+    const int32_t page_size = std::max(1, d_.cache.page_size);
+    const auto pages_of = [&](int32_t keys) { return (size_t)((keys + (int64_t)page_size - 1) / page_size); };
+    if (d_.prefix_len) plan_->pages.assign(d_.prefix_pages, d_.prefix_pages + pages_of(d_.prefix_len));
+    plan_->positions.resize(d_.cu_q[d_.nseq]);
+    qattn_shared_info& info = plan_->info;
+    info.tokens = d_.cu_q[d_.nseq];
+    info.keys = d_.prefix_len;
+    for (int32_t i = 0; i < d_.nseq; ++i) {
+      Sequence s{d_.cu_q[i], d_.cu_q[i + 1] - d_.cu_q[i], d_.own_len[i], 0, kOwnRows};
+      if (d_.own_pages) {
+        s.source = kOwnPages;
+        s.base = (int32_t)plan_->pages.size();
+        const size_t n = pages_of(s.keys);
+        plan_->pages.insert(plan_->pages.end(), d_.own_pages + page, d_.own_pages + page + n);
+        page += n;
+      } else {
+        s.base = first_row;
+        first_row += s.keys;
+      }
+      info.keys += s.keys;
+      for (int32_t j = 0; j < s.queries; ++j) {
+        const int64_t at = (int64_t)d_.prefix_len + s.keys - s.queries + j;
+        plan_->positions[s.first + j] = (int32_t)std::max<int64_t>(at, -1);
+        if (at < 0) continue;
+        int64_t seen = at + 1;
+        if (local()) {
+          const int64_t always = std::min<int64_t>(seen, d_.prefix);
+          seen = always + std::max<int64_t>(0, at - std::max(at - window() + 1, always) + 1);
+        }
+        info.pairs += seen;
+      }
+      if (s.queries) sequences_.push_back(s);
+    }
+    info.flops = 4ll * d_.cache.head_dim * d_.q_heads * info.pairs;
+  }
+
+  // The tiles of `keys` keys from `position` on that queries at least .. greatest can see, as segments.
+  void add_segs(std::vector<SharedSeg>* out, SharedSeg s, int tile, int32_t least, int32_t greatest) const {
+    const int64_t end = std::min<int64_t>(s.keys, (int64_t)greatest - s.position + 1);
+    if (end <= 0) return;
+    const auto tiles = [&](int64_t n) { return (int32_t)((n + tile - 1) / tile); };
+    const auto add = [&](int32_t a, int32_t b) {
+      if (a >= b) return;
+      s.tile_begin = a;
+      s.tile_end = b;
+      out->push_back(s);
+    };
+    if (!local()) return add(0, tiles(end));
+    const int64_t always = std::clamp<int64_t>((int64_t)d_.prefix - s.position, 0, end);
+    const int64_t start = std::clamp<int64_t>((int64_t)least - window() + 1 - s.position, 0, end);
+    if (start / tile <= tiles(always)) return add(0, start < end ? tiles(end) : tiles(always));
+    add(0, tiles(always));
+    add((int32_t)(start / tile), start < end ? tiles(end) : (int32_t)(start / tile));
+  }
+
+  // A block's segments: the prefix, and the own keys of its sequences that are not left to flat items.
+  Draft block(int64_t row0, int64_t rows, size_t first_sequence, int kind, bool with_own) const {
+    const int tile = kind == kTall ? kTallKeys : kFlatKeys;
+    Draft b;
+    b.item = SharedItem{(int32_t)row0, (int32_t)rows, 0, 0, -1, 0, kind, 0, 0, {0, 0, 0}};
+    const int32_t t0 = (int32_t)(row0 / group_), t1 = (int32_t)((row0 + rows - 1) / group_);
+    b.item.least = *std::min_element(&plan_->positions[t0], &plan_->positions[t1] + 1);
+    b.item.greatest = *std::max_element(&plan_->positions[t0], &plan_->positions[t1] + 1);
+    if (d_.prefix_len)
+      add_segs(&b.segs, SharedSeg{kPrefixPages, 0, d_.prefix_len, 0, 0, 0, (int32_t)row0, (int32_t)(row0 + rows)}, tile,
+               b.item.least, b.item.greatest);
+    for (size_t i = first_sequence; with_own && i < sequences_.size() && sequences_[i].first <= t1; ++i) {
+      const Sequence& s = sequences_[i];
+      if (flat_own(s)) continue;
+      const int64_t begin = std::max<int64_t>(row0, (int64_t)s.first * group_);
+      const int64_t end = std::min<int64_t>(row0 + rows, ((int64_t)s.first + s.queries) * group_);
+      if (begin >= end || !s.keys) continue;
+      add_segs(&b.segs, SharedSeg{s.source, s.base, s.keys, d_.prefix_len, 0, 0, (int32_t)begin, (int32_t)end}, tile,
+               plan_->positions[begin / group_], plan_->positions[(end - 1) / group_]);
+    }
+    for (const SharedSeg& s : b.segs) b.item.tiles += s.tile_end - s.tile_begin;
+    return b;
+  }
+
+  bool flat_own(const Sequence& s) const { return !flat_all_ && (int64_t)s.queries * group_ <= kFlatRows; }
+
+  // Blocks of stacked rows: `aligned` starts a block at every sequence of a block's rows or more.
+  std::vector<Draft> blocks(bool aligned) const {
+    std::vector<Draft> out;
+    int64_t begin = -1, end = 0;  // pending rows
+    size_t first = 0;             // a sequence at or before them
+    const auto flush = [&](int64_t upto) {
+      while (begin >= 0 && begin < upto) {
+        while (first < sequences_.size() && ((int64_t)sequences_[first].first + sequences_[first].queries) * group_ <= begin) ++first;
+        const int64_t rows = std::min<int64_t>(kTallRows, upto - begin);
+        out.push_back(block(begin, rows, first, kTall, true));
+        begin += rows;
+      }
+      begin = -1;
+    };
+    for (const Sequence& s : sequences_) {
+      if (!d_.prefix_len && flat_own(s)) {
+        flush(end);
+        continue;
+      }
+      const int64_t row = (int64_t)s.first * group_, rows = (int64_t)s.queries * group_;
+      if (begin < 0 || row != end || (aligned && rows >= kTallRows)) {
+        flush(end);
+        begin = row;
+      }
+      end = row + rows;
+    }
+    flush(end);
+    return out;
+  }
+
+  void draft() {
+    if (sequences_.empty()) return;
+    const int64_t rows = (int64_t)plan_->positions.size() * group_;
+    if (rows <= kFlatRows && sequences_.size() == 1) {
+      // One short sequence: prefix and own keys in one item.
+      flat_all_ = true;
+      drafts_.push_back(block((int64_t)sequences_[0].first * group_, rows, 0, kFlat, true));
+    } else if (rows <= kFlatRows) {
+      if (d_.prefix_len) drafts_.push_back(block(0, rows, 0, kFlat, false));
+    } else {
+      const auto tiles = [](const std::vector<Draft>& v) {
+        int64_t n = 0;
+        for (const Draft& b : v) n += b.item.tiles + 2;
+        return n;
+      };
+      std::vector<Draft> a = blocks(true), b = blocks(false);
+      drafts_ = tiles(a) <= tiles(b) ? std::move(a) : std::move(b);
+    }
+    if (!flat_all_)
+      for (const Sequence& s : sequences_)
+        if (flat_own(s) && s.keys) {
+          Draft f;
+          const int64_t row0 = (int64_t)s.first * group_, n = (int64_t)s.queries * group_;
+          f.item = SharedItem{(int32_t)row0, (int32_t)n, 0, 0, -1, 0, kFlat, plan_->positions[s.first],
+                              plan_->positions[s.first + s.queries - 1], {0, 0, 0}};
+          add_segs(&f.segs, SharedSeg{s.source, s.base, s.keys, d_.prefix_len, 0, 0, (int32_t)row0, (int32_t)(row0 + n)},
+                   kFlatKeys, f.item.least, f.item.greatest);
+          for (const SharedSeg& g : f.segs) f.item.tiles += g.tile_end - g.tile_begin;
+          drafts_.push_back(std::move(f));
+        }
+    drafts_.erase(std::remove_if(drafts_.begin(), drafts_.end(), [](const Draft& b) { return b.item.tiles == 0; }),
+                  drafts_.end());
+    // Rows of two items are merged, and with them all rows of those items.
+    std::vector<int32_t> cover(rows, 0);
+    for (const Draft& b : drafts_)
+      for (int32_t r = 0; r < b.item.rows; ++r) ++cover[b.item.row0 + r];
+    for (Draft& b : drafts_)
+      for (int32_t r = 0; r < b.item.rows; ++r) b.merged |= cover[b.item.row0 + r] > 1;
+  }
+
+  static int chunks_for(const Draft& b, double target) {
+    // Flat chunks are whole rounds of the four wavefronts.
+    const double unit = b.item.kind == kTall ? 1.0 : kFlatRound;
+    const int n = b.item.kind == kTall ? b.item.tiles : (b.item.tiles + 3) / 4;
+    const double fixed = b.item.kind == kTall ? kTallItem : kFlatItem;
+    const int fit = std::max(1, (int)std::floor((target - fixed) / unit));
+    return (n + fit - 1) / fit;
+  }
+
+  // The time at which the last slot ends, longest item first.
+  double span(double target, bool* split) const {
+    std::vector<double> costs;
+    double partial_rows = 0;
+    for (const Draft& b : drafts_) {
+      const int c = chunks_for(b, target);
+      const int units = b.item.kind == kTall ? b.item.tiles : (b.item.tiles + 3) / 4;
+      const bool part = c > 1 || b.merged;
+      if (part) partial_rows += (double)c * b.item.rows;
+      *split |= part;
+      for (int i = 0; i < c; ++i) {
+        const int n = units * (i + 1) / c - units * i / c;
+        costs.push_back((part ? kPartial : 0) + (b.item.kind == kTall ? kTallItem + n : kFlatItem + kFlatRound * n));
+      }
+      if ((int)costs.size() > kMostSimulated) return 1e30;
+    }
+    std::sort(costs.begin(), costs.end(), std::greater<double>());
+    std::priority_queue<double, std::vector<double>, std::greater<double>> ends;
+    double last = 0;
+    for (double c : costs) {
+      double start = 0;
+      if ((int)ends.size() == slots_) {
+        start = ends.top();
+        ends.pop();
+      }
+      ends.push(start + c);
+      last = std::max(last, start + c);
+    }
+    // Partial rows are written and read once each: about 4 TB/s, a unit being about 1 us.
+    return last + (*split ? kMergeLaunch + partial_rows * d_.cache.kv_heads * d_.cache.head_dim * 8 / 4e6 : 0);
+  }
+
+  void cut() {
+    double longest = 0, best_span = 1e30, best = 0;
+    for (const Draft& b : drafts_) longest = std::max(longest, b.cost(b.item.tiles));
+    for (double target = longest; target > 1.9; target *= target > longest / 2 ? 0.85 : 0.7) {
+      bool split = false;
+      const double s = span(target, &split);
+      if (target == longest || s < best_span * 0.97) {
+        best_span = s;
+        best = target;
+      }
+    }
+    if (best_span >= 1e30) best = longest;
+    for (Draft& b : drafts_) b.chunks = best > 0 ? chunks_for(b, best) : 1;
+  }
+
+  void emit() {
+    std::vector<std::pair<double, SharedItem>> items;
+    for (Draft& b : drafts_) {
+      const int rows = b.item.rows;
+      const bool part = b.chunks > 1 || b.merged;
+      if (part) {
+        b.first_part = (int32_t)plan_->partial_rows;
+        plan_->partial_rows += (int64_t)b.chunks * rows;
+      }
+      const int round = b.item.kind == kTall ? 1 : 4;
+      const int units = (b.item.tiles + round - 1) / round;
+      for (int c = 0; c < b.chunks; ++c) {
+        int begin = std::min(b.item.tiles, (int)((int64_t)units * c / b.chunks) * round);
+        int end = std::min(b.item.tiles, (int)((int64_t)units * (c + 1) / b.chunks) * round);
+        SharedItem it = b.item;
+        it.seg_begin = (int32_t)plan_->segs.size();
+        it.tiles = end - begin;
+        it.part = part ? b.first_part + c * rows : -1;
+        for (SharedSeg s : b.segs) {
+          const int n = s.tile_end - s.tile_begin;
+          if (begin < n && end > 0) {
+            s.tile_end = s.tile_begin + std::min(n, end);
+            s.tile_begin += std::max(0, begin);
+            plan_->segs.push_back(s);
+          }
+          begin -= n;
+          end -= n;
+        }
+        it.seg_end = (int32_t)plan_->segs.size();
+        items.emplace_back(b.cost(it.tiles), it);
+      }
+    }
+    std::stable_sort(items.begin(), items.end(), [](const auto& a, const auto& b) { return a.first > b.first; });
+    for (const auto& i : items) plan_->items.push_back(i.second);
+    merge_rows();
+    plan_->info.items = (int32_t)plan_->items.size();
+    plan_->info.merged_rows = (int32_t)plan_->merges.size();
+    plan_->info.partial_rows = plan_->partial_rows;
+  }
+
+  // Rows with partial results, and rows that no item computes (merged from nothing: zeros).
+  void merge_rows() {
+    const int64_t rows = (int64_t)plan_->positions.size() * group_;
+    std::vector<SharedMerge> all(rows, SharedMerge{});
+    std::vector<uint8_t> direct(rows, 0);
+    for (const Draft& b : drafts_)
+      for (int32_t r = 0; r < b.item.rows; ++r) {
+        const int64_t row = (int64_t)b.item.row0 + r;
+        if (b.chunks == 1 && !b.merged) {
+          direct[row] = 1;
+          continue;
+        }
+        SharedMerge& m = all[row];
+        m.group[m.group[0].count ? 1 : 0] = {b.first_part + r, b.chunks, b.item.rows};
+      }
+    for (int64_t row = 0; row < rows; ++row)
+      if (!direct[row]) {
+        all[row].row = (int32_t)row;
+        plan_->merges.push_back(all[row]);
+      }
+  }
+
+  const qattn_shared_desc& d_;
+  SharedPlan* plan_;
+  const int group_;
+  const int slots_;
+  bool flat_all_ = false;
+  std::vector<Sequence> sequences_;
+  std::vector<Draft> drafts_;
+};
+
+}  // namespace
+
+void plan_shared(const qattn_shared_desc& d, int compute_units, SharedPlan* plan) { Planner(d, compute_units, plan).run(); }
+
+}  // namespace qattn

@@ -122,6 +122,34 @@ class KvCache(ctypes.Structure):
     ]
 
 
+class SharedDesc(ctypes.Structure):
+    """qattn_shared_desc."""
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("o", ctypes.c_void_p),
+        ("q_row_stride", ctypes.c_int64), ("o_row_stride", ctypes.c_int64),
+        ("q_heads", ctypes.c_int32),
+        ("cache", KvCache),
+        ("prefix_pages", ctypes.c_void_p), ("prefix_len", ctypes.c_int32),
+        ("cu_q", ctypes.c_void_p), ("nseq", ctypes.c_int32),
+        ("own_len", ctypes.c_void_p), ("own_pages", ctypes.c_void_p),
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("k_row_stride", ctypes.c_int64), ("v_row_stride", ctypes.c_int64),
+        ("mask", ctypes.c_int32), ("prefix", ctypes.c_int32), ("window", ctypes.c_int32),
+        ("scale", ctypes.c_double),
+    ]
+
+
+class SharedInfo(ctypes.Structure):
+    """qattn_shared_info."""
+    _fields_ = [
+        ("tokens", ctypes.c_int64), ("keys", ctypes.c_int64), ("pairs", ctypes.c_int64), ("flops", ctypes.c_int64),
+        ("items", ctypes.c_int32), ("merged_rows", ctypes.c_int32), ("partial_rows", ctypes.c_int64),
+    ]
+
+    def as_dict(self):
+        return {name: getattr(self, name) for name, _ in self._fields_}
+
+
 def build():
     """Compile libqattn.so for gfx950 with the package Makefile."""
     subprocess.run(["make", "-s", "-C", PKG_DIR, "lib"], check=True)
@@ -193,6 +221,14 @@ def lib():
         "qattn_rope": (ctypes.c_int, [vp, ctypes.POINTER(RopeDesc), vp]),
         "qattn_kv_write": (ctypes.c_int, [vp, ctypes.POINTER(KvCache), vp, i64, vp, i64, vp, i64, vp]),
         "qattn_kv_read": (ctypes.c_int, [vp, ctypes.POINTER(KvCache), vp, i64, vp, i64, vp, i64, vp]),
+        "qattn_shared_run_create": (ctypes.c_int, [vp, ctypes.POINTER(SharedDesc), pvp]),
+        "qattn_shared_run_encode": (ctypes.c_int, [vp, vp]),
+        "qattn_shared_run_update": (ctypes.c_int, [vp, vp, i32, vp, i32, vp, vp]),
+        "qattn_shared_run_rebind": (ctypes.c_int, [vp, vp, vp, ctypes.POINTER(KvCache), vp, vp]),
+        "qattn_shared_run_destroy": (None, [vp]),
+        "qattn_shared_run_get_info": (ctypes.c_int, [vp, ctypes.POINTER(SharedInfo)]),
+        "qattn_shared_plan_describe": (ctypes.c_int, [ctypes.POINTER(SharedDesc), vp, i64, ctypes.POINTER(i64),
+                                                      ctypes.POINTER(SharedInfo)]),
         "qattn_model_create": (ctypes.c_int, [vp, ctypes.POINTER(ModelDesc), pvp]),
         "qattn_model_destroy": (None, [vp]),
         "qattn_model_plan_create": (ctypes.c_int, [vp, i32, i32, pvp]),
@@ -254,6 +290,58 @@ def make_kv_cache(k, v, pages, page_size, kv_heads=HKV, head_dim=HD, dtype=F16, 
     """Build a qattn_kv_cache over device addresses: codes [pages, kv_heads, page_size, head_dim],
     scales f32 [pages, kv_heads, page_size]."""
     return KvCache(k, v, k_scale, v_scale, pages, page_size, kv_heads, head_dim, dtype, format)
+
+
+def _i32(a):
+    return None if a is None else np.ascontiguousarray(a, dtype=np.int32)
+
+
+def _page_counts(prefix_len, own_len, page_size):
+    return -(-int(prefix_len) // page_size), int(np.sum(-(-np.asarray(own_len, np.int64) // page_size)))
+
+
+def _shared_arrays(prefix_pages, prefix_len, cu_q, own_len, own_pages, page_size):
+    """The host arrays of a shared run as int32, their lengths checked."""
+    prefix_pages, cu, own, own_pages = _i32(prefix_pages), _i32(cu_q), _i32(own_len), _i32(own_pages)
+    if len(own) != len(cu) - 1:
+        raise ValueError(f"own_len has {len(own)} entries for {len(cu) - 1} sequences")
+    if page_size > 0 and prefix_len >= 0 and (own >= 0).all():
+        need = _page_counts(prefix_len, own, page_size)
+        for name, pages, n in (("prefix_pages", prefix_pages, need[0]), ("own_pages", own_pages, need[1])):
+            if pages is not None and len(pages) < n:
+                raise ValueError(f"{name} has {len(pages)} entries, {n} are needed")
+    return prefix_pages, cu, own, own_pages
+
+
+def make_shared_desc(q, o, cache, cu_q, own_len, q_heads=HQ, prefix_pages=None, prefix_len=0, own_pages=None, k=None,
+                     v=None, q_row_stride=None, o_row_stride=None, k_row_stride=None, v_row_stride=None,
+                     mask=MASK_CAUSAL, prefix=176, window=432, scale=0.0):
+    """Build a qattn_shared_desc.  q/o/k/v are device addresses; cache a qattn_kv_cache
+    (make_kv_cache); the page lists, cu_q and own_len host arrays, which the desc keeps."""
+    width, kv_width = q_heads * cache.head_dim, cache.kv_heads * cache.head_dim
+    arrays = _shared_arrays(prefix_pages, prefix_len, cu_q, own_len, own_pages, cache.page_size)
+    at = [None if a is None else a.ctypes.data for a in arrays]
+    d = SharedDesc(q, o, width if q_row_stride is None else q_row_stride, width if o_row_stride is None else o_row_stride,
+                   q_heads, cache, at[0], prefix_len, at[1], len(arrays[1]) - 1, at[2], at[3], k, v,
+                   kv_width if k_row_stride is None else k_row_stride,
+                   kv_width if v_row_stride is None else v_row_stride, mask, prefix, window, scale)
+    d._arrays = arrays
+    return d
+
+
+def shared_plan(desc):
+    """Host-only planner of a shared run: (plan as a dict of arrays, SharedInfo); the layout is
+    qattn_shared_plan_describe's."""
+    n, info = ctypes.c_int64(0), SharedInfo()
+    _check(lib().qattn_shared_plan_describe(ctypes.byref(desc), None, 0, ctypes.byref(n), ctypes.byref(info)))
+    words = np.zeros(n.value, np.int32)
+    _check(lib().qattn_shared_plan_describe(ctypes.byref(desc), _np_ptr(words), n.value, ctypes.byref(n), None))
+    counts, at, out = words[:5], 8, {}
+    for name, count, width in zip(("items", "segments", "merges", "positions", "pages"), counts, (12, 8, 8, 1, 1)):
+        part = words[at:at + count * width]
+        out[name] = part if width == 1 else part.reshape(count, width)
+        at += count * width
+    return out, info
 
 
 def plan_slots(desc, max_slots=0):
@@ -374,6 +462,41 @@ class Run:
     def destroy(self):
         if self.handle:
             lib().qattn_run_destroy(self.handle)
+            self.handle = None
+
+
+class SharedRun:
+    """A planned launch of the attention behind one shared prefix (qattn_shared_run)."""
+
+    def __init__(self, ctx, desc):
+        self.ctx = ctx
+        self.page_size = desc.cache.page_size
+        h = ctypes.c_void_p()
+        _check(lib().qattn_shared_run_create(ctx.handle, ctypes.byref(desc), ctypes.byref(h)), ctx.handle)
+        self.handle = h.value
+
+    def encode(self, stream=None):
+        _check(lib().qattn_shared_run_encode(self.handle, stream), self.ctx.handle)
+
+    def update(self, cu_q, own_len, prefix_pages=None, prefix_len=0, own_pages=None):
+        """New lengths and pages for the same tensors (qattn_shared_run_update)."""
+        arrays = _shared_arrays(prefix_pages, prefix_len, cu_q, own_len, own_pages, self.page_size)
+        at = [None if a is None else a.ctypes.data for a in arrays]
+        _check(lib().qattn_shared_run_update(self.handle, at[0], prefix_len, at[1], len(arrays[1]) - 1, at[2], at[3]),
+               self.ctx.handle)
+
+    def rebind(self, q, o, cache, k=None, v=None):
+        """Other tensors and another cache of the same geometry (qattn_shared_run_rebind)."""
+        _check(lib().qattn_shared_run_rebind(self.handle, q, o, ctypes.byref(cache), k, v), self.ctx.handle)
+
+    def info(self):
+        i = SharedInfo()
+        _check(lib().qattn_shared_run_get_info(self.handle, ctypes.byref(i)), self.ctx.handle)
+        return i
+
+    def destroy(self):
+        if self.handle:
+            lib().qattn_shared_run_destroy(self.handle)
             self.handle = None
 
 
@@ -555,6 +678,9 @@ class Context:
         _check(lib().qattn_kv_read(self.handle, ctypes.byref(cache), slots_ptr, tokens, k_ptr,
                                    width if k_row_stride is None else k_row_stride, v_ptr,
                                    width if v_row_stride is None else v_row_stride, stream), self.handle)
+
+    def shared_run(self, desc):
+        return SharedRun(self, desc)
 
     def model(self, token_embd, output_norm, layers, eps=1e-6, rope_theta=1e6, mask=MASK_PREFIX_LOCAL,
               prefix=176, window=432, flags=0):
