@@ -29,9 +29,11 @@ struct SharedItem {
   int32_t pad[3];
 };
 // Tiles tile_begin .. tile_end - 1 (of the item kind's size) of `keys` keys, seen by rows row_begin ..
-// row_end - 1 only.  base: the source's first page number (an index into the plan's list) or row.
+// row_end - 1 only.  base: the source's first page number (an index into the plan's list) or row.  whole:
+// every row of the item sees every key of these tiles.
 struct SharedSeg {
-  int32_t source, base, keys, position, tile_begin, tile_end, row_begin, row_end;
+  int32_t source, whole, base, keys, position, tile_begin, tile_end, row_begin, row_end;
+  int32_t pad[3];
 };
 // A row whose results are merged: `count` partial rows from `first` on, `step` apart, in two groups.
 struct SharedMerge {
@@ -41,7 +43,7 @@ struct SharedMerge {
   } group[2];
   int32_t pad;
 };
-static_assert(sizeof(SharedItem) == 48 && sizeof(SharedSeg) == 32 && sizeof(SharedMerge) == 32, "plan words");
+static_assert(sizeof(SharedItem) == 48 && sizeof(SharedSeg) == 48 && sizeof(SharedMerge) == 32, "plan words");
 
 struct SharedPlan {
   std::vector<SharedItem> items;

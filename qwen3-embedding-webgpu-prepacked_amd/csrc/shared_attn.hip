@@ -76,10 +76,6 @@ __device__ inline float rows_sum(float x) {
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return half_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
-__device__ inline int wave_min(int x) {
-  for (int d = 32; d; d >>= 1) x = min(x, __shfl_xor(x, d));
-  return __builtin_amdgcn_readfirstlane(x);
-}
 __device__ inline int wave_max(int x) {
   for (int d = 32; d; d >>= 1) x = max(x, __shfl_xor(x, d));
   return __builtin_amdgcn_readfirstlane(x);
@@ -100,14 +96,14 @@ struct Cursor {
     tile = seg.tile_begin;
   }
   __device__ void read() {
-    seg = SharedSeg{words[0], words[1], words[2], words[3], words[4], words[5], words[6], words[7]};
+    seg = SharedSeg{words[0], words[1], words[2], words[3], words[4], words[5], words[6], words[7], words[8], {0, 0, 0}};
   }
   // `n` tiles on; the item has that many.
   __device__ void advance(int n) {
     tile += n;
     while (tile >= seg.tile_end) {
       const int over = tile - seg.tile_end;
-      words += 8;
+      words += sizeof(SharedSeg) / 4;
       read();
       tile = seg.tile_begin + over;
     }
@@ -158,8 +154,9 @@ __device__ inline void expand(u32x4 codes, float scale, u32x4 (&out)[2]) {
 
 // ---- values that a row must not see ----------------------------------------------------------------
 // A masked key's p is 0, but 0 times an infinity or NaN is NaN.  In tiles that some row of the item sees
-// only part of, such elements of V are replaced by 0 on their way into LDS, and where there were any,
-// the rows that do see the key get them added afterwards (p times an infinity is that infinity).
+// only part of, such elements of V are replaced by 0 on their way into LDS, and if there were any, the
+// rows that do see the key get them added at the end (p times an infinity is that infinity, whatever the
+// reference).
 template <bool BF16>
 __device__ inline bool drop_nonfinite(u32x4& chunk) {
   constexpr uint32_t kExp = Elem<BF16>::kExponent;
@@ -186,14 +183,26 @@ __device__ inline f4 value_at(const SharedParams& p, const SharedSeg& s, int key
   return f4{widen<BF16, 0>(x[0]), widen<BF16, 1>(x[0]), widen<BF16, 0>(x[1]), widen<BF16, 1>(x[1])};
 }
 __device__ inline float nonfinite(float v, bool seen) { return seen && !(fabsf(v) < INFINITY) ? v : 0.f; }
-
-// Does every row of [row_begin, row_end) with positions in [least, greatest] see every existing key of the
-// `size` keys from `first` on?
-__device__ inline bool all_seen(const SharedParams& p, const SharedSeg& s, int first, int size, int row_begin, int row_end,
-                                int least, int greatest) {
-  const int from = s.position + first, to = s.position + min(s.keys, first + size) - 1;
-  return s.row_begin <= row_begin && s.row_end >= row_end && to <= least &&
-         (p.mask == QATTN_MASK_CAUSAL || to < p.prefix || from > greatest - p.window);
+// Calls add(value, seen) for every key of the item's tiles first, first + step, ... (of `size` keys) that not
+// all rows see: value(d) is elements d .. d + 3 of its V, seen whether row `row` at position `at` sees it.
+template <bool BF16, int FORMAT, int DIM, class Add>
+__device__ inline void each_nonfinite(const SharedParams& p, const SharedItem& it, int kvh, int row, int at, int size, int first,
+                                      int step, Add add) {
+  Cursor c(p, it.seg_begin);
+  c.advance(first);
+  for (int t = first;;) {
+    const SharedSeg s = c.seg;
+    if (!s.whole) {
+      const int mine = row >= s.row_begin && row < s.row_end ? at : -1;
+      for (int key = c.tile * size; key < min(s.keys, (c.tile + 1) * size); ++key) {
+        const int pos = s.position + key;
+        add([&](int d) { return value_at<BF16, FORMAT, DIM>(p, s, key, kvh, d); },
+            pos <= mine && (p.mask == QATTN_MASK_CAUSAL || pos < p.prefix || pos > mine - p.window));
+      }
+    }
+    if ((t += step) >= it.tiles) return;
+    c.advance(step);
+  }
 }
 
 // ---- tall items -----------------------------------------------------------------------------------
@@ -213,49 +222,64 @@ struct Tall {
   __device__ static uint32_t k_at(int r, int c) { return r * kRow + ((c ^ (DIM == 128 ? r & 15 : (r >> 1) & 7)) << 4); }
   __device__ static uint32_t v_at(int r, int c) { return r * kRow + ((c ^ (DIM == 128 ? (r & 3) << 2 : (r & 2) << 1)) << 4); }
 
+  // Where this lane's rows of a tile lie.  Keys past the last stand on it: a row that does not see the last
+  // key either makes the tile a partly seen one, whose infinities and NaN are taken out.
+  struct Spot {
+    int source, base;
+    int key[kLoads16], page[kLoads16];
+  };
+  __device__ static Spot spot(const SharedParams& p, const SharedSeg& s, int tile, int wave, int lane) {
+    Spot at;
+    at.source = s.source;
+    at.base = s.base;
+    const int last = s.keys - 1, first = tile * kTallKeys;
+    if (s.source == kOwnRows) {
+#pragma unroll
+      for (int j = 0; j < kLoads16; ++j) at.key[j] = min(first + (j * 4 + wave) * kRows16 + lane / kChunks16, last);
+    } else {
+#pragma unroll
+      for (int j = 0; j < (kCodes ? kLoads8 : kLoads16); ++j) {
+        at.key[j] = min(first + (kCodes ? (j * 4 + wave) * kRows8 + lane / kChunks8 : (j * 4 + wave) * kRows16 + lane / kChunks16), last);
+        at.page[j] = p.pages[s.base + (at.key[j] >> p.page_shift)];
+      }
+    }
+    return at;
+  }
+
   u32x4 raw[2][kLoads16];
   float scale[2][kCodes ? kLoads8 : 1];
 
-  // Key tile `tile` into registers.
-  __device__ void load(const SharedParams& p, const SharedSeg& s, int tile, int kvh, int wave, int lane) {
-    if (!kCodes || s.source == kOwnRows) {
+  // K (I = 0) or V (1) of a tile into registers.
+  template <int I>
+  __device__ void load(const SharedParams& p, const Spot& at, int kvh, int lane) {
+    if (at.source == kOwnRows) {
+      const char* rows = reinterpret_cast<const char*>(p.rows[I] + (int64_t)at.base * p.row_stride[I] + kvh * DIM);
+      const uint32_t stride = (uint32_t)p.row_stride[I] * 2;
 #pragma unroll
-      for (int j = 0; j < kLoads16; ++j) {
-        const Group g = group_at<FORMAT, DIM>(p, s, tile * kTallKeys + (j * 4 + wave) * kRows16, kRows16, kvh);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t stride = s.source == kOwnRows ? (uint32_t)p.row_stride[i] * 2 : kRow;
-          raw[i][j] = load16(buffer(g.base[i], g.count ? (g.count - 1) * stride + kRow : 0),
-                             (lane / kChunks16) * stride + (lane % kChunks16) * 16);
-        }
-      }
+      for (int j = 0; j < kLoads16; ++j)
+        raw[I][j] = *reinterpret_cast<const u32x4*>(rows + (uint64_t)(uint32_t)at.key[j] * stride + (lane % kChunks16) * 16);
     } else {
+      constexpr int kBytes = kCodes ? DIM : kRow, kChunks = kBytes / 16;
+      const uint32_t page_rows = (uint32_t)p.kv_heads << p.page_shift, head = (uint32_t)kvh << p.page_shift;
+      const uint32_t mask = (1u << p.page_shift) - 1;
 #pragma unroll
-      for (int j = 0; j < kLoads8; ++j) {
-        const Group g = group_at<FORMAT, DIM>(p, s, tile * kTallKeys + (j * 4 + wave) * kRows8, kRows8, kvh);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          raw[i][j] = load16(buffer(g.base[i], g.count * DIM), lane * 16);
-          scale[i][kCodes ? j : 0] = __uint_as_float(
-              __builtin_amdgcn_raw_buffer_load_b32(buffer(g.scale[i], g.count * 4), (lane / kChunks8) * 4, 0, 0));
-        }
+      for (int j = 0; j < (kCodes ? kLoads8 : kLoads16); ++j) {
+        const uint32_t row = head + (at.key[j] & mask);
+        const uint64_t byte = (uint64_t)(uint32_t)at.page[j] * (page_rows * kBytes) + (row * kBytes + (lane % kChunks) * 16);
+        raw[I][j] = *reinterpret_cast<const u32x4*>(p.cache[I] + byte);
+        if constexpr (kCodes)
+          scale[I][j] = *reinterpret_cast<const float*>(reinterpret_cast<const char*>(p.cache_scale[I]) +
+                                                        ((uint64_t)(uint32_t)at.page[j] * (page_rows * 4) + row * 4));
       }
     }
   }
 
-  // The loaded tile into LDS as 16-bit elements.  partly: some row sees only part of it; returns whether
-  // this wavefront's V had infinities or NaN then.
-  __device__ bool store(char* k, char* v, const SharedSeg& s, int wave, int lane, bool partly) {
-    bool any = false;
-    if (!kCodes || s.source == kOwnRows) {
+  // The loaded K into LDS as 16-bit elements.
+  __device__ void store_k(char* k, bool rows, int wave, int lane) {
+    if (!kCodes || rows) {
 #pragma unroll
-      for (int j = 0; j < kLoads16; ++j) {
-        const int r = (j * 4 + wave) * kRows16 + lane / kChunks16, c = lane % kChunks16;
-        *reinterpret_cast<u32x4*>(k + k_at(r, c)) = raw[0][j];
-        u32x4 x = raw[1][j];
-        if (partly) any |= drop_nonfinite<BF16>(x);
-        *reinterpret_cast<u32x4*>(v + v_at(r, c)) = x;
-      }
+      for (int j = 0; j < kLoads16; ++j)
+        *reinterpret_cast<u32x4*>(k + k_at((j * 4 + wave) * kRows16 + lane / kChunks16, lane % kChunks16)) = raw[0][j];
     } else {
 #pragma unroll
       for (int j = 0; j < kLoads8; ++j) {
@@ -264,12 +288,28 @@ struct Tall {
         expand<BF16, FORMAT>(raw[0][j], scale[0][kCodes ? j : 0], x);
         *reinterpret_cast<u32x4*>(k + k_at(r, c)) = x[0];
         *reinterpret_cast<u32x4*>(k + k_at(r, c + 1)) = x[1];
-        expand<BF16, FORMAT>(raw[1][j], scale[1][kCodes ? j : 0], x);
+      }
+    }
+  }
+  // V likewise.  partly: some row sees only part of the tile; returns whether this wavefront's part had
+  // infinities or NaN then.
+  __device__ bool store_v(char* v, bool rows, int wave, int lane, bool partly) {
+    bool any = false;
+    const auto put = [&](int r, int c, u32x4 x) {
+      if (partly) any |= drop_nonfinite<BF16>(x);
+      *reinterpret_cast<u32x4*>(v + v_at(r, c)) = x;
+    };
+    if (!kCodes || rows) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (partly) any |= drop_nonfinite<BF16>(x[h]);
-          *reinterpret_cast<u32x4*>(v + v_at(r, c + h)) = x[h];
-        }
+      for (int j = 0; j < kLoads16; ++j) put((j * 4 + wave) * kRows16 + lane / kChunks16, lane % kChunks16, raw[1][j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kLoads8; ++j) {
+        const int r = (j * 4 + wave) * kRows8 + lane / kChunks8, c = 2 * (lane % kChunks8);
+        u32x4 x[2];
+        expand<BF16, FORMAT>(raw[1][j], scale[1][kCodes ? j : 0], x);
+        put(r, c, x[0]);
+        put(r, c + 1, x[1]);
       }
     }
     return partly && __any(any);
@@ -280,7 +320,7 @@ struct Tall {
 __device__ constexpr int key_off(int r) { return 32 * (r >> 4) + 8 * ((r & 15) >> 2) + (r & 3); }
 
 template <bool BF16, int FORMAT, int DIM>
-__device__ inline void tall_item(const SharedParams& p, const SharedItem& it, int kvh, char* lds, uint32_t* flags) {
+__device__ inline void tall_item(const SharedParams& p, const SharedItem& it, int kvh, char* lds, uint32_t* dropped) {
   typedef Tall<BF16, FORMAT, DIM> T;
   constexpr int kBlocks = DIM / 32, kSteps = DIM / 16;
   const int lane = threadIdx.x & 63, lq = lane & 31, hl = lane >> 5;
@@ -292,16 +332,51 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
   const int token = exists ? row / p.group : 0;
   const int head = kvh * p.group + row - token * p.group;
   const int at = exists ? p.positions[token] : -1;
-  const int least = wave_min(exists ? at : kMaxPosition), greatest = wave_max(at);
   const bool local = p.mask != QATTN_MASK_CAUSAL;
+  const auto k_buf = [&](int t) { return lds + (t & 1) * T::kTile; };
+  const auto v_buf = [&](int t) { return lds + (2 + (t & 1)) * T::kTile; };
 
+  // What the scores of a tile need to know of it.
+  struct Info {
+    int whole, from, last, row_begin, row_end;  // from: position of its first key; last: of its segment's last
+  };
+  // Tile t is in LDS while tile t + 1 is in registers, asked for an iteration ago.
+  Cursor ahead(p, it.seg_begin);
+  T tile;
+  typename T::Spot spot = T::spot(p, ahead.seg, ahead.tile, wave, lane);
+  int asked = 0;
+  bool rows = false;  // the tile in registers: 16-bit rows
+  Info now{}, next{};
+  bool found = false;  // infinities or NaN were dropped from V
+  if (threadIdx.x == 0) *dropped = 0;
+  const auto ask = [&]() {
+    tile.template load<0>(p, spot, kvh, lane);
+    tile.template load<1>(p, spot, kvh, lane);
+    rows = spot.source == kOwnRows;
+    const SharedSeg& s = ahead.seg;
+    next = Info{s.whole, s.position + ahead.tile * kTallKeys, s.position + s.keys - 1, s.row_begin, s.row_end};
+    if (++asked < it.tiles) {
+      ahead.advance(1);
+      spot = T::spot(p, ahead.seg, ahead.tile, wave, lane);
+    }
+  };
+  const auto keep = [&](int t) {
+    tile.store_k(k_buf(t), rows, wave, lane);
+    found |= tile.store_v(v_buf(t), rows, wave, lane, !next.whole);
+  };
+
+  ask();
   // Q (B operand of S^T = K Q^T): this lane's row, dims 16 st + 8 hl .. + 7 at step st.
   u32x4 q[kSteps];
   {
     const uint16_t* src = p.q + (int64_t)token * p.q_stride + head * DIM + 8 * hl;
 #pragma unroll
     for (int st = 0; st < kSteps; ++st) q[st] = exists ? *reinterpret_cast<const u32x4*>(src + 16 * st) : u32x4{};
+    // Here, once: a use inside the loop would wait for its tile's loads too.
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st) asm volatile("" : "+v"(q[st]));
   }
+  const int greatest = wave_max(at);
 
   f16x o[kBlocks];
 #pragma unroll
@@ -317,52 +392,33 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
 #pragma unroll
     for (int db = 0; db < kBlocks; ++db) v_read[db] = T::v_at(r, 4 * db + 2 * (G & 1) + ((a & 3) >> 1)) + ((a & 1) << 3);
   }
-
-  Cursor ahead(p, it.seg_begin), now = ahead;
-  T tile;
-  const auto partly = [&](const Cursor& c) {
-    return !all_seen(p, c.seg, c.tile * kTallKeys, kTallKeys, it.row0, end_row, it.least, it.greatest);
-  };
-  const auto put = [&](int buf) {
-    const bool part = partly(ahead);
-    const bool any = tile.store(lds + buf * 2 * T::kTile, lds + buf * 2 * T::kTile + T::kTile, ahead.seg, wave, lane, part);
-    if (part && lane == 0) flags[4 * buf + wave] = any;
-  };
-
-  tile.load(p, ahead.seg, ahead.tile, kvh, wave, lane);
-  put(0);
-  if (it.tiles > 1) {
-    ahead.advance(1);
-    tile.load(p, ahead.seg, ahead.tile, kvh, wave, lane);
-  }
+  keep(0);
+  now = next;
+  if (it.tiles > 1) ask();
   for (int t = 0; t < it.tiles; ++t) {
-    // The tile is in LDS, and every wavefront is done with the other buffer.
+    // Tile t is in LDS, and every wavefront is done with the other buffers.
     __syncthreads();
+    const Info cur = now;
     if (t + 1 < it.tiles) {
-      put((t + 1) & 1);
-      if (t + 2 < it.tiles) {
-        ahead.advance(1);
-        tile.load(p, ahead.seg, ahead.tile, kvh, wave, lane);
-      }
+      keep(t + 1);
+      now = next;
+      if (t + 2 < it.tiles) ask();
     }
-    const SharedSeg& s = now.seg;
-    const int first = now.tile * kTallKeys, from = s.position + first;
-    if (s.row_begin < wave_end && s.row_end > wave_row && from <= greatest) {
-      const char* k = lds + (t & 1) * 2 * T::kTile;
-      const char* v = k + T::kTile;
+    // Does some row of this wavefront see some key of the tile?
+    if (cur.whole || (cur.row_begin < wave_end && cur.row_end > wave_row && cur.from <= greatest)) {
+      const char* k = k_buf(t);
+      const char* v = v_buf(t);
       f16x sc[2] = {};
 #pragma unroll
       for (int st = 0; st < kSteps; ++st)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
           sc[h] = mfma32<BF16>(*reinterpret_cast<const u32x4*>(k + T::k_at(lq + 32 * h, 2 * st + hl)), q[st], sc[h]);
-      const bool mine = row >= s.row_begin && row < s.row_end;
-      const int limit = min(mine ? at : -1, s.position + s.keys - 1);
-      if (first + kTallKeys > s.keys ||
-          !all_seen(p, s, first, kTallKeys, wave_row, wave_end, least, greatest)) {
+      const int mine = row >= cur.row_begin && row < cur.row_end ? at : -1;
+      if (!cur.whole) {
         // Offsets from this lane's first key: the last one seen, and where the prefix and the window leave a gap.
-        const int base = from + 4 * hl, last = limit - base;
-        const int gap = local ? p.prefix - base : kMaxPosition, window = (mine ? at : -1) - p.window - base;
+        const int base = cur.from + 4 * hl, last = min(mine, cur.last) - base;
+        const int gap = local ? p.prefix - base : kMaxPosition, window = mine - p.window - base;
 #pragma unroll
         for (int r = 0; r < 32; ++r) {
           const int off = key_off(r);
@@ -375,51 +431,51 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
       for (int r = 3; r < 31; r += 2) top = fmaxf(fmaxf(top, sc[r >> 4][r & 15]), sc[(r + 1) >> 4][(r + 1) & 15]);
       top = half_max(fmaxf(top, sc[1][15])) * p.scale_log2;
       if (__any(top > m + kLazy || (m == kNone && top > kNone))) {
-        const float next = top > m + kLazy || m == kNone ? fmaxf(top, m) : m;
-        const float keep = m == next ? 1.f : __builtin_amdgcn_exp2f(m - next);
+        const float moved = top > m + kLazy || m == kNone ? fmaxf(top, m) : m;
+        const float shrink = m == moved ? 1.f : __builtin_amdgcn_exp2f(m - moved);
 #pragma unroll
-        for (int db = 0; db < kBlocks; ++db) o[db] *= keep;
-        l *= keep;
-        m = next;
+        for (int db = 0; db < kBlocks; ++db) o[db] *= shrink;
+        l *= shrink;
+        m = moved;
       }
       const float ref = m == kNone ? 0.f : m;
       u32x4 pf[4];
+      float l1 = 0.f;
 #pragma unroll
       for (int r = 0; r < 32; r += 2) {
         const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[r >> 4][r & 15], p.scale_log2, -ref));
         const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[r >> 4][(r & 15) + 1], p.scale_log2, -ref));
-        l += p0 + p1;
+        l += p0;
+        l1 += p1;
         pf[r >> 3][(r & 7) >> 1] = narrow2<BF16>(p0, p1);
       }
+      l += l1;
+      {
 #pragma unroll
-      for (int st = 0; st < 4; ++st)
+        for (int st = 0; st < 4; ++st)
 #pragma unroll
-        for (int db = 0; db < kBlocks; ++db) {
-          const char* src = v + v_read[db] + st * 16 * T::kRow;
-          const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)src));
-          const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(src + 8 * T::kRow)));
-          o[db] = mfma32<BF16>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pf[st], o[db]);
-        }
-      if (partly(now)) {
-        const uint32_t* f = flags + 4 * (t & 1);
-        if (__builtin_amdgcn_readfirstlane(f[0] | f[1] | f[2] | f[3])) {
-          for (int key = first; key < min(s.keys, first + kTallKeys); ++key) {
-            const int pos = s.position + key;
-            const bool seen = pos <= limit && (!local || pos < p.prefix || pos > (mine ? at : -1) - p.window);
-#pragma unroll
-            for (int db = 0; db < kBlocks; ++db)
-#pragma unroll
-              for (int g = 0; g < 4; ++g) {
-                const f4 x = value_at<BF16, FORMAT, DIM>(p, s, key, kvh, 32 * db + 8 * g + 4 * hl);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[db][4 * g + e] += nonfinite(x[e], seen);
-              }
+          for (int db = 0; db < kBlocks; ++db) {
+            const char* src = v + v_read[db] + st * 16 * T::kRow;
+            const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)src));
+            const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(src + 8 * T::kRow)));
+            o[db] = mfma32<BF16>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pf[st], o[db]);
           }
-        }
       }
     }
-    if (t + 1 < it.tiles) now.advance(1);
   }
+  if (found && lane == 0) *dropped = 1;
+  __syncthreads();
+  if (*dropped)
+    each_nonfinite<BF16, FORMAT, DIM>(p, it, kvh, row, at, kTallKeys, 0, 1, [&](auto value, bool seen) {
+#pragma unroll
+      for (int db = 0; db < kBlocks; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f4 x = value(32 * db + 8 * g + 4 * hl);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[db][4 * g + e] += nonfinite(x[e], seen);
+        }
+    });
 
   // O^T: this lane holds dims 32 db + 8 g + 4 hl .. + 3 of its row.
   l = half_sum(l);
@@ -572,6 +628,7 @@ __device__ inline void flat_item(const SharedParams& p, const SharedItem& it, in
   const int vr = 4 * c + (n >> 2);
 
   if (wave < it.tiles) {
+    bool found = false;  // infinities or NaN were dropped from V
     Cursor now(p, it.seg_begin);
     now.advance(wave);
     T tile;
@@ -587,8 +644,8 @@ __device__ inline void flat_item(const SharedParams& p, const SharedItem& it, in
 #pragma unroll
         for (int st = 0; st < T::kSteps; ++st) sc[b] = mfma16<BF16>(a[st], q[st], sc[b]);
       }
-      const bool part = !all_seen(p, s, first, kFlatKeys, it.row0, end_row, it.least, it.greatest);
-      const bool poisoned = tile.store(lds, s, lane, part);
+      const bool part = !s.whole;
+      found |= tile.store(lds, s, lane, part);
       if (t + 4 < it.tiles) {
         now.advance(4);
         tile.load(p, now.seg, now.tile, kvh, lane);
@@ -596,7 +653,7 @@ __device__ inline void flat_item(const SharedParams& p, const SharedItem& it, in
       const bool mine = row >= s.row_begin && row < s.row_end;
       const int limit = min(mine ? at : -1, s.position + s.keys - 1);
       const int window_from = (mine ? at : -1) - p.window;
-      if (part || first + kFlatKeys > s.keys) {
+      if (part) {
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
           const int pos = from + 16 * (r >> 2) + 4 * c + (r & 3);
@@ -631,19 +688,16 @@ __device__ inline void flat_item(const SharedParams& p, const SharedItem& it, in
         const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(src + 16 * T::kRow)));
         o[db] = mfma16<BF16>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pf, o[db]);
       }
-      if (poisoned) {
-        for (int key = first; key < min(s.keys, first + kFlatKeys); ++key) {
-          const int pos = s.position + key;
-          const bool seen = pos <= limit && (!local || pos < p.prefix || pos > window_from);
-#pragma unroll
-          for (int db = 0; db < kBlocks; ++db) {
-            const f4 x = value_at<BF16, FORMAT, DIM>(p, s, key, kvh, 16 * db + 4 * c);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[db][e] += nonfinite(x[e], seen);
-          }
-        }
-      }
     }
+    if (found)
+      each_nonfinite<BF16, FORMAT, DIM>(p, it, kvh, row, at, kFlatKeys, wave, 4, [&](auto value, bool seen) {
+#pragma unroll
+        for (int db = 0; db < kBlocks; ++db) {
+          const f4 x = value(16 * db + 4 * c);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[db][e] += nonfinite(x[e], seen);
+        }
+      });
   }
 
   // The four wavefronts' sums: lane (n, c) holds dims 16 db + 4 c .. + 3 of row n.
@@ -713,19 +767,39 @@ __global__ __launch_bounds__(kSharedThreads) void shared_merge_kernel(SharedPara
     const SharedMerge::Group& of = e.group[g];
     return ((int64_t)of.first + (int64_t)(g ? i - e.group[0].count : i) * of.step) * p.kv_heads + kvh;
   };
-  float top = kNone;
-  for (int i = lane; i < count; i += 64) top = fmaxf(top, p.part_ml[part_at(i)].x);
-  for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-  const float ref = top == kNone ? 0.f : top;
+  // Up to 64 partial rows at a time, one weight to a lane; their rows' loads go out eight at a time.
   constexpr int kDims = DIM / 64;
-  float sum = 0.f, x[kDims] = {};
-  for (int i = 0; i < count; ++i) {
-    const int64_t part = part_at(i);
-    const float2 ml = p.part_ml[part];
-    const float f = __builtin_amdgcn_exp2f(ml.x - ref);
-    sum += f * ml.y;
+  float top = kNone, sum = 0.f, x[kDims] = {};
+  for (int i0 = 0; i0 < count; i0 += 64) {
+    const int n = min(64, count - i0);
+    const float2 ml = lane < n ? p.part_ml[part_at(i0 + lane)] : float2{kNone, 0.f};
+    float most = ml.x;
+    for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
+    most = fmaxf(most, top);
+    const float ref = most == kNone ? 0.f : most;
+    const float rescale = __builtin_amdgcn_exp2f(top - ref), weight = __builtin_amdgcn_exp2f(ml.x - ref);
+    float part_sum = weight * ml.y;
+    for (int d = 32; d; d >>= 1) part_sum += __shfl_xor(part_sum, d);
+    sum = (i0 ? sum * rescale : 0.f) + part_sum;
 #pragma unroll
-    for (int k = 0; k < kDims; ++k) x[k] += f * p.part_o[part * DIM + kDims * lane + k];
+    for (int k = 0; k < kDims; ++k) x[k] *= i0 ? rescale : 0.f;
+    top = most;
+    for (int j0 = 0; j0 < n; j0 += 8) {
+      float y[8][kDims];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float* src = p.part_o + part_at(i0 + min(j0 + j, n - 1)) * DIM + kDims * lane;
+#pragma unroll
+        for (int k = 0; k < kDims; ++k) y[j][k] = src[k];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j0 + j < n) {
+          const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), j0 + j));
+#pragma unroll
+          for (int k = 0; k < kDims; ++k) x[k] += f * y[j][k];
+        }
+    }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int token = e.row / p.group;

@@ -124,7 +124,7 @@ class Planner {
     b.item.least = *std::min_element(&plan_->positions[t0], &plan_->positions[t1] + 1);
     b.item.greatest = *std::max_element(&plan_->positions[t0], &plan_->positions[t1] + 1);
     if (d_.prefix_len)
-      add_segs(&b.segs, SharedSeg{kPrefixPages, 0, d_.prefix_len, 0, 0, 0, (int32_t)row0, (int32_t)(row0 + rows)}, tile,
+      add_segs(&b.segs, SharedSeg{kPrefixPages, 0, 0, d_.prefix_len, 0, 0, 0, (int32_t)row0, (int32_t)(row0 + rows)}, tile,
                b.item.least, b.item.greatest);
     for (size_t i = first_sequence; with_own && i < sequences_.size() && sequences_[i].first <= t1; ++i) {
       const Sequence& s = sequences_[i];
@@ -132,11 +132,36 @@ class Planner {
       const int64_t begin = std::max<int64_t>(row0, (int64_t)s.first * group_);
       const int64_t end = std::min<int64_t>(row0 + rows, ((int64_t)s.first + s.queries) * group_);
       if (begin >= end || !s.keys) continue;
-      add_segs(&b.segs, SharedSeg{s.source, s.base, s.keys, d_.prefix_len, 0, 0, (int32_t)begin, (int32_t)end}, tile,
+      add_segs(&b.segs, SharedSeg{s.source, 0, s.base, s.keys, d_.prefix_len, 0, 0, (int32_t)begin, (int32_t)end}, tile,
                plan_->positions[begin / group_], plan_->positions[(end - 1) / group_]);
     }
-    for (const SharedSeg& s : b.segs) b.item.tiles += s.tile_end - s.tile_begin;
+    finish(&b);
     return b;
+  }
+
+  // Counts a draft's tiles and takes apart the ones that all its rows see wholly, which the kernel neither
+  // masks nor looks through.
+  void finish(Draft* b) const {
+    const int tile = b->item.kind == kTall ? kTallKeys : kFlatKeys;
+    std::vector<SharedSeg> segs;
+    segs.swap(b->segs);
+    for (const SharedSeg& s : segs) {
+      b->item.tiles += s.tile_end - s.tile_begin;
+      const bool all_rows = s.row_begin == b->item.row0 && s.row_end == b->item.row0 + b->item.rows;
+      const auto whole = [&](int t) {
+        const int64_t from = (int64_t)s.position + (int64_t)t * tile, to = from + tile - 1;
+        return all_rows && (int64_t)(t + 1) * tile <= s.keys && to <= b->item.least &&
+               (!local() || to < d_.prefix || from > b->item.greatest - window());
+      };
+      for (int t = s.tile_begin; t < s.tile_end;) {
+        SharedSeg part = s;
+        part.whole = whole(t);
+        part.tile_begin = t;
+        while (t < s.tile_end && whole(t) == (part.whole != 0)) ++t;
+        part.tile_end = t;
+        b->segs.push_back(part);
+      }
+    }
   }
 
   bool flat_own(const Sequence& s) const { return !flat_all_ && (int64_t)s.queries * group_ <= kFlatRows; }
@@ -196,9 +221,9 @@ class Planner {
           const int64_t row0 = (int64_t)s.first * group_, n = (int64_t)s.queries * group_;
           f.item = SharedItem{(int32_t)row0, (int32_t)n, 0, 0, -1, 0, kFlat, plan_->positions[s.first],
                               plan_->positions[s.first + s.queries - 1], {0, 0, 0}};
-          add_segs(&f.segs, SharedSeg{s.source, s.base, s.keys, d_.prefix_len, 0, 0, (int32_t)row0, (int32_t)(row0 + n)},
+          add_segs(&f.segs, SharedSeg{s.source, 0, s.base, s.keys, d_.prefix_len, 0, 0, (int32_t)row0, (int32_t)(row0 + n)},
                    kFlatKeys, f.item.least, f.item.greatest);
-          for (const SharedSeg& g : f.segs) f.item.tiles += g.tile_end - g.tile_begin;
+          finish(&f);
           drafts_.push_back(std::move(f));
         }
     drafts_.erase(std::remove_if(drafts_.begin(), drafts_.end(), [](const Draft& b) { return b.item.tiles == 0; }),

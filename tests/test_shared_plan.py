@@ -44,8 +44,8 @@ def check_plan(qattn, prefix, queries, own, heads=16, kv=8, page=64, paged=True,
         at = plan["positions"][r // group]
         assert least <= at.min() and greatest >= at.max()
         segs = plan["segments"][s0:s1]
-        assert sum(s[5] - s[4] for s in segs) == tiles and s1 > s0
-        for source, base, keys, pos0, t0, t1, lo, hi in segs:
+        assert sum(s[6] - s[5] for s in segs) == tiles and s1 > s0
+        for source, whole, base, keys, pos0, t0, t1, lo, hi in segs[:, :9]:
             assert 0 <= t0 < t1 <= -(-keys // TILE[kind])
             assert row0 <= lo < hi <= row0 + rows
             if source == 0:
@@ -58,6 +58,10 @@ def check_plan(qattn, prefix, queries, own, heads=16, kv=8, page=64, paged=True,
                 sees = (r >= lo) & (r < hi)
             key = np.arange(t0 * TILE[kind], min(t1 * TILE[kind], keys))
             counts[np.ix_(r[sees], pos0 + key)] += 1
+            if whole:
+                assert sees.all() and t1 * TILE[kind] <= keys
+                assert all(ref.visible(position[x // group], pos0 + t1 * TILE[kind], mask, always, window)[pos0 + key].all()
+                           for x in r)
         if part < 0:
             writes[r] += 1
         else:
