@@ -76,11 +76,6 @@ __device__ inline float rows_sum(float x) {
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return half_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
-__device__ inline int wave_max(int x) {
-  for (int d = 32; d; d >>= 1) x = max(x, __shfl_xor(x, d));
-  return __builtin_amdgcn_readfirstlane(x);
-}
-
 __device__ inline SharedItem item_at(const SharedParams& p, int i) {
   const const_i32* w = (const const_i32*)(p.items + i);
   return SharedItem{w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7], w[8], {0, 0, 0}};
@@ -213,8 +208,8 @@ struct Tall {
   static constexpr int kTile = kTallKeys * kRow;        // of K or V
   static constexpr int kLds = 4 * kTile;                // K and V, double buffered
   // 16-byte chunks of a row in memory, rows of a wavefront's load, loads per tile: of 16-bit rows, codes.
-  static constexpr int kChunks16 = kRow / 16, kRows16 = 64 / kChunks16, kLoads16 = kTallKeys / (4 * kRows16);
-  static constexpr int kChunks8 = DIM / 16, kRows8 = 64 / kChunks8, kLoads8 = kTallKeys / (4 * kRows8);
+  static constexpr int kChunks16 = kRow / 16, kRows16 = 64 / kChunks16, kLoads16 = 16 / kRows16;
+  static constexpr int kChunks8 = DIM / 16, kRows8 = 64 / kChunks8, kLoads8 = 16 / kRows8;
   static constexpr bool kCodes = FORMAT != QATTN_KV_16BIT;
 
   // 16-byte chunk c of row r, swizzled so that 16 rows' reads of one chunk (K) and the transposed reads
@@ -222,28 +217,24 @@ struct Tall {
   __device__ static uint32_t k_at(int r, int c) { return r * kRow + ((c ^ (DIM == 128 ? r & 15 : (r >> 1) & 7)) << 4); }
   __device__ static uint32_t v_at(int r, int c) { return r * kRow + ((c ^ (DIM == 128 ? (r & 3) << 2 : (r & 2) << 1)) << 4); }
 
-  // Where this lane's rows of a tile lie.  Keys past the last stand on it: a row that does not see the last
-  // key either makes the tile a partly seen one, whose infinities and NaN are taken out.
+  // Where the 16 rows of a tile that this wavefront loads lie: within one page.  Rows of keys past the last
+  // are read as they are, if a page holds them (their tile is not whole: their scores are masked, and
+  // infinities and NaN of their V taken out), or as the last key's.
   struct Spot {
-    int source, base;
-    int key[kLoads16], page[kLoads16];
+    int source, keys;  // keys from the first of the 16 rows on: <= 0 if none of them exist
+    int64_t row;       // of the pool (all KV heads' rows), or of p.rows
   };
-  __device__ static Spot spot(const SharedParams& p, const SharedSeg& s, int tile, int wave, int lane) {
-    Spot at;
-    at.source = s.source;
-    at.base = s.base;
-    const int last = s.keys - 1, first = tile * kTallKeys;
-    if (s.source == kOwnRows) {
-#pragma unroll
-      for (int j = 0; j < kLoads16; ++j) at.key[j] = min(first + (j * 4 + wave) * kRows16 + lane / kChunks16, last);
-    } else {
-#pragma unroll
-      for (int j = 0; j < (kCodes ? kLoads8 : kLoads16); ++j) {
-        at.key[j] = min(first + (kCodes ? (j * 4 + wave) * kRows8 + lane / kChunks8 : (j * 4 + wave) * kRows16 + lane / kChunks16), last);
-        at.page[j] = p.pages[s.base + (at.key[j] >> p.page_shift)];
-      }
-    }
-    return at;
+  // `page`: its page number, for pages.
+  __device__ static Spot spot(const SharedParams& p, const SharedSeg& s, int tile, int page, int kvh, int wave) {
+    const int first = tile * kTallKeys + 16 * wave;
+    if (s.source == kOwnRows) return Spot{s.source, s.keys - first, (int64_t)s.base + first};
+    const int in_page = first & ((1 << p.page_shift) - 1);
+    return Spot{s.source, s.keys - first, (((int64_t)page * p.kv_heads + kvh) << p.page_shift) + in_page};
+  }
+  // The page of that spot, as a vector load: it is waited for with the tile's other loads.
+  __device__ static int page_of(const SharedParams& p, const SharedSeg& s, int tile, int wave, int zero) {
+    if (s.source == kOwnRows) return 0;
+    return p.pages[zero + s.base + (min(tile * kTallKeys + 16 * wave, s.keys - 1) >> p.page_shift)];
   }
 
   u32x4 raw[2][kLoads16];
@@ -253,23 +244,22 @@ struct Tall {
   template <int I>
   __device__ void load(const SharedParams& p, const Spot& at, int kvh, int lane) {
     if (at.source == kOwnRows) {
-      const char* rows = reinterpret_cast<const char*>(p.rows[I] + (int64_t)at.base * p.row_stride[I] + kvh * DIM);
-      const uint32_t stride = (uint32_t)p.row_stride[I] * 2;
+      // at.row + a lane's row may be past the last key: that one's row instead.
+      const char* rows = reinterpret_cast<const char*>(p.rows[I] + kvh * DIM) + (lane % kChunks16) * 16;
+      const int64_t stride = p.row_stride[I] * 2;
 #pragma unroll
       for (int j = 0; j < kLoads16; ++j)
-        raw[I][j] = *reinterpret_cast<const u32x4*>(rows + (uint64_t)(uint32_t)at.key[j] * stride + (lane % kChunks16) * 16);
+        raw[I][j] = *reinterpret_cast<const u32x4*>(rows + (at.row + min(j * kRows16 + lane / kChunks16, at.keys - 1)) * stride);
     } else {
-      constexpr int kBytes = kCodes ? DIM : kRow, kChunks = kBytes / 16;
-      const uint32_t page_rows = (uint32_t)p.kv_heads << p.page_shift, head = (uint32_t)kvh << p.page_shift;
-      const uint32_t mask = (1u << p.page_shift) - 1;
+      constexpr int kBytes = kCodes ? DIM : kRow;
+      const char* rows = p.cache[I] + at.row * kBytes;
 #pragma unroll
-      for (int j = 0; j < (kCodes ? kLoads8 : kLoads16); ++j) {
-        const uint32_t row = head + (at.key[j] & mask);
-        const uint64_t byte = (uint64_t)(uint32_t)at.page[j] * (page_rows * kBytes) + (row * kBytes + (lane % kChunks) * 16);
-        raw[I][j] = *reinterpret_cast<const u32x4*>(p.cache[I] + byte);
-        if constexpr (kCodes)
-          scale[I][j] = *reinterpret_cast<const float*>(reinterpret_cast<const char*>(p.cache_scale[I]) +
-                                                        ((uint64_t)(uint32_t)at.page[j] * (page_rows * 4) + row * 4));
+      for (int j = 0; j < (kCodes ? kLoads8 : kLoads16); ++j)
+        raw[I][j] = *reinterpret_cast<const u32x4*>(rows + (uint32_t)(lane * 16 + j * 1024));
+      if constexpr (kCodes) {
+        const float* scales = p.cache_scale[I] + at.row;
+#pragma unroll
+        for (int j = 0; j < kLoads8; ++j) scale[I][j] = scales[(uint32_t)(lane / kChunks8 + j * kRows8)];
       }
     }
   }
@@ -279,11 +269,11 @@ struct Tall {
     if (!kCodes || rows) {
 #pragma unroll
       for (int j = 0; j < kLoads16; ++j)
-        *reinterpret_cast<u32x4*>(k + k_at((j * 4 + wave) * kRows16 + lane / kChunks16, lane % kChunks16)) = raw[0][j];
+        *reinterpret_cast<u32x4*>(k + k_at(16 * wave + j * kRows16 + lane / kChunks16, lane % kChunks16)) = raw[0][j];
     } else {
 #pragma unroll
       for (int j = 0; j < kLoads8; ++j) {
-        const int r = (j * 4 + wave) * kRows8 + lane / kChunks8, c = 2 * (lane % kChunks8);
+        const int r = 16 * wave + j * kRows8 + lane / kChunks8, c = 2 * (lane % kChunks8);
         u32x4 x[2];
         expand<BF16, FORMAT>(raw[0][j], scale[0][kCodes ? j : 0], x);
         *reinterpret_cast<u32x4*>(k + k_at(r, c)) = x[0];
@@ -301,11 +291,11 @@ struct Tall {
     };
     if (!kCodes || rows) {
 #pragma unroll
-      for (int j = 0; j < kLoads16; ++j) put((j * 4 + wave) * kRows16 + lane / kChunks16, lane % kChunks16, raw[1][j]);
+      for (int j = 0; j < kLoads16; ++j) put(16 * wave + j * kRows16 + lane / kChunks16, lane % kChunks16, raw[1][j]);
     } else {
 #pragma unroll
       for (int j = 0; j < kLoads8; ++j) {
-        const int r = (j * 4 + wave) * kRows8 + lane / kChunks8, c = 2 * (lane % kChunks8);
+        const int r = 16 * wave + j * kRows8 + lane / kChunks8, c = 2 * (lane % kChunks8);
         u32x4 x[2];
         expand<BF16, FORMAT>(raw[1][j], scale[1][kCodes ? j : 0], x);
         put(r, c, x[0]);
@@ -319,6 +309,9 @@ struct Tall {
 // Offset of accumulator element r (0 .. 31 over the two 32-key blocks) from the tile's first key + 4 hl.
 __device__ constexpr int key_off(int r) { return 32 * (r >> 4) + 8 * ((r & 15) >> 2) + (r & 3); }
 
+// Iteration t computes the scores of tile t, then its weights while the matrix cores add P(t - 1) V(t - 1);
+// K(t + 1) and V(t), in registers since the iteration before, go to LDS, and K(t + 2) and V(t + 1) are asked
+// for.
 template <bool BF16, int FORMAT, int DIM>
 __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, int kvh, char* lds, uint32_t* dropped) {
   typedef Tall<BF16, FORMAT, DIM> T;
@@ -326,7 +319,6 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
   const int lane = threadIdx.x & 63, lq = lane & 31, hl = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int end_row = it.row0 + it.rows, wave_row = it.row0 + 32 * wave;
-  const int wave_end = min(end_row, wave_row + 32);
   const int row = wave_row + lq;
   const bool exists = row < end_row;
   const int token = exists ? row / p.group : 0;
@@ -340,32 +332,36 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
   struct Info {
     int whole, from, last, row_begin, row_end;  // from: position of its first key; last: of its segment's last
   };
-  // Tile t is in LDS while tile t + 1 is in registers, asked for an iteration ago.
-  Cursor ahead(p, it.seg_begin);
+  Cursor ahead(p, it.seg_begin);  // the next K tile to ask for, its page on the way
   T tile;
-  typename T::Spot spot = T::spot(p, ahead.seg, ahead.tile, wave, lane);
+  int zero = 0;
+  asm volatile("" : "+v"(zero));
+  int page = T::page_of(p, ahead.seg, ahead.tile, wave, zero);
+  typename T::Spot spot{}, spot_v{};
   int asked = 0;
-  bool rows = false;  // the tile in registers: 16-bit rows
-  Info now{}, next{};
-  bool found = false;  // infinities or NaN were dropped from V
+  bool whole_v = true;  // the V tile in registers
+  bool found = false;   // infinities or NaN were dropped from V
   if (threadIdx.x == 0) *dropped = 0;
-  const auto ask = [&]() {
+  Info now{}, next{};   // of the scores to come, of the K tile in registers
+  // K of the next tile, if there is one, and V of the tile before it.
+  const auto ask_k = [&]() {
+    if (asked == it.tiles) return;
+    spot = T::spot(p, ahead.seg, ahead.tile, __builtin_amdgcn_readfirstlane(page), kvh, wave);
     tile.template load<0>(p, spot, kvh, lane);
-    tile.template load<1>(p, spot, kvh, lane);
-    rows = spot.source == kOwnRows;
     const SharedSeg& s = ahead.seg;
     next = Info{s.whole, s.position + ahead.tile * kTallKeys, s.position + s.keys - 1, s.row_begin, s.row_end};
     if (++asked < it.tiles) {
       ahead.advance(1);
-      spot = T::spot(p, ahead.seg, ahead.tile, wave, lane);
+      page = T::page_of(p, ahead.seg, ahead.tile, wave, zero);
     }
   };
-  const auto keep = [&](int t) {
-    tile.store_k(k_buf(t), rows, wave, lane);
-    found |= tile.store_v(v_buf(t), rows, wave, lane, !next.whole);
+  const auto ask_v = [&](bool whole) {
+    tile.template load<1>(p, spot_v, kvh, lane);
+    whole_v = whole;
   };
+  const auto keep_v = [&](int t) { found |= tile.store_v(v_buf(t), spot_v.source == kOwnRows, wave, lane, !whole_v); };
 
-  ask();
+  ask_k();  // K(0)
   // Q (B operand of S^T = K Q^T): this lane's row, dims 16 st + 8 hl .. + 7 at step st.
   u32x4 q[kSteps];
   {
@@ -376,8 +372,6 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
 #pragma unroll
     for (int st = 0; st < kSteps; ++st) asm volatile("" : "+v"(q[st]));
   }
-  const int greatest = wave_max(at);
-
   f16x o[kBlocks];
 #pragma unroll
   for (int db = 0; db < kBlocks; ++db) o[db] = f16x{};
@@ -392,77 +386,138 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
 #pragma unroll
     for (int db = 0; db < kBlocks; ++db) v_read[db] = T::v_at(r, 4 * db + 2 * (G & 1) + ((a & 3) >> 1)) + ((a & 1) << 3);
   }
-  keep(0);
+  // O^T += V^T P^T for the tile in `v`.  Step st covers keys 16 st .. 16 st + 15; slot j of half hl is key
+  // 16 st + 8 (j >> 2) + 4 hl + (j & 3), whose p is element j of pf[st].
+  const auto v_frag = [&](const char* v, int i) {
+    const char* src = v + v_read[i % kBlocks] + i / kBlocks * 16 * T::kRow;
+    const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)src));
+    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(src + 8 * T::kRow)));
+    return u32x4{lo[0], lo[1], hi[0], hi[1]};
+  };
+  // beside(i): other work, issued after product i.  Operands are read kDeep products ahead; the scheduling
+  // barriers keep the compiler from reading them all at once, for which there are no registers.
+  constexpr int kDeep = 2;
+  const auto add_pv = [&](const char* v, const u32x4 (&pf)[4], auto beside) {
+    u32x4 a[kDeep];
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i) a[i] = v_frag(v, i);
+#pragma unroll
+    for (int i = 0; i < 4 * kBlocks; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+      o[i % kBlocks] = mfma32<BF16>(a[i % kDeep], pf[i / kBlocks], o[i % kBlocks]);
+      if (i + kDeep < 4 * kBlocks) a[i % kDeep] = v_frag(v, i + kDeep);
+      beside(i);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  const auto nothing = [](int) {};
+  // p of elements r, r + 1.
+  const auto weights = [&](const f16x (&sc)[2], int r, float ref, u32x4 (&pf)[4], float& sum) {
+    const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[r >> 4][r & 15], p.scale_log2, -ref));
+    const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[r >> 4][(r & 15) + 1], p.scale_log2, -ref));
+    sum += p0 + p1;
+    pf[r >> 3][(r & 7) >> 1] = narrow2<BF16>(p0, p1);
+  };
+
+  tile.store_k(k_buf(0), spot.source == kOwnRows, wave, lane);
   now = next;
-  if (it.tiles > 1) ask();
-  for (int t = 0; t < it.tiles; ++t) {
-    // Tile t is in LDS, and every wavefront is done with the other buffers.
+  spot_v = spot;
+  ask_v(now.whole);
+  ask_k();
+  // Scores of tile t, masked.
+  const auto scores = [&](const Info& cur, const char* k, f16x (&sc)[2]) {
+    // Rows lq and lq + 32, chunk 2 st + hl: its swizzled place is 2 st xor'ed onto chunk hl's.  (Formed here:
+    // hoisted, the addresses of all steps would take a register each.)
+    uint32_t place = T::k_at(lq, hl) - lq * T::kRow;
+    asm volatile("" : "+v"(place));
+    const auto k_frag = [&](int i) {
+      return *reinterpret_cast<const u32x4*>(k + lq * T::kRow + ((uint32_t)(i >> 1 << 5) ^ place) + 32 * (i & 1) * T::kRow);
+    };
+    constexpr int kAhead = 4;
+    u32x4 a[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) a[i] = k_frag(i);
+#pragma unroll
+    for (int i = 0; i < 2 * kSteps; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+      sc[i & 1] = mfma32<BF16>(a[i % kAhead], q[i >> 1], i < 2 ? f16x{} : sc[i & 1]);
+      if (i + kAhead < 2 * kSteps) a[i % kAhead] = k_frag(i + kAhead);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (!cur.whole) {
+      // Offsets from this lane's first key: the last one seen, and where the prefix and the window leave a gap.
+      const int mine = row >= cur.row_begin && row < cur.row_end ? at : -1;
+      const int base = cur.from + 4 * hl, last = min(mine, cur.last) - base;
+      const int gap = local ? p.prefix - base : kMaxPosition, window = mine - p.window - base;
+#pragma unroll
+      for (int r = 0; r < 32; ++r) {
+        const int off = key_off(r);
+        const bool hidden = (int)(off > last) | ((int)(off >= gap) & (int)(off <= window));
+        sc[r >> 4][r & 15] = hidden ? kNone : sc[r >> 4][r & 15];
+      }
+    }
+  };
+  // Moves the row's reference if the tile calls for it; returns what the sums so far are to be scaled by.
+  const auto refer = [&](const f16x (&sc)[2]) {
+    float top = fmaxf(fmaxf(sc[0][0], sc[0][1]), sc[0][2]);
+#pragma unroll
+    for (int r = 3; r < 31; r += 2) top = fmaxf(fmaxf(top, sc[r >> 4][r & 15]), sc[(r + 1) >> 4][(r + 1) & 15]);
+    top = half_max(fmaxf(top, sc[1][15])) * p.scale_log2;
+    const float moved = top > m + kLazy ? top : m;  // from -inf too: any score exceeds it
+    const float shrink = m == moved ? 1.f : __builtin_amdgcn_exp2f(m - moved);
+    m = moved;
+    return shrink;
+  };
+  const auto put_next = [&](int t) {
+    keep_v(t);
+    if (t + 1 < it.tiles) {
+      tile.store_k(k_buf(t + 1), spot.source == kOwnRows, wave, lane);
+      now = next;
+      spot_v = spot;
+      ask_v(now.whole);
+      ask_k();
+    }
+  };
+
+  u32x4 pf[4];
+  {
     __syncthreads();
     const Info cur = now;
-    if (t + 1 < it.tiles) {
-      keep(t + 1);
-      now = next;
-      if (t + 2 < it.tiles) ask();
-    }
-    // Does some row of this wavefront see some key of the tile?
-    if (cur.whole || (cur.row_begin < wave_end && cur.row_end > wave_row && cur.from <= greatest)) {
-      const char* k = k_buf(t);
-      const char* v = v_buf(t);
-      f16x sc[2] = {};
+    put_next(0);
+    f16x sc[2];
+    scores(cur, k_buf(0), sc);
+    refer(sc);
+    const float ref = m == kNone ? 0.f : m;
 #pragma unroll
-      for (int st = 0; st < kSteps; ++st)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          sc[h] = mfma32<BF16>(*reinterpret_cast<const u32x4*>(k + T::k_at(lq + 32 * h, 2 * st + hl)), q[st], sc[h]);
-      const int mine = row >= cur.row_begin && row < cur.row_end ? at : -1;
-      if (!cur.whole) {
-        // Offsets from this lane's first key: the last one seen, and where the prefix and the window leave a gap.
-        const int base = cur.from + 4 * hl, last = min(mine, cur.last) - base;
-        const int gap = local ? p.prefix - base : kMaxPosition, window = mine - p.window - base;
-#pragma unroll
-        for (int r = 0; r < 32; ++r) {
-          const int off = key_off(r);
-          const bool hidden = (int)(off > last) | ((int)(off >= gap) & (int)(off <= window));
-          sc[r >> 4][r & 15] = hidden ? kNone : sc[r >> 4][r & 15];
-        }
-      }
-      float top = fmaxf(fmaxf(sc[0][0], sc[0][1]), sc[0][2]);
-#pragma unroll
-      for (int r = 3; r < 31; r += 2) top = fmaxf(fmaxf(top, sc[r >> 4][r & 15]), sc[(r + 1) >> 4][(r + 1) & 15]);
-      top = half_max(fmaxf(top, sc[1][15])) * p.scale_log2;
-      if (__any(top > m + kLazy || (m == kNone && top > kNone))) {
-        const float moved = top > m + kLazy || m == kNone ? fmaxf(top, m) : m;
-        const float shrink = m == moved ? 1.f : __builtin_amdgcn_exp2f(m - moved);
-#pragma unroll
-        for (int db = 0; db < kBlocks; ++db) o[db] *= shrink;
-        l *= shrink;
-        m = moved;
-      }
-      const float ref = m == kNone ? 0.f : m;
-      u32x4 pf[4];
-      float l1 = 0.f;
-#pragma unroll
-      for (int r = 0; r < 32; r += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[r >> 4][r & 15], p.scale_log2, -ref));
-        const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[r >> 4][(r & 15) + 1], p.scale_log2, -ref));
-        l += p0;
-        l1 += p1;
-        pf[r >> 3][(r & 7) >> 1] = narrow2<BF16>(p0, p1);
-      }
-      l += l1;
-      {
-#pragma unroll
-        for (int st = 0; st < 4; ++st)
-#pragma unroll
-          for (int db = 0; db < kBlocks; ++db) {
-            const char* src = v + v_read[db] + st * 16 * T::kRow;
-            const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)src));
-            const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(src + 8 * T::kRow)));
-            o[db] = mfma32<BF16>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pf[st], o[db]);
-          }
-      }
-    }
+    for (int r = 0; r < 32; r += 2) weights(sc, r, ref, pf, l);
   }
+  for (int t = 1; t < it.tiles; ++t) {
+    // K(t) and V(t - 1) are in LDS, and every wavefront is done with the other buffers.
+    __syncthreads();
+    const Info cur = now;
+    put_next(t);
+    f16x sc[2];
+    scores(cur, k_buf(t), sc);
+    const float shrink = refer(sc);
+    const float ref = m == kNone ? 0.f : m;
+    // The weights beside the matrix cores' work on the tile before.
+    u32x4 next_pf[4];
+    float sum = 0.f;
+    constexpr int kEach = 32 / (4 * kBlocks);
+    add_pv(v_buf(t - 1), pf, [&](int i) {
+#pragma unroll
+      for (int r = kEach * i; r < kEach * (i + 1); r += 2) weights(sc, r, ref, next_pf, sum);
+    });
+    if (__any(shrink != 1.f)) {
+#pragma unroll
+      for (int db = 0; db < kBlocks; ++db) o[db] *= shrink;
+    }
+    l = l * shrink + sum;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pf[i] = next_pf[i];
+  }
+  __syncthreads();
+  add_pv(v_buf(it.tiles - 1), pf, nothing);
   if (found && lane == 0) *dropped = 1;
   __syncthreads();
   if (*dropped)
