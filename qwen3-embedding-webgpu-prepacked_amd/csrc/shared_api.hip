@@ -260,7 +260,7 @@ int check_shared(qattn_ctx* ctx, const qattn_shared_desc* d) {
 int make_shared_plan(qattn_ctx* ctx, const qattn_shared_desc& d, int compute_units, SharedPlan* plan) {
   plan_shared(d, compute_units, plan);
   const int64_t heads = d.cache.kv_heads;
-  if ((int64_t)plan->items.size() * heads > kMaxSharedGroups || ((int64_t)plan->merges.size() * heads + 3) / 4 > kMaxSharedGroups ||
+  if ((int64_t)plan->items.size() * heads > kMaxSharedGroups || (int64_t)plan->merges.size() * heads > kMaxSharedGroups ||
       plan->partial_rows >= ((int64_t)1 << 31))
     return fail(ctx, QATTN_EINVAL, "too many rows for one launch (%zu items, %zu merged rows, %lld KV heads)", plan->items.size(),
                 plan->merges.size(), (long long)heads);
@@ -367,6 +367,7 @@ int install_shared_plan(qattn_shared_run* run, const qattn_shared_desc& d) {
   p.part_ml = reinterpret_cast<float2*>(p.part_o + values * d.cache.head_dim);
   p.n_items = (int32_t)plan.items.size();
   p.n_merges = (int32_t)plan.merges.size();
+  p.most_parts = plan.most_parts;
   p.kv_heads = d.cache.kv_heads;
   p.group = d.q_heads / d.cache.kv_heads;
   while ((1 << p.page_shift) < d.cache.page_size) ++p.page_shift;

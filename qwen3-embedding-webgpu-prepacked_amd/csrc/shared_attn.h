@@ -52,6 +52,7 @@ struct SharedPlan {
   std::vector<int32_t> positions;  // of each query
   std::vector<int32_t> pages;
   int64_t partial_rows = 0;
+  int32_t most_parts = 0;  // partial rows of a merged row, at most
   qattn_shared_info info{};
 };
 // `d`: validated.  compute_units: of the device.
@@ -71,7 +72,7 @@ struct SharedParams {
   const int32_t* pages;
   float* part_o;                // [partial row][kv_heads][head_dim]
   float2* part_ml;              // [partial row][kv_heads]: the row's reference (log2) and sum
-  int32_t n_items, n_merges, kv_heads, group, page_shift;
+  int32_t n_items, n_merges, most_parts, kv_heads, group, page_shift;
   int32_t mask, prefix, window;
   float scale_log2;
 };

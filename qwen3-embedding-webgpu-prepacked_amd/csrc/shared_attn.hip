@@ -807,62 +807,79 @@ __global__ __launch_bounds__(kSharedThreads, 2) void shared_attn_kernel(SharedPa
     flat_item<BF16, FORMAT, DIM>(p, it, kvh, lds, stats);
 }
 
-// One wavefront per merged row and KV head: sum over its partial rows of 2^(m_i - max m) times the row's
-// sums; a partial row that saw no key has m = -inf and weighs 0.  Without partial rows: zeros.
-template <bool BF16, int DIM>
+// Merged rows: sum over a row's partial rows of 2^(m_i - max m) times its sums; a partial row that saw no
+// key has m = -inf and weighs 0.  Without partial rows: zeros.  DIM / 4 lanes hold a row, a float4 each, and a
+// lane's loads go out eight partial rows at a time.  WIDE: a whole workgroup takes one row, its groups of
+// lanes every kGroups'th partial row (rows cut into many chunks: a chain of loads would set the time);
+// else each group takes a row of its own.  Bound by latency: three dependent accesses.
+template <bool BF16, int DIM, bool WIDE>
 __global__ __launch_bounds__(kSharedThreads) void shared_merge_kernel(SharedParams p) {
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int64_t index = (int64_t)blockIdx.x * 4 + wave;
-  if (index >= (int64_t)p.n_merges * p.kv_heads) return;
+  constexpr int kLanes = DIM / 4, kGroups = kSharedThreads / kLanes;
+  __shared__ f4 sums[WIDE ? kSharedThreads : 1];
+  __shared__ float2 stats[WIDE ? kGroups : 1];
+  const int group = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
+  const int64_t index = WIDE ? blockIdx.x : (int64_t)blockIdx.x * kGroups + group;
+  const bool exists = index < (int64_t)p.n_merges * p.kv_heads;
   const int kvh = (int)(index % p.kv_heads);
-  const SharedMerge e = p.merges[index / p.kv_heads];
+  SharedMerge e{};
+  if (exists) e = p.merges[index / p.kv_heads];
   const int count = e.group[0].count + e.group[1].count;
-  const auto part_at = [&](int i) {
-    const int g = i >= e.group[0].count;
-    const SharedMerge::Group& of = e.group[g];
-    return ((int64_t)of.first + (int64_t)(g ? i - e.group[0].count : i) * of.step) * p.kv_heads + kvh;
-  };
-  // Up to 64 partial rows at a time, one weight to a lane; their rows' loads go out eight at a time.
-  constexpr int kDims = DIM / 64;
-  float top = kNone, sum = 0.f, x[kDims] = {};
-  for (int i0 = 0; i0 < count; i0 += 64) {
-    const int n = min(64, count - i0);
-    const float2 ml = lane < n ? p.part_ml[part_at(i0 + lane)] : float2{kNone, 0.f};
-    float most = ml.x;
-    for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
-    most = fmaxf(most, top);
-    const float ref = most == kNone ? 0.f : most;
-    const float rescale = __builtin_amdgcn_exp2f(top - ref), weight = __builtin_amdgcn_exp2f(ml.x - ref);
-    float part_sum = weight * ml.y;
-    for (int d = 32; d; d >>= 1) part_sum += __shfl_xor(part_sum, d);
-    sum = (i0 ? sum * rescale : 0.f) + part_sum;
+  constexpr int kFirst = WIDE ? 1 : 0, kStep = WIDE ? kGroups : 1, kBatch = 8;
+  float top = kNone, sum = 0.f;
+  f4 x = {};
+  for (int i0 = kFirst * group; i0 < count; i0 += kBatch * kStep) {
+    float2 ml[kBatch];
+    f4 y[kBatch];
 #pragma unroll
-    for (int k = 0; k < kDims; ++k) x[k] *= i0 ? rescale : 0.f;
-    top = most;
-    for (int j0 = 0; j0 < n; j0 += 8) {
-      float y[8][kDims];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float* src = p.part_o + part_at(i0 + min(j0 + j, n - 1)) * DIM + kDims * lane;
-#pragma unroll
-        for (int k = 0; k < kDims; ++k) y[j][k] = src[k];
+    for (int j = 0; j < kBatch; ++j) {
+      const int i = i0 + j * kStep;
+      ml[j] = float2{kNone, 0.f};
+      y[j] = f4{};
+      if (i < count) {
+        const bool second = i >= e.group[0].count;
+        const int64_t row = second ? e.group[1].first + (int64_t)(i - e.group[0].count) * e.group[1].step
+                                   : e.group[0].first + (int64_t)i * e.group[0].step;
+        const int64_t part = row * p.kv_heads + kvh;
+        ml[j] = p.part_ml[part];
+        y[j] = *reinterpret_cast<const f4*>(p.part_o + part * DIM + 4 * lane);
       }
+    }
+    float most = top;
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j0 + j < n) {
-          const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), j0 + j));
+    for (int j = 0; j < kBatch; ++j) most = fmaxf(most, ml[j].x);
+    const float ref = most == kNone ? 0.f : most, keep = __builtin_amdgcn_exp2f(top - ref);
+    sum *= keep;
+    x *= keep;
 #pragma unroll
-          for (int k = 0; k < kDims; ++k) x[k] += f * y[j][k];
-        }
+    for (int j = 0; j < kBatch; ++j) {
+      const float f = __builtin_amdgcn_exp2f(ml[j].x - ref);
+      sum += f * ml[j].y;
+      x += f * y[j];
+    }
+    top = most;
+  }
+  if constexpr (WIDE) {
+    sums[threadIdx.x] = x;
+    if (lane == 0) stats[group] = float2{top, sum};
+    __syncthreads();
+    if (group) return;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) top = fmaxf(top, stats[g].x);
+    const float ref = top == kNone ? 0.f : top;
+    sum = 0.f;
+    x = f4{};
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      const float f = __builtin_amdgcn_exp2f(stats[g].x - ref);
+      sum += f * stats[g].y;
+      x += f * sums[g * kLanes + lane];
     }
   }
+  if (!exists) return;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int token = e.row / p.group;
-  uint16_t* dst = p.o + (int64_t)token * p.o_stride + (kvh * p.group + e.row - token * p.group) * DIM + kDims * lane;
-  if constexpr (kDims == 2)
-    *reinterpret_cast<uint32_t*>(dst) = narrow2<BF16>(x[0] * inv, x[1] * inv);
-  else
-    *dst = (uint16_t)narrow2<BF16>(x[0] * inv, 0.f);
+  uint16_t* dst = p.o + (int64_t)token * p.o_stride + (kvh * p.group + e.row - token * p.group) * DIM + 4 * lane;
+  *reinterpret_cast<u32x2*>(dst) = u32x2{narrow2<BF16>(x[0] * inv, x[1] * inv), narrow2<BF16>(x[2] * inv, x[3] * inv)};
 }
 
 template <bool BF16, int FORMAT, int DIM>
@@ -882,8 +899,13 @@ hipError_t launch(const SharedParams& p, int format, hipStream_t stream) {
     if (e != hipSuccess) return e;
   }
   if (p.n_merges > 0) {
-    const int64_t waves = (int64_t)p.n_merges * p.kv_heads;
-    hipLaunchKernelGGL((shared_merge_kernel<BF16, DIM>), dim3((unsigned)((waves + 3) / 4)), dim3(kSharedThreads), 0, stream, p);
+    const int64_t rows = (int64_t)p.n_merges * p.kv_heads;
+    constexpr int kGroups = kSharedThreads / (DIM / 4);
+    if (p.most_parts > 8)
+      hipLaunchKernelGGL((shared_merge_kernel<BF16, DIM, true>), dim3((unsigned)rows), dim3(kSharedThreads), 0, stream, p);
+    else
+      hipLaunchKernelGGL((shared_merge_kernel<BF16, DIM, false>), dim3((unsigned)((rows + kGroups - 1) / kGroups)),
+                         dim3(kSharedThreads), 0, stream, p);
     return hipGetLastError();
   }
   return hipSuccess;

@@ -8,8 +8,7 @@
 // more rows than that.
 //
 // Cuts.  Items are cut along their keys where that shortens the launch: the planner compares the time at
-// which the last of the GPU's slots ends, for a range of chunk sizes, by a cost model in units of one
-// 64-key tile of a full block.
+// which the last of the GPU's slots ends, for a range of chunk sizes, by a cost model.
 #include <algorithm>
 #include <cmath>
 #include <queue>
@@ -20,9 +19,11 @@ namespace qattn {
 
 namespace {
 
-// Costs in units of a block's 64-key tile, from measured launches: an item's start and end, a round of four
-// 32-key tiles of a flat item, and the second launch.
-constexpr double kTallItem = 1.5, kFlatItem = 1.0, kFlatRound = 0.4, kPartial = 0.5, kMergeLaunch = 2.0;
+// Costs in microseconds, from measured launches (two workgroups to a CU): an item's start and end, a 64-key
+// tile of a full block, a round of four 32-key tiles of a flat item, an item's partial results, the second
+// launch, and the partial rows' bytes (written and read).
+constexpr double kTallItem = 3.0, kTallTile = 2.3, kFlatItem = 2.0, kFlatRound = 1.4, kPartial = 1.0, kMergeLaunch = 4.0;
+constexpr double kBytesPerUs = 5e6;
 constexpr int kMostSimulated = 16384;
 
 struct Sequence {
@@ -36,7 +37,7 @@ struct Draft {
   bool merged = false;  // its rows have partial results elsewhere too
   int chunks = 1, first_part = 0;
   double cost(int tiles) const {
-    return item.kind == kTall ? kTallItem + tiles : kFlatItem + kFlatRound * ((tiles + 3) / 4);
+    return item.kind == kTall ? kTallItem + kTallTile * tiles : kFlatItem + kFlatRound * ((tiles + 3) / 4);
   }
 };
 
@@ -238,7 +239,7 @@ class Planner {
 
   static int chunks_for(const Draft& b, double target) {
     // Flat chunks are whole rounds of the four wavefronts.
-    const double unit = b.item.kind == kTall ? 1.0 : kFlatRound;
+    const double unit = b.item.kind == kTall ? kTallTile : kFlatRound;
     const int n = b.item.kind == kTall ? b.item.tiles : (b.item.tiles + 3) / 4;
     const double fixed = b.item.kind == kTall ? kTallItem : kFlatItem;
     const int fit = std::max(1, (int)std::floor((target - fixed) / unit));
@@ -257,7 +258,7 @@ class Planner {
       *split |= part;
       for (int i = 0; i < c; ++i) {
         const int n = units * (i + 1) / c - units * i / c;
-        costs.push_back((part ? kPartial : 0) + (b.item.kind == kTall ? kTallItem + n : kFlatItem + kFlatRound * n));
+        costs.push_back((part ? kPartial : 0) + (b.item.kind == kTall ? kTallItem + kTallTile * n : kFlatItem + kFlatRound * n));
       }
       if ((int)costs.size() > kMostSimulated) return 1e30;
     }
@@ -273,14 +274,13 @@ class Planner {
       ends.push(start + c);
       last = std::max(last, start + c);
     }
-    // Partial rows are written and read once each: about 4 TB/s, a unit being about 1 us.
-    return last + (*split ? kMergeLaunch + partial_rows * d_.cache.kv_heads * d_.cache.head_dim * 8 / 4e6 : 0);
+    return last + (*split ? kMergeLaunch + partial_rows * d_.cache.kv_heads * d_.cache.head_dim * 8 / kBytesPerUs : 0);
   }
 
   void cut() {
     double longest = 0, best_span = 1e30, best = 0;
     for (const Draft& b : drafts_) longest = std::max(longest, b.cost(b.item.tiles));
-    for (double target = longest; target > 1.9; target *= target > longest / 2 ? 0.85 : 0.7) {
+    for (double target = longest; target > kTallItem + kTallTile; target *= target > longest / 2 ? 0.85 : 0.7) {
       bool split = false;
       const double s = span(target, &split);
       if (target == longest || s < best_span * 0.97) {
@@ -350,6 +350,7 @@ class Planner {
     for (int64_t row = 0; row < rows; ++row)
       if (!direct[row]) {
         all[row].row = (int32_t)row;
+        plan_->most_parts = std::max(plan_->most_parts, all[row].group[0].count + all[row].group[1].count);
         plan_->merges.push_back(all[row]);
       }
   }
