@@ -464,7 +464,8 @@ int qattn_shared_run_get_info(const qattn_shared_run* run, qattn_shared_info* in
 /* Host-only planning (no device; 256 compute units): the plan as int32 words, the counts first:
  * {items, segments, merged rows, tokens, page numbers, 0, 0, 0}, then per item {first row, rows, first
  * segment, end segment, first partial row or -1, key tiles, kind (0: 128-row blocks over 64-key tiles,
- * 1: 16-row blocks over 32-key tiles), least query position, greatest, 0, 0, 0}, per segment {source
+ * 1: 16-row blocks over 32-key tiles), least query position, greatest, 0, 0, 0,
+ * a copy of the first segment, the pages of the first eight 16-key groups}, per segment {source
  * (0 prefix pages, 1 own pages, 2 own rows), whether every row sees all its keys, first page number or
  * first row, keys, position of key 0, first tile, end tile, first row, end row, 0, 0, 0}, per merged row {row, then for up to two groups of partial
  * results: first partial row, count, distance between them, and 0}, per token its position, and the

@@ -494,7 +494,7 @@ int qattn_shared_plan_describe(const qattn_shared_desc* desc, int32_t* words, in
   if (rc) return rc;
   const int32_t head[8] = {(int32_t)plan.items.size(), (int32_t)plan.segs.size(), (int32_t)plan.merges.size(),
                            (int32_t)plan.positions.size(), (int32_t)plan.pages.size(), 0, 0, 0};
-  *count = 8 + (int64_t)plan.items.size() * 12 + (int64_t)plan.segs.size() * 12 + (int64_t)plan.merges.size() * 8 +
+  *count = 8 + (int64_t)plan.items.size() * 32 + (int64_t)plan.segs.size() * 12 + (int64_t)plan.merges.size() * 8 +
            (int64_t)plan.positions.size() + (int64_t)plan.pages.size();
   if (info) *info = plan.info;
   if (!words) return QATTN_OK;

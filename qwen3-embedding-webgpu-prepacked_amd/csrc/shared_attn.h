@@ -21,19 +21,23 @@ constexpr int32_t kMaxPosition = 1 << 30;
 enum SharedSource { kPrefixPages = 0, kOwnPages = 1, kOwnRows = 2 };
 enum SharedKind { kTall = 0, kFlat = 1 };
 
-// Rows row0 .. row0 + rows - 1 over the tiles of segments seg_begin .. seg_end - 1.  Results go to the output
-// (part < 0) or, unnormalised, to partial rows part, part + 1, ...
-struct SharedItem {
-  int32_t row0, rows, seg_begin, seg_end, part, tiles, kind;
-  int32_t least, greatest;  // query positions among the rows
-  int32_t pad[3];
-};
 // Tiles tile_begin .. tile_end - 1 (of the item kind's size) of `keys` keys, seen by rows row_begin ..
 // row_end - 1 only.  base: the source's first page number (an index into the plan's list) or row.  whole:
 // every row of the item sees every key of these tiles.
 struct SharedSeg {
   int32_t source, whole, base, keys, position, tile_begin, tile_end, row_begin, row_end;
   int32_t pad[3];
+};
+// Rows row0 .. row0 + rows - 1 over the tiles of segments seg_begin .. seg_end - 1.  Results go to the output
+// (part < 0) or, unnormalised, to partial rows part, part + 1, ...  The first segment, and the pages of the
+// first tiles' 16-key groups (tall: four, flat: two for each wavefront's first tile), come with the item, so
+// that a workgroup asks for its first keys after one dependent load.
+struct SharedItem {
+  int32_t row0, rows, seg_begin, seg_end, part, tiles, kind;
+  int32_t least, greatest;  // query positions among the rows
+  int32_t pad[3];
+  SharedSeg seg;
+  int32_t page[8];
 };
 // A row whose results are merged: `count` partial rows from `first` on, `step` apart, in two groups.
 struct SharedMerge {
@@ -43,7 +47,7 @@ struct SharedMerge {
   } group[2];
   int32_t pad;
 };
-static_assert(sizeof(SharedItem) == 48 && sizeof(SharedSeg) == 48 && sizeof(SharedMerge) == 32, "plan words");
+static_assert(sizeof(SharedItem) == 128 && sizeof(SharedSeg) == 48 && sizeof(SharedMerge) == 32, "plan words");
 
 struct SharedPlan {
   std::vector<SharedItem> items;

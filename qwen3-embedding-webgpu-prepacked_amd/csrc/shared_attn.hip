@@ -76,9 +76,16 @@ __device__ inline float rows_sum(float x) {
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return half_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
+__device__ inline SharedSeg seg_at(const const_i32* w) {
+  return SharedSeg{w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7], w[8], {0, 0, 0}};
+}
+// All of an item but its pages.
 __device__ inline SharedItem item_at(const SharedParams& p, int i) {
   const const_i32* w = (const const_i32*)(p.items + i);
-  return SharedItem{w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7], w[8], {0, 0, 0}};
+  return SharedItem{w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7], w[8], {0, 0, 0}, seg_at(w + 12), {}};
+}
+__device__ inline int item_page(const SharedParams& p, int i, int group) {
+  return ((const const_i32*)(p.items + i))[24 + group];
 }
 
 // The tiles of an item one after another, through its segments.
@@ -86,20 +93,15 @@ struct Cursor {
   const const_i32* words;
   int tile;
   SharedSeg seg;
-  __device__ Cursor(const SharedParams& p, int first) : words((const const_i32*)(p.segs + first)) {
-    read();
-    tile = seg.tile_begin;
-  }
-  __device__ void read() {
-    seg = SharedSeg{words[0], words[1], words[2], words[3], words[4], words[5], words[6], words[7], words[8], {0, 0, 0}};
-  }
+  __device__ Cursor(const SharedParams& p, const SharedItem& it)
+      : words((const const_i32*)(p.segs + it.seg_begin)), tile(it.seg.tile_begin), seg(it.seg) {}
   // `n` tiles on; the item has that many.
   __device__ void advance(int n) {
     tile += n;
     while (tile >= seg.tile_end) {
       const int over = tile - seg.tile_end;
       words += sizeof(SharedSeg) / 4;
-      read();
+      seg = seg_at(words);
       tile = seg.tile_begin + over;
     }
   }
@@ -112,8 +114,11 @@ struct Group {
   int count;             // keys of the group that exist
   uint32_t stride;       // bytes between rows
 };
+__device__ inline int page_at(const SharedParams& p, const SharedSeg& s, int first) {
+  return s.source == kOwnRows ? 0 : ((const const_i32*)p.pages)[s.base + (min(first, s.keys - 1) >> p.page_shift)];
+}
 template <int FORMAT, int DIM>
-__device__ inline Group group_at(const SharedParams& p, const SharedSeg& s, int first, int size, int kvh) {
+__device__ inline Group group_at(const SharedParams& p, const SharedSeg& s, int first, int size, int page, int kvh) {
   Group g;
   g.count = min(max(s.keys - first, 0), size);
   if (s.source == kOwnRows) {
@@ -125,7 +130,6 @@ __device__ inline Group group_at(const SharedParams& p, const SharedSeg& s, int 
   } else {
     constexpr int kRow = FORMAT == QATTN_KV_16BIT ? 2 * DIM : DIM;
     const int in_page = first & ((1 << p.page_shift) - 1);
-    const int page = ((const const_i32*)p.pages)[s.base + (min(first, s.keys - 1) >> p.page_shift)];
     const int64_t row = (((int64_t)page * p.kv_heads + kvh) << p.page_shift) + in_page;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -167,7 +171,7 @@ __device__ inline bool drop_nonfinite(u32x4& chunk) {
 // Elements d .. d + 3 of key `key`'s V.
 template <bool BF16, int FORMAT, int DIM>
 __device__ inline f4 value_at(const SharedParams& p, const SharedSeg& s, int key, int kvh, int d) {
-  const Group g = group_at<FORMAT, DIM>(p, s, key, 1, kvh);
+  const Group g = group_at<FORMAT, DIM>(p, s, key, 1, page_at(p, s, key), kvh);
   u32x2 x;
   if (FORMAT == QATTN_KV_16BIT || s.source == kOwnRows) {
     x = *reinterpret_cast<const u32x2*>(g.base[1] + 2 * d);
@@ -183,7 +187,7 @@ __device__ inline float nonfinite(float v, bool seen) { return seen && !(fabsf(v
 template <bool BF16, int FORMAT, int DIM, class Add>
 __device__ inline void each_nonfinite(const SharedParams& p, const SharedItem& it, int kvh, int row, int at, int size, int first,
                                       int step, Add add) {
-  Cursor c(p, it.seg_begin);
+  Cursor c(p, it);
   c.advance(first);
   for (int t = first;;) {
     const SharedSeg s = c.seg;
@@ -313,7 +317,7 @@ __device__ constexpr int key_off(int r) { return 32 * (r >> 4) + 8 * ((r & 15) >
 // K(t + 1) and V(t), in registers since the iteration before, go to LDS, and K(t + 2) and V(t + 1) are asked
 // for.
 template <bool BF16, int FORMAT, int DIM>
-__device__ inline void tall_item(const SharedParams& p, const SharedItem& it, int kvh, char* lds, uint32_t* dropped) {
+__device__ inline void tall_item(const SharedParams& p, const SharedItem& it, int index, int kvh, char* lds, uint32_t* dropped) {
   typedef Tall<BF16, FORMAT, DIM> T;
   constexpr int kBlocks = DIM / 32, kSteps = DIM / 16;
   const int lane = threadIdx.x & 63, lq = lane & 31, hl = lane >> 5;
@@ -332,11 +336,11 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
   struct Info {
     int whole, from, last, row_begin, row_end;  // from: position of its first key; last: of its segment's last
   };
-  Cursor ahead(p, it.seg_begin);  // the next K tile to ask for, its page on the way
+  Cursor ahead(p, it);  // the next K tile to ask for, its page on the way
   T tile;
   int zero = 0;
   asm volatile("" : "+v"(zero));
-  int page = T::page_of(p, ahead.seg, ahead.tile, wave, zero);
+  int page = item_page(p, index, wave);
   typename T::Spot spot{}, spot_v{};
   int asked = 0;
   bool whole_v = true;  // the V tile in registers
@@ -437,6 +441,7 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
     u32x4 a[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) a[i] = k_frag(i);
+    __builtin_amdgcn_s_setprio(1);  // before the other wavefront's vector work
 #pragma unroll
     for (int i = 0; i < 2 * kSteps; ++i) {
       __builtin_amdgcn_sched_barrier(0);
@@ -444,16 +449,20 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
       if (i + kAhead < 2 * kSteps) a[i % kAhead] = k_frag(i + kAhead);
     }
     __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(0);
     if (!cur.whole) {
       // Offsets from this lane's first key: the last one seen, and where the prefix and the window leave a gap.
       const int mine = row >= cur.row_begin && row < cur.row_end ? at : -1;
       const int base = cur.from + 4 * hl, last = min(mine, cur.last) - base;
-      const int gap = local ? p.prefix - base : kMaxPosition, window = mine - p.window - base;
 #pragma unroll
-      for (int r = 0; r < 32; ++r) {
-        const int off = key_off(r);
-        const bool hidden = (int)(off > last) | ((int)(off >= gap) & (int)(off <= window));
-        sc[r >> 4][r & 15] = hidden ? kNone : sc[r >> 4][r & 15];
+      for (int r = 0; r < 32; ++r) sc[r >> 4][r & 15] = key_off(r) > last ? kNone : sc[r >> 4][r & 15];
+      if (local && cur.from + kTallKeys > p.prefix && cur.from <= it.greatest - p.window) {
+        const int gap = p.prefix - base, window = mine - p.window - base;
+#pragma unroll
+        for (int r = 0; r < 32; ++r) {
+          const int off = key_off(r);
+          sc[r >> 4][r & 15] = (int)(off >= gap) & (int)(off <= window) ? kNone : sc[r >> 4][r & 15];
+        }
       }
     }
   };
@@ -506,7 +515,9 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
     constexpr int kEach = 32 / (4 * kBlocks);
     add_pv(v_buf(t - 1), pf, [&](int i) {
 #pragma unroll
-      for (int r = kEach * i; r < kEach * (i + 1); r += 2) weights(sc, r, ref, next_pf, sum);
+      for (int r = kEach * i; r < kEach * (i + 1); r += 2) {
+        weights(sc, r, ref, next_pf, sum);
+      }
     });
     if (__any(shrink != 1.f)) {
 #pragma unroll
@@ -581,11 +592,11 @@ struct Flat {
   u32x4 k[2][kSteps], v[2][kLoads16];
   float ks[2], vs[2][kCodes ? kLoads8 : 1];
 
-  __device__ void load(const SharedParams& p, const SharedSeg& s, int tile, int kvh, int lane) {
+  __device__ void load(const SharedParams& p, const SharedSeg& s, int tile, const int (&page)[2], int kvh, int lane) {
     const int key = lane & 15, c = lane >> 4;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      const Group g = group_at<FORMAT, DIM>(p, s, tile * kFlatKeys + 16 * b, 16, kvh);
+      const Group g = group_at<FORMAT, DIM>(p, s, tile * kFlatKeys + 16 * b, 16, page[b], kvh);
       if (!kCodes || s.source == kOwnRows) {
         uint32_t stride[2];
 #pragma unroll
@@ -654,7 +665,7 @@ struct Flat {
 };
 
 template <bool BF16, int FORMAT, int DIM>
-__device__ inline void flat_item(const SharedParams& p, const SharedItem& it, int kvh, char* lds_all, float2* stats) {
+__device__ inline void flat_item(const SharedParams& p, const SharedItem& it, int index, int kvh, char* lds_all, float2* stats) {
   typedef Flat<BF16, FORMAT, DIM> T;
   constexpr int kBlocks = DIM / 16;
   const int lane = threadIdx.x & 63, n = lane & 15, c = lane >> 4;
@@ -684,10 +695,11 @@ __device__ inline void flat_item(const SharedParams& p, const SharedItem& it, in
 
   if (wave < it.tiles) {
     bool found = false;  // infinities or NaN were dropped from V
-    Cursor now(p, it.seg_begin);
+    Cursor now(p, it);
     now.advance(wave);
     T tile;
-    tile.load(p, now.seg, now.tile, kvh, lane);
+    int page[2] = {item_page(p, index, 2 * wave), item_page(p, index, 2 * wave + 1)};
+    tile.load(p, now.seg, now.tile, page, kvh, lane);
     for (int t = wave; t < it.tiles; t += 4) {
       const SharedSeg s = now.seg;
       const int first = now.tile * kFlatKeys, from = s.position + first;
@@ -703,7 +715,8 @@ __device__ inline void flat_item(const SharedParams& p, const SharedItem& it, in
       found |= tile.store(lds, s, lane, part);
       if (t + 4 < it.tiles) {
         now.advance(4);
-        tile.load(p, now.seg, now.tile, kvh, lane);
+        for (int b = 0; b < 2; ++b) page[b] = page_at(p, now.seg, now.tile * kFlatKeys + 16 * b);
+        tile.load(p, now.seg, now.tile, page, kvh, lane);
       }
       const bool mine = row >= s.row_begin && row < s.row_end;
       const int limit = min(mine ? at : -1, s.position + s.keys - 1);
@@ -800,11 +813,12 @@ __global__ __launch_bounds__(kSharedThreads, 2) void shared_attn_kernel(SharedPa
   __shared__ __attribute__((aligned(1024))) char lds[Tall<BF16, FORMAT, DIM>::kLds];
   __shared__ __attribute__((aligned(16))) float2 stats[4 * kFlatRows];
   const int kvh = (int)(blockIdx.x % (uint32_t)p.kv_heads);
-  const SharedItem it = item_at(p, (int)(blockIdx.x / (uint32_t)p.kv_heads));
+  const int index = (int)(blockIdx.x / (uint32_t)p.kv_heads);
+  const SharedItem it = item_at(p, index);
   if (it.kind == kTall)
-    tall_item<BF16, FORMAT, DIM>(p, it, kvh, lds, reinterpret_cast<uint32_t*>(stats));
+    tall_item<BF16, FORMAT, DIM>(p, it, index, kvh, lds, reinterpret_cast<uint32_t*>(stats));
   else
-    flat_item<BF16, FORMAT, DIM>(p, it, kvh, lds, stats);
+    flat_item<BF16, FORMAT, DIM>(p, it, index, kvh, lds, stats);
 }
 
 // Merged rows: sum over a row's partial rows of 2^(m_i - max m) times its sums; a partial row that saw no

@@ -120,7 +120,7 @@ class Planner {
   Draft block(int64_t row0, int64_t rows, size_t first_sequence, int kind, bool with_own) const {
     const int tile = kind == kTall ? kTallKeys : kFlatKeys;
     Draft b;
-    b.item = SharedItem{(int32_t)row0, (int32_t)rows, 0, 0, -1, 0, kind, 0, 0, {0, 0, 0}};
+    b.item = SharedItem{(int32_t)row0, (int32_t)rows, 0, 0, -1, 0, kind};
     const int32_t t0 = (int32_t)(row0 / group_), t1 = (int32_t)((row0 + rows - 1) / group_);
     b.item.least = *std::min_element(&plan_->positions[t0], &plan_->positions[t1] + 1);
     b.item.greatest = *std::max_element(&plan_->positions[t0], &plan_->positions[t1] + 1);
@@ -221,7 +221,7 @@ class Planner {
           Draft f;
           const int64_t row0 = (int64_t)s.first * group_, n = (int64_t)s.queries * group_;
           f.item = SharedItem{(int32_t)row0, (int32_t)n, 0, 0, -1, 0, kFlat, plan_->positions[s.first],
-                              plan_->positions[s.first + s.queries - 1], {0, 0, 0}};
+                              plan_->positions[s.first + s.queries - 1]};
           add_segs(&f.segs, SharedSeg{s.source, 0, s.base, s.keys, d_.prefix_len, 0, 0, (int32_t)row0, (int32_t)(row0 + n)},
                    kFlatKeys, f.item.least, f.item.greatest);
           finish(&f);
@@ -321,6 +321,7 @@ class Planner {
           end -= n;
         }
         it.seg_end = (int32_t)plan_->segs.size();
+        first_pages(&it);
         items.emplace_back(b.cost(it.tiles), it);
       }
     }
@@ -330,6 +331,22 @@ class Planner {
     plan_->info.items = (int32_t)plan_->items.size();
     plan_->info.merged_rows = (int32_t)plan_->merges.size();
     plan_->info.partial_rows = plan_->partial_rows;
+  }
+
+  // The item's own copy of its first segment and of the pages of its first tiles.
+  void first_pages(SharedItem* it) const {
+    it->seg = plan_->segs[it->seg_begin];
+    const int tile = it->kind == kTall ? kTallKeys : kFlatKeys;
+    int32_t seg = it->seg_begin, at = it->seg.tile_begin;
+    for (int i = 0; i < 8; ++i) {
+      const SharedSeg& s = plan_->segs[seg];
+      const int32_t first = at * tile + 16 * i % tile;
+      it->page[i] = s.source == kOwnRows ? 0 : plan_->pages[s.base + std::min(first, s.keys - 1) / d_.cache.page_size];
+      if ((16 * (i + 1)) % tile) continue;
+      if (++at < s.tile_end) continue;
+      if (++seg == it->seg_end) break;  // no further tile
+      at = plan_->segs[seg].tile_begin;
+    }
   }
 
   // Rows with partial results, and rows that no item computes (merged from nothing: zeros).

@@ -45,6 +45,10 @@ def check_plan(qattn, prefix, queries, own, heads=16, kv=8, page=64, paged=True,
         assert least <= at.min() and greatest >= at.max()
         segs = plan["segments"][s0:s1]
         assert sum(s[6] - s[5] for s in segs) == tiles and s1 > s0
+        assert np.array_equal(it[12:24], segs[0])
+        groups = [(s, k) for s in segs for k in range(s[5] * TILE[kind], s[6] * TILE[kind], 16)][:8]
+        for (s, k), got in zip(groups, it[24:]):
+            assert got == (0 if s[0] == 2 else plan["pages"][s[2] + min(k, s[3] - 1) // page])
         for source, whole, base, keys, pos0, t0, t1, lo, hi in segs[:, :9]:
             assert 0 <= t0 < t1 <= -(-keys // TILE[kind])
             assert row0 <= lo < hi <= row0 + rows
