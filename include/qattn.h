@@ -379,7 +379,8 @@ enum qattn_kv_format {
 };
 /* A paged cache in the caller's device memory: slot s is row s % page_size of page s / page_size;
  * codes [pages][kv_heads][page_size][head_dim], scales [pages][kv_heads][page_size].  Device
- * pointers 16-byte aligned; page_size a power of two in [16, 4096]; head_dim 64 or 128. */
+ * pointers 16-byte aligned; page_size a power of two in [16, 4096]; head_dim 64 or 128;
+ * pages*page_size*kv_heads below 2^35. */
 typedef struct qattn_kv_cache {
   void* k;
   void* v;
@@ -462,14 +463,15 @@ typedef struct qattn_shared_info {
 } qattn_shared_info;
 int qattn_shared_run_get_info(const qattn_shared_run* run, qattn_shared_info* info);
 /* Host-only planning (no device; 256 compute units): the plan as int32 words, the counts first:
- * {items, segments, merged rows, tokens, page numbers, 0, 0, 0}, then per item {first row, rows, first
+ * {items, segments, merged rows, tokens, groups, 0, 0, 0}, then per item {first row, rows, first
  * segment, end segment, first partial row or -1, key tiles, kind (0: 128-row blocks over 64-key tiles,
  * 1: 16-row blocks over 32-key tiles), least query position, greatest, 0, 0, 0,
- * a copy of the first segment, the pages of the first eight 16-key groups}, per segment {source
- * (0 prefix pages, 1 own pages, 2 own rows), whether every row sees all its keys, first page number or
- * first row, keys, position of key 0, first tile, end tile, first row, end row, 0, 0, 0}, per merged row {row, then for up to two groups of partial
+ * a copy of the first segment, the first eight groups}, per segment {source
+ * (0 prefix pages, 1 own pages, 2 own rows), whether every row sees all its keys, first group (an
+ * index) or first row, keys, position of key 0, first tile, end tile, first row, end row, 0, 0, 0}, per merged row {row, then for up to two groups of partial
  * results: first partial row, count, distance between them, and 0}, per token its position, and the
- * page numbers.  words NULL: only *count. */
+ * groups: each 16 keys of a page, as its first pool row of KV head 0 over 16; a source's filled up to
+ * whole 64-key tiles.  words NULL: only *count. */
 int qattn_shared_plan_describe(const qattn_shared_desc* desc, int32_t* words, int64_t capacity, int64_t* count,
                                qattn_shared_info* info);
 

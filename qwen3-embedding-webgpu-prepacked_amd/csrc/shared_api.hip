@@ -35,7 +35,8 @@ int check_kv_cache(qattn_ctx* ctx, const qattn_kv_cache* c, bool needs_pages) {
   if (!needs_pages) return QATTN_OK;
   if (c->page_size < 16 || c->page_size > 4096 || (c->page_size & (c->page_size - 1)))
     return fail(ctx, QATTN_EINVAL, "page_size %d: a power of two in [16, 4096]", c->page_size);
-  if (c->pages < 1) return fail(ctx, QATTN_EINVAL, "pages %d: at least 1", c->pages);
+  if (c->pages < 1 || (int64_t)c->pages * c->page_size * c->kv_heads >= (int64_t)1 << 35)
+    return fail(ctx, QATTN_EINVAL, "pages %d: at least 1, pages*page_size*kv_heads below 2^35", c->pages);
   if (!c->k || !c->v || !aligned16(c->k) || !aligned16(c->v))
     return fail(ctx, QATTN_EINVAL, "cache k/v NULL or not 16-byte aligned");
   if (c->format != QATTN_KV_16BIT && (!c->k_scale || !c->v_scale || !aligned16(c->k_scale) || !aligned16(c->v_scale)))
@@ -320,7 +321,7 @@ int install_shared_plan(qattn_shared_run* run, const qattn_shared_desc& d) {
   const size_t segs = put(plan.segs.data(), plan.segs.size() * sizeof(SharedSeg));
   const size_t merges = put(plan.merges.data(), plan.merges.size() * sizeof(SharedMerge));
   const size_t positions = put(plan.positions.data(), plan.positions.size() * sizeof(int32_t));
-  const size_t pages = put(plan.pages.data(), plan.pages.size() * sizeof(int32_t));
+  const size_t groups = put(plan.groups.data(), plan.groups.size() * sizeof(int32_t));
   DeviceGuard g(ctx->device);
   const int next = run->cur < 0 ? 0 : run->cur ^ 1;
   if (run->cur >= 0 && (rc = retire_shared(run, run->cur))) return rc;
@@ -362,7 +363,7 @@ int install_shared_plan(qattn_shared_run* run, const qattn_shared_desc& d) {
   p.segs = reinterpret_cast<const SharedSeg*>(image + segs);
   p.merges = reinterpret_cast<const SharedMerge*>(image + merges);
   p.positions = reinterpret_cast<const int32_t*>(image + positions);
-  p.pages = reinterpret_cast<const int32_t*>(image + pages);
+  p.groups = reinterpret_cast<const int32_t*>(image + groups);
   p.part_o = static_cast<float*>(run->partials);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + values * d.cache.head_dim);
   p.n_items = (int32_t)plan.items.size();
@@ -493,9 +494,9 @@ int qattn_shared_plan_describe(const qattn_shared_desc* desc, int32_t* words, in
   }
   if (rc) return rc;
   const int32_t head[8] = {(int32_t)plan.items.size(), (int32_t)plan.segs.size(), (int32_t)plan.merges.size(),
-                           (int32_t)plan.positions.size(), (int32_t)plan.pages.size(), 0, 0, 0};
+                           (int32_t)plan.positions.size(), (int32_t)plan.groups.size(), 0, 0, 0};
   *count = 8 + (int64_t)plan.items.size() * 32 + (int64_t)plan.segs.size() * 12 + (int64_t)plan.merges.size() * 8 +
-           (int64_t)plan.positions.size() + (int64_t)plan.pages.size();
+           (int64_t)plan.positions.size() + (int64_t)plan.groups.size();
   if (info) *info = plan.info;
   if (!words) return QATTN_OK;
   if (capacity < *count) return fail(nullptr, QATTN_EINVAL, "capacity %lld < %lld words", (long long)capacity, (long long)*count);
@@ -508,7 +509,7 @@ int qattn_shared_plan_describe(const qattn_shared_desc* desc, int32_t* words, in
   put(plan.segs.data(), plan.segs.size() * sizeof(SharedSeg));
   put(plan.merges.data(), plan.merges.size() * sizeof(SharedMerge));
   put(plan.positions.data(), plan.positions.size() * sizeof(int32_t));
-  put(plan.pages.data(), plan.pages.size() * sizeof(int32_t));
+  put(plan.groups.data(), plan.groups.size() * sizeof(int32_t));
   return QATTN_OK;
 }
 

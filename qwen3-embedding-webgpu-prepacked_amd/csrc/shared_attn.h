@@ -22,22 +22,24 @@ enum SharedSource { kPrefixPages = 0, kOwnPages = 1, kOwnRows = 2 };
 enum SharedKind { kTall = 0, kFlat = 1 };
 
 // Tiles tile_begin .. tile_end - 1 (of the item kind's size) of `keys` keys, seen by rows row_begin ..
-// row_end - 1 only.  base: the source's first page number (an index into the plan's list) or row.  whole:
-// every row of the item sees every key of these tiles.
+// row_end - 1 only.  base: where the source's groups begin in the plan's list, or its first row.  A group is 16
+// keys of a page: its number times 16 is the pool row (of KV head 0) of the first; a source's list is
+// filled up to whole 64-key tiles with its last group.  whole: every row of the item sees every key of
+// these tiles.
 struct SharedSeg {
   int32_t source, whole, base, keys, position, tile_begin, tile_end, row_begin, row_end;
   int32_t pad[3];
 };
 // Rows row0 .. row0 + rows - 1 over the tiles of segments seg_begin .. seg_end - 1.  Results go to the output
-// (part < 0) or, unnormalised, to partial rows part, part + 1, ...  The first segment, and the pages of the
-// first tiles' 16-key groups (tall: four, flat: two for each wavefront's first tile), come with the item, so
-// that a workgroup asks for its first keys after one dependent load.
+// (part < 0) or, unnormalised, to partial rows part, part + 1, ...  The first segment, and the groups of the
+// first tiles (tall: one for each wavefront, flat: two for each wavefront's first tile), come with the item,
+// so that a workgroup asks for its first keys after one dependent load.
 struct SharedItem {
   int32_t row0, rows, seg_begin, seg_end, part, tiles, kind;
   int32_t least, greatest;  // query positions among the rows
   int32_t pad[3];
   SharedSeg seg;
-  int32_t page[8];
+  int32_t group[8];
 };
 // A row whose results are merged: `count` partial rows from `first` on, `step` apart, in two groups.
 struct SharedMerge {
@@ -54,7 +56,7 @@ struct SharedPlan {
   std::vector<SharedSeg> segs;
   std::vector<SharedMerge> merges;
   std::vector<int32_t> positions;  // of each query
-  std::vector<int32_t> pages;
+  std::vector<int32_t> groups;
   int64_t partial_rows = 0;
   int32_t most_parts = 0;  // partial rows of a merged row, at most
   qattn_shared_info info{};
@@ -73,7 +75,7 @@ struct SharedParams {
   const SharedSeg* segs;
   const SharedMerge* merges;
   const int32_t* positions;
-  const int32_t* pages;
+  const int32_t* groups;
   float* part_o;                // [partial row][kv_heads][head_dim]
   float2* part_ml;              // [partial row][kv_heads]: the row's reference (log2) and sum
   int32_t n_items, n_merges, most_parts, kv_heads, group, page_shift;

@@ -51,14 +51,6 @@ __device__ inline f4 mfma16(u32x4 a, u32x4 b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(T8, a), __builtin_bit_cast(T8, b), c, 0, 0, 0);
 }
 
-// Raw buffer over `bytes` bytes: loads past its end give zeros.
-__device__ inline __amdgpu_buffer_rsrc_t buffer(const void* base, int bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00020000);
-}
-__device__ inline u32x4 load16(__amdgpu_buffer_rsrc_t rs, uint32_t offset) {
-  return __builtin_amdgcn_raw_buffer_load_b128(rs, offset, 0, 0);
-}
-
 // Combined with the other half-wavefront (lane ^ 32), and with the other 16-lane rows (lane ^ 16, ^ 32).
 __device__ inline float half_max(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -79,13 +71,13 @@ __device__ inline float rows_sum(float x) {
 __device__ inline SharedSeg seg_at(const const_i32* w) {
   return SharedSeg{w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7], w[8], {0, 0, 0}};
 }
-// All of an item but its pages.
+// All of an item but its groups.
 __device__ inline SharedItem item_at(const SharedParams& p, int i) {
   const const_i32* w = (const const_i32*)(p.items + i);
   return SharedItem{w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7], w[8], {0, 0, 0}, seg_at(w + 12), {}};
 }
-__device__ inline int item_page(const SharedParams& p, int i, int group) {
-  return ((const const_i32*)(p.items + i))[24 + group];
+__device__ inline int item_group(const SharedParams& p, int i, int which) {
+  return ((const const_i32*)(p.items + i))[24 + which];
 }
 
 // The tiles of an item one after another, through its segments.
@@ -107,37 +99,39 @@ struct Cursor {
   }
 };
 
-// Where the rows of an aligned group of keys (within one page: groups are of 16 keys at most) lie.
-struct Group {
-  const char* base[2];   // key `first`'s row of K, V for this KV head
-  const float* scale[2];
-  int count;             // keys of the group that exist
-  uint32_t stride;       // bytes between rows
-};
-__device__ inline int page_at(const SharedParams& p, const SharedSeg& s, int first) {
-  return s.source == kOwnRows ? 0 : ((const const_i32*)p.pages)[s.base + (min(first, s.keys - 1) >> p.page_shift)];
-}
+// This KV head's keys: uniform pointers, K's and V's.
 template <int FORMAT, int DIM>
-__device__ inline Group group_at(const SharedParams& p, const SharedSeg& s, int first, int size, int page, int kvh) {
-  Group g;
-  g.count = min(max(s.keys - first, 0), size);
-  if (s.source == kOwnRows) {
+struct Keys {
+  static constexpr bool kCodes = FORMAT != QATTN_KV_16BIT;
+  static constexpr int kBytes = kCodes ? DIM : 2 * DIM;  // of a pool row
+  const char* cache[2];
+  const char* scale[2];
+  const char* rows[2];
+  uint32_t stride[2];  // bytes between rows
+  __device__ Keys(const SharedParams& p, int kvh) {
+    const int64_t head = (int64_t)kvh << p.page_shift;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      g.base[i] = reinterpret_cast<const char*>(p.rows[i] + ((int64_t)s.base + first) * p.row_stride[i] + kvh * DIM);
-      g.scale[i] = nullptr;
-    }
-  } else {
-    constexpr int kRow = FORMAT == QATTN_KV_16BIT ? 2 * DIM : DIM;
-    const int in_page = first & ((1 << p.page_shift) - 1);
-    const int64_t row = (((int64_t)page * p.kv_heads + kvh) << p.page_shift) + in_page;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      g.base[i] = p.cache[i] + row * kRow;
-      g.scale[i] = p.cache_scale[i] + row;
+      cache[i] = p.cache[i] + head * kBytes;
+      scale[i] = reinterpret_cast<const char*>(p.cache_scale[i] + head);
+      rows[i] = reinterpret_cast<const char*>(p.rows[i] + kvh * DIM);
+      stride[i] = (uint32_t)p.row_stride[i] * 2;
     }
   }
-  return g;
+  // Byte `offset` of a group (its 16 rows lie together; offset below their bytes), and of its scales.
+  __device__ const char* in_group(int i, uint32_t group, uint32_t offset) const {
+    return cache[i] + ((uint64_t)group * (16 * kBytes) | offset);
+  }
+  __device__ float scale_of(int i, uint32_t group, uint32_t row) const {
+    return *reinterpret_cast<const float*>(scale[i] + ((uint64_t)group * 64 | 4 * row));
+  }
+  __device__ const char* row(int i, uint32_t row, uint32_t offset) const {
+    return rows[i] + ((uint64_t)row * stride[i] + offset);
+  }
+};
+// The group of key `first` of a segment, loaded as a vector: it is waited for with the tile's other loads.
+__device__ inline uint32_t group_of(const SharedParams& p, const SharedSeg& s, int first, int zero) {
+  return s.source == kOwnRows ? 0 : (uint32_t)p.groups[zero + s.base + (first >> 4)];
 }
 
 // 16 codes as two 16-byte chunks of 16-bit elements.
@@ -170,14 +164,20 @@ __device__ inline bool drop_nonfinite(u32x4& chunk) {
 }
 // Elements d .. d + 3 of key `key`'s V.
 template <bool BF16, int FORMAT, int DIM>
-__device__ inline f4 value_at(const SharedParams& p, const SharedSeg& s, int key, int kvh, int d) {
-  const Group g = group_at<FORMAT, DIM>(p, s, key, 1, page_at(p, s, key), kvh);
+__device__ inline f4 value_at(const SharedParams& p, const Keys<FORMAT, DIM>& keys, const SharedSeg& s, int key, int d) {
   u32x2 x;
-  if (FORMAT == QATTN_KV_16BIT || s.source == kOwnRows) {
-    x = *reinterpret_cast<const u32x2*>(g.base[1] + 2 * d);
+  if (s.source == kOwnRows) {
+    x = *reinterpret_cast<const u32x2*>(keys.row(1, s.base + key, 2 * d));
   } else {
-    const uint32_t codes = *reinterpret_cast<const uint32_t*>(g.base[1] + d);
-    x = FORMAT == QATTN_KV_E4M3 ? e4m3_elems<BF16>(codes, *g.scale[1]) : int8_elems<BF16>(codes, *g.scale[1]);
+    const uint32_t group = group_of(p, s, key, 0), row = key & 15;
+    const char* at = keys.in_group(1, group, row * keys.kBytes + (keys.kCodes ? d : 2 * d));
+    if constexpr (FORMAT == QATTN_KV_16BIT) {
+      x = *reinterpret_cast<const u32x2*>(at);
+    } else {
+      const uint32_t codes = *reinterpret_cast<const uint32_t*>(at);
+      const float scale = keys.scale_of(1, group, row);
+      x = FORMAT == QATTN_KV_E4M3 ? e4m3_elems<BF16>(codes, scale) : int8_elems<BF16>(codes, scale);
+    }
   }
   return f4{widen<BF16, 0>(x[0]), widen<BF16, 1>(x[0]), widen<BF16, 0>(x[1]), widen<BF16, 1>(x[1])};
 }
@@ -185,8 +185,8 @@ __device__ inline float nonfinite(float v, bool seen) { return seen && !(fabsf(v
 // Calls add(value, seen) for every key of the item's tiles first, first + step, ... (of `size` keys) that not
 // all rows see: value(d) is elements d .. d + 3 of its V, seen whether row `row` at position `at` sees it.
 template <bool BF16, int FORMAT, int DIM, class Add>
-__device__ inline void each_nonfinite(const SharedParams& p, const SharedItem& it, int kvh, int row, int at, int size, int first,
-                                      int step, Add add) {
+__device__ inline void each_nonfinite(const SharedParams& p, const Keys<FORMAT, DIM>& keys, const SharedItem& it, int row, int at,
+                                      int size, int first, int step, Add add) {
   Cursor c(p, it);
   c.advance(first);
   for (int t = first;;) {
@@ -195,7 +195,7 @@ __device__ inline void each_nonfinite(const SharedParams& p, const SharedItem& i
       const int mine = row >= s.row_begin && row < s.row_end ? at : -1;
       for (int key = c.tile * size; key < min(s.keys, (c.tile + 1) * size); ++key) {
         const int pos = s.position + key;
-        add([&](int d) { return value_at<BF16, FORMAT, DIM>(p, s, key, kvh, d); },
+        add([&](int d) { return value_at<BF16, FORMAT, DIM>(p, keys, s, key, d); },
             pos <= mine && (p.mask == QATTN_MASK_CAUSAL || pos < p.prefix || pos > mine - p.window));
       }
     }
@@ -221,92 +221,62 @@ struct Tall {
   __device__ static uint32_t k_at(int r, int c) { return r * kRow + ((c ^ (DIM == 128 ? r & 15 : (r >> 1) & 7)) << 4); }
   __device__ static uint32_t v_at(int r, int c) { return r * kRow + ((c ^ (DIM == 128 ? (r & 3) << 2 : (r & 2) << 1)) << 4); }
 
-  // Where the 16 rows of a tile that this wavefront loads lie: within one page.  Rows of keys past the last
-  // are read as they are, if a page holds them (their tile is not whole: their scores are masked, and
-  // infinities and NaN of their V taken out), or as the last key's.
+  // Where the 16 rows of a tile that this wavefront loads lie.  Rows of keys past the last are read as they
+  // are, if a page holds them (their tile is not whole: their scores are masked, and infinities and NaN of
+  // their V taken out), or as the last key's.
   struct Spot {
-    int source, keys;  // keys from the first of the 16 rows on: <= 0 if none of them exist
-    int64_t row;       // of the pool (all KV heads' rows), or of p.rows
+    uint32_t group;  // of pages
+    int row, left;   // of p.rows: the first, and how many further there are
+    bool rows;
   };
-  // `page`: its page number, for pages.
-  __device__ static Spot spot(const SharedParams& p, const SharedSeg& s, int tile, int page, int kvh, int wave) {
-    const int first = tile * kTallKeys + 16 * wave;
-    if (s.source == kOwnRows) return Spot{s.source, s.keys - first, (int64_t)s.base + first};
-    const int in_page = first & ((1 << p.page_shift) - 1);
-    return Spot{s.source, s.keys - first, (((int64_t)page * p.kv_heads + kvh) << p.page_shift) + in_page};
-  }
-  // The page of that spot, as a vector load: it is waited for with the tile's other loads.
-  __device__ static int page_of(const SharedParams& p, const SharedSeg& s, int tile, int wave, int zero) {
-    if (s.source == kOwnRows) return 0;
-    return p.pages[zero + s.base + (min(tile * kTallKeys + 16 * wave, s.keys - 1) >> p.page_shift)];
-  }
 
   u32x4 raw[2][kLoads16];
   float scale[2][kCodes ? kLoads8 : 1];
 
   // K (I = 0) or V (1) of a tile into registers.
   template <int I>
-  __device__ void load(const SharedParams& p, const Spot& at, int kvh, int lane) {
-    if (at.source == kOwnRows) {
-      // at.row + a lane's row may be past the last key: that one's row instead.
-      const char* rows = reinterpret_cast<const char*>(p.rows[I] + kvh * DIM) + (lane % kChunks16) * 16;
-      const int64_t stride = p.row_stride[I] * 2;
+  __device__ void load(const Keys<FORMAT, DIM>& keys, const Spot& at, int lane) {
+    if (at.rows) {
 #pragma unroll
       for (int j = 0; j < kLoads16; ++j)
-        raw[I][j] = *reinterpret_cast<const u32x4*>(rows + (at.row + min(j * kRows16 + lane / kChunks16, at.keys - 1)) * stride);
+        raw[I][j] = *reinterpret_cast<const u32x4*>(
+            keys.row(I, at.row + min(j * kRows16 + lane / kChunks16, at.left), lane % kChunks16 * 16));
     } else {
-      constexpr int kBytes = kCodes ? DIM : kRow;
-      const char* rows = p.cache[I] + at.row * kBytes;
+      const char* src = keys.in_group(I, at.group, lane * 16);
 #pragma unroll
-      for (int j = 0; j < (kCodes ? kLoads8 : kLoads16); ++j)
-        raw[I][j] = *reinterpret_cast<const u32x4*>(rows + (uint32_t)(lane * 16 + j * 1024));
+      for (int j = 0; j < (kCodes ? kLoads8 : kLoads16); ++j) raw[I][j] = *reinterpret_cast<const u32x4*>(src + j * 1024);
       if constexpr (kCodes) {
-        const float* scales = p.cache_scale[I] + at.row;
 #pragma unroll
-        for (int j = 0; j < kLoads8; ++j) scale[I][j] = scales[(uint32_t)(lane / kChunks8 + j * kRows8)];
+        for (int j = 0; j < kLoads8; ++j) scale[I][j] = keys.scale_of(I, at.group, lane / kChunks8 + j * kRows8);
       }
     }
   }
 
-  // The loaded K into LDS as 16-bit elements.
-  __device__ void store_k(char* k, bool rows, int wave, int lane) {
-    if (!kCodes || rows) {
-#pragma unroll
-      for (int j = 0; j < kLoads16; ++j)
-        *reinterpret_cast<u32x4*>(k + k_at(16 * wave + j * kRows16 + lane / kChunks16, lane % kChunks16)) = raw[0][j];
-    } else {
-#pragma unroll
-      for (int j = 0; j < kLoads8; ++j) {
-        const int r = 16 * wave + j * kRows8 + lane / kChunks8, c = 2 * (lane % kChunks8);
-        u32x4 x[2];
-        expand<BF16, FORMAT>(raw[0][j], scale[0][kCodes ? j : 0], x);
-        *reinterpret_cast<u32x4*>(k + k_at(r, c)) = x[0];
-        *reinterpret_cast<u32x4*>(k + k_at(r, c + 1)) = x[1];
-      }
-    }
-  }
-  // V likewise.  partly: some row sees only part of the tile; returns whether this wavefront's part had
-  // infinities or NaN then.
-  __device__ bool store_v(char* v, bool rows, int wave, int lane, bool partly) {
+  // Half h of the loaded K (I = 0) or V (1) into LDS as 16-bit elements.  partly: infinities and NaN are
+  // taken out (of V, in tiles that some row sees only part of); returns whether this lane had any.
+  template <int I>
+  __device__ bool store(char* lds, bool rows, int wave, int lane, int h, bool partly) {
     bool any = false;
     const auto put = [&](int r, int c, u32x4 x) {
-      if (partly) any |= drop_nonfinite<BF16>(x);
-      *reinterpret_cast<u32x4*>(v + v_at(r, c)) = x;
+      if (I && partly) any |= drop_nonfinite<BF16>(x);
+      *reinterpret_cast<u32x4*>(lds + (I ? v_at(r, c) : k_at(r, c))) = x;
     };
     if (!kCodes || rows) {
 #pragma unroll
-      for (int j = 0; j < kLoads16; ++j) put(16 * wave + j * kRows16 + lane / kChunks16, lane % kChunks16, raw[1][j]);
+      for (int j = h * kLoads16 / 2; j < (h + 1) * kLoads16 / 2; ++j)
+        put(16 * wave + j * kRows16 + lane / kChunks16, lane % kChunks16, raw[I][j]);
     } else {
+      constexpr int kEach = (kLoads8 + 1) / 2;
 #pragma unroll
-      for (int j = 0; j < kLoads8; ++j) {
+      for (int j = h * kEach; j < (h + 1) * kEach && j < kLoads8; ++j) {
         const int r = 16 * wave + j * kRows8 + lane / kChunks8, c = 2 * (lane % kChunks8);
         u32x4 x[2];
-        expand<BF16, FORMAT>(raw[1][j], scale[1][kCodes ? j : 0], x);
+        expand<BF16, FORMAT>(raw[I][j], scale[I][kCodes ? j : 0], x);
         put(r, c, x[0]);
         put(r, c + 1, x[1]);
       }
     }
-    return partly && __any(any);
+    return any;
   }
 };
 
@@ -336,11 +306,12 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
   struct Info {
     int whole, from, last, row_begin, row_end;  // from: position of its first key; last: of its segment's last
   };
-  Cursor ahead(p, it);  // the next K tile to ask for, its page on the way
+  const Keys<FORMAT, DIM> keys(p, kvh);
+  Cursor ahead(p, it);  // the next K tile to ask for, its group on the way
   T tile;
   int zero = 0;
   asm volatile("" : "+v"(zero));
-  int page = item_page(p, index, wave);
+  uint32_t group = item_group(p, index, wave);
   typename T::Spot spot{}, spot_v{};
   int asked = 0;
   bool whole_v = true;  // the V tile in registers
@@ -350,20 +321,20 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
   // K of the next tile, if there is one, and V of the tile before it.
   const auto ask_k = [&]() {
     if (asked == it.tiles) return;
-    spot = T::spot(p, ahead.seg, ahead.tile, __builtin_amdgcn_readfirstlane(page), kvh, wave);
-    tile.template load<0>(p, spot, kvh, lane);
     const SharedSeg& s = ahead.seg;
+    const int first = ahead.tile * kTallKeys + 16 * wave;
+    spot.rows = s.source == kOwnRows;
+    spot.group = group;
+    spot.row = s.base + min(first, s.keys - 1);
+    spot.left = max(s.keys - 1 - first, 0);
+    tile.template load<0>(keys, spot, lane);
     next = Info{s.whole, s.position + ahead.tile * kTallKeys, s.position + s.keys - 1, s.row_begin, s.row_end};
     if (++asked < it.tiles) {
       ahead.advance(1);
-      page = T::page_of(p, ahead.seg, ahead.tile, wave, zero);
+      group = group_of(p, ahead.seg, ahead.tile * kTallKeys + 16 * wave, zero);
     }
   };
-  const auto ask_v = [&](bool whole) {
-    tile.template load<1>(p, spot_v, kvh, lane);
-    whole_v = whole;
-  };
-  const auto keep_v = [&](int t) { found |= tile.store_v(v_buf(t), spot_v.source == kOwnRows, wave, lane, !whole_v); };
+  const auto ask_v = [&]() { tile.template load<1>(keys, spot_v, lane); };
 
   ask_k();  // K(0)
   // Q (B operand of S^T = K Q^T): this lane's row, dims 16 st + 8 hl .. + 7 at step st.
@@ -423,13 +394,16 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
     pf[r >> 3][(r & 7) >> 1] = narrow2<BF16>(p0, p1);
   };
 
-  tile.store_k(k_buf(0), spot.source == kOwnRows, wave, lane);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) tile.template store<0>(k_buf(0), spot.rows, wave, lane, h, false);
   now = next;
   spot_v = spot;
-  ask_v(now.whole);
+  whole_v = now.whole;
+  ask_v();
   ask_k();
   // Scores of tile t, masked.
-  const auto scores = [&](const Info& cur, const char* k, f16x (&sc)[2]) {
+  // (beside(i): other work, issued after product i.)
+  const auto scores = [&](const Info& cur, const char* k, f16x (&sc)[2], auto beside) {
     // Rows lq and lq + 32, chunk 2 st + hl: its swizzled place is 2 st xor'ed onto chunk hl's.  (Formed here:
     // hoisted, the addresses of all steps would take a register each.)
     uint32_t place = T::k_at(lq, hl) - lq * T::kRow;
@@ -447,6 +421,7 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
       __builtin_amdgcn_sched_barrier(0);
       sc[i & 1] = mfma32<BF16>(a[i % kAhead], q[i >> 1], i < 2 ? f16x{} : sc[i & 1]);
       if (i + kAhead < 2 * kSteps) a[i % kAhead] = k_frag(i + kAhead);
+      beside(i);
     }
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_setprio(0);
@@ -477,14 +452,31 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
     m = moved;
     return shrink;
   };
-  const auto put_next = [&](int t) {
-    keep_v(t);
-    if (t + 1 < it.tiles) {
-      tile.store_k(k_buf(t + 1), spot.source == kOwnRows, wave, lane);
-      now = next;
-      spot_v = spot;
-      ask_v(now.whole);
-      ask_k();
+  // Beside the products of S(t): V(t) and K(t + 1) go to LDS, V(t + 1) and K(t + 2) are asked for.
+  const auto move_on = [&](int t, int i) {
+    constexpr int kEvery = kSteps / 4;
+    if (i % kEvery) return;
+    const bool more = t + 1 < it.tiles;
+    switch (i / kEvery) {
+      case 1: found |= tile.template store<1>(v_buf(t), spot_v.rows, wave, lane, 0, !whole_v); break;
+      case 2: found |= tile.template store<1>(v_buf(t), spot_v.rows, wave, lane, 1, !whole_v); break;
+      case 3:
+        if (more) tile.template store<0>(k_buf(t + 1), spot.rows, wave, lane, 0, false);
+        break;
+      case 4:
+        if (more) tile.template store<0>(k_buf(t + 1), spot.rows, wave, lane, 1, false);
+        break;
+      case 5:
+        if (more) {
+          now = next;
+          spot_v = spot;
+          whole_v = now.whole;
+          ask_v();
+        }
+        break;
+      case 6:
+        if (more) ask_k();
+        break;
     }
   };
 
@@ -492,9 +484,8 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
   {
     __syncthreads();
     const Info cur = now;
-    put_next(0);
     f16x sc[2];
-    scores(cur, k_buf(0), sc);
+    scores(cur, k_buf(0), sc, [&](int i) { move_on(0, i); });
     refer(sc);
     const float ref = m == kNone ? 0.f : m;
 #pragma unroll
@@ -504,9 +495,8 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
     // K(t) and V(t - 1) are in LDS, and every wavefront is done with the other buffers.
     __syncthreads();
     const Info cur = now;
-    put_next(t);
     f16x sc[2];
-    scores(cur, k_buf(t), sc);
+    scores(cur, k_buf(t), sc, [&](int i) { move_on(t, i); });
     const float shrink = refer(sc);
     const float ref = m == kNone ? 0.f : m;
     // The weights beside the matrix cores' work on the tile before.
@@ -529,10 +519,10 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
   }
   __syncthreads();
   add_pv(v_buf(it.tiles - 1), pf, nothing);
-  if (found && lane == 0) *dropped = 1;
+  if (found) *dropped = 1;
   __syncthreads();
   if (*dropped)
-    each_nonfinite<BF16, FORMAT, DIM>(p, it, kvh, row, at, kTallKeys, 0, 1, [&](auto value, bool seen) {
+    each_nonfinite<BF16, FORMAT, DIM>(p, keys, it, row, at, kTallKeys, 0, 1, [&](auto value, bool seen) {
 #pragma unroll
       for (int db = 0; db < kBlocks; ++db)
 #pragma unroll
@@ -592,33 +582,35 @@ struct Flat {
   u32x4 k[2][kSteps], v[2][kLoads16];
   float ks[2], vs[2][kCodes ? kLoads8 : 1];
 
-  __device__ void load(const SharedParams& p, const SharedSeg& s, int tile, const int (&page)[2], int kvh, int lane) {
+  // Tile `tile` of segment s, whose two groups are `group`.  (Rows past the last key: as in Tall.)
+  __device__ void load(const Keys<FORMAT, DIM>& keys, const SharedSeg& s, int tile, const uint32_t (&group)[2], int lane) {
     const int key = lane & 15, c = lane >> 4;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      const Group g = group_at<FORMAT, DIM>(p, s, tile * kFlatKeys + 16 * b, 16, page[b], kvh);
-      if (!kCodes || s.source == kOwnRows) {
-        uint32_t stride[2];
+      if (s.source == kOwnRows) {
+        const int first = tile * kFlatKeys + 16 * b, last = s.keys - 1;
+        const char* src = keys.row(0, s.base + min(first + key, last), 32 * c);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) stride[i] = s.source == kOwnRows ? (uint32_t)p.row_stride[i] * 2 : kRow;
-        const auto bk = buffer(g.base[0], g.count ? (g.count - 1) * stride[0] + kRow : 0);
-        const auto bv = buffer(g.base[1], g.count ? (g.count - 1) * stride[1] + kRow : 0);
-#pragma unroll
-        for (int st = 0; st < kSteps; ++st) k[b][st] = load16(bk, key * stride[0] + 128 * (st >> 1) + 32 * c + 16 * (st & 1));
+        for (int st = 0; st < kSteps; ++st) k[b][st] = *reinterpret_cast<const u32x4*>(src + 128 * (st >> 1) + 16 * (st & 1));
 #pragma unroll
         for (int j = 0; j < kLoads16; ++j)
-          v[b][j] = load16(bv, (j * kRows16 + lane / kChunks16) * stride[1] + (lane % kChunks16) * 16);
+          v[b][j] = *reinterpret_cast<const u32x4*>(
+              keys.row(1, s.base + min(first + j * kRows16 + lane / kChunks16, last), lane % kChunks16 * 16));
       } else {
-        const auto bk = buffer(g.base[0], g.count * DIM), bv = buffer(g.base[1], g.count * DIM);
-        const auto sk = buffer(g.scale[0], g.count * 4), sv = buffer(g.scale[1], g.count * 4);
+        const char* src = keys.in_group(0, group[b], key * keys.kBytes + (kCodes ? 16 : 32) * c);
+        const char* rows = keys.in_group(1, group[b], lane * 16);
+        if constexpr (kCodes) {
 #pragma unroll
-        for (int h = 0; h < DIM / 64; ++h) k[b][h] = load16(bk, key * DIM + 64 * h + 16 * c);
-        ks[b] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(sk, key * 4, 0, 0));
+          for (int h = 0; h < DIM / 64; ++h) k[b][h] = *reinterpret_cast<const u32x4*>(src + 64 * h);
+          ks[b] = keys.scale_of(0, group[b], key);
+        } else {
 #pragma unroll
-        for (int j = 0; j < kLoads8; ++j) {
-          v[b][j] = load16(bv, j * 1024 + lane * 16);
-          vs[b][kCodes ? j : 0] =
-              __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(sv, (j * kRows8 + lane / kChunks8) * 4, 0, 0));
+          for (int st = 0; st < kSteps; ++st) k[b][st] = *reinterpret_cast<const u32x4*>(src + 128 * (st >> 1) + 16 * (st & 1));
+        }
+#pragma unroll
+        for (int j = 0; j < (kCodes ? kLoads8 : kLoads16); ++j) {
+          v[b][j] = *reinterpret_cast<const u32x4*>(rows + j * 1024);
+          if constexpr (kCodes) vs[b][j] = keys.scale_of(1, group[b], j * kRows8 + lane / kChunks8);
         }
       }
     }
@@ -693,13 +685,24 @@ __device__ inline void flat_item(const SharedParams& p, const SharedItem& it, in
   // V^T: the 16 lanes of group c read keys 4 c .. 4 c + 3 (and 16 more) by the 16 dims of a block.
   const int vr = 4 * c + (n >> 2);
 
+  const Keys<FORMAT, DIM> keys(p, kvh);
   if (wave < it.tiles) {
     bool found = false;  // infinities or NaN were dropped from V
     Cursor now(p, it);
     now.advance(wave);
     T tile;
-    int page[2] = {item_page(p, index, 2 * wave), item_page(p, index, 2 * wave + 1)};
-    tile.load(p, now.seg, now.tile, page, kvh, lane);
+    uint32_t group[2] = {(uint32_t)item_group(p, index, 2 * wave), (uint32_t)item_group(p, index, 2 * wave + 1)};
+    tile.load(keys, now.seg, now.tile, group, lane);
+    // The next tile's groups are on the way while this one is worked on.
+    int zero = 0;
+    asm volatile("" : "+v"(zero));
+    Cursor ahead = now;
+    const auto ask_groups = [&]() {
+      ahead.advance(4);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) group[b] = group_of(p, ahead.seg, ahead.tile * kFlatKeys + 16 * b, zero);
+    };
+    if (wave + 4 < it.tiles) ask_groups();
     for (int t = wave; t < it.tiles; t += 4) {
       const SharedSeg s = now.seg;
       const int first = now.tile * kFlatKeys, from = s.position + first;
@@ -714,9 +717,9 @@ __device__ inline void flat_item(const SharedParams& p, const SharedItem& it, in
       const bool part = !s.whole;
       found |= tile.store(lds, s, lane, part);
       if (t + 4 < it.tiles) {
-        now.advance(4);
-        for (int b = 0; b < 2; ++b) page[b] = page_at(p, now.seg, now.tile * kFlatKeys + 16 * b);
-        tile.load(p, now.seg, now.tile, page, kvh, lane);
+        now = ahead;
+        tile.load(keys, now.seg, now.tile, group, lane);
+        if (t + 8 < it.tiles) ask_groups();
       }
       const bool mine = row >= s.row_begin && row < s.row_end;
       const int limit = min(mine ? at : -1, s.position + s.keys - 1);
@@ -758,7 +761,7 @@ __device__ inline void flat_item(const SharedParams& p, const SharedItem& it, in
       }
     }
     if (found)
-      each_nonfinite<BF16, FORMAT, DIM>(p, it, kvh, row, at, kFlatKeys, wave, 4, [&](auto value, bool seen) {
+      each_nonfinite<BF16, FORMAT, DIM>(p, keys, it, row, at, kFlatKeys, wave, 4, [&](auto value, bool seen) {
 #pragma unroll
         for (int db = 0; db < kBlocks; ++db) {
           const f4 x = value(16 * db + 4 * c);

@@ -60,10 +60,19 @@ class Planner {
 
   void read() {
     int32_t first_row = 0;
-    size_t page = 0;
     const int32_t page_size = std::max(1, d_.cache.page_size);
-    const auto pages_of = [&](int32_t keys) { return (size_t)((keys + (int64_t)page_size - 1) / page_size); };
-    if (d_.prefix_len) plan_->pages.assign(d_.prefix_pages, d_.prefix_pages + pages_of(d_.prefix_len));
+    const int32_t page_groups = d_.cache.kv_heads * (page_size / 16);
+    // Appends the groups of `keys` keys, and takes `pages` past their pages.
+    const auto add_groups = [&](const int32_t*& pages, int32_t keys) {
+      const int32_t groups = (int32_t)(((int64_t)keys + 15) / 16);
+      for (int32_t i = 0; i < groups; ++i)
+        plan_->groups.push_back(pages[i / (page_size / 16)] * page_groups + i % (page_size / 16));
+      while (groups && plan_->groups.size() % 4) plan_->groups.push_back(plan_->groups.back());
+      pages += ((int64_t)keys + page_size - 1) / page_size;
+    };
+    const int32_t* pages = d_.prefix_pages;
+    if (d_.prefix_len) add_groups(pages, d_.prefix_len);
+    pages = d_.own_pages;
     plan_->positions.resize(d_.cu_q[d_.nseq]);
     qattn_shared_info& info = plan_->info;
     info.tokens = d_.cu_q[d_.nseq];
@@ -72,10 +81,8 @@ class Planner {
       Sequence s{d_.cu_q[i], d_.cu_q[i + 1] - d_.cu_q[i], d_.own_len[i], 0, kOwnRows};
       if (d_.own_pages) {
         s.source = kOwnPages;
-        s.base = (int32_t)plan_->pages.size();
-        const size_t n = pages_of(s.keys);
-        plan_->pages.insert(plan_->pages.end(), d_.own_pages + page, d_.own_pages + page + n);
-        page += n;
+        s.base = (int32_t)plan_->groups.size();
+        add_groups(pages, s.keys);
       } else {
         s.base = first_row;
         first_row += s.keys;
@@ -321,7 +328,7 @@ class Planner {
           end -= n;
         }
         it.seg_end = (int32_t)plan_->segs.size();
-        first_pages(&it);
+        first_groups(&it);
         items.emplace_back(b.cost(it.tiles), it);
       }
     }
@@ -333,15 +340,15 @@ class Planner {
     plan_->info.partial_rows = plan_->partial_rows;
   }
 
-  // The item's own copy of its first segment and of the pages of its first tiles.
-  void first_pages(SharedItem* it) const {
+  // The item's own copy of its first segment and of the groups of its first tiles.
+  void first_groups(SharedItem* it) const {
     it->seg = plan_->segs[it->seg_begin];
     const int tile = it->kind == kTall ? kTallKeys : kFlatKeys;
     int32_t seg = it->seg_begin, at = it->seg.tile_begin;
     for (int i = 0; i < 8; ++i) {
       const SharedSeg& s = plan_->segs[seg];
       const int32_t first = at * tile + 16 * i % tile;
-      it->page[i] = s.source == kOwnRows ? 0 : plan_->pages[s.base + std::min(first, s.keys - 1) / d_.cache.page_size];
+      it->group[i] = s.source == kOwnRows ? 0 : plan_->groups[s.base + first / 16];
       if ((16 * (i + 1)) % tile) continue;
       if (++at < s.tile_end) continue;
       if (++seg == it->seg_end) break;  // no further tile

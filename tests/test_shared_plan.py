@@ -31,8 +31,15 @@ def check_plan(qattn, prefix, queries, own, heads=16, kv=8, page=64, paged=True,
     own = np.asarray(own, np.int64)
     position = np.concatenate([prefix + n - m + np.arange(m) for m, n in zip(queries, own)] + [np.zeros(0)]).astype(np.int64)
     assert np.array_equal(plan["positions"], np.maximum(position, -1))
-    assert np.array_equal(plan["pages"], order[:sum(need)])
-    first_page = np.cumsum([need[0]] + need[1:])[:-1] if paged and len(need) > 1 else None
+    # groups of 16 keys in page order, each source's filled up to whole tiles
+    tables = np.split(order[:sum(need)], np.cumsum(need)[:-1])
+    groups, first_group = [], []
+    for table, n in zip(tables, [prefix] + (list(own) if paged else [])):
+        first_group.append(len(groups))
+        k = np.arange(0, n, 16)
+        groups += list((table[k // page] * kv * page + k % page) // 16)
+        groups += [groups[-1]] * (-len(groups) % 4) if n else []
+    assert np.array_equal(plan["groups"], groups)
     first_row = np.concatenate([[0], np.cumsum(own)])
     top = prefix + int(own.max(initial=0))
     counts = np.zeros((T * group, max(top, 1)), np.int16)  # visits of (row, key position)
@@ -46,9 +53,8 @@ def check_plan(qattn, prefix, queries, own, heads=16, kv=8, page=64, paged=True,
         segs = plan["segments"][s0:s1]
         assert sum(s[6] - s[5] for s in segs) == tiles and s1 > s0
         assert np.array_equal(it[12:24], segs[0])
-        groups = [(s, k) for s in segs for k in range(s[5] * TILE[kind], s[6] * TILE[kind], 16)][:8]
-        for (s, k), got in zip(groups, it[24:]):
-            assert got == (0 if s[0] == 2 else plan["pages"][s[2] + min(k, s[3] - 1) // page])
+        for (s, k), got in zip([(s, k) for s in segs for k in range(s[5] * TILE[kind], s[6] * TILE[kind], 16)], it[24:]):
+            assert got == (0 if s[0] == 2 else groups[s[2] + k // 16])
         for source, whole, base, keys, pos0, t0, t1, lo, hi in segs[:, :9]:
             assert 0 <= t0 < t1 <= -(-keys // TILE[kind])
             assert row0 <= lo < hi <= row0 + rows
@@ -58,7 +64,7 @@ def check_plan(qattn, prefix, queries, own, heads=16, kv=8, page=64, paged=True,
             else:
                 i = seq[lo // group]
                 assert (seq[np.arange(lo, hi) // group] == i).all() and keys == own[i] and pos0 == prefix
-                assert base == (first_page[i] if paged else first_row[i]) and source == (1 if paged else 2)
+                assert base == (first_group[1 + i] if paged else first_row[i]) and source == (1 if paged else 2)
                 sees = (r >= lo) & (r < hi)
             key = np.arange(t0 * TILE[kind], min(t1 * TILE[kind], keys))
             counts[np.ix_(r[sees], pos0 + key)] += 1
