@@ -434,7 +434,7 @@ typedef struct qattn_shared_desc {
 /* Tensors 16-byte aligned, strides multiples of 8 elements up to 2^24 and at least the heads' width;
  * page numbers in [0, pages); positions below 2^30; at most 2^22 rows (queries * q_heads / kv_heads).
  * The run plans the launch on the host, as qattn_run_create does: rows (query, head of the group) of
- * all sequences are stacked, so that a tile of prefix keys is read once for up to 128 rows; long key
+ * all sequences are stacked, so that a tile of prefix keys is read once for up to 256 rows; long key
  * ranges of few rows are spread over workgroups and their partial results merged by a second launch. */
 int qattn_shared_run_create(qattn_ctx* ctx, const qattn_shared_desc* desc, qattn_shared_run** out);
 /* Enqueues the launch.  Launches of one run must not overlap on the device: they share its workspace.
@@ -464,14 +464,14 @@ typedef struct qattn_shared_info {
 int qattn_shared_run_get_info(const qattn_shared_run* run, qattn_shared_info* info);
 /* Host-only planning (no device; 256 compute units): the plan as int32 words, the counts first:
  * {items, segments, merged rows, tokens, groups, 0, 0, 0}, then per item {first row, rows, first
- * segment, end segment, first partial row or -1, key tiles, kind (0: 128-row blocks over 64-key tiles,
- * 1: 16-row blocks over 32-key tiles), least query position, greatest, 0, 0, 0,
+ * segment, end segment, first partial row or -1, key tiles, kind (0, 1: blocks of 256, 128 rows over
+ * 128-key tiles, 2: of 16 rows over 32-key tiles), least query position, greatest, 0, 0, 0,
  * a copy of the first segment, the first eight groups}, per segment {source
  * (0 prefix pages, 1 own pages, 2 own rows), whether every row sees all its keys, first group (an
  * index) or first row, keys, position of key 0, first tile, end tile, first row, end row, 0, 0, 0}, per merged row {row, then for up to two groups of partial
  * results: first partial row, count, distance between them, and 0}, per token its position, and the
  * groups: each 16 keys of a page, as its first pool row of KV head 0 over 16; a source's filled up to
- * whole 64-key tiles.  words NULL: only *count. */
+ * whole 128-key tiles.  words NULL: only *count. */
 int qattn_shared_plan_describe(const qattn_shared_desc* desc, int32_t* words, int64_t capacity, int64_t* count,
                                qattn_shared_info* info);
 

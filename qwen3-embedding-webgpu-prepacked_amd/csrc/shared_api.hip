@@ -366,7 +366,9 @@ int install_shared_plan(qattn_shared_run* run, const qattn_shared_desc& d) {
   p.groups = reinterpret_cast<const int32_t*>(image + groups);
   p.part_o = static_cast<float*>(run->partials);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + values * d.cache.head_dim);
-  p.n_items = (int32_t)plan.items.size();
+  p.n_blocks = (int32_t)plan.items.size() - plan.flat_items;
+  p.n_flat = plan.flat_items;
+  p.flat_first = plan.flat_first;
   p.n_merges = (int32_t)plan.merges.size();
   p.most_parts = plan.most_parts;
   p.kv_heads = d.cache.kv_heads;

@@ -13,18 +13,21 @@
 
 namespace qattn {
 
-constexpr int kSharedThreads = 256;
-constexpr int kTallRows = 128, kTallKeys = 64;  // 4 wavefronts x 32 rows share a tile of 64 keys
-constexpr int kFlatRows = 16, kFlatKeys = 32;   // 4 wavefronts x the same 16 rows, a tile of 32 keys each
+constexpr int kSharedThreads = 512;
+// Tall: eight wavefronts x 32 rows share a tile of 128 keys.  Split: four x 32 rows, twice: one four takes the
+// tile's first 64 keys, the other its last.  Flat: four wavefronts x the same 16 rows, a tile of 32 keys
+// each; a workgroup takes two flat items.
+constexpr int kTallRows = 256, kSplitRows = 128, kTallKeys = 128;
+constexpr int kFlatRows = 16, kFlatKeys = 32;
 constexpr int32_t kMaxPosition = 1 << 30;
 
 enum SharedSource { kPrefixPages = 0, kOwnPages = 1, kOwnRows = 2 };
-enum SharedKind { kTall = 0, kFlat = 1 };
+enum SharedKind { kTall = 0, kSplit = 1, kFlat = 2 };
 
 // Tiles tile_begin .. tile_end - 1 (of the item kind's size) of `keys` keys, seen by rows row_begin ..
 // row_end - 1 only.  base: where the source's groups begin in the plan's list, or its first row.  A group is 16
 // keys of a page: its number times 16 is the pool row (of KV head 0) of the first; a source's list is
-// filled up to whole 64-key tiles with its last group.  whole: every row of the item sees every key of
+// filled up to whole 128-key tiles with its last group.  whole: every row of the item sees every key of
 // these tiles.
 struct SharedSeg {
   int32_t source, whole, base, keys, position, tile_begin, tile_end, row_begin, row_end;
@@ -32,7 +35,7 @@ struct SharedSeg {
 };
 // Rows row0 .. row0 + rows - 1 over the tiles of segments seg_begin .. seg_end - 1.  Results go to the output
 // (part < 0) or, unnormalised, to partial rows part, part + 1, ...  The first segment, and the groups of the
-// first tiles (tall: one for each wavefront, flat: two for each wavefront's first tile), come with the item,
+// first tiles (one for each wavefront; flat: two for each wavefront's first tile), come with the item,
 // so that a workgroup asks for its first keys after one dependent load.
 struct SharedItem {
   int32_t row0, rows, seg_begin, seg_end, part, tiles, kind;
@@ -58,6 +61,8 @@ struct SharedPlan {
   std::vector<int32_t> positions;  // of each query
   std::vector<int32_t> groups;
   int64_t partial_rows = 0;
+  int32_t flat_items = 0;  // the last of them
+  bool flat_first = false;
   int32_t most_parts = 0;  // partial rows of a merged row, at most
   qattn_shared_info info{};
 };
@@ -78,7 +83,9 @@ struct SharedParams {
   const int32_t* groups;
   float* part_o;                // [partial row][kv_heads][head_dim]
   float2* part_ml;              // [partial row][kv_heads]: the row's reference (log2) and sum
-  int32_t n_items, n_merges, most_parts, kv_heads, group, page_shift;
+  int32_t n_blocks, n_flat;     // items that are not flat, and flat ones, which follow them in the list
+  int32_t flat_first;           // the flat items' workgroups come first
+  int32_t n_merges, most_parts, kv_heads, group, page_shift;
   int32_t mask, prefix, window;
   float scale_log2;
 };

@@ -2,15 +2,16 @@
 //
 // o[r] = sum_j p_rj v_j / sum_j p_rj, p_rj = 2^(c q_r . k_j - m_r), over the keys that row r sees: the
 // prefix's, read from a paged cache that may hold 8-bit codes, and its sequence's own.  Rows of all
-// sequences are stacked (row = query * group + head of the group), so one tile of prefix keys serves 128
-// rows, whatever sequences they belong to.  Two kinds of item share a launch:
-//   tall  128 rows, 32 to a wavefront, over 64-key tiles that the four wavefronts share in LDS;
-//         S^T = K Q^T and O^T = V^T P^T on 32x32x16 MFMAs, a query row to a lane.  Codes become 16-bit
-//         elements once, on their way into LDS.  Bound by the matrix cores, the softmax's exponentials
-//         and LDS reads.
-//   flat  16 rows over 32-key tiles, every fourth tile to a wavefront, which keeps its own sum; K goes from
-//         memory straight into the MFMA operand, V through the wavefront's own 8 KiB of LDS for the
-//         transposed read; the four sums are joined at the end.  Bound by the cache's bytes.
+// sequences are stacked (row = query * group + head of the group), so one tile of prefix keys serves 256 or
+// 128 rows, whatever sequences they belong to.  Two kinds of work share a launch:
+//   blocks  256 or 128 rows, 32 to a wavefront, over 128-key tiles that eight wavefronts share in LDS (with
+//           128 rows, each half of the tile goes to four of them, and their sums are joined at the end);
+//           S^T = K Q^T and O^T = V^T P^T on 32x32x16 MFMAs, a query row to a lane.  Codes become 16-bit
+//           elements once, on their way into LDS.  Bound by the matrix cores, the softmax's exponentials
+//           and the latency between them: one workgroup fills a CU's LDS and half its registers.
+//   flat    16 rows over 32-key tiles, every fourth tile to a wavefront, which keeps its own sum; K goes from
+//           memory straight into the MFMA operand, V through the wavefront's own 8 KiB of LDS for the
+//           transposed read; the four sums are joined at the end.  Bound by the cache's bytes.
 // An item whose rows have keys elsewhere too (other chunks, other items) leaves its unnormalised f32
 // sums, the row's reference m and its sum of p; shared_merge_kernel joins them.
 //
@@ -31,6 +32,7 @@ typedef short s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s4 lds_s4;
 typedef __attribute__((address_space(4))) const int32_t const_i32;
 
+constexpr int kMergeThreads = 256;
 constexpr float kLazy = 8.f;
 constexpr float kNone = -INFINITY;
 
@@ -68,6 +70,11 @@ __device__ inline float rows_sum(float x) {
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return half_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
+__device__ inline int wave_max(int x) {
+  for (int d = 32; d; d >>= 1) x = max(x, __shfl_xor(x, d));
+  return __builtin_amdgcn_readfirstlane(x);
+}
+
 __device__ inline SharedSeg seg_at(const const_i32* w) {
   return SharedSeg{w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7], w[8], {0, 0, 0}};
 }
@@ -210,7 +217,7 @@ template <bool BF16, int FORMAT, int DIM>
 struct Tall {
   static constexpr int kRow = 2 * DIM;                  // bytes of a row in LDS
   static constexpr int kTile = kTallKeys * kRow;        // of K or V
-  static constexpr int kLds = 4 * kTile;                // K and V, double buffered
+  static constexpr int kLds = 4 * kTile;                // K and V, double buffered; O of four wavefronts in f32
   // 16-byte chunks of a row in memory, rows of a wavefront's load, loads per tile: of 16-bit rows, codes.
   static constexpr int kChunks16 = kRow / 16, kRows16 = 64 / kChunks16, kLoads16 = 16 / kRows16;
   static constexpr int kChunks8 = DIM / 16, kRows8 = 64 / kChunks8, kLoads8 = 16 / kRows8;
@@ -252,10 +259,10 @@ struct Tall {
     }
   }
 
-  // Half h of the loaded K (I = 0) or V (1) into LDS as 16-bit elements.  partly: infinities and NaN are
+  // The loaded K (I = 0) or V (1) into LDS as 16-bit elements.  partly: infinities and NaN are
   // taken out (of V, in tiles that some row sees only part of); returns whether this lane had any.
   template <int I>
-  __device__ bool store(char* lds, bool rows, int wave, int lane, int h, bool partly) {
+  __device__ bool store(char* lds, bool rows, int wave, int lane, bool partly) {
     bool any = false;
     const auto put = [&](int r, int c, u32x4 x) {
       if (I && partly) any |= drop_nonfinite<BF16>(x);
@@ -263,12 +270,11 @@ struct Tall {
     };
     if (!kCodes || rows) {
 #pragma unroll
-      for (int j = h * kLoads16 / 2; j < (h + 1) * kLoads16 / 2; ++j)
+      for (int j = 0; j < kLoads16; ++j)
         put(16 * wave + j * kRows16 + lane / kChunks16, lane % kChunks16, raw[I][j]);
     } else {
-      constexpr int kEach = (kLoads8 + 1) / 2;
 #pragma unroll
-      for (int j = h * kEach; j < (h + 1) * kEach && j < kLoads8; ++j) {
+      for (int j = 0; j < kLoads8; ++j) {
         const int r = 16 * wave + j * kRows8 + lane / kChunks8, c = 2 * (lane % kChunks8);
         u32x4 x[2];
         expand<BF16, FORMAT>(raw[I][j], scale[I][kCodes ? j : 0], x);
@@ -283,44 +289,42 @@ struct Tall {
 // Offset of accumulator element r (0 .. 31 over the two 32-key blocks) from the tile's first key + 4 hl.
 __device__ constexpr int key_off(int r) { return 32 * (r >> 4) + 8 * ((r & 15) >> 2) + (r & 3); }
 
-// Iteration t computes the scores of tile t, then its weights while the matrix cores add P(t - 1) V(t - 1);
-// K(t + 1) and V(t), in registers since the iteration before, go to LDS, and K(t + 2) and V(t + 1) are asked
-// for.
+// Tile t is in LDS while tile t + 1 is in registers or on its way there: at the end of an iteration those go
+// into the other buffers and tile t + 2 is asked for.
 template <bool BF16, int FORMAT, int DIM>
-__device__ inline void tall_item(const SharedParams& p, const SharedItem& it, int index, int kvh, char* lds, uint32_t* dropped) {
+__device__ inline void tall_item(const SharedParams& p, const SharedItem& it, int index, int kvh, char* lds, float2* stats,
+                                 uint32_t* dropped) {
   typedef Tall<BF16, FORMAT, DIM> T;
   constexpr int kBlocks = DIM / 32, kSteps = DIM / 16;
   const int lane = threadIdx.x & 63, lq = lane & 31, hl = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int end_row = it.row0 + it.rows, wave_row = it.row0 + 32 * wave;
+  // The wavefront's rows, and its 64-key parts of a tile: both, or one of them.
+  const bool split = it.kind == kSplit;
+  const int part_begin = split ? wave >> 2 : 0, part_end = split ? part_begin + 1 : 2;
+  const int end_row = it.row0 + it.rows, wave_row = it.row0 + 32 * (split ? wave & 3 : wave);
   const int row = wave_row + lq;
   const bool exists = row < end_row;
   const int token = exists ? row / p.group : 0;
   const int head = kvh * p.group + row - token * p.group;
   const int at = exists ? p.positions[token] : -1;
   const bool local = p.mask != QATTN_MASK_CAUSAL;
-  const auto k_buf = [&](int t) { return lds + (t & 1) * T::kTile; };
-  const auto v_buf = [&](int t) { return lds + (2 + (t & 1)) * T::kTile; };
 
   // What the scores of a tile need to know of it.
   struct Info {
     int whole, from, last, row_begin, row_end;  // from: position of its first key; last: of its segment's last
   };
   const Keys<FORMAT, DIM> keys(p, kvh);
-  Cursor ahead(p, it);  // the next K tile to ask for, its group on the way
+  Cursor ahead(p, it);  // the next tile to ask for, its group on the way
   T tile;
   int zero = 0;
   asm volatile("" : "+v"(zero));
   uint32_t group = item_group(p, index, wave);
-  typename T::Spot spot{}, spot_v{};
+  typename T::Spot spot{};
   int asked = 0;
-  bool whole_v = true;  // the V tile in registers
-  bool found = false;   // infinities or NaN were dropped from V
+  bool found = false;  // infinities or NaN were dropped from V
   if (threadIdx.x == 0) *dropped = 0;
-  Info now{}, next{};   // of the scores to come, of the K tile in registers
-  // K of the next tile, if there is one, and V of the tile before it.
-  const auto ask_k = [&]() {
-    if (asked == it.tiles) return;
+  Info next{};  // of the tile in registers
+  const auto ask = [&]() {
     const SharedSeg& s = ahead.seg;
     const int first = ahead.tile * kTallKeys + 16 * wave;
     spot.rows = s.source == kOwnRows;
@@ -328,15 +332,20 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
     spot.row = s.base + min(first, s.keys - 1);
     spot.left = max(s.keys - 1 - first, 0);
     tile.template load<0>(keys, spot, lane);
+    tile.template load<1>(keys, spot, lane);
     next = Info{s.whole, s.position + ahead.tile * kTallKeys, s.position + s.keys - 1, s.row_begin, s.row_end};
     if (++asked < it.tiles) {
       ahead.advance(1);
       group = group_of(p, ahead.seg, ahead.tile * kTallKeys + 16 * wave, zero);
     }
   };
-  const auto ask_v = [&]() { tile.template load<1>(keys, spot_v, lane); };
+  const auto keep = [&](int t) {
+    char* buf = lds + (t & 1) * 2 * T::kTile;
+    tile.template store<0>(buf, spot.rows, wave, lane, false);
+    found |= tile.template store<1>(buf + T::kTile, spot.rows, wave, lane, !next.whole);
+  };
 
-  ask_k();  // K(0)
+  ask();
   // Q (B operand of S^T = K Q^T): this lane's row, dims 16 st + 8 hl .. + 7 at step st.
   u32x4 q[kSteps];
   {
@@ -347,13 +356,15 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
 #pragma unroll
     for (int st = 0; st < kSteps; ++st) asm volatile("" : "+v"(q[st]));
   }
+  const int greatest = wave_max(at);
+
   f16x o[kBlocks];
 #pragma unroll
   for (int db = 0; db < kBlocks; ++db) o[db] = f16x{};
   float m = kNone, l = 0.f;
 
   // LDS read addresses.  K: rows lq, lq + 32.  V^T through the transposing read: in each 16-lane group G
-  // lane a reads 4 elements of key 4 (G >> 1) + (a >> 2) (+ 16 t, + 8) at dims 32 db + 16 (G & 1) + 4 (a & 3)
+  // lane a reads 4 elements of key 4 (G >> 1) + (a >> 2) (+ 16 st, + 8) at dims 32 db + 16 (G & 1) + 4 (a & 3)
   // and receives those keys' elements of dim 32 db + 16 (G & 1) + a.
   uint32_t v_read[kBlocks];
   {
@@ -361,77 +372,40 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
 #pragma unroll
     for (int db = 0; db < kBlocks; ++db) v_read[db] = T::v_at(r, 4 * db + 2 * (G & 1) + ((a & 3) >> 1)) + ((a & 1) << 3);
   }
-  // O^T += V^T P^T for the tile in `v`.  Step st covers keys 16 st .. 16 st + 15; slot j of half hl is key
-  // 16 st + 8 (j >> 2) + 4 hl + (j & 3), whose p is element j of pf[st].
-  const auto v_frag = [&](const char* v, int i) {
-    const char* src = v + v_read[i % kBlocks] + i / kBlocks * 16 * T::kRow;
-    const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)src));
-    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(src + 8 * T::kRow)));
-    return u32x4{lo[0], lo[1], hi[0], hi[1]};
-  };
-  // beside(i): other work, issued after product i.  Operands are read kDeep products ahead; the scheduling
-  // barriers keep the compiler from reading them all at once, for which there are no registers.
-  constexpr int kDeep = 2;
-  const auto add_pv = [&](const char* v, const u32x4 (&pf)[4], auto beside) {
-    u32x4 a[kDeep];
+  // Scores, weights and sums of the 64 keys at k, v, of which the first stands at position `from`.  Operands
+  // are read ahead; the scheduling barriers keep the compiler from reading them all at once, for which there
+  // are no registers.
+  const auto add_part = [&](const Info& cur, int from, const char* k, const char* v) {
+    f16x sc[2];
+    {
+      // Rows lq and lq + 32, chunk 2 st + hl: its swizzled place is 2 st xor'ed onto chunk hl's.  (Formed here:
+      // hoisted, the addresses of all steps would take a register each.)
+      uint32_t place = T::k_at(lq, hl) - lq * T::kRow;
+      asm volatile("" : "+v"(place));
+      const auto k_frag = [&](int i) {
+        return *reinterpret_cast<const u32x4*>(k + lq * T::kRow + ((uint32_t)(i >> 1 << 5) ^ place) + 32 * (i & 1) * T::kRow);
+      };
+      constexpr int kAhead = 4;
+      u32x4 a[kAhead];
 #pragma unroll
-    for (int i = 0; i < kDeep; ++i) a[i] = v_frag(v, i);
+      for (int i = 0; i < kAhead; ++i) a[i] = k_frag(i);
+      __builtin_amdgcn_s_setprio(1);  // before the other wavefront's vector work
 #pragma unroll
-    for (int i = 0; i < 4 * kBlocks; ++i) {
+      for (int i = 0; i < 2 * kSteps; ++i) {
+        __builtin_amdgcn_sched_barrier(0);
+        sc[i & 1] = mfma32<BF16>(a[i % kAhead], q[i >> 1], i < 2 ? f16x{} : sc[i & 1]);
+        if (i + kAhead < 2 * kSteps) a[i % kAhead] = k_frag(i + kAhead);
+      }
       __builtin_amdgcn_sched_barrier(0);
-      o[i % kBlocks] = mfma32<BF16>(a[i % kDeep], pf[i / kBlocks], o[i % kBlocks]);
-      if (i + kDeep < 4 * kBlocks) a[i % kDeep] = v_frag(v, i + kDeep);
-      beside(i);
+      __builtin_amdgcn_s_setprio(0);
     }
-    __builtin_amdgcn_sched_barrier(0);
-  };
-  const auto nothing = [](int) {};
-  // p of elements r, r + 1.
-  const auto weights = [&](const f16x (&sc)[2], int r, float ref, u32x4 (&pf)[4], float& sum) {
-    const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[r >> 4][r & 15], p.scale_log2, -ref));
-    const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[r >> 4][(r & 15) + 1], p.scale_log2, -ref));
-    sum += p0 + p1;
-    pf[r >> 3][(r & 7) >> 1] = narrow2<BF16>(p0, p1);
-  };
-
-#pragma unroll
-  for (int h = 0; h < 2; ++h) tile.template store<0>(k_buf(0), spot.rows, wave, lane, h, false);
-  now = next;
-  spot_v = spot;
-  whole_v = now.whole;
-  ask_v();
-  ask_k();
-  // Scores of tile t, masked.
-  // (beside(i): other work, issued after product i.)
-  const auto scores = [&](const Info& cur, const char* k, f16x (&sc)[2], auto beside) {
-    // Rows lq and lq + 32, chunk 2 st + hl: its swizzled place is 2 st xor'ed onto chunk hl's.  (Formed here:
-    // hoisted, the addresses of all steps would take a register each.)
-    uint32_t place = T::k_at(lq, hl) - lq * T::kRow;
-    asm volatile("" : "+v"(place));
-    const auto k_frag = [&](int i) {
-      return *reinterpret_cast<const u32x4*>(k + lq * T::kRow + ((uint32_t)(i >> 1 << 5) ^ place) + 32 * (i & 1) * T::kRow);
-    };
-    constexpr int kAhead = 4;
-    u32x4 a[kAhead];
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) a[i] = k_frag(i);
-    __builtin_amdgcn_s_setprio(1);  // before the other wavefront's vector work
-#pragma unroll
-    for (int i = 0; i < 2 * kSteps; ++i) {
-      __builtin_amdgcn_sched_barrier(0);
-      sc[i & 1] = mfma32<BF16>(a[i % kAhead], q[i >> 1], i < 2 ? f16x{} : sc[i & 1]);
-      if (i + kAhead < 2 * kSteps) a[i % kAhead] = k_frag(i + kAhead);
-      beside(i);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_setprio(0);
     if (!cur.whole) {
       // Offsets from this lane's first key: the last one seen, and where the prefix and the window leave a gap.
       const int mine = row >= cur.row_begin && row < cur.row_end ? at : -1;
-      const int base = cur.from + 4 * hl, last = min(mine, cur.last) - base;
+      const int base = from + 4 * hl, last = min(mine, cur.last) - base;
 #pragma unroll
       for (int r = 0; r < 32; ++r) sc[r >> 4][r & 15] = key_off(r) > last ? kNone : sc[r >> 4][r & 15];
-      if (local && cur.from + kTallKeys > p.prefix && cur.from <= it.greatest - p.window) {
+      if (local && from + 64 > p.prefix && from <= it.greatest - p.window) {
         const int gap = p.prefix - base, window = mine - p.window - base;
 #pragma unroll
         for (int r = 0; r < 32; ++r) {
@@ -440,88 +414,75 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
         }
       }
     }
-  };
-  // Moves the row's reference if the tile calls for it; returns what the sums so far are to be scaled by.
-  const auto refer = [&](const f16x (&sc)[2]) {
     float top = fmaxf(fmaxf(sc[0][0], sc[0][1]), sc[0][2]);
 #pragma unroll
     for (int r = 3; r < 31; r += 2) top = fmaxf(fmaxf(top, sc[r >> 4][r & 15]), sc[(r + 1) >> 4][(r + 1) & 15]);
     top = half_max(fmaxf(top, sc[1][15])) * p.scale_log2;
-    const float moved = top > m + kLazy ? top : m;  // from -inf too: any score exceeds it
-    const float shrink = m == moved ? 1.f : __builtin_amdgcn_exp2f(m - moved);
-    m = moved;
-    return shrink;
-  };
-  // Beside the products of S(t): V(t) and K(t + 1) go to LDS, V(t + 1) and K(t + 2) are asked for.
-  const auto move_on = [&](int t, int i) {
-    constexpr int kEvery = kSteps / 4;
-    if (i % kEvery) return;
-    const bool more = t + 1 < it.tiles;
-    switch (i / kEvery) {
-      case 1: found |= tile.template store<1>(v_buf(t), spot_v.rows, wave, lane, 0, !whole_v); break;
-      case 2: found |= tile.template store<1>(v_buf(t), spot_v.rows, wave, lane, 1, !whole_v); break;
-      case 3:
-        if (more) tile.template store<0>(k_buf(t + 1), spot.rows, wave, lane, 0, false);
-        break;
-      case 4:
-        if (more) tile.template store<0>(k_buf(t + 1), spot.rows, wave, lane, 1, false);
-        break;
-      case 5:
-        if (more) {
-          now = next;
-          spot_v = spot;
-          whole_v = now.whole;
-          ask_v();
-        }
-        break;
-      case 6:
-        if (more) ask_k();
-        break;
-    }
-  };
-
-  u32x4 pf[4];
-  {
-    __syncthreads();
-    const Info cur = now;
-    f16x sc[2];
-    scores(cur, k_buf(0), sc, [&](int i) { move_on(0, i); });
-    refer(sc);
-    const float ref = m == kNone ? 0.f : m;
-#pragma unroll
-    for (int r = 0; r < 32; r += 2) weights(sc, r, ref, pf, l);
-  }
-  for (int t = 1; t < it.tiles; ++t) {
-    // K(t) and V(t - 1) are in LDS, and every wavefront is done with the other buffers.
-    __syncthreads();
-    const Info cur = now;
-    f16x sc[2];
-    scores(cur, k_buf(t), sc, [&](int i) { move_on(t, i); });
-    const float shrink = refer(sc);
-    const float ref = m == kNone ? 0.f : m;
-    // The weights beside the matrix cores' work on the tile before.
-    u32x4 next_pf[4];
-    float sum = 0.f;
-    constexpr int kEach = 32 / (4 * kBlocks);
-    add_pv(v_buf(t - 1), pf, [&](int i) {
-#pragma unroll
-      for (int r = kEach * i; r < kEach * (i + 1); r += 2) {
-        weights(sc, r, ref, next_pf, sum);
-      }
-    });
-    if (__any(shrink != 1.f)) {
+    if (__any(top > m + kLazy)) {  // from -inf too: any score exceeds it
+      const float moved = top > m + kLazy ? top : m;
+      const float shrink = m == moved ? 1.f : __builtin_amdgcn_exp2f(m - moved);
+      m = moved;
+      l *= shrink;
 #pragma unroll
       for (int db = 0; db < kBlocks; ++db) o[db] *= shrink;
     }
-    l = l * shrink + sum;
+    const float ref = m == kNone ? 0.f : m;
+    // Slot j of half hl at step st is key 16 st + 8 (j >> 2) + 4 hl + (j & 3): element 8 st + j of the scores.
+    u32x4 pf[4];
+    float sum[2] = {};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) pf[i] = next_pf[i];
+    for (int r = 0; r < 32; r += 2) {
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[r >> 4][r & 15], p.scale_log2, -ref));
+      const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[r >> 4][(r & 15) + 1], p.scale_log2, -ref));
+      sum[0] += p0;
+      sum[1] += p1;
+      pf[r >> 3][(r & 7) >> 1] = narrow2<BF16>(p0, p1);
+    }
+    l += sum[0] + sum[1];
+    const auto v_frag = [&](int i) {
+      const char* src = v + v_read[i % kBlocks] + i / kBlocks * 16 * T::kRow;
+      const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)src));
+      const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(src + 8 * T::kRow)));
+      return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    };
+    constexpr int kDeep = 4;
+    u32x4 a[kDeep];
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i) a[i] = v_frag(i);
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int i = 0; i < 4 * kBlocks; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+      o[i % kBlocks] = mfma32<BF16>(a[i % kDeep], pf[i / kBlocks], o[i % kBlocks]);
+      if (i + kDeep < 4 * kBlocks) a[i % kDeep] = v_frag(i + kDeep);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(0);
+  };
+
+  keep(0);
+  Info now = next;
+  if (it.tiles > 1) ask();
+  for (int t = 0; t < it.tiles; ++t) {
+    __syncthreads();
+    const char* buf = lds + (t & 1) * 2 * T::kTile;
+    // Parts of which some row of this wavefront sees a key.
+    if (wave_row < end_row && (now.whole || (now.row_begin < wave_row + 32 && now.row_end > wave_row))) {
+      for (int part = part_begin; part < part_end; ++part) {
+        const int from = now.from + 64 * part;
+        if (now.whole || from <= min(greatest, now.last))
+          add_part(now, from, buf + part * 64 * T::kRow, buf + T::kTile + part * 64 * T::kRow);
+      }
+    }
+    if (t + 1 < it.tiles) {
+      keep(t + 1);
+      now = next;
+      if (t + 2 < it.tiles) ask();
+    }
   }
-  __syncthreads();
-  add_pv(v_buf(it.tiles - 1), pf, nothing);
   if (found) *dropped = 1;
   __syncthreads();
-  if (*dropped)
+  if (*dropped && part_begin == 0)
     each_nonfinite<BF16, FORMAT, DIM>(p, keys, it, row, at, kTallKeys, 0, 1, [&](auto value, bool seen) {
 #pragma unroll
       for (int db = 0; db < kBlocks; ++db)
@@ -533,8 +494,31 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
         }
     });
 
-  // O^T: this lane holds dims 32 db + 8 g + 4 hl .. + 3 of its row.
   l = half_sum(l);
+  if (split) {
+    // The sums of wavefront w + 4 join those of w, over the tiles' LDS.
+    f4* sums = reinterpret_cast<f4*>(lds) + (wave & 3) * (DIM / 8) * 64 + lane;
+    if (wave >= 4) {
+#pragma unroll
+      for (int i = 0; i < DIM / 8; ++i)
+        sums[64 * i] = f4{o[i >> 2][4 * (i & 3)], o[i >> 2][4 * (i & 3) + 1], o[i >> 2][4 * (i & 3) + 2], o[i >> 2][4 * (i & 3) + 3]};
+      if (hl == 0) stats[32 * (wave & 3) + lq] = float2{m, l};
+    }
+    __syncthreads();
+    if (wave >= 4) return;
+    const float2 other = stats[32 * wave + lq];
+    const float top = fmaxf(m, other.x), ref = top == kNone ? 0.f : top;
+    const float f0 = __builtin_amdgcn_exp2f(m - ref), f1 = __builtin_amdgcn_exp2f(other.x - ref);
+    l = f0 * l + f1 * other.y;
+    m = top;
+#pragma unroll
+    for (int i = 0; i < DIM / 8; ++i) {
+      const f4 x = sums[64 * i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i >> 2][4 * (i & 3) + e] = f0 * o[i >> 2][4 * (i & 3) + e] + f1 * x[e];
+    }
+  }
+  // O^T: this lane holds dims 32 db + 8 g + 4 hl .. + 3 of its row.
   if (it.part < 0) {
     const float inv = l == 0.f ? 0.f : 1.f / l;  // a NaN stays one
     uint16_t* dst = p.o + (int64_t)token * p.o_stride + head * DIM + 8 * hl;
@@ -661,7 +645,7 @@ __device__ inline void flat_item(const SharedParams& p, const SharedItem& it, in
   typedef Flat<BF16, FORMAT, DIM> T;
   constexpr int kBlocks = DIM / 16;
   const int lane = threadIdx.x & 63, n = lane & 15, c = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
   char* lds = lds_all + wave * (T::kLds / 4);
   const int end_row = it.row0 + it.rows, row = it.row0 + n;
   const bool exists = row < end_row;
@@ -778,7 +762,7 @@ __device__ inline void flat_item(const SharedParams& p, const SharedItem& it, in
   for (int db = 0; db < kBlocks; ++db) *reinterpret_cast<f4*>(own + n * DIM + 16 * db + 4 * c) = o[db];
   if (c == 0) stats[16 * wave + n] = float2{m, l};
   __syncthreads();
-  const int r = threadIdx.x >> 4, d = (threadIdx.x & 15) * (DIM / 16);
+  const int r = (threadIdx.x & 255) >> 4, d = (threadIdx.x & 15) * (DIM / 16);
   if (it.row0 + r >= end_row) return;
   float2 st[4];
   float top = kNone, sum = 0.f;
@@ -813,15 +797,25 @@ __device__ inline void flat_item(const SharedParams& p, const SharedItem& it, in
 
 template <bool BF16, int FORMAT, int DIM>
 __global__ __launch_bounds__(kSharedThreads, 2) void shared_attn_kernel(SharedParams p) {
-  __shared__ __attribute__((aligned(1024))) char lds[Tall<BF16, FORMAT, DIM>::kLds];
-  __shared__ __attribute__((aligned(16))) float2 stats[4 * kFlatRows];
+  constexpr int kTallLds = Tall<BF16, FORMAT, DIM>::kLds, kFlatLds = Flat<BF16, FORMAT, DIM>::kLds;
+  static_assert(kTallLds >= 2 * kFlatLds && kTallLds >= 4 * 32 * DIM * 4, "two flat items; O of four wavefronts");
+  __shared__ __attribute__((aligned(1024))) char lds[kTallLds];
+  __shared__ __attribute__((aligned(16))) float2 stats[128];
+  __shared__ uint32_t dropped;
   const int kvh = (int)(blockIdx.x % (uint32_t)p.kv_heads);
-  const int index = (int)(blockIdx.x / (uint32_t)p.kv_heads);
-  const SharedItem it = item_at(p, index);
-  if (it.kind == kTall)
-    tall_item<BF16, FORMAT, DIM>(p, it, index, kvh, lds, reinterpret_cast<uint32_t*>(stats));
-  else
-    flat_item<BF16, FORMAT, DIM>(p, it, index, kvh, lds, stats);
+  const int unit = (int)(blockIdx.x / (uint32_t)p.kv_heads);
+  const int pairs = (p.n_flat + 1) / 2;
+  const int block = p.flat_first ? unit - pairs : unit;
+  if (block >= 0 && block < p.n_blocks) {
+    tall_item<BF16, FORMAT, DIM>(p, item_at(p, block), block, kvh, lds, stats, &dropped);
+  } else {
+    const int half = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+    const int flat = 2 * (p.flat_first ? unit : unit - p.n_blocks) + half;
+    const int index = p.n_blocks + min(flat, p.n_flat - 1);
+    SharedItem it = item_at(p, index);
+    if (flat >= p.n_flat) it.rows = it.tiles = 0;  // the last pair's second half: along for the barrier
+    flat_item<BF16, FORMAT, DIM>(p, it, index, kvh, lds + half * kFlatLds, stats + 64 * half);
+  }
 }
 
 // Merged rows: sum over a row's partial rows of 2^(m_i - max m) times its sums; a partial row that saw no
@@ -830,9 +824,9 @@ __global__ __launch_bounds__(kSharedThreads, 2) void shared_attn_kernel(SharedPa
 // lanes every kGroups'th partial row (rows cut into many chunks: a chain of loads would set the time);
 // else each group takes a row of its own.  Bound by latency: three dependent accesses.
 template <bool BF16, int DIM, bool WIDE>
-__global__ __launch_bounds__(kSharedThreads) void shared_merge_kernel(SharedParams p) {
-  constexpr int kLanes = DIM / 4, kGroups = kSharedThreads / kLanes;
-  __shared__ f4 sums[WIDE ? kSharedThreads : 1];
+__global__ __launch_bounds__(kMergeThreads) void shared_merge_kernel(SharedParams p) {
+  constexpr int kLanes = DIM / 4, kGroups = kMergeThreads / kLanes;
+  __shared__ f4 sums[WIDE ? kMergeThreads : 1];
   __shared__ float2 stats[WIDE ? kGroups : 1];
   const int group = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
   const int64_t index = WIDE ? blockIdx.x : (int64_t)blockIdx.x * kGroups + group;
@@ -901,12 +895,12 @@ __global__ __launch_bounds__(kSharedThreads) void shared_merge_kernel(SharedPara
 
 template <bool BF16, int FORMAT, int DIM>
 void launch_attn(const SharedParams& p, hipStream_t stream) {
-  hipLaunchKernelGGL((shared_attn_kernel<BF16, FORMAT, DIM>), dim3((unsigned)p.n_items * p.kv_heads), dim3(kSharedThreads),
-                     0, stream, p);
+  const unsigned units = p.n_blocks + (p.n_flat + 1) / 2;
+  hipLaunchKernelGGL((shared_attn_kernel<BF16, FORMAT, DIM>), dim3(units * p.kv_heads), dim3(kSharedThreads), 0, stream, p);
 }
 template <bool BF16, int DIM>
 hipError_t launch(const SharedParams& p, int format, hipStream_t stream) {
-  if (p.n_items > 0) {
+  if (p.n_blocks + p.n_flat > 0) {
     switch (format) {
       case QATTN_KV_16BIT: launch_attn<BF16, QATTN_KV_16BIT, DIM>(p, stream); break;
       case QATTN_KV_E4M3: launch_attn<BF16, QATTN_KV_E4M3, DIM>(p, stream); break;
@@ -917,12 +911,12 @@ hipError_t launch(const SharedParams& p, int format, hipStream_t stream) {
   }
   if (p.n_merges > 0) {
     const int64_t rows = (int64_t)p.n_merges * p.kv_heads;
-    constexpr int kGroups = kSharedThreads / (DIM / 4);
+    constexpr int kGroups = kMergeThreads / (DIM / 4);
     if (p.most_parts > 8)
-      hipLaunchKernelGGL((shared_merge_kernel<BF16, DIM, true>), dim3((unsigned)rows), dim3(kSharedThreads), 0, stream, p);
+      hipLaunchKernelGGL((shared_merge_kernel<BF16, DIM, true>), dim3((unsigned)rows), dim3(kMergeThreads), 0, stream, p);
     else
       hipLaunchKernelGGL((shared_merge_kernel<BF16, DIM, false>), dim3((unsigned)((rows + kGroups - 1) / kGroups)),
-                         dim3(kSharedThreads), 0, stream, p);
+                         dim3(kMergeThreads), 0, stream, p);
     return hipGetLastError();
   }
   return hipSuccess;

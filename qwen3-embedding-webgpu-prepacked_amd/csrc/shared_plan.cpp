@@ -1,14 +1,14 @@
 // shared_plan.cpp -- host planner of the attention behind one shared prefix.
 //
-// Row blocks.  The rows of all sequences are stacked and cut into blocks of 128, so that short sequences
-// fill a block together and a tile of prefix keys is read once for all its rows.  A block also visits
-// the own keys of its sequences, one segment each, in which only their rows see anything.  Sequences
-// of up to 16 rows (single tokens) would waste most of a block on their own keys: those go to items of
-// 16 rows whose four wavefronts take a tile of keys each, and so do the prefix's if the launch has no
-// more rows than that.
+// Row blocks.  The rows of all sequences are stacked and cut into blocks of 256 or 128, so that short
+// sequences fill a block together and a tile of prefix keys is read once for all its rows.  A block also
+// visits the own keys of its sequences, one segment each, in which only their rows see anything.
+// Sequences of up to 16 rows (single tokens) would waste most of a block on their own keys: those go to
+// items of 16 rows whose four wavefronts take a tile of keys each, and so do the prefix's if the launch has
+// no more rows than that.
 //
-// Cuts.  Items are cut along their keys where that shortens the launch: the planner compares the time at
-// which the last of the GPU's slots ends, for a range of chunk sizes, by a cost model.
+// Cuts.  Items are cut along their keys where that shortens the launch.  The planner compares, for both block
+// sizes and a range of chunk sizes, the time at which the last of the GPU's slots ends, by a cost model.
 #include <algorithm>
 #include <cmath>
 #include <queue>
@@ -19,11 +19,11 @@ namespace qattn {
 
 namespace {
 
-// Costs in microseconds, from measured launches (two workgroups to a CU): an item's start and end, a 64-key
-// tile of a full block, a round of four 32-key tiles of a flat item, an item's partial results, the second
-// launch, and the partial rows' bytes (written and read).
-constexpr double kTallItem = 3.0, kTallTile = 2.3, kFlatItem = 2.0, kFlatRound = 1.4, kPartial = 1.0, kMergeLaunch = 4.0;
-constexpr double kBytesPerUs = 5e6;
+// Costs in microseconds, from measured launches (one workgroup to a CU): an item's start and end, a 128-key
+// tile of a 256- and of a 128-row block, a round of four 32-key tiles of a pair of flat items, an item's
+// partial results, the second launch, and the partial rows' bytes (written and read).
+constexpr double kBlockItem = 4.0, kTallTile = 3.6, kSplitTile = 2.0, kFlatItem = 3.0, kFlatRound = 1.4;
+constexpr double kPartial = 1.0, kMergeLaunch = 4.0, kBytesPerUs = 5e6;
 constexpr int kMostSimulated = 16384;
 
 struct Sequence {
@@ -36,25 +36,27 @@ struct Draft {
   std::vector<SharedSeg> segs;
   bool merged = false;  // its rows have partial results elsewhere too
   int chunks = 1, first_part = 0;
-  double cost(int tiles) const {
-    return item.kind == kTall ? kTallItem + kTallTile * tiles : kFlatItem + kFlatRound * ((tiles + 3) / 4);
-  }
+  // Units of work that cuts leave whole (tiles; rounds of the four wavefronts), and their cost.
+  int units() const { return item.kind == kFlat ? (item.tiles + 3) / 4 : item.tiles; }
+  double fixed() const { return item.kind == kFlat ? kFlatItem : kBlockItem; }
+  double unit() const { return item.kind == kFlat ? kFlatRound : item.kind == kTall ? kTallTile : kSplitTile; }
+  double cost(int n) const { return fixed() + unit() * n; }
 };
 
 class Planner {
  public:
   Planner(const qattn_shared_desc& d, int compute_units, SharedPlan* plan)
       : d_(d), plan_(plan), group_(d.q_heads / d.cache.kv_heads),
-        slots_(std::max(1, 2 * compute_units / d.cache.kv_heads)) {}
+        slots_(std::max(1, compute_units / d.cache.kv_heads)) {}
 
   void run() {
     read();
     draft();
-    cut();
     emit();
   }
 
  private:
+  static int tile_of(int kind) { return kind == kFlat ? kFlatKeys : kTallKeys; }
   bool local() const { return d_.mask == QATTN_MASK_PREFIX_LOCAL; }
   int64_t window() const { return std::min<int64_t>(d_.window, kMaxPosition); }
 
@@ -67,7 +69,7 @@ class Planner {
       const int32_t groups = (int32_t)(((int64_t)keys + 15) / 16);
       for (int32_t i = 0; i < groups; ++i)
         plan_->groups.push_back(pages[i / (page_size / 16)] * page_groups + i % (page_size / 16));
-      while (groups && plan_->groups.size() % 4) plan_->groups.push_back(plan_->groups.back());
+      while (groups && plan_->groups.size() % (kTallKeys / 16)) plan_->groups.push_back(plan_->groups.back());
       pages += ((int64_t)keys + page_size - 1) / page_size;
     };
     const int32_t* pages = d_.prefix_pages;
@@ -125,7 +127,7 @@ class Planner {
 
   // A block's segments: the prefix, and the own keys of its sequences that are not left to flat items.
   Draft block(int64_t row0, int64_t rows, size_t first_sequence, int kind, bool with_own) const {
-    const int tile = kind == kTall ? kTallKeys : kFlatKeys;
+    const int tile = tile_of(kind);
     Draft b;
     b.item = SharedItem{(int32_t)row0, (int32_t)rows, 0, 0, -1, 0, kind};
     const int32_t t0 = (int32_t)(row0 / group_), t1 = (int32_t)((row0 + rows - 1) / group_);
@@ -150,7 +152,7 @@ class Planner {
   // Counts a draft's tiles and takes apart the ones that all its rows see wholly, which the kernel neither
   // masks nor looks through.
   void finish(Draft* b) const {
-    const int tile = b->item.kind == kTall ? kTallKeys : kFlatKeys;
+    const int tile = tile_of(b->item.kind);
     std::vector<SharedSeg> segs;
     segs.swap(b->segs);
     for (const SharedSeg& s : segs) {
@@ -175,15 +177,16 @@ class Planner {
   bool flat_own(const Sequence& s) const { return !flat_all_ && (int64_t)s.queries * group_ <= kFlatRows; }
 
   // Blocks of stacked rows: `aligned` starts a block at every sequence of a block's rows or more.
-  std::vector<Draft> blocks(bool aligned) const {
+  std::vector<Draft> blocks(int kind, bool aligned) const {
+    const int64_t most = kind == kTall ? kTallRows : kSplitRows;
     std::vector<Draft> out;
     int64_t begin = -1, end = 0;  // pending rows
     size_t first = 0;             // a sequence at or before them
     const auto flush = [&](int64_t upto) {
       while (begin >= 0 && begin < upto) {
         while (first < sequences_.size() && ((int64_t)sequences_[first].first + sequences_[first].queries) * group_ <= begin) ++first;
-        const int64_t rows = std::min<int64_t>(kTallRows, upto - begin);
-        out.push_back(block(begin, rows, first, kTall, true));
+        const int64_t rows = std::min<int64_t>(most, upto - begin);
+        out.push_back(block(begin, rows, first, kind, true));
         begin += rows;
       }
       begin = -1;
@@ -194,7 +197,7 @@ class Planner {
         continue;
       }
       const int64_t row = (int64_t)s.first * group_, rows = (int64_t)s.queries * group_;
-      if (begin < 0 || row != end || (aligned && rows >= kTallRows)) {
+      if (begin < 0 || row != end || (aligned && rows >= most)) {
         flush(end);
         begin = row;
       }
@@ -204,25 +207,17 @@ class Planner {
     return out;
   }
 
+  // The drafts that suit the batch best, cut.
   void draft() {
     if (sequences_.empty()) return;
     const int64_t rows = (int64_t)plan_->positions.size() * group_;
+    std::vector<Draft> flat;
     if (rows <= kFlatRows && sequences_.size() == 1) {
       // One short sequence: prefix and own keys in one item.
       flat_all_ = true;
-      drafts_.push_back(block((int64_t)sequences_[0].first * group_, rows, 0, kFlat, true));
-    } else if (rows <= kFlatRows) {
-      if (d_.prefix_len) drafts_.push_back(block(0, rows, 0, kFlat, false));
+      flat.push_back(block((int64_t)sequences_[0].first * group_, rows, 0, kFlat, true));
     } else {
-      const auto tiles = [](const std::vector<Draft>& v) {
-        int64_t n = 0;
-        for (const Draft& b : v) n += b.item.tiles + 2;
-        return n;
-      };
-      std::vector<Draft> a = blocks(true), b = blocks(false);
-      drafts_ = tiles(a) <= tiles(b) ? std::move(a) : std::move(b);
-    }
-    if (!flat_all_)
+      if (rows <= kFlatRows && d_.prefix_len) flat.push_back(block(0, rows, 0, kFlat, false));
       for (const Sequence& s : sequences_)
         if (flat_own(s) && s.keys) {
           Draft f;
@@ -232,43 +227,62 @@ class Planner {
           add_segs(&f.segs, SharedSeg{s.source, 0, s.base, s.keys, d_.prefix_len, 0, 0, (int32_t)row0, (int32_t)(row0 + n)},
                    kFlatKeys, f.item.least, f.item.greatest);
           finish(&f);
-          drafts_.push_back(std::move(f));
+          flat.push_back(std::move(f));
         }
-    drafts_.erase(std::remove_if(drafts_.begin(), drafts_.end(), [](const Draft& b) { return b.item.tiles == 0; }),
-                  drafts_.end());
-    // Rows of two items are merged, and with them all rows of those items.
-    std::vector<int32_t> cover(rows, 0);
-    for (const Draft& b : drafts_)
+    }
+    double best = 0;
+    const auto consider = [&](std::vector<Draft> blocks) {
+      blocks.insert(blocks.end(), flat.begin(), flat.end());
+      mark_merged(&blocks, rows);
+      const double s = cut(&blocks);
+      if (!drafts_.empty() && s >= best) return;
+      best = s;
+      drafts_ = std::move(blocks);
+    };
+    if (rows <= kFlatRows) return consider({});
+    for (int kind : {kTall, kSplit}) {
+      // Aligned blocks straddle fewer sequences, the others waste fewer rows: fewer tiles decide.
+      const auto tiles = [](const std::vector<Draft>& v) {
+        int64_t n = 0;
+        for (const Draft& b : v) n += b.item.tiles + 2;
+        return n;
+      };
+      std::vector<Draft> a = blocks(kind, true), b = blocks(kind, false);
+      consider(tiles(a) <= tiles(b) ? std::move(a) : std::move(b));
+    }
+  }
+
+  // Drops drafts that see nothing; rows of two items are merged, and with them all rows of those items.
+  static void mark_merged(std::vector<Draft>* drafts, int64_t rows) {
+    drafts->erase(std::remove_if(drafts->begin(), drafts->end(), [](const Draft& b) { return b.item.tiles == 0; }), drafts->end());
+    std::vector<uint8_t> cover(rows, 0);
+    for (const Draft& b : *drafts)
       for (int32_t r = 0; r < b.item.rows; ++r) ++cover[b.item.row0 + r];
-    for (Draft& b : drafts_)
+    for (Draft& b : *drafts)
       for (int32_t r = 0; r < b.item.rows; ++r) b.merged |= cover[b.item.row0 + r] > 1;
   }
 
   static int chunks_for(const Draft& b, double target) {
-    // Flat chunks are whole rounds of the four wavefronts.
-    const double unit = b.item.kind == kTall ? kTallTile : kFlatRound;
-    const int n = b.item.kind == kTall ? b.item.tiles : (b.item.tiles + 3) / 4;
-    const double fixed = b.item.kind == kTall ? kTallItem : kFlatItem;
-    const int fit = std::max(1, (int)std::floor((target - fixed) / unit));
+    const int n = b.units(), fit = std::max(1, (int)std::floor((target - b.fixed()) / b.unit()));
     return (n + fit - 1) / fit;
   }
 
-  // The time at which the last slot ends, longest item first.
-  double span(double target, bool* split) const {
-    std::vector<double> costs;
+  // The time at which the last slot ends, longest unit first, two flat items to a unit.
+  double span(const std::vector<Draft>& drafts, double target) const {
+    std::vector<double> costs, flat;
     double partial_rows = 0;
-    for (const Draft& b : drafts_) {
-      const int c = chunks_for(b, target);
-      const int units = b.item.kind == kTall ? b.item.tiles : (b.item.tiles + 3) / 4;
+    bool split = false;
+    for (const Draft& b : drafts) {
+      const int c = chunks_for(b, target), units = b.units();
       const bool part = c > 1 || b.merged;
       if (part) partial_rows += (double)c * b.item.rows;
-      *split |= part;
-      for (int i = 0; i < c; ++i) {
-        const int n = units * (i + 1) / c - units * i / c;
-        costs.push_back((part ? kPartial : 0) + (b.item.kind == kTall ? kTallItem + kTallTile * n : kFlatItem + kFlatRound * n));
-      }
-      if ((int)costs.size() > kMostSimulated) return 1e30;
+      split |= part;
+      auto& to = b.item.kind == kFlat ? flat : costs;
+      for (int i = 0; i < c; ++i) to.push_back((part ? kPartial : 0) + b.cost(units * (i + 1) / c - units * i / c));
+      if (costs.size() + flat.size() > kMostSimulated) return 1e30;
     }
+    std::sort(flat.begin(), flat.end(), std::greater<double>());
+    for (size_t i = 0; i < flat.size(); i += 2) costs.push_back(flat[i]);
     std::sort(costs.begin(), costs.end(), std::greater<double>());
     std::priority_queue<double, std::vector<double>, std::greater<double>> ends;
     double last = 0;
@@ -281,22 +295,27 @@ class Planner {
       ends.push(start + c);
       last = std::max(last, start + c);
     }
-    return last + (*split ? kMergeLaunch + partial_rows * d_.cache.kv_heads * d_.cache.head_dim * 8 / kBytesPerUs : 0);
+    return last + (split ? kMergeLaunch + partial_rows * d_.cache.kv_heads * d_.cache.head_dim * 8 / kBytesPerUs : 0);
   }
 
-  void cut() {
-    double longest = 0, best_span = 1e30, best = 0;
-    for (const Draft& b : drafts_) longest = std::max(longest, b.cost(b.item.tiles));
-    for (double target = longest; target > kTallItem + kTallTile; target *= target > longest / 2 ? 0.85 : 0.7) {
-      bool split = false;
-      const double s = span(target, &split);
-      if (target == longest || s < best_span * 0.97) {
+  // Chooses every draft's chunks; returns the launch's time.
+  double cut(std::vector<Draft>* drafts) const {
+    double longest = 0;
+    for (const Draft& b : *drafts) longest = std::max(longest, b.cost(b.units()));
+    double best_span = span(*drafts, longest), best = longest;
+    for (double target = longest * 0.85; target > kBlockItem + kSplitTile; target *= target > longest / 2 ? 0.85 : 0.7) {
+      const double s = span(*drafts, target);
+      if (s < best_span * 0.97) {
         best_span = s;
         best = target;
       }
     }
-    if (best_span >= 1e30) best = longest;
-    for (Draft& b : drafts_) b.chunks = best > 0 ? chunks_for(b, best) : 1;
+    double total = 0;
+    for (Draft& b : *drafts) {
+      b.chunks = best > 0 ? chunks_for(b, best) : 1;
+      total += b.cost(b.units());
+    }
+    return best_span < 1e30 ? best_span : total / slots_;  // too many to simulate: the slots are full
   }
 
   void emit() {
@@ -308,8 +327,7 @@ class Planner {
         b.first_part = (int32_t)plan_->partial_rows;
         plan_->partial_rows += (int64_t)b.chunks * rows;
       }
-      const int round = b.item.kind == kTall ? 1 : 4;
-      const int units = (b.item.tiles + round - 1) / round;
+      const int round = b.item.kind == kFlat ? 4 : 1, units = b.units();
       for (int c = 0; c < b.chunks; ++c) {
         int begin = std::min(b.item.tiles, (int)((int64_t)units * c / b.chunks) * round);
         int end = std::min(b.item.tiles, (int)((int64_t)units * (c + 1) / b.chunks) * round);
@@ -329,11 +347,18 @@ class Planner {
         }
         it.seg_end = (int32_t)plan_->segs.size();
         first_groups(&it);
-        items.emplace_back(b.cost(it.tiles), it);
+        items.emplace_back(b.cost((it.tiles + round - 1) / round), it);
       }
     }
+    // Longest first, the flat items behind the others (their workgroups may come first all the same).
     std::stable_sort(items.begin(), items.end(), [](const auto& a, const auto& b) { return a.first > b.first; });
-    for (const auto& i : items) plan_->items.push_back(i.second);
+    std::stable_partition(items.begin(), items.end(), [](const auto& i) { return i.second.kind != kFlat; });
+    for (const auto& i : items) {
+      plan_->items.push_back(i.second);
+      plan_->flat_items += i.second.kind == kFlat;
+    }
+    const size_t blocks = plan_->items.size() - plan_->flat_items;
+    plan_->flat_first = blocks && plan_->flat_items && items[blocks].first > items[0].first;
     merge_rows();
     plan_->info.items = (int32_t)plan_->items.size();
     plan_->info.merged_rows = (int32_t)plan_->merges.size();
@@ -343,7 +368,7 @@ class Planner {
   // The item's own copy of its first segment and of the groups of its first tiles.
   void first_groups(SharedItem* it) const {
     it->seg = plan_->segs[it->seg_begin];
-    const int tile = it->kind == kTall ? kTallKeys : kFlatKeys;
+    const int tile = tile_of(it->kind);
     int32_t seg = it->seg_begin, at = it->seg.tile_begin;
     for (int i = 0; i < 8; ++i) {
       const SharedSeg& s = plan_->segs[seg];

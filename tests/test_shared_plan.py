@@ -6,7 +6,7 @@ import pytest
 import shared_ref as ref
 
 FAKE = 0x100000  # aligned stand-in device address
-TILE, ROWS = {0: 64, 1: 32}, {0: 128, 1: 16}
+TILE, ROWS = {0: 128, 1: 128, 2: 32}, {0: 256, 1: 128, 2: 16}
 
 
 def make(qattn, prefix, queries, own, heads=16, kv=8, dim=128, page=64, paged=True, mask=0, always=176, window=432,
@@ -38,7 +38,7 @@ def check_plan(qattn, prefix, queries, own, heads=16, kv=8, page=64, paged=True,
         first_group.append(len(groups))
         k = np.arange(0, n, 16)
         groups += list((table[k // page] * kv * page + k % page) // 16)
-        groups += [groups[-1]] * (-len(groups) % 4) if n else []
+        groups += [groups[-1]] * (-len(groups) % 8) if n else []
     assert np.array_equal(plan["groups"], groups)
     first_row = np.concatenate([[0], np.cumsum(own)])
     top = prefix + int(own.max(initial=0))
@@ -140,13 +140,13 @@ def test_plans_of_random_batches(qattn):
 def test_plan_fills_the_chip_for_few_rows(qattn):
     # 64 tokens behind 8,192 keys: one block of rows per KV head, cut until most slots have work
     _, info = qattn.shared_plan(make(qattn, 8192, [1] * 64, [200] * 64)[0])
-    assert info.items * 8 >= 512
-    # a full batch needs no cuts
+    assert info.items * 8 >= 400
+    # a full batch fills it too
     _, info = qattn.shared_plan(make(qattn, 5000, [500] * 16, [500] * 16, paged=False)[0])
-    assert info.items * 8 >= 512
+    assert info.items * 8 >= 400
     # masks skip whole tiles of the prefix
     plan, _ = qattn.shared_plan(make(qattn, 8192, [100], [100], mask=1)[0])
-    assert sum(i[5] for i in plan["items"]) <= 2 * (3 + 9 + 2) and plan["items"][:, 6].max() == 0
+    assert sum(i[5] for i in plan["items"]) <= 2 * (2 + 6 + 2) and plan["items"][:, 6].max() <= 1
 
 
 def refuses(qattn, needle, change, **kw):
