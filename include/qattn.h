@@ -463,15 +463,18 @@ typedef struct qattn_shared_info {
 } qattn_shared_info;
 int qattn_shared_run_get_info(const qattn_shared_run* run, qattn_shared_info* info);
 /* Host-only planning (no device; 256 compute units): the plan as int32 words, the counts first:
- * {items, segments, merged rows, tokens, groups, 0, 0, 0}, then per item {first row, rows, first
- * segment, end segment, first partial row or -1, key tiles, kind (0, 1: blocks of 256, 128 rows over
- * 128-key tiles, 2: of 16 rows over 32-key tiles), least query position, greatest, 0, 0, 0,
- * a copy of the first segment, the first eight groups}, per segment {source
+ * {items, segments, merged rows, tokens, groups, runs, 0, 0}, then per item (32 words) {first row, rows,
+ * first segment, end segment, first partial row or -1, key tiles, kind (0, 1: blocks of 256, 128 rows
+ * over 128-key tiles, 2: of 16 rows over 32-key tiles), least query position, greatest, 0, 0, 0, a copy
+ * of the first segment, the eight groups of the first tile (kind 2: 0)}, per segment {source
  * (0 prefix pages, 1 own pages, 2 own rows), whether every row sees all its keys, first group (an
- * index) or first row, keys, position of key 0, first tile, end tile, first row, end row, 0, 0, 0}, per merged row {row, then for up to two groups of partial
- * results: first partial row, count, distance between them, and 0}, per token its position, and the
- * groups: each 16 keys of a page, as its first pool row of KV head 0 over 16; a source's filled up to
- * whole 128-key tiles.  words NULL: only *count. */
+ * index) or first row, keys, position of key 0, first tile, end tile, first row, end row, 0, 0, 0},
+ * per merged row {row, then for up to two groups of partial results: first partial row, count,
+ * distance between them, and 0}, per token its position, and the groups: each 16 keys of a page, as
+ * its first pool row of KV head 0 over 16; a source's filled up to whole 128-key tiles.  Then the
+ * runs of the items of kind 2, eight to an item (16 words): {the first nine words of a segment, its
+ * first tile the run's, the segment, tiles, the first tile's two groups, 0, 0, 0}.
+ * words NULL: only *count. */
 int qattn_shared_plan_describe(const qattn_shared_desc* desc, int32_t* words, int64_t capacity, int64_t* count,
                                qattn_shared_info* info);
 

@@ -319,6 +319,7 @@ int install_shared_plan(qattn_shared_run* run, const qattn_shared_desc& d) {
   };
   const size_t items = put(plan.items.data(), plan.items.size() * sizeof(SharedItem));
   const size_t segs = put(plan.segs.data(), plan.segs.size() * sizeof(SharedSeg));
+  const size_t starts = put(plan.starts.data(), plan.starts.size() * sizeof(SharedStart));
   const size_t merges = put(plan.merges.data(), plan.merges.size() * sizeof(SharedMerge));
   const size_t positions = put(plan.positions.data(), plan.positions.size() * sizeof(int32_t));
   const size_t groups = put(plan.groups.data(), plan.groups.size() * sizeof(int32_t));
@@ -361,6 +362,7 @@ int install_shared_plan(qattn_shared_run* run, const qattn_shared_desc& d) {
   const char* image = static_cast<const char*>(run->image[next]);
   p.items = reinterpret_cast<const SharedItem*>(image + items);
   p.segs = reinterpret_cast<const SharedSeg*>(image + segs);
+  p.starts = reinterpret_cast<const SharedStart*>(image + starts);
   p.merges = reinterpret_cast<const SharedMerge*>(image + merges);
   p.positions = reinterpret_cast<const int32_t*>(image + positions);
   p.groups = reinterpret_cast<const int32_t*>(image + groups);
@@ -496,9 +498,9 @@ int qattn_shared_plan_describe(const qattn_shared_desc* desc, int32_t* words, in
   }
   if (rc) return rc;
   const int32_t head[8] = {(int32_t)plan.items.size(), (int32_t)plan.segs.size(), (int32_t)plan.merges.size(),
-                           (int32_t)plan.positions.size(), (int32_t)plan.groups.size(), 0, 0, 0};
-  *count = 8 + (int64_t)plan.items.size() * 32 + (int64_t)plan.segs.size() * 12 + (int64_t)plan.merges.size() * 8 +
-           (int64_t)plan.positions.size() + (int64_t)plan.groups.size();
+                           (int32_t)plan.positions.size(), (int32_t)plan.groups.size(), (int32_t)plan.starts.size(), 0, 0};
+  *count = 8 + (int64_t)(plan.items.size() * 32 + plan.segs.size() * 12 + plan.merges.size() * 8 + plan.positions.size() +
+                         plan.groups.size() + plan.starts.size() * 16);
   if (info) *info = plan.info;
   if (!words) return QATTN_OK;
   if (capacity < *count) return fail(nullptr, QATTN_EINVAL, "capacity %lld < %lld words", (long long)capacity, (long long)*count);
@@ -512,6 +514,7 @@ int qattn_shared_plan_describe(const qattn_shared_desc* desc, int32_t* words, in
   put(plan.merges.data(), plan.merges.size() * sizeof(SharedMerge));
   put(plan.positions.data(), plan.positions.size() * sizeof(int32_t));
   put(plan.groups.data(), plan.groups.size() * sizeof(int32_t));
+  put(plan.starts.data(), plan.starts.size() * sizeof(SharedStart));
   return QATTN_OK;
 }
 

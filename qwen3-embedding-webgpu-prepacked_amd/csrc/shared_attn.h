@@ -15,10 +15,9 @@ namespace qattn {
 
 constexpr int kSharedThreads = 512;
 // Tall: eight wavefronts x 32 rows share a tile of 128 keys.  Split: four x 32 rows, twice: one four takes the
-// tile's first 64 keys, the other its last.  Flat: four wavefronts x the same 16 rows, a tile of 32 keys
-// each; a workgroup takes two flat items.
+// tile's first 64 keys, the other its last.  Flat: eight wavefronts x the same 16 rows, a tile of 32 keys each.
 constexpr int kTallRows = 256, kSplitRows = 128, kTallKeys = 128;
-constexpr int kFlatRows = 16, kFlatKeys = 32;
+constexpr int kFlatRows = 16, kFlatKeys = 32, kFlatWaves = 8;
 constexpr int32_t kMaxPosition = 1 << 30;
 
 enum SharedSource { kPrefixPages = 0, kOwnPages = 1, kOwnRows = 2 };
@@ -34,15 +33,22 @@ struct SharedSeg {
   int32_t pad[3];
 };
 // Rows row0 .. row0 + rows - 1 over the tiles of segments seg_begin .. seg_end - 1.  Results go to the output
-// (part < 0) or, unnormalised, to partial rows part, part + 1, ...  The first segment, and the groups of the
-// first tiles (one for each wavefront; flat: two for each wavefront's first tile), come with the item,
-// so that a workgroup asks for its first keys after one dependent load.
+// (part < 0) or, unnormalised, to partial rows part, part + 1, ...  The first segment and the groups of a
+// block's first tile come with the item, so that a workgroup asks for its first keys after one dependent load.
 struct SharedItem {
   int32_t row0, rows, seg_begin, seg_end, part, tiles, kind;
   int32_t least, greatest;  // query positions among the rows
   int32_t pad[3];
   SharedSeg seg;
   int32_t group[8];
+};
+// The tiles that one wavefront of a flat item takes, one after another: `tiles` of them, from tile_begin of
+// its copy of segment `seg` on; `group`: the first one's.
+struct SharedStart {
+  int32_t source, whole, base, keys, position, tile_begin, tile_end, row_begin, row_end;
+  int32_t seg, tiles;
+  int32_t group[2];
+  int32_t pad[3];
 };
 // A row whose results are merged: `count` partial rows from `first` on, `step` apart, in two groups.
 struct SharedMerge {
@@ -52,11 +58,13 @@ struct SharedMerge {
   } group[2];
   int32_t pad;
 };
-static_assert(sizeof(SharedItem) == 128 && sizeof(SharedSeg) == 48 && sizeof(SharedMerge) == 32, "plan words");
+static_assert(sizeof(SharedItem) == 128 && sizeof(SharedSeg) == 48 && sizeof(SharedStart) == 64 && sizeof(SharedMerge) == 32,
+              "plan words");
 
 struct SharedPlan {
   std::vector<SharedItem> items;
   std::vector<SharedSeg> segs;
+  std::vector<SharedStart> starts;  // kFlatWaves to a flat item, in their order
   std::vector<SharedMerge> merges;
   std::vector<int32_t> positions;  // of each query
   std::vector<int32_t> groups;
@@ -78,6 +86,7 @@ struct SharedParams {
   int64_t q_stride, o_stride, row_stride[2];
   const SharedItem* items;
   const SharedSeg* segs;
+  const SharedStart* starts;
   const SharedMerge* merges;
   const int32_t* positions;
   const int32_t* groups;

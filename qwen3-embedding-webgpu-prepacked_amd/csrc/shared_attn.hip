@@ -87,22 +87,20 @@ __device__ inline int item_group(const SharedParams& p, int i, int which) {
   return ((const const_i32*)(p.items + i))[24 + which];
 }
 
-// The tiles of an item one after another, through its segments.
+// Tiles one after another, through segments: of a block, or of one wavefront of a flat item.
 struct Cursor {
   const const_i32* words;
   int tile;
   SharedSeg seg;
   __device__ Cursor(const SharedParams& p, const SharedItem& it)
       : words((const const_i32*)(p.segs + it.seg_begin)), tile(it.seg.tile_begin), seg(it.seg) {}
-  // `n` tiles on; the item has that many.
-  __device__ void advance(int n) {
-    tile += n;
-    while (tile >= seg.tile_end) {
-      const int over = tile - seg.tile_end;
-      words += sizeof(SharedSeg) / 4;
-      seg = seg_at(words);
-      tile = seg.tile_begin + over;
-    }
+  __device__ Cursor(const SharedParams& p, const const_i32* start)
+      : words((const const_i32*)(p.segs + start[9])), tile(start[5]), seg(seg_at(start)) {}
+  __device__ void advance() {
+    if (++tile < seg.tile_end) return;
+    words += sizeof(SharedSeg) / 4;
+    seg = seg_at(words);
+    tile = seg.tile_begin;
   }
 };
 
@@ -158,16 +156,22 @@ __device__ inline void expand(u32x4 codes, float scale, u32x4 (&out)[2]) {
 // rows that do see the key get them added at the end (p times an infinity is that infinity, whatever the
 // reference).
 template <bool BF16>
-__device__ inline bool drop_nonfinite(u32x4& chunk) {
+__device__ inline void drop_nonfinite(u32x4& chunk) {
   constexpr uint32_t kExp = Elem<BF16>::kExponent;
-  bool any = false;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const bool low = (chunk[e] & kExp) == kExp, high = ((chunk[e] >> 16) & kExp) == kExp;
-    any |= low | high;
     chunk[e] &= (low ? 0xFFFF0000u : 0xFFFFFFFFu) & (high ? 0x0000FFFFu : 0xFFFFFFFFu);
   }
-  return any;
+}
+// Bits 15 and 31 of the result are set if `seen`'s were or an element is infinite or NaN: adding the
+// exponent's lowest bit carries out of an exponent of ones, and of no other.
+template <bool BF16>
+__device__ inline uint32_t see_nonfinite(uint32_t seen, u32x4 chunk) {
+  constexpr uint32_t kExp = Elem<BF16>::kExponent, kLow = kExp & (0u - kExp);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) seen |= (chunk[e] & (kExp << 16 | kExp)) + (kLow << 16 | kLow);
+  return seen;
 }
 // Elements d .. d + 3 of key `key`'s V.
 template <bool BF16, int FORMAT, int DIM>
@@ -192,11 +196,9 @@ __device__ inline float nonfinite(float v, bool seen) { return seen && !(fabsf(v
 // Calls add(value, seen) for every key of the item's tiles first, first + step, ... (of `size` keys) that not
 // all rows see: value(d) is elements d .. d + 3 of its V, seen whether row `row` at position `at` sees it.
 template <bool BF16, int FORMAT, int DIM, class Add>
-__device__ inline void each_nonfinite(const SharedParams& p, const Keys<FORMAT, DIM>& keys, const SharedItem& it, int row, int at,
-                                      int size, int first, int step, Add add) {
-  Cursor c(p, it);
-  c.advance(first);
-  for (int t = first;;) {
+__device__ inline void each_nonfinite(const SharedParams& p, const Keys<FORMAT, DIM>& keys, Cursor c, int tiles, int row,
+                                      int at, int size, Add add) {
+  for (int t = 0;;) {
     const SharedSeg s = c.seg;
     if (!s.whole) {
       const int mine = row >= s.row_begin && row < s.row_end ? at : -1;
@@ -206,8 +208,8 @@ __device__ inline void each_nonfinite(const SharedParams& p, const Keys<FORMAT, 
             pos <= mine && (p.mask == QATTN_MASK_CAUSAL || pos < p.prefix || pos > mine - p.window));
       }
     }
-    if ((t += step) >= it.tiles) return;
-    c.advance(step);
+    if (++t >= tiles) return;
+    c.advance();
   }
 }
 
@@ -260,29 +262,36 @@ struct Tall {
   }
 
   // The loaded K (I = 0) or V (1) into LDS as 16-bit elements.  partly: infinities and NaN are
-  // taken out (of V, in tiles that some row sees only part of); returns whether this lane had any.
+  // taken out (of V, in tiles that some row sees only part of); returns whether there were any.
   template <int I>
   __device__ bool store(char* lds, bool rows, int wave, int lane, bool partly) {
-    bool any = false;
-    const auto put = [&](int r, int c, u32x4 x) {
-      if (I && partly) any |= drop_nonfinite<BF16>(x);
-      *reinterpret_cast<u32x4*>(lds + (I ? v_at(r, c) : k_at(r, c))) = x;
-    };
-    if (!kCodes || rows) {
+    const auto each = [&](auto put) {
+      if (!kCodes || rows) {
 #pragma unroll
-      for (int j = 0; j < kLoads16; ++j)
-        put(16 * wave + j * kRows16 + lane / kChunks16, lane % kChunks16, raw[I][j]);
-    } else {
+        for (int j = 0; j < kLoads16; ++j)
+          put(16 * wave + j * kRows16 + lane / kChunks16, lane % kChunks16, raw[I][j]);
+      } else {
 #pragma unroll
-      for (int j = 0; j < kLoads8; ++j) {
-        const int r = 16 * wave + j * kRows8 + lane / kChunks8, c = 2 * (lane % kChunks8);
-        u32x4 x[2];
-        expand<BF16, FORMAT>(raw[I][j], scale[I][kCodes ? j : 0], x);
-        put(r, c, x[0]);
-        put(r, c + 1, x[1]);
+        for (int j = 0; j < kLoads8; ++j) {
+          const int r = 16 * wave + j * kRows8 + lane / kChunks8, c = 2 * (lane % kChunks8);
+          u32x4 x[2];
+          expand<BF16, FORMAT>(raw[I][j], scale[I][kCodes ? j : 0], x);
+          put(r, c, x[0]);
+          put(r, c + 1, x[1]);
+        }
       }
-    }
-    return any;
+    };
+    uint32_t seen = 0;
+    each([&](int r, int c, u32x4 x) {
+      if (I && partly) seen = see_nonfinite<BF16>(seen, x);
+      *reinterpret_cast<u32x4*>(lds + (I ? v_at(r, c) : k_at(r, c))) = x;
+    });
+    if (!I || !partly || !__any(seen & 0x80008000u)) return false;
+    each([&](int r, int c, u32x4 x) {
+      drop_nonfinite<BF16>(x);
+      *reinterpret_cast<u32x4*>(lds + v_at(r, c)) = x;
+    });
+    return true;
   }
 };
 
@@ -335,7 +344,7 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
     tile.template load<1>(keys, spot, lane);
     next = Info{s.whole, s.position + ahead.tile * kTallKeys, s.position + s.keys - 1, s.row_begin, s.row_end};
     if (++asked < it.tiles) {
-      ahead.advance(1);
+      ahead.advance();
       group = group_of(p, ahead.seg, ahead.tile * kTallKeys + 16 * wave, zero);
     }
   };
@@ -483,7 +492,7 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
   if (found) *dropped = 1;
   __syncthreads();
   if (*dropped && part_begin == 0)
-    each_nonfinite<BF16, FORMAT, DIM>(p, keys, it, row, at, kTallKeys, 0, 1, [&](auto value, bool seen) {
+    each_nonfinite<BF16, FORMAT, DIM>(p, keys, Cursor(p, it), it.tiles, row, at, kTallKeys, [&](auto value, bool seen) {
 #pragma unroll
       for (int db = 0; db < kBlocks; ++db)
 #pragma unroll
@@ -551,12 +560,12 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
 template <bool BF16, int FORMAT, int DIM>
 struct Flat {
   static constexpr int kRow = 2 * DIM;
-  static constexpr int kLds = 4 * kFlatKeys * kRow;  // each wavefront's V tile, later its 16 rows of O in f32
+  static constexpr int kLds = kFlatWaves * kFlatKeys * kRow;  // each wavefront's V tile, later its 16 rows of O in f32
   static constexpr int kSteps = DIM / 32;            // K: two 16-byte loads of codes, four of 16-bit elements per 128 dims
   static constexpr int kChunks16 = kRow / 16, kRows16 = 64 / kChunks16, kLoads16 = 16 / kRows16;
   static constexpr int kChunks8 = DIM / 16, kRows8 = 64 / kChunks8, kLoads8 = 16 / kRows8;
   static constexpr bool kCodes = FORMAT != QATTN_KV_16BIT;
-  static_assert(kLds >= 4 * kFlatRows * DIM * 4, "O of four wavefronts");
+  static_assert(kLds >= kFlatWaves * kFlatRows * DIM * 4, "O of the wavefronts");
 
   // Eight rows by two chunks cover all 64 banks.
   __device__ static uint32_t v_at(int r, int c) { return r * kRow + ((c ^ (DIM == 128 ? (r & 7) << 1 : (r & 6))) << 4); }
@@ -615,28 +624,35 @@ struct Flat {
     }
   }
   __device__ bool store(char* lds, const SharedSeg& s, int lane, bool partly) const {
-    bool any = false;
-    const auto put = [&](int r, int c, u32x4 x) {
-      if (partly) any |= drop_nonfinite<BF16>(x);
-      *reinterpret_cast<u32x4*>(lds + v_at(r, c)) = x;
-    };
+    const auto each = [&](auto put) {
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      if (!kCodes || s.source == kOwnRows) {
+      for (int b = 0; b < 2; ++b) {
+        if (!kCodes || s.source == kOwnRows) {
 #pragma unroll
-        for (int j = 0; j < kLoads16; ++j) put(16 * b + j * kRows16 + lane / kChunks16, lane % kChunks16, v[b][j]);
-      } else {
+          for (int j = 0; j < kLoads16; ++j) put(16 * b + j * kRows16 + lane / kChunks16, lane % kChunks16, v[b][j]);
+        } else {
 #pragma unroll
-        for (int j = 0; j < kLoads8; ++j) {
-          const int r = 16 * b + j * kRows8 + lane / kChunks8, c = 2 * (lane % kChunks8);
-          u32x4 x[2];
-          expand<BF16, FORMAT>(v[b][j], vs[b][kCodes ? j : 0], x);
-          put(r, c, x[0]);
-          put(r, c + 1, x[1]);
+          for (int j = 0; j < kLoads8; ++j) {
+            const int r = 16 * b + j * kRows8 + lane / kChunks8, c = 2 * (lane % kChunks8);
+            u32x4 x[2];
+            expand<BF16, FORMAT>(v[b][j], vs[b][kCodes ? j : 0], x);
+            put(r, c, x[0]);
+            put(r, c + 1, x[1]);
+          }
         }
       }
-    }
-    return partly && __any(any);
+    };
+    uint32_t seen = 0;
+    each([&](int r, int c, u32x4 x) {
+      if (partly) seen = see_nonfinite<BF16>(seen, x);
+      *reinterpret_cast<u32x4*>(lds + v_at(r, c)) = x;
+    });
+    if (!partly || !__any(seen & 0x80008000u)) return false;
+    each([&](int r, int c, u32x4 x) {
+      drop_nonfinite<BF16>(x);
+      *reinterpret_cast<u32x4*>(lds + v_at(r, c)) = x;
+    });
+    return true;
   }
 };
 
@@ -645,12 +661,12 @@ __device__ inline void flat_item(const SharedParams& p, const SharedItem& it, in
   typedef Flat<BF16, FORMAT, DIM> T;
   constexpr int kBlocks = DIM / 16;
   const int lane = threadIdx.x & 63, n = lane & 15, c = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
-  char* lds = lds_all + wave * (T::kLds / 4);
-  const int end_row = it.row0 + it.rows, row = it.row0 + n;
-  const bool exists = row < end_row;
-  const int token = exists ? row / p.group : 0;
-  const int at = exists ? p.positions[token] : -1;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  char* lds = lds_all + wave * (T::kLds / kFlatWaves);
+  // Lanes past the item's rows repeat the last one; their results go nowhere.
+  const int end_row = it.row0 + it.rows, row = min(it.row0 + n, end_row - 1);
+  const int token = row / p.group;
+  const int at = p.positions[token];
   const bool local = p.mask != QATTN_MASK_CAUSAL;
 
   // Q (B operand): this lane's row, the dims of K's chunks.
@@ -659,8 +675,7 @@ __device__ inline void flat_item(const SharedParams& p, const SharedItem& it, in
     const int head = kvh * p.group + row - token * p.group;
     const uint16_t* src = p.q + (int64_t)token * p.q_stride + head * DIM + 16 * c;
 #pragma unroll
-    for (int st = 0; st < T::kSteps; ++st)
-      q[st] = exists ? *reinterpret_cast<const u32x4*>(src + 64 * (st >> 1) + 8 * (st & 1)) : u32x4{};
+    for (int st = 0; st < T::kSteps; ++st) q[st] = *reinterpret_cast<const u32x4*>(src + 64 * (st >> 1) + 8 * (st & 1));
   }
   f4 o[kBlocks];
 #pragma unroll
@@ -670,24 +685,25 @@ __device__ inline void flat_item(const SharedParams& p, const SharedItem& it, in
   const int vr = 4 * c + (n >> 2);
 
   const Keys<FORMAT, DIM> keys(p, kvh);
-  if (wave < it.tiles) {
+  const const_i32* start = (const const_i32*)(p.starts + index * kFlatWaves + wave);
+  const int tiles = start[10];
+  if (tiles) {
     bool found = false;  // infinities or NaN were dropped from V
-    Cursor now(p, it);
-    now.advance(wave);
+    Cursor now(p, start);
     T tile;
-    uint32_t group[2] = {(uint32_t)item_group(p, index, 2 * wave), (uint32_t)item_group(p, index, 2 * wave + 1)};
+    uint32_t group[2] = {(uint32_t)start[11], (uint32_t)start[12]};
     tile.load(keys, now.seg, now.tile, group, lane);
     // The next tile's groups are on the way while this one is worked on.
     int zero = 0;
     asm volatile("" : "+v"(zero));
     Cursor ahead = now;
     const auto ask_groups = [&]() {
-      ahead.advance(4);
+      ahead.advance();
 #pragma unroll
       for (int b = 0; b < 2; ++b) group[b] = group_of(p, ahead.seg, ahead.tile * kFlatKeys + 16 * b, zero);
     };
-    if (wave + 4 < it.tiles) ask_groups();
-    for (int t = wave; t < it.tiles; t += 4) {
+    if (tiles > 1) ask_groups();
+    for (int t = 0; t < tiles; ++t) {
       const SharedSeg s = now.seg;
       const int first = now.tile * kFlatKeys, from = s.position + first;
       f4 sc[2] = {};
@@ -700,10 +716,10 @@ __device__ inline void flat_item(const SharedParams& p, const SharedItem& it, in
       }
       const bool part = !s.whole;
       found |= tile.store(lds, s, lane, part);
-      if (t + 4 < it.tiles) {
+      if (t + 1 < tiles) {
         now = ahead;
         tile.load(keys, now.seg, now.tile, group, lane);
-        if (t + 8 < it.tiles) ask_groups();
+        if (t + 2 < tiles) ask_groups();
       }
       const bool mine = row >= s.row_begin && row < s.row_end;
       const int limit = min(mine ? at : -1, s.position + s.keys - 1);
@@ -745,7 +761,7 @@ __device__ inline void flat_item(const SharedParams& p, const SharedItem& it, in
       }
     }
     if (found)
-      each_nonfinite<BF16, FORMAT, DIM>(p, keys, it, row, at, kFlatKeys, wave, 4, [&](auto value, bool seen) {
+      each_nonfinite<BF16, FORMAT, DIM>(p, keys, Cursor(p, start), tiles, row, at, kFlatKeys, [&](auto value, bool seen) {
 #pragma unroll
         for (int db = 0; db < kBlocks; ++db) {
           const f4 x = value(16 * db + 4 * c);
@@ -755,30 +771,30 @@ __device__ inline void flat_item(const SharedParams& p, const SharedItem& it, in
       });
   }
 
-  // The four wavefronts' sums: lane (n, c) holds dims 16 db + 4 c .. + 3 of row n.
+  // The wavefronts' sums: lane (n, c) holds dims 16 db + 4 c .. + 3 of row n.
   l = rows_sum(l);
   float* own = reinterpret_cast<float*>(lds);
 #pragma unroll
   for (int db = 0; db < kBlocks; ++db) *reinterpret_cast<f4*>(own + n * DIM + 16 * db + 4 * c) = o[db];
-  if (c == 0) stats[16 * wave + n] = float2{m, l};
+  if (c == 0) stats[kFlatRows * wave + n] = float2{m, l};
   __syncthreads();
-  const int r = (threadIdx.x & 255) >> 4, d = (threadIdx.x & 15) * (DIM / 16);
+  constexpr int kLanes = kSharedThreads / kFlatRows, kEach = DIM / kLanes;
+  typedef float Part __attribute__((ext_vector_type(kEach)));
+  const int r = threadIdx.x / kLanes, d = threadIdx.x % kLanes * kEach;
   if (it.row0 + r >= end_row) return;
-  float2 st[4];
+  float2 st[kFlatWaves];
   float top = kNone, sum = 0.f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    st[w] = stats[16 * w + r];
+  for (int w = 0; w < kFlatWaves; ++w) {
+    st[w] = stats[kFlatRows * w + r];
     top = fmaxf(top, st[w].x);
   }
-  float x[DIM / 16] = {};
+  Part x = {};
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
+  for (int w = 0; w < kFlatWaves; ++w) {
     const float f = __builtin_amdgcn_exp2f(st[w].x - (top == kNone ? 0.f : top));
     sum += f * st[w].y;
-    const float* src = reinterpret_cast<const float*>(lds_all + w * (T::kLds / 4)) + r * DIM + d;
-#pragma unroll
-    for (int e = 0; e < DIM / 16; ++e) x[e] += f * src[e];
+    x += f * *reinterpret_cast<const Part*>(reinterpret_cast<const float*>(lds_all + w * (T::kLds / kFlatWaves)) + r * DIM + d);
   }
   const int out_row = it.row0 + r, out_token = out_row / p.group;
   if (it.part < 0) {
@@ -786,11 +802,10 @@ __device__ inline void flat_item(const SharedParams& p, const SharedItem& it, in
     uint32_t* dst = reinterpret_cast<uint32_t*>(p.o + (int64_t)out_token * p.o_stride +
                                                 (kvh * p.group + out_row - out_token * p.group) * DIM + d);
 #pragma unroll
-    for (int e = 0; e < DIM / 16; e += 2) dst[e / 2] = narrow2<BF16>(x[e] * inv, x[e + 1] * inv);
+    for (int e = 0; e < kEach; e += 2) dst[e / 2] = narrow2<BF16>(x[e] * inv, x[e + 1] * inv);
   } else {
     const int64_t part = ((int64_t)it.part + r) * p.kv_heads + kvh;
-#pragma unroll
-    for (int e = 0; e < DIM / 16; ++e) p.part_o[part * DIM + d + e] = x[e];
+    *reinterpret_cast<Part*>(p.part_o + part * DIM + d) = x;
     if (d == 0) p.part_ml[part] = float2{top, sum};
   }
 }
@@ -798,24 +813,27 @@ __device__ inline void flat_item(const SharedParams& p, const SharedItem& it, in
 template <bool BF16, int FORMAT, int DIM>
 __global__ __launch_bounds__(kSharedThreads, 2) void shared_attn_kernel(SharedParams p) {
   constexpr int kTallLds = Tall<BF16, FORMAT, DIM>::kLds, kFlatLds = Flat<BF16, FORMAT, DIM>::kLds;
-  static_assert(kTallLds >= 2 * kFlatLds && kTallLds >= 4 * 32 * DIM * 4, "two flat items; O of four wavefronts");
+  static_assert(kTallLds >= kFlatLds && kTallLds >= 4 * 32 * DIM * 4, "O of four wavefronts");
   __shared__ __attribute__((aligned(1024))) char lds[kTallLds];
   __shared__ __attribute__((aligned(16))) float2 stats[128];
   __shared__ uint32_t dropped;
   const int kvh = (int)(blockIdx.x % (uint32_t)p.kv_heads);
   const int unit = (int)(blockIdx.x / (uint32_t)p.kv_heads);
-  const int pairs = (p.n_flat + 1) / 2;
-  const int block = p.flat_first ? unit - pairs : unit;
-  if (block >= 0 && block < p.n_blocks) {
-    tall_item<BF16, FORMAT, DIM>(p, item_at(p, block), block, kvh, lds, stats, &dropped);
-  } else {
-    const int half = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
-    const int flat = 2 * (p.flat_first ? unit : unit - p.n_blocks) + half;
-    const int index = p.n_blocks + min(flat, p.n_flat - 1);
-    SharedItem it = item_at(p, index);
-    if (flat >= p.n_flat) it.rows = it.tiles = 0;  // the last pair's second half: along for the barrier
-    flat_item<BF16, FORMAT, DIM>(p, it, index, kvh, lds + half * kFlatLds, stats + 64 * half);
-  }
+  const int index = !p.flat_first ? unit : unit < p.n_flat ? p.n_blocks + unit : unit - p.n_flat;
+  const SharedItem it = item_at(p, index);
+  if (index < p.n_blocks)
+    tall_item<BF16, FORMAT, DIM>(p, it, index, kvh, lds, stats, &dropped);
+  else
+    flat_item<BF16, FORMAT, DIM>(p, it, index - p.n_blocks, kvh, lds, stats);
+}
+
+// Launches of flat items alone: with half the LDS, a workgroup starts sooner.
+template <bool BF16, int FORMAT, int DIM>
+__global__ __launch_bounds__(kSharedThreads, 2) void shared_flat_kernel(SharedParams p) {
+  __shared__ __attribute__((aligned(1024))) char lds[Flat<BF16, FORMAT, DIM>::kLds];
+  __shared__ __attribute__((aligned(16))) float2 stats[kFlatWaves * kFlatRows];
+  const int kvh = (int)(blockIdx.x % (uint32_t)p.kv_heads), index = (int)(blockIdx.x / (uint32_t)p.kv_heads);
+  flat_item<BF16, FORMAT, DIM>(p, item_at(p, index), index, kvh, lds, stats);
 }
 
 // Merged rows: sum over a row's partial rows of 2^(m_i - max m) times its sums; a partial row that saw no
@@ -895,8 +913,11 @@ __global__ __launch_bounds__(kMergeThreads) void shared_merge_kernel(SharedParam
 
 template <bool BF16, int FORMAT, int DIM>
 void launch_attn(const SharedParams& p, hipStream_t stream) {
-  const unsigned units = p.n_blocks + (p.n_flat + 1) / 2;
-  hipLaunchKernelGGL((shared_attn_kernel<BF16, FORMAT, DIM>), dim3(units * p.kv_heads), dim3(kSharedThreads), 0, stream, p);
+  const dim3 grid((unsigned)(p.n_blocks + p.n_flat) * p.kv_heads);
+  if (p.n_blocks == 0)
+    hipLaunchKernelGGL((shared_flat_kernel<BF16, FORMAT, DIM>), grid, dim3(kSharedThreads), 0, stream, p);
+  else
+    hipLaunchKernelGGL((shared_attn_kernel<BF16, FORMAT, DIM>), grid, dim3(kSharedThreads), 0, stream, p);
 }
 template <bool BF16, int DIM>
 hipError_t launch(const SharedParams& p, int format, hipStream_t stream) {

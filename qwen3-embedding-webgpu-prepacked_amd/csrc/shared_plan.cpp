@@ -11,6 +11,8 @@
 // sizes and a range of chunk sizes, the time at which the last of the GPU's slots ends, by a cost model.
 #include <algorithm>
 #include <cmath>
+#include <cstddef>
+#include <cstring>
 #include <queue>
 
 #include "shared_attn.h"
@@ -19,12 +21,13 @@ namespace qattn {
 
 namespace {
 
-// Costs in microseconds, from measured launches (one workgroup to a CU): an item's start and end, a 128-key
-// tile of a 256- and of a 128-row block, a round of four 32-key tiles of a pair of flat items, an item's
-// partial results, the second launch, and the partial rows' bytes (written and read).
-constexpr double kBlockItem = 4.0, kTallTile = 3.6, kSplitTile = 2.0, kFlatItem = 3.0, kFlatRound = 1.4;
-constexpr double kPartial = 1.0, kMergeLaunch = 4.0, kBytesPerUs = 5e6;
-constexpr int kMostSimulated = 16384;
+// Costs in microseconds, from measured launches (one workgroup to a CU): a block, and each of its 128-key tiles
+// with 256 and with 128 rows; a flat item, and the bytes that it reads; partial results; the second launch;
+// bytes that all items read from memory.
+constexpr double kBlockItem = 5.9, kTallTile = 4.0, kSplitTile = 2.4, kFlatItem = 3.2, kItemBytesPerUs = 45e3;
+constexpr double kFlatRound = 0.3, kFlatInt8 = 1.1, kFlatMasked = 0.4;
+constexpr double kPartial = 0.5, kMergeLaunch = 2.8, kBytesPerUs = 5e6;
+constexpr int kMostSimulated = 16384, kMostFlatRows = 512;
 
 struct Sequence {
   int32_t first, queries, keys;  // first query; own keys
@@ -34,20 +37,18 @@ struct Sequence {
 struct Draft {
   SharedItem item;
   std::vector<SharedSeg> segs;
+  int masked = 0;       // tiles that not every row sees whole
   bool merged = false;  // its rows have partial results elsewhere too
   int chunks = 1, first_part = 0;
-  // Units of work that cuts leave whole (tiles; rounds of the four wavefronts), and their cost.
-  int units() const { return item.kind == kFlat ? (item.tiles + 3) / 4 : item.tiles; }
-  double fixed() const { return item.kind == kFlat ? kFlatItem : kBlockItem; }
-  double unit() const { return item.kind == kFlat ? kFlatRound : item.kind == kTall ? kTallTile : kSplitTile; }
-  double cost(int n) const { return fixed() + unit() * n; }
+  int units() const { return item.kind == kFlat ? (item.tiles + kFlatWaves - 1) / kFlatWaves : item.tiles; }
 };
 
 class Planner {
  public:
   Planner(const qattn_shared_desc& d, int compute_units, SharedPlan* plan)
       : d_(d), plan_(plan), group_(d.q_heads / d.cache.kv_heads),
-        slots_(std::max(1, compute_units / d.cache.kv_heads)) {}
+        slots_(std::max(1, compute_units / d.cache.kv_heads)),
+        key_bytes_(d.cache.head_dim * (d.cache.format == QATTN_KV_16BIT ? 4 : 2)) {}
 
   void run() {
     read();
@@ -125,20 +126,26 @@ class Planner {
     add((int32_t)(start / tile), start < end ? tiles(end) : (int32_t)(start / tile));
   }
 
-  // A block's segments: the prefix, and the own keys of its sequences that are not left to flat items.
-  Draft block(int64_t row0, int64_t rows, size_t first_sequence, int kind, bool with_own) const {
+  // Sequences by the rows that they have: whose own keys an item visits.
+  enum Own { kLong = 1, kShort = 2, kAll = 3 };
+  bool chosen(const Sequence& s, Own own) const {
+    return own & ((int64_t)s.queries * group_ <= kFlatRows ? kShort : kLong);
+  }
+
+  // A block's segments: the prefix if asked for, and the own keys of its sequences that `own` names.
+  Draft block(int64_t row0, int64_t rows, size_t first_sequence, int kind, bool prefix, Own own) const {
     const int tile = tile_of(kind);
     Draft b;
     b.item = SharedItem{(int32_t)row0, (int32_t)rows, 0, 0, -1, 0, kind};
     const int32_t t0 = (int32_t)(row0 / group_), t1 = (int32_t)((row0 + rows - 1) / group_);
     b.item.least = *std::min_element(&plan_->positions[t0], &plan_->positions[t1] + 1);
     b.item.greatest = *std::max_element(&plan_->positions[t0], &plan_->positions[t1] + 1);
-    if (d_.prefix_len)
+    if (prefix && d_.prefix_len)
       add_segs(&b.segs, SharedSeg{kPrefixPages, 0, 0, d_.prefix_len, 0, 0, 0, (int32_t)row0, (int32_t)(row0 + rows)}, tile,
                b.item.least, b.item.greatest);
-    for (size_t i = first_sequence; with_own && i < sequences_.size() && sequences_[i].first <= t1; ++i) {
+    for (size_t i = first_sequence; i < sequences_.size() && sequences_[i].first <= t1; ++i) {
       const Sequence& s = sequences_[i];
-      if (flat_own(s)) continue;
+      if (!chosen(s, own)) continue;
       const int64_t begin = std::max<int64_t>(row0, (int64_t)s.first * group_);
       const int64_t end = std::min<int64_t>(row0 + rows, ((int64_t)s.first + s.queries) * group_);
       if (begin >= end || !s.keys) continue;
@@ -169,16 +176,16 @@ class Planner {
         part.tile_begin = t;
         while (t < s.tile_end && whole(t) == (part.whole != 0)) ++t;
         part.tile_end = t;
+        if (!part.whole) b->masked += part.tile_end - part.tile_begin;
         b->segs.push_back(part);
       }
     }
   }
 
-  bool flat_own(const Sequence& s) const { return !flat_all_ && (int64_t)s.queries * group_ <= kFlatRows; }
-
-  // Blocks of stacked rows: `aligned` starts a block at every sequence of a block's rows or more.
-  std::vector<Draft> blocks(int kind, bool aligned) const {
-    const int64_t most = kind == kTall ? kTallRows : kSplitRows;
+  // Blocks of stacked rows of the sequences that have something to visit: `aligned` starts a block at every
+  // sequence of a block's rows or more.
+  std::vector<Draft> blocks(int kind, bool aligned, bool prefix, Own own) const {
+    const int64_t most = kind == kTall ? kTallRows : kind == kSplit ? kSplitRows : kFlatRows;
     std::vector<Draft> out;
     int64_t begin = -1, end = 0;  // pending rows
     size_t first = 0;             // a sequence at or before them
@@ -186,13 +193,13 @@ class Planner {
       while (begin >= 0 && begin < upto) {
         while (first < sequences_.size() && ((int64_t)sequences_[first].first + sequences_[first].queries) * group_ <= begin) ++first;
         const int64_t rows = std::min<int64_t>(most, upto - begin);
-        out.push_back(block(begin, rows, first, kind, true));
+        out.push_back(block(begin, rows, first, kind, prefix, own));
         begin += rows;
       }
       begin = -1;
     };
     for (const Sequence& s : sequences_) {
-      if (!d_.prefix_len && flat_own(s)) {
+      if (!(prefix && d_.prefix_len) && !chosen(s, own)) {
         flush(end);
         continue;
       }
@@ -207,48 +214,47 @@ class Planner {
     return out;
   }
 
+  // The fewest tiles: aligned blocks straddle fewer sequences, the others waste fewer rows.
+  std::vector<Draft> best_blocks(int kind, bool prefix, Own own) const {
+    const auto tiles = [](const std::vector<Draft>& v) {
+      int64_t n = 0;
+      for (const Draft& b : v) n += b.item.tiles + 2;
+      return n;
+    };
+    std::vector<Draft> a = blocks(kind, true, prefix, own), b = blocks(kind, false, prefix, own);
+    return tiles(a) <= tiles(b) ? a : b;
+  }
+
   // The drafts that suit the batch best, cut.
   void draft() {
-    if (sequences_.empty()) return;
     const int64_t rows = (int64_t)plan_->positions.size() * group_;
-    std::vector<Draft> flat;
-    if (rows <= kFlatRows && sequences_.size() == 1) {
-      // One short sequence: prefix and own keys in one item.
-      flat_all_ = true;
-      flat.push_back(block((int64_t)sequences_[0].first * group_, rows, 0, kFlat, true));
-    } else {
-      if (rows <= kFlatRows && d_.prefix_len) flat.push_back(block(0, rows, 0, kFlat, false));
-      for (const Sequence& s : sequences_)
-        if (flat_own(s) && s.keys) {
-          Draft f;
-          const int64_t row0 = (int64_t)s.first * group_, n = (int64_t)s.queries * group_;
-          f.item = SharedItem{(int32_t)row0, (int32_t)n, 0, 0, -1, 0, kFlat, plan_->positions[s.first],
-                              plan_->positions[s.first + s.queries - 1]};
-          add_segs(&f.segs, SharedSeg{s.source, 0, s.base, s.keys, d_.prefix_len, 0, 0, (int32_t)row0, (int32_t)(row0 + n)},
-                   kFlatKeys, f.item.least, f.item.greatest);
-          finish(&f);
-          flat.push_back(std::move(f));
-        }
-    }
     double best = 0;
-    const auto consider = [&](std::vector<Draft> blocks) {
-      blocks.insert(blocks.end(), flat.begin(), flat.end());
-      mark_merged(&blocks, rows);
-      const double s = cut(&blocks);
+    const auto consider = [&](std::vector<Draft> drafts, const std::vector<Draft>& more) {
+      drafts.insert(drafts.end(), more.begin(), more.end());
+      mark_merged(&drafts, rows);
+      const double s = cut(&drafts);
       if (!drafts_.empty() && s >= best) return;
       best = s;
-      drafts_ = std::move(blocks);
+      drafts_ = std::move(drafts);
     };
-    if (rows <= kFlatRows) return consider({});
+    // The own keys of short sequences, which waste most of a larger block: in flat items, several
+    // sequences to an item or each by itself.
+    const std::vector<Draft> packed = blocks(kFlat, false, false, kShort);
+    std::vector<Draft> single;
+    for (size_t i = 0; i < sequences_.size(); ++i) {
+      const Sequence& s = sequences_[i];
+      if (s.keys && chosen(s, kShort))
+        single.push_back(block((int64_t)s.first * group_, (int64_t)s.queries * group_, i, kFlat, false, kShort));
+    }
+    if (rows <= kMostFlatRows) {
+      consider(blocks(kFlat, false, true, kAll), {});
+      consider(blocks(kFlat, false, true, kLong), single);
+    }
+    if (rows <= kFlatRows) return;
     for (int kind : {kTall, kSplit}) {
-      // Aligned blocks straddle fewer sequences, the others waste fewer rows: fewer tiles decide.
-      const auto tiles = [](const std::vector<Draft>& v) {
-        int64_t n = 0;
-        for (const Draft& b : v) n += b.item.tiles + 2;
-        return n;
-      };
-      std::vector<Draft> a = blocks(kind, true), b = blocks(kind, false);
-      consider(tiles(a) <= tiles(b) ? std::move(a) : std::move(b));
+      const std::vector<Draft> large = best_blocks(kind, true, kLong);
+      consider(large, single);
+      if (packed.size() < single.size()) consider(large, packed);
     }
   }
 
@@ -262,27 +268,35 @@ class Planner {
       for (int32_t r = 0; r < b.item.rows; ++r) b.merged |= cover[b.item.row0 + r] > 1;
   }
 
-  static int chunks_for(const Draft& b, double target) {
-    const int n = b.units(), fit = std::max(1, (int)std::floor((target - b.fixed()) / b.unit()));
+  // The time that an item takes: fixed, and for each unit of work (cuts leave it whole: a tile; a round
+  // of the eight wavefronts).
+  static double fixed(const Draft& b) { return b.item.kind == kFlat ? kFlatItem : kBlockItem; }
+  double unit(const Draft& b) const {
+    if (b.item.kind != kFlat) return b.item.kind == kTall ? kTallTile : kSplitTile;
+    return kFlatRound + kFlatWaves * kFlatKeys * key_bytes_ / kItemBytesPerUs + (d_.cache.format == QATTN_KV_INT8 ? kFlatInt8 : 0) +
+           kFlatMasked * b.masked / std::max(1, b.item.tiles);
+  }
+  double cost(const Draft& b, int units) const { return fixed(b) + unit(b) * units; }
+
+  int chunks_for(const Draft& b, double target) const {
+    const int n = b.units(), fit = std::max(1, (int)std::floor((target - fixed(b)) / unit(b)));
     return (n + fit - 1) / fit;
   }
 
-  // The time at which the last slot ends, longest unit first, two flat items to a unit.
+  // The time at which the last slot ends, longest item first, or the flat items' bytes have been read.
   double span(const std::vector<Draft>& drafts, double target) const {
-    std::vector<double> costs, flat;
-    double partial_rows = 0;
+    std::vector<double> costs;
+    double partial_rows = 0, flat_keys = 0;
     bool split = false;
     for (const Draft& b : drafts) {
       const int c = chunks_for(b, target), units = b.units();
       const bool part = c > 1 || b.merged;
       if (part) partial_rows += (double)c * b.item.rows;
       split |= part;
-      auto& to = b.item.kind == kFlat ? flat : costs;
-      for (int i = 0; i < c; ++i) to.push_back((part ? kPartial : 0) + b.cost(units * (i + 1) / c - units * i / c));
-      if (costs.size() + flat.size() > kMostSimulated) return 1e30;
+      if (b.item.kind == kFlat) flat_keys += (double)b.item.tiles * kFlatKeys;
+      for (int i = 0; i < c; ++i) costs.push_back((part ? kPartial : 0) + cost(b, units * (i + 1) / c - units * i / c));
+      if (costs.size() > kMostSimulated) return 1e30;
     }
-    std::sort(flat.begin(), flat.end(), std::greater<double>());
-    for (size_t i = 0; i < flat.size(); i += 2) costs.push_back(flat[i]);
     std::sort(costs.begin(), costs.end(), std::greater<double>());
     std::priority_queue<double, std::vector<double>, std::greater<double>> ends;
     double last = 0;
@@ -295,17 +309,18 @@ class Planner {
       ends.push(start + c);
       last = std::max(last, start + c);
     }
+    last = std::max(last, kFlatItem + flat_keys * key_bytes_ * d_.cache.kv_heads / kBytesPerUs);
     return last + (split ? kMergeLaunch + partial_rows * d_.cache.kv_heads * d_.cache.head_dim * 8 / kBytesPerUs : 0);
   }
 
   // Chooses every draft's chunks; returns the launch's time.
   double cut(std::vector<Draft>* drafts) const {
     double longest = 0;
-    for (const Draft& b : *drafts) longest = std::max(longest, b.cost(b.units()));
+    for (const Draft& b : *drafts) longest = std::max(longest, cost(b, b.units()));
     double best_span = span(*drafts, longest), best = longest;
-    for (double target = longest * 0.85; target > kBlockItem + kSplitTile; target *= target > longest / 2 ? 0.85 : 0.7) {
+    for (double target = longest * 0.85; target > kFlatItem; target *= target > longest / 2 ? 0.85 : 0.7) {
       const double s = span(*drafts, target);
-      if (s < best_span * 0.97) {
+      if (s < best_span * 0.98) {
         best_span = s;
         best = target;
       }
@@ -313,7 +328,7 @@ class Planner {
     double total = 0;
     for (Draft& b : *drafts) {
       b.chunks = best > 0 ? chunks_for(b, best) : 1;
-      total += b.cost(b.units());
+      total += cost(b, b.units());
     }
     return best_span < 1e30 ? best_span : total / slots_;  // too many to simulate: the slots are full
   }
@@ -327,7 +342,7 @@ class Planner {
         b.first_part = (int32_t)plan_->partial_rows;
         plan_->partial_rows += (int64_t)b.chunks * rows;
       }
-      const int round = b.item.kind == kFlat ? 4 : 1, units = b.units();
+      const int round = b.item.kind == kFlat ? kFlatWaves : 1, units = b.units();
       for (int c = 0; c < b.chunks; ++c) {
         int begin = std::min(b.item.tiles, (int)((int64_t)units * c / b.chunks) * round);
         int end = std::min(b.item.tiles, (int)((int64_t)units * (c + 1) / b.chunks) * round);
@@ -346,8 +361,9 @@ class Planner {
           end -= n;
         }
         it.seg_end = (int32_t)plan_->segs.size();
-        first_groups(&it);
-        items.emplace_back(b.cost((it.tiles + round - 1) / round), it);
+        if (it.kind != kFlat) first_groups(&it);
+        it.seg = plan_->segs[it.seg_begin];
+        items.emplace_back(cost(b, (it.tiles + round - 1) / round), it);
       }
     }
     // Longest first, the flat items behind the others (their workgroups may come first all the same).
@@ -355,7 +371,9 @@ class Planner {
     std::stable_partition(items.begin(), items.end(), [](const auto& i) { return i.second.kind != kFlat; });
     for (const auto& i : items) {
       plan_->items.push_back(i.second);
-      plan_->flat_items += i.second.kind == kFlat;
+      if (i.second.kind != kFlat) continue;
+      ++plan_->flat_items;
+      add_starts(i.second);
     }
     const size_t blocks = plan_->items.size() - plan_->flat_items;
     plan_->flat_first = blocks && plan_->flat_items && items[blocks].first > items[0].first;
@@ -365,19 +383,34 @@ class Planner {
     plan_->info.partial_rows = plan_->partial_rows;
   }
 
-  // The item's own copy of its first segment and of the groups of its first tiles.
+  int32_t group_at(const SharedSeg& s, int32_t key) const { return s.source == kOwnRows ? 0 : plan_->groups[s.base + key / 16]; }
+
+  // A block's copy of the groups of its first tile.
   void first_groups(SharedItem* it) const {
-    it->seg = plan_->segs[it->seg_begin];
-    const int tile = tile_of(it->kind);
-    int32_t seg = it->seg_begin, at = it->seg.tile_begin;
-    for (int i = 0; i < 8; ++i) {
-      const SharedSeg& s = plan_->segs[seg];
-      const int32_t first = at * tile + 16 * i % tile;
-      it->group[i] = s.source == kOwnRows ? 0 : plan_->groups[s.base + first / 16];
-      if ((16 * (i + 1)) % tile) continue;
-      if (++at < s.tile_end) continue;
-      if (++seg == it->seg_end) break;  // no further tile
-      at = plan_->segs[seg].tile_begin;
+    const SharedSeg& s = plan_->segs[it->seg_begin];
+    for (int i = 0; i < kTallKeys / 16; ++i) it->group[i] = group_at(s, s.tile_begin * kTallKeys + 16 * i);
+  }
+
+  // A flat item's tiles, in runs for its wavefronts.
+  void add_starts(const SharedItem& it) const {
+    int32_t seg = it.seg_begin, tile = it.seg.tile_begin;
+    for (int w = 0; w < kFlatWaves; ++w) {
+      SharedStart start{};
+      start.tiles = (int32_t)((int64_t)it.tiles * (w + 1) / kFlatWaves - (int64_t)it.tiles * w / kFlatWaves);
+      if (start.tiles) {
+        const SharedSeg& s = plan_->segs[seg];
+        std::memcpy(&start, &s, offsetof(SharedStart, seg));
+        start.tile_begin = tile;
+        start.seg = seg;
+        for (int b = 0; b < 2; ++b) start.group[b] = group_at(s, tile * kFlatKeys + 16 * b);
+      }
+      plan_->starts.push_back(start);
+      for (int n = start.tiles; n;) {
+        const int step = std::min(n, plan_->segs[seg].tile_end - tile);
+        n -= step;
+        tile += step;
+        if (tile == plan_->segs[seg].tile_end && ++seg < it.seg_end) tile = plan_->segs[seg].tile_begin;
+      }
     }
   }
 
@@ -408,7 +441,7 @@ class Planner {
   SharedPlan* plan_;
   const int group_;
   const int slots_;
-  bool flat_all_ = false;
+  const double key_bytes_;  // of a key's K and V for one KV head
   std::vector<Sequence> sequences_;
   std::vector<Draft> drafts_;
 };

@@ -336,8 +336,8 @@ def shared_plan(desc):
     _check(lib().qattn_shared_plan_describe(ctypes.byref(desc), None, 0, ctypes.byref(n), ctypes.byref(info)))
     words = np.zeros(n.value, np.int32)
     _check(lib().qattn_shared_plan_describe(ctypes.byref(desc), _np_ptr(words), n.value, ctypes.byref(n), None))
-    counts, at, out = words[:5], 8, {}
-    for name, count, width in zip(("items", "segments", "merges", "positions", "groups"), counts, (32, 12, 8, 1, 1)):
+    counts, at, out = words[:6], 8, {}
+    for name, count, width in zip(("items", "segments", "merges", "positions", "groups", "runs"), counts, (32, 12, 8, 1, 1, 16)):
         part = words[at:at + count * width]
         out[name] = part if width == 1 else part.reshape(count, width)
         at += count * width

@@ -351,7 +351,7 @@ class Graph:
 def test_captured_launches(ctx, qattn):
     """A graph of a step's launches (rope, cache write, attention, merge), replayed on new inputs and
     compared with the eager step every time."""
-    heads, kv, dim, page, n, P = 16, 8, 128, 16, 6, 400
+    heads, kv, dim, page, n, P = 16, 8, 128, 16, 6, 4000
     rng = np.random.default_rng(3)
     f16 = lambda *shape: rng.standard_normal(shape).astype(np.float16).view(np.uint16)  # noqa: E731
     pages = P // page + n

@@ -43,7 +43,7 @@ def check_plan(qattn, prefix, queries, own, heads=16, kv=8, page=64, paged=True,
     first_row = np.concatenate([[0], np.cumsum(own)])
     top = prefix + int(own.max(initial=0))
     counts = np.zeros((T * group, max(top, 1)), np.int16)  # visits of (row, key position)
-    writes, parts = np.zeros(T * group, int), {}
+    writes, parts, flat = np.zeros(T * group, int), {}, 0
     for it in plan["items"]:
         row0, rows, s0, s1, part, tiles, kind, least, greatest = it[:9]
         assert 1 <= rows <= ROWS[kind] and 0 <= row0 and row0 + rows <= T * group and tiles >= 1
@@ -53,8 +53,19 @@ def check_plan(qattn, prefix, queries, own, heads=16, kv=8, page=64, paged=True,
         segs = plan["segments"][s0:s1]
         assert sum(s[6] - s[5] for s in segs) == tiles and s1 > s0
         assert np.array_equal(it[12:24], segs[0])
-        for (s, k), got in zip([(s, k) for s in segs for k in range(s[5] * TILE[kind], s[6] * TILE[kind], 16)], it[24:]):
-            assert got == (0 if s[0] == 2 else groups[s[2] + k // 16])
+        group_at = lambda s, k: 0 if s[0] == 2 else groups[s[2] + k // 16]  # noqa: E731
+        visits = [(s0 + i, s, t) for i, s in enumerate(segs) for t in range(s[5], s[6])]
+        if kind == 2:
+            runs, done = plan["runs"][8 * flat:8 * flat + 8], 0
+            flat += 1
+            assert (runs[:, 10] <= -(-tiles // 8)).all() and runs[:, 10].sum() == tiles
+            for run in runs[runs[:, 10] > 0]:
+                i, s, t = visits[done]
+                assert run[5] == t and run[9] == i and np.array_equal(np.delete(run[:9], 5), np.delete(s[:9], 5))
+                assert list(run[11:13]) == [group_at(s, 32 * t), group_at(s, 32 * t + 16)]
+                done += run[10]
+        else:
+            assert list(it[24:]) == [group_at(segs[0], 128 * segs[0][5] + 16 * i) for i in range(8)]
         for source, whole, base, keys, pos0, t0, t1, lo, hi in segs[:, :9]:
             assert 0 <= t0 < t1 <= -(-keys // TILE[kind])
             assert row0 <= lo < hi <= row0 + rows
@@ -78,6 +89,7 @@ def check_plan(qattn, prefix, queries, own, heads=16, kv=8, page=64, paged=True,
             for j in range(rows):
                 assert part + j not in parts and 0 <= part + j < info.partial_rows
                 parts[part + j] = row0 + j
+    assert len(plan["runs"]) == 8 * flat
     used = set()
     for m in plan["merges"]:
         writes[m[0]] += 1
@@ -138,15 +150,18 @@ def test_plans_of_random_batches(qattn):
 
 
 def test_plan_fills_the_chip_for_few_rows(qattn):
-    # 64 tokens behind 8,192 keys: one block of rows per KV head, cut until most slots have work
-    _, info = qattn.shared_plan(make(qattn, 8192, [1] * 64, [200] * 64)[0])
-    assert info.items * 8 >= 400
+    # 64 tokens behind 8,192 keys, cut until most of the 32 slots of a KV head have work
+    plan, _ = qattn.shared_plan(make(qattn, 8192, [1] * 64, [200] * 64)[0])
+    assert len(plan["items"]) >= 24
     # a full batch fills it too
     _, info = qattn.shared_plan(make(qattn, 5000, [500] * 16, [500] * 16, paged=False)[0])
     assert info.items * 8 >= 400
     # masks skip whole tiles of the prefix
     plan, _ = qattn.shared_plan(make(qattn, 8192, [100], [100], mask=1)[0])
-    assert sum(i[5] for i in plan["items"]) <= 2 * (2 + 6 + 2) and plan["items"][:, 6].max() <= 1
+    blocks = {}
+    for it in plan["items"]:
+        blocks[it[0]] = blocks.get(it[0], 0) + it[5] * TILE[it[6]]
+    assert max(blocks.values()) <= (2 + 6 + 2) * 128
 
 
 def refuses(qattn, needle, change, **kw):
