@@ -771,11 +771,13 @@ __device__ inline void flat_item(const SharedParams& p, const SharedItem& it, in
       });
   }
 
-  // The wavefronts' sums: lane (n, c) holds dims 16 db + 4 c .. + 3 of row n.
+  // The wavefronts' sums: lane (n, c) holds dims 16 db + 4 c .. + 3 of row n.  Rows start at the same bank: their
+  // 16-byte chunks are swizzled.
+  const auto chunk_at = [](int r, int chunk) { return r * DIM + ((chunk ^ (r & 3) << 2) << 2); };
   l = rows_sum(l);
   float* own = reinterpret_cast<float*>(lds);
 #pragma unroll
-  for (int db = 0; db < kBlocks; ++db) *reinterpret_cast<f4*>(own + n * DIM + 16 * db + 4 * c) = o[db];
+  for (int db = 0; db < kBlocks; ++db) *reinterpret_cast<f4*>(own + chunk_at(n, 4 * db + c)) = o[db];
   if (c == 0) stats[kFlatRows * wave + n] = float2{m, l};
   __syncthreads();
   constexpr int kLanes = kSharedThreads / kFlatRows, kEach = DIM / kLanes;
@@ -794,7 +796,7 @@ __device__ inline void flat_item(const SharedParams& p, const SharedItem& it, in
   for (int w = 0; w < kFlatWaves; ++w) {
     const float f = __builtin_amdgcn_exp2f(st[w].x - (top == kNone ? 0.f : top));
     sum += f * st[w].y;
-    x += f * *reinterpret_cast<const Part*>(reinterpret_cast<const float*>(lds_all + w * (T::kLds / kFlatWaves)) + r * DIM + d);
+    x += f * *reinterpret_cast<const Part*>(reinterpret_cast<const float*>(lds_all + w * (T::kLds / kFlatWaves)) + chunk_at(r, d / 4) + d % 4);
   }
   const int out_row = it.row0 + r, out_token = out_row / p.group;
   if (it.part < 0) {
