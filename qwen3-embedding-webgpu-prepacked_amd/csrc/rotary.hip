@@ -4,7 +4,7 @@
 // A pair (a, b) turns by angle = position * f: (a cos - b sin, b cos + a sin).  The angle is reduced in
 // f64, in turns: position * (f / 2 pi) minus its floor, so positions of 2^31 still have 2^-22 turns; the
 // fraction goes to sincospif in f32 (2^-25 turns).  One (cos, sin) serves every head of its token: a
-// workgroup computes those of its tokens into LDS, then its threads stream the heads.
+// workgroup takes one token, computes those into LDS, then its threads stream the heads.
 // Bound by memory: 4 bytes moved per element for about two operations.
 #include "shared_ops.h"
 
@@ -15,18 +15,16 @@ namespace qattn {
 namespace {
 
 constexpr int kRotaryThreads = 256;
-constexpr int kRotaryTable = 256;  // (cos, sin) pairs of a workgroup's tokens
+constexpr int kMaxPairs = QATTN_MAX_ROPE_DIM / 2;
 
 // WIDE: 16-byte accesses of eight elements (every address and width a multiple of eight elements); else
 // one pair or one element at a time.
 template <bool BF16, bool INTERLEAVED, bool WIDE>
 __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
-  __shared__ float2 table[kRotaryTable];
-  const int64_t first = (int64_t)blockIdx.x * a.block_tokens;
-  const int count = (int)(a.tokens - first < a.block_tokens ? a.tokens - first : a.block_tokens);
-  for (int i = threadIdx.x; i < count * a.pairs; i += kRotaryThreads) {
-    const int t = i / a.pairs, pair = i - t * a.pairs;
-    const double turn = (double)a.positions[first + t] * a.turns[pair];
+  __shared__ float2 table[kMaxPairs];
+  const int64_t token = blockIdx.x;
+  for (int i = threadIdx.x; i < a.pairs; i += kRotaryThreads) {
+    const double turn = (double)a.positions[token] * a.turns[i];
     float s, c;
     sincospif(2.f * (float)(turn - floor(turn)), &s, &c);
     table[i] = float2{c * a.magnitude, s * a.magnitude * a.sign};
@@ -36,16 +34,14 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
   // the elements that pass through.
   const int turned = WIDE ? (INTERLEAVED ? a.pairs / 4 : a.pairs / 8) : a.pairs;
   const int units = turned + (WIDE ? a.tail / 8 : a.tail);
-  const int total = count * a.heads * units;
+  const int total = a.heads * units;
   for (int i = threadIdx.x; i < total; i += kRotaryThreads) {
-    const int row = i / units, unit = i - row * units;
-    const int t = row / a.heads, head = row - t * a.heads;
+    const int head = i / units, unit = i - head * units;
     const bool is_q = head < a.heads_q;
     const RopeBlockArgs& b = is_q ? a.q : a.k;
     const int64_t column = (int64_t)(is_q ? head : head - a.heads_q) * a.head_dim;
-    const uint16_t* x = b.x + (first + t) * b.x_stride + column;
-    uint16_t* out = b.out + (first + t) * b.out_stride + column;
-    const float2* cs = table + t * a.pairs;
+    const uint16_t* x = b.x + token * b.x_stride + column;
+    uint16_t* out = b.out + token * b.out_stride + column;
     if (unit >= turned) {
       const int c = 2 * a.pairs + (unit - turned) * (WIDE ? 8 : 1);
       if constexpr (WIDE)
@@ -55,7 +51,7 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
     } else if constexpr (!WIDE) {
       const int ia = INTERLEAVED ? 2 * unit : unit, ib = INTERLEAVED ? 2 * unit + 1 : unit + a.pairs;
       const float xa = widen<BF16, 0>(x[ia]), xb = widen<BF16, 0>(x[ib]);
-      const float2 r = cs[unit];
+      const float2 r = table[unit];
       const uint32_t y = narrow2<BF16>(xa * r.x - xb * r.y, xb * r.x + xa * r.y);
       out[ia] = (uint16_t)y;
       out[ib] = (uint16_t)(y >> 16);
@@ -65,7 +61,7 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float xa = widen<BF16, 0>(v[e]), xb = widen<BF16, 1>(v[e]);
-        const float2 r = cs[4 * unit + e];
+        const float2 r = table[4 * unit + e];
         y[e] = narrow2<BF16>(xa * r.x - xb * r.y, xb * r.x + xa * r.y);
       }
       *reinterpret_cast<u32x4*>(out + 8 * unit) = y;
@@ -75,7 +71,7 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
       u32x4 ya, yb;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float2 r0 = cs[8 * unit + 2 * e], r1 = cs[8 * unit + 2 * e + 1];
+        const float2 r0 = table[8 * unit + 2 * e], r1 = table[8 * unit + 2 * e + 1];
         const float a0 = widen<BF16, 0>(va[e]), a1 = widen<BF16, 1>(va[e]);
         const float b0 = widen<BF16, 0>(vb[e]), b1 = widen<BF16, 1>(vb[e]);
         ya[e] = narrow2<BF16>(a0 * r0.x - b0 * r0.y, a1 * r1.x - b1 * r1.y);
@@ -97,11 +93,9 @@ void launch(const RotaryArgs& a, bool wide, dim3 grid, hipStream_t stream) {
 
 }  // namespace
 
-hipError_t launch_rotary(const RotaryArgs& args, bool bf16, bool interleaved, bool wide, hipStream_t stream) {
-  if (args.tokens <= 0) return hipSuccess;
-  RotaryArgs a = args;
-  a.block_tokens = 1;
-  const dim3 grid((unsigned)((a.tokens + a.block_tokens - 1) / a.block_tokens));
+hipError_t launch_rotary(const RotaryArgs& a, bool bf16, bool interleaved, bool wide, hipStream_t stream) {
+  if (a.tokens <= 0) return hipSuccess;
+  const dim3 grid((unsigned)a.tokens);
   if (bf16)
     interleaved ? launch<true, true>(a, wide, grid, stream) : launch<true, false>(a, wide, grid, stream);
   else

@@ -20,7 +20,6 @@ struct RotaryArgs {
   int32_t heads_q, heads;  // heads of q, of q and k together
   int32_t head_dim, pairs;
   int32_t tail;            // elements from tail_begin on that are copied (0 in place)
-  int32_t block_tokens;    // tokens of a workgroup
   float sign, magnitude;
   double turns[QATTN_MAX_ROPE_DIM / 2];  // turns per position of each pair
 };
