@@ -394,8 +394,7 @@ typedef struct qattn_kv_cache {
  * (likewise v), goes to slot slots[t], a device array of `tokens` int64; a slot outside
  * [0, pages*page_size) writes nothing (padding), and no slot may be named twice in a call.  Rows 16-byte
  * aligned, strides multiples of 8 elements, >= kv_heads*head_dim; tokens below 2^24 and
- * tokens*kv_heads*head_dim below 2^35.  Enqueued on `stream`; allocates
- * nothing. */
+ * tokens*kv_heads*head_dim below 2^34.  Enqueued on `stream`; allocates nothing. */
 int qattn_kv_write(qattn_ctx* ctx, const qattn_kv_cache* cache, const void* k, int64_t k_row_stride,
                    const void* v, int64_t v_row_stride, const int64_t* slots, int64_t tokens,
                    qattn_stream_t stream);

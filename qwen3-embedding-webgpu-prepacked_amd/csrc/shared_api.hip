@@ -20,7 +20,7 @@ constexpr int32_t kMaxKvHeads = 256;
 constexpr int32_t kMaxRopeHeads = 4096;
 // Of a row-wise launch, whose grid has to stay below 2^32 threads.
 constexpr int64_t kMaxRowTokens = ((int64_t)1 << 24) - 1;
-constexpr int64_t kMaxRowValues = ((int64_t)1 << 35) - 1;  // tokens * kv_heads * head_dim: eight to a thread
+constexpr int64_t kMaxRowValues = ((int64_t)1 << 34) - 1;  // tokens * kv_heads * head_dim
 constexpr int64_t kMaxSharedRows = (int64_t)1 << 22;       // queries * heads of a group
 constexpr int64_t kMaxSharedStride = (int64_t)1 << 24;     // elements: 16 rows of it within a 32-bit offset
 constexpr int64_t kMaxSharedGroups = (int64_t)1 << 23;     // workgroups of a launch
@@ -93,7 +93,7 @@ int kv_args(qattn_ctx* ctx, const qattn_kv_cache* cache, const void* k, int64_t 
   if (tokens < 0 || tokens > kMaxRowTokens) return fail(ctx, QATTN_EINVAL, "tokens %lld outside [0, 2^24)", (long long)tokens);
   if (!tokens) return QATTN_OK;
   if (tokens * cache->kv_heads * cache->head_dim > kMaxRowValues)
-    return fail(ctx, QATTN_EINVAL, "tokens*kv_heads*head_dim must be below 2^35");
+    return fail(ctx, QATTN_EINVAL, "tokens*kv_heads*head_dim must be below 2^34");
   if (!k || !v || !slots) return fail(ctx, QATTN_EINVAL, "k/v/slots is NULL");
   if (!aligned16(k) || !aligned16(v) || (reinterpret_cast<uintptr_t>(slots) & 7))
     return fail(ctx, QATTN_EINVAL, "k/v not 16-byte or slots not 8-byte aligned");

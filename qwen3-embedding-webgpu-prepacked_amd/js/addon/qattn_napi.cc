@@ -15,6 +15,7 @@
 #include <cstring>
 #include <set>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "../../../include/qattn.h"
@@ -44,6 +45,7 @@ struct Run;
 struct Model;
 struct Plan;
 struct Evt;
+struct SharedRun;
 struct Ctx {
   qattn_ctx* ctx = nullptr;
   int refs = 1;  // the context handle's own reference
@@ -52,6 +54,7 @@ struct Ctx {
   std::set<Model*> models;
   std::set<Plan*> plans;
   std::set<Evt*> evts;
+  std::set<SharedRun*> shared_runs;
   int async_busy = 0;  // synchronizeAsync / readAfterAsync waits on worker threads
 };
 // An event on the context stream (marks the end of one submitted batch).  While a readAfterAsync
@@ -98,6 +101,7 @@ struct Plan {
 };
 
 void release_device(Ctx* c);
+void destroy_shared_runs(Ctx* c);
 void unref(Ctx* c) {
   if (--c->refs == 0) {
     release_device(c);
@@ -190,6 +194,7 @@ void release_device(Ctx* c) {
       qattn_run_destroy(r->run);
       r->run = nullptr;
     }
+  destroy_shared_runs(c);
   for (Buf* b : c->bufs)
     if (b->ptr) {
       qattn_buffer_free(c->ctx, b->ptr);
@@ -1334,6 +1339,449 @@ napi_value ReadAfterAsync(napi_env env, napi_callback_info info) {
   return promise;
 }
 
+// ---- requests behind one shared prefix: rotary positions, the paged cache, attention over it ------------
+
+// A device tensor of a descriptor object: obj[name], a buffer of context `c`, from obj[name + "Offset"]
+// bytes on.  Alignment is the C ABI's to check.
+struct Tensor {
+  Buf* buf = nullptr;
+  int64_t off = 0;
+  napi_value js = nullptr;
+  void* ptr() const { return buf ? static_cast<char*>(buf->ptr) + off : nullptr; }
+  // rows of `width` elements, `stride` apart (negative sizes are the C ABI's to reject)
+  bool holds(int64_t rows, int64_t stride, int64_t width, int64_t bytes) const {
+    if (rows <= 0 || stride < 0 || width <= 0) return true;
+    const unsigned __int128 elems = (unsigned __int128)(rows - 1) * (uint64_t)stride + (uint64_t)width;
+    return elems * (uint64_t)bytes + (uint64_t)off <= buf->bytes;
+  }
+};
+bool tensor_of(napi_env env, napi_value obj, const char* name, const Ctx* c, bool required, Tensor* out) {
+  napi_value v;
+  if (!prop(env, obj, name, &v)) {
+    if (required) napi_throw_type_error(env, nullptr, (std::string("missing ") + name).c_str());
+    return !required;
+  }
+  Buf* b = live_buf(env, v);
+  if (!b) return false;
+  if (b->owner != c) {
+    napi_throw_error(env, nullptr, (std::string(name) + " belongs to another context").c_str());
+    return false;
+  }
+  *out = Tensor{b, 0, v};
+  if (prop(env, obj, (std::string(name) + "Offset").c_str(), &v) && !get_i64(env, v, &out->off)) out->off = -1;
+  if (out->off < 0 || (uint64_t)out->off > b->bytes) {
+    napi_throw_range_error(env, nullptr, (std::string(name) + "Offset lies outside the buffer").c_str());
+    return false;
+  }
+  return true;
+}
+bool past_buffer(napi_env env, const char* name) {
+  napi_throw_range_error(env, nullptr, (std::string(name) + ": rows x stride exceed the device buffer").c_str());
+  return false;
+}
+// Numbers of a descriptor object; one that is not a number fails (with a TypeError, once).
+struct Numbers {
+  napi_env env;
+  napi_value obj;
+  bool ok = true;
+  void bad(const char* name) {
+    if (ok) napi_throw_type_error(env, nullptr, (std::string(name) + " must be a number").c_str());
+    ok = false;
+  }
+  int64_t wide(const char* name, int64_t dflt) {
+    napi_value v;
+    if (ok && prop(env, obj, name, &v) && !get_i64(env, v, &dflt)) bad(name);
+    return dflt;
+  }
+  int32_t i32(const char* name, int64_t dflt) {
+    const int64_t x = wide(name, dflt);
+    if (ok && (x < INT32_MIN || x > INT32_MAX)) {
+      napi_throw_range_error(env, nullptr, (std::string(name) + " is out of range").c_str());
+      ok = false;
+    }
+    return (int32_t)x;
+  }
+  double real(const char* name, double dflt) {
+    napi_value v;
+    if (ok && prop(env, obj, name, &v) && napi_get_value_double(env, v, &dflt) != napi_ok) bad(name);
+    return dflt;
+  }
+};
+
+bool rope_block(napi_env env, napi_value desc, const char* name, const Ctx* c, int64_t tokens, int64_t head_dim,
+                qattn_rope_block* out) {
+  napi_value obj;
+  if (!prop(env, desc, name, &obj)) return true;
+  Numbers n{env, obj};
+  Tensor x, y;
+  out->heads = n.i32("heads", 0);
+  out->x_row_stride = n.wide("xStride", (int64_t)out->heads * head_dim);
+  if (!n.ok || !tensor_of(env, obj, "x", c, true, &x) || !tensor_of(env, obj, "out", c, false, &y)) return false;
+  const bool in_place = !y.buf;
+  if (in_place) y = x;
+  out->out_row_stride = n.wide("outStride", y.ptr() == x.ptr() ? out->x_row_stride : (int64_t)out->heads * head_dim);
+  if (!n.ok) return false;
+  out->x = x.ptr();
+  out->out = y.ptr();
+  if (!x.holds(tokens, out->x_row_stride, out->heads * head_dim, 2)) return past_buffer(env, name);
+  if (!y.holds(tokens, out->out_row_stride, out->heads * head_dim, 2)) return past_buffer(env, name);
+  return true;
+}
+
+// rope(ctx, desc)  (qattn_rope)
+napi_value Rope(napi_env env, napi_callback_info info) {
+  napi_value argv[2];
+  if (!args_of(env, info, 2, argv)) return nullptr;
+  Ctx* c = live_ctx(env, argv[0]);
+  if (!c) return nullptr;
+  qattn_rope_desc d{};
+  Numbers n{env, argv[1]};
+  d.tokens = n.wide("tokens", 0);
+  d.dtype = n.i32("dtype", QATTN_DTYPE_F16);
+  d.head_dim = n.i32("headDim", 128);
+  d.rotary_dim = n.i32("rotaryDim", d.head_dim);
+  d.layout = n.i32("layout", QATTN_ROPE_HALF);
+  d.scaling = n.i32("scaling", QATTN_ROPE_PLAIN);
+  d.inverse = n.i32("inverse", 0);
+  d.theta = n.real("theta", 1e6);
+  d.factor = n.real("factor", 1.0);
+  d.original_context = n.real("originalContext", 32768);
+  d.beta_fast = n.real("betaFast", 32);
+  d.beta_slow = n.real("betaSlow", 1);
+  d.magnitude = n.real("magnitude", 0);
+  Tensor positions;
+  if (!n.ok || !tensor_of(env, argv[1], "positions", c, true, &positions)) return nullptr;
+  if (!positions.holds(d.tokens, 1, 1, 4)) {
+    past_buffer(env, "positions");
+    return nullptr;
+  }
+  d.positions = static_cast<const int32_t*>(positions.ptr());
+  if (!rope_block(env, argv[1], "q", c, d.tokens, d.head_dim, &d.q) || !rope_block(env, argv[1], "k", c, d.tokens, d.head_dim, &d.k))
+    return nullptr;
+  int rc = qattn_rope(c->ctx, &d, nullptr);
+  if (rc) return throw_qattn(env, rc, c->ctx);
+  return undefined(env);
+}
+
+// A cache object {k, v, kScale, vScale, pages, pageSize, kvHeads, headDim, dtype, format}, whose buffers
+// hold its pages if there are any.
+bool read_cache(napi_env env, napi_value obj, const Ctx* c, qattn_kv_cache* out, std::vector<Tensor>* tensors) {
+  Numbers n{env, obj};
+  *out = qattn_kv_cache{};
+  out->pages = n.i32("pages", 0);
+  out->page_size = n.i32("pageSize", 0);
+  out->kv_heads = n.i32("kvHeads", 8);
+  out->head_dim = n.i32("headDim", 128);
+  out->dtype = n.i32("dtype", QATTN_DTYPE_F16);
+  out->format = n.i32("format", QATTN_KV_16BIT);
+  if (!n.ok) return false;
+  const int64_t vectors = out->pages < 0 || out->page_size < 0 || out->kv_heads < 0 || out->kv_heads > 4096 ? 0
+                          : (int64_t)out->pages * out->page_size > (int64_t)1 << 48 ? (int64_t)1 << 60
+                                                                                     : (int64_t)out->pages * out->page_size * out->kv_heads;
+  const bool codes = out->format != QATTN_KV_16BIT;
+  for (const char* name : {"k", "v", "kScale", "vScale"}) {
+    const bool scale = std::strlen(name) > 1;
+    if (scale && !codes) continue;
+    Tensor t;
+    if (!tensor_of(env, obj, name, c, vectors > 0, &t)) return false;
+    if (t.buf && !t.holds(vectors, scale ? 1 : out->head_dim, scale ? 1 : out->head_dim, scale ? 4 : codes ? 1 : 2))
+      return past_buffer(env, name);
+    if (!std::strcmp(name, "k")) out->k = t.ptr();
+    if (!std::strcmp(name, "v")) out->v = t.ptr();
+    if (!std::strcmp(name, "kScale")) out->k_scale = static_cast<float*>(t.ptr());
+    if (!std::strcmp(name, "vScale")) out->v_scale = static_cast<float*>(t.ptr());
+    if (t.buf && tensors) tensors->push_back(t);
+  }
+  return true;
+}
+
+// kvWrite(ctx, cache, {k, v, slots, tokens, kStride, vStride}) / kvRead: K and V rows into and out of
+// the cache (qattn_kv_write, qattn_kv_read)
+napi_value KvRows(napi_env env, napi_callback_info info, bool write) {
+  napi_value argv[3];
+  if (!args_of(env, info, 3, argv)) return nullptr;
+  Ctx* c = live_ctx(env, argv[0]);
+  if (!c) return nullptr;
+  qattn_kv_cache cache;
+  if (!read_cache(env, argv[1], c, &cache, nullptr)) return nullptr;
+  Tensor k, v, slots;
+  if (!tensor_of(env, argv[2], "k", c, true, &k) || !tensor_of(env, argv[2], "v", c, true, &v) ||
+      !tensor_of(env, argv[2], "slots", c, true, &slots))
+    return nullptr;
+  Numbers n{env, argv[2]};
+  const int64_t width = (int64_t)cache.kv_heads * cache.head_dim;
+  const int64_t tokens = n.wide("tokens", 0), ks = n.wide("kStride", width), vs = n.wide("vStride", width);
+  if (!n.ok) return nullptr;
+  if (!k.holds(tokens, ks, width, 2)) {
+    past_buffer(env, "k");
+    return nullptr;
+  }
+  if (!v.holds(tokens, vs, width, 2)) {
+    past_buffer(env, "v");
+    return nullptr;
+  }
+  if (!slots.holds(tokens, 1, 1, 8)) {
+    past_buffer(env, "slots");
+    return nullptr;
+  }
+  const int64_t* s = static_cast<const int64_t*>(slots.ptr());
+  int rc = write ? qattn_kv_write(c->ctx, &cache, k.ptr(), ks, v.ptr(), vs, s, tokens, nullptr)
+                 : qattn_kv_read(c->ctx, &cache, s, tokens, k.ptr(), ks, v.ptr(), vs, nullptr);
+  if (rc) return throw_qattn(env, rc, c->ctx);
+  return undefined(env);
+}
+napi_value KvWrite(napi_env env, napi_callback_info info) { return KvRows(env, info, true); }
+napi_value KvRead(napi_env env, napi_callback_info info) { return KvRows(env, info, false); }
+
+// The batch of a shared run: host arrays, copied by the library.
+struct SharedBatch {
+  std::vector<int32_t> prefix_pages, cu, own, own_pages;
+  int32_t prefix_len = 0;
+  int64_t own_rows = 0;
+  bool paged = false;
+};
+bool read_batch(napi_env env, napi_value obj, int32_t page_size, SharedBatch* b) {
+  napi_value v;
+  Numbers n{env, obj};
+  b->prefix_len = n.i32("prefixLength", 0);
+  if (!n.ok) return false;
+  if (!prop(env, obj, "cuSeqlens", &v) || !get_i32_array(env, v, &b->cu) || b->cu.size() < 2 ||
+      !prop(env, obj, "ownLengths", &v) || !get_i32_array(env, v, &b->own) || b->own.size() + 1 != b->cu.size()) {
+    napi_throw_type_error(env, nullptr, "cuSeqlens must hold nseq+1 offsets and ownLengths nseq lengths");
+    return false;
+  }
+  if (prop(env, obj, "prefixPages", &v) && !get_i32_array(env, v, &b->prefix_pages)) {
+    napi_throw_type_error(env, nullptr, "prefixPages must be an Int32Array");
+    return false;
+  }
+  b->paged = prop(env, obj, "ownPages", &v);
+  if (b->paged && !get_i32_array(env, v, &b->own_pages)) {
+    napi_throw_type_error(env, nullptr, "ownPages must be an Int32Array");
+    return false;
+  }
+  // The page lists hold what the lengths ask for (negative lengths are the C ABI's to reject).
+  if (page_size < 1) page_size = 1;
+  const auto pages = [&](int64_t keys) { return keys > 0 ? (keys + page_size - 1) / page_size : 0; };
+  int64_t own = 0;
+  for (int32_t x : b->own) {
+    own += pages(x);
+    b->own_rows += std::max(x, 0);
+  }
+  if ((int64_t)b->prefix_pages.size() < pages(b->prefix_len) || (b->paged && (int64_t)b->own_pages.size() < own)) {
+    napi_throw_range_error(env, nullptr, "prefixPages/ownPages: fewer pages than the lengths need");
+    return false;
+  }
+  return true;
+}
+
+// A run holds a reference on each buffer bound to it, and the tensors that its batches have to fit.
+struct SharedRun {
+  Ctx* owner = nullptr;
+  qattn_shared_run* run = nullptr;
+  qattn_shared_desc desc{};  // geometry and strides
+  Tensor q, o, k, v;
+  std::vector<napi_ref> bound_refs;
+  std::vector<const Buf*> bound;
+};
+bool batch_fits(napi_env env, const SharedRun& r, const SharedBatch& b) {
+  const qattn_shared_desc& d = r.desc;
+  const int64_t width = (int64_t)d.q_heads * d.cache.head_dim, kv_width = (int64_t)d.cache.kv_heads * d.cache.head_dim;
+  if (!r.q.holds(b.cu.back(), d.q_row_stride, width, 2)) return past_buffer(env, "q");
+  if (!r.o.holds(b.cu.back(), d.o_row_stride, width, 2)) return past_buffer(env, "o");
+  if (b.paged) return true;
+  if (!r.k.buf || !r.v.buf) {
+    if (b.own_rows == 0) return true;
+    napi_throw_type_error(env, nullptr, "own keys need ownPages, or k and v rows");
+    return false;
+  }
+  if (!r.k.holds(b.own_rows, d.k_row_stride, kv_width, 2)) return past_buffer(env, "k");
+  if (!r.v.holds(b.own_rows, d.v_row_stride, kv_width, 2)) return past_buffer(env, "v");
+  return true;
+}
+bool shared_tensors(napi_env env, napi_value obj, const Ctx* c, SharedRun* r, std::vector<Tensor>* all) {
+  napi_value cache;
+  if (!prop(env, obj, "cache", &cache)) {
+    napi_throw_type_error(env, nullptr, "missing cache");
+    return false;
+  }
+  if (!tensor_of(env, obj, "q", c, true, &r->q) || !tensor_of(env, obj, "o", c, true, &r->o) ||
+      !tensor_of(env, obj, "k", c, false, &r->k) || !tensor_of(env, obj, "v", c, false, &r->v) ||
+      !read_cache(env, cache, c, &r->desc.cache, all))
+    return false;
+  for (const Tensor* t : {&r->q, &r->o, &r->k, &r->v})
+    if (t->buf) all->push_back(*t);
+  return true;
+}
+napi_value bind_tensors(napi_env env, SharedRun* r, const std::vector<Tensor>& all) {
+  for (napi_ref ref : r->bound_refs) napi_delete_reference(env, ref);
+  r->bound_refs.clear();
+  r->bound.clear();
+  for (const Tensor& t : all) {
+    napi_ref ref;
+    NAPI_OK(env, napi_create_reference(env, t.js, 1, &ref));
+    r->bound_refs.push_back(ref);
+    r->bound.push_back(t.buf);
+  }
+  return undefined(env);
+}
+void destroy_shared_runs(Ctx* c) {
+  for (SharedRun* r : c->shared_runs)
+    if (r->run) {
+      qattn_shared_run_destroy(r->run);
+      r->run = nullptr;
+    }
+}
+void finalize_shared_run(napi_env env, void* data, void*) {
+  auto* r = static_cast<SharedRun*>(data);
+  Ctx* c = r->owner;
+  if (r->run && c->ctx) qattn_shared_run_destroy(r->run);
+  for (napi_ref ref : r->bound_refs) napi_delete_reference(env, ref);
+  c->shared_runs.erase(r);
+  delete r;
+  unref(c);
+}
+SharedRun* live_shared_run(napi_env env, napi_value v) {
+  SharedRun* r = get_external<SharedRun>(env, v, "shared attention run");
+  if (r && (!r->run || !r->owner->ctx)) {
+    napi_throw_error(env, nullptr, r->run ? "context was destroyed" : "shared attention run was destroyed");
+    return nullptr;
+  }
+  if (r)
+    for (const Buf* b : r->bound)
+      if (!b->ptr) {
+        napi_throw_error(env, nullptr, "a device buffer bound to this run was freed");
+        return nullptr;
+      }
+  return r;
+}
+
+// createSharedRun(ctx, desc) -> external (qattn_shared_run_create)
+napi_value CreateSharedRun(napi_env env, napi_callback_info info) {
+  napi_value argv[2];
+  if (!args_of(env, info, 2, argv)) return nullptr;
+  Ctx* c = live_ctx(env, argv[0]);
+  if (!c) return nullptr;
+  SharedRun made;
+  std::vector<Tensor> all;
+  if (!shared_tensors(env, argv[1], c, &made, &all)) return nullptr;
+  qattn_shared_desc& d = made.desc;
+  Numbers n{env, argv[1]};
+  d.q_heads = n.i32("qHeads", 16);
+  const int64_t width = (int64_t)d.q_heads * d.cache.head_dim, kv_width = (int64_t)d.cache.kv_heads * d.cache.head_dim;
+  d.q_row_stride = n.wide("qStride", width);
+  d.o_row_stride = n.wide("oStride", width);
+  d.k_row_stride = n.wide("kStride", kv_width);
+  d.v_row_stride = n.wide("vStride", kv_width);
+  d.mask = n.i32("mask", QATTN_MASK_CAUSAL);
+  d.prefix = n.i32("prefix", 176);
+  d.window = n.i32("window", 432);
+  d.scale = n.real("scale", 0);
+  SharedBatch b;
+  if (!n.ok || !read_batch(env, argv[1], d.cache.page_size, &b) || !batch_fits(env, made, b)) return nullptr;
+  d.q = made.q.ptr();
+  d.o = made.o.ptr();
+  d.k = made.k.ptr();
+  d.v = made.v.ptr();
+  d.prefix_pages = b.prefix_pages.data();
+  d.prefix_len = b.prefix_len;
+  d.cu_q = b.cu.data();
+  d.nseq = (int32_t)b.own.size();
+  d.own_len = b.own.data();
+  static const int32_t no_pages[1] = {0};
+  d.own_pages = !b.paged ? nullptr : b.own_pages.empty() ? no_pages : b.own_pages.data();
+  if (!d.prefix_pages) d.prefix_pages = no_pages;
+  int rc = qattn_shared_run_create(c->ctx, &d, &made.run);
+  if (rc) return throw_qattn(env, rc, c->ctx);
+  made.owner = c;
+  auto* r = new SharedRun(made);
+  c->shared_runs.insert(r);
+  ++c->refs;
+  napi_value out;
+  NAPI_OK(env, napi_create_external(env, r, finalize_shared_run, nullptr, &out));
+  if (!bind_tensors(env, r, all)) return nullptr;
+  return out;
+}
+
+// updateSharedRun(run, batch): new lengths and pages for the same tensors (qattn_shared_run_update)
+napi_value UpdateSharedRun(napi_env env, napi_callback_info info) {
+  napi_value argv[2];
+  if (!args_of(env, info, 2, argv)) return nullptr;
+  SharedRun* r = live_shared_run(env, argv[0]);
+  if (!r) return nullptr;
+  SharedBatch b;
+  if (!read_batch(env, argv[1], r->desc.cache.page_size, &b) || !batch_fits(env, *r, b)) return nullptr;
+  static const int32_t no_pages[1] = {0};
+  int rc = qattn_shared_run_update(r->run, b.prefix_pages.empty() ? no_pages : b.prefix_pages.data(), b.prefix_len, b.cu.data(),
+                                   (int32_t)b.own.size(), b.own.data(),
+                                   !b.paged ? nullptr : b.own_pages.empty() ? no_pages : b.own_pages.data());
+  if (rc) return throw_qattn(env, rc, r->owner->ctx);
+  return undefined(env);
+}
+
+// rebindSharedRun(run, {q, o, cache, k, v}, batch): other tensors of the same strides, a cache of the same
+// geometry (qattn_shared_run_rebind); batch: the one that the run holds, whose rows the tensors have to fit
+napi_value RebindSharedRun(napi_env env, napi_callback_info info) {
+  napi_value argv[3];
+  if (!args_of(env, info, 3, argv)) return nullptr;
+  SharedRun* r = live_shared_run(env, argv[0]);
+  if (!r) return nullptr;
+  SharedRun next;
+  std::vector<Tensor> all;
+  next.desc = r->desc;
+  SharedBatch b;
+  if (!shared_tensors(env, argv[1], r->owner, &next, &all) || !read_batch(env, argv[2], r->desc.cache.page_size, &b) ||
+      !batch_fits(env, next, b))
+    return nullptr;
+  int rc = qattn_shared_run_rebind(r->run, next.q.ptr(), next.o.ptr(), &next.desc.cache, next.k.ptr(), next.v.ptr());
+  if (rc) return throw_qattn(env, rc, r->owner->ctx);
+  r->q = next.q;
+  r->o = next.o;
+  r->k = next.k;
+  r->v = next.v;
+  return bind_tensors(env, r, all);
+}
+
+napi_value EncodeSharedRun(napi_env env, napi_callback_info info) {
+  napi_value argv[1];
+  if (!args_of(env, info, 1, argv)) return nullptr;
+  SharedRun* r = live_shared_run(env, argv[0]);
+  if (!r) return nullptr;
+  int rc = qattn_shared_run_encode(r->run, nullptr);
+  if (rc) return throw_qattn(env, rc, r->owner->ctx);
+  return undefined(env);
+}
+
+napi_value DestroySharedRun(napi_env env, napi_callback_info info) {
+  napi_value argv[1];
+  if (!args_of(env, info, 1, argv)) return nullptr;
+  SharedRun* r = get_external<SharedRun>(env, argv[0], "shared attention run");
+  if (!r) return nullptr;
+  if (r->run && r->owner->ctx) qattn_shared_run_destroy(r->run);
+  r->run = nullptr;
+  return bind_tensors(env, r, {});
+}
+
+// sharedRunInfo(run) -> {tokens, keys, pairs, flops, items, mergedRows, partialRows}
+napi_value SharedRunInfo(napi_env env, napi_callback_info info) {
+  napi_value argv[1];
+  if (!args_of(env, info, 1, argv)) return nullptr;
+  SharedRun* r = live_shared_run(env, argv[0]);
+  if (!r) return nullptr;
+  qattn_shared_info i{};
+  int rc = qattn_shared_run_get_info(r->run, &i);
+  if (rc) return throw_qattn(env, rc, r->owner->ctx);
+  napi_value out, v;
+  NAPI_OK(env, napi_create_object(env, &out));
+  const std::pair<const char*, int64_t> fields[] = {{"tokens", i.tokens}, {"keys", i.keys}, {"pairs", i.pairs},
+                                                    {"flops", i.flops}, {"items", i.items}, {"mergedRows", i.merged_rows},
+                                                    {"partialRows", i.partial_rows}};
+  for (const auto& f : fields) {
+    NAPI_OK(env, napi_create_double(env, (double)f.second, &v));
+    NAPI_OK(env, napi_set_named_property(env, out, f.first, v));
+  }
+  return out;
+}
+
 napi_value AbiVersion(napi_env env, napi_callback_info) {
   napi_value v;
   napi_create_int32(env, qattn_abi_version(), &v);
@@ -1362,6 +1810,11 @@ napi_value Init(napi_env env, napi_value exports) {
       {"runModelPlan", RunModelPlan}, {"profileModelPlan", ProfileModelPlan},
       {"createEvent", CreateEvent},   {"recordEvent", RecordEvent},
       {"destroyEvent", DestroyEvent}, {"readAfterAsync", ReadAfterAsync},
+      {"rope", Rope},                 {"kvWrite", KvWrite},
+      {"kvRead", KvRead},             {"createSharedRun", CreateSharedRun},
+      {"updateSharedRun", UpdateSharedRun}, {"rebindSharedRun", RebindSharedRun},
+      {"encodeSharedRun", EncodeSharedRun}, {"destroySharedRun", DestroySharedRun},
+      {"sharedRunInfo", SharedRunInfo},
   };
   for (const Fn& f : fns) {
     napi_value fn;

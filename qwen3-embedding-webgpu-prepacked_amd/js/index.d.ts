@@ -140,6 +140,80 @@ export class CompactQ4Matmul {
       options?: { inputStride?: number; outputStride?: number }): void;
 }
 
+// ---- requests behind one shared prefix: rotary positions, a paged K/V cache, attention over it.
+export type DtypeName = 'f16' | 'bf16';
+/** Head h of token t at element t * xStride + h * headDim; without `out` in place.  Strides in
+ *  elements (default heads * headDim), offsets in bytes. */
+export interface RopeBlock {
+  x: DeviceBuffer; heads: number; out?: DeviceBuffer; xStride?: number; outStride?: number;
+  xOffset?: number; outOffset?: number;
+}
+export interface RopeOptions {
+  q: RopeBlock; k?: RopeBlock;
+  /** Int32 per token, on the device. */
+  positions: DeviceBuffer; positionsOffset?: number; tokens: number;
+  dtype?: DtypeName; headDim?: number;
+  /** The first elements of a head that turn (default headDim); the others pass through. */
+  rotaryDim?: number;
+  layout?: 'half' | 'interleaved'; scaling?: 'plain' | 'linear' | 'yarn';
+  theta?: number; factor?: number; originalContext?: number; betaFast?: number; betaSlow?: number; magnitude?: number;
+  /** The rotation back, which also maps the output's gradient to the input's. */
+  inverse?: boolean;
+}
+export class RotaryPositions {
+  constructor(context: DeviceContext);
+  run(options: RopeOptions): void;
+}
+/** Strides in elements, offsets in bytes. */
+export interface KvRowOptions {
+  kStride?: number; vStride?: number; kOffset?: number; vOffset?: number; slotsOffset?: number;
+}
+/** Slot s is row s % pageSize of page floor(s / pageSize). */
+export class PagedKvCache {
+  constructor(context: DeviceContext, options: {
+    pages: number; pageSize: number; kvHeads?: number; headDim?: 64 | 128; dtype?: DtypeName;
+    format?: '16bit' | 'e4m3' | 'int8';
+  });
+  readonly pages: number;
+  readonly pageSize: number;
+  /** slots: BigInt64 per token, on the device; none twice in a write. */
+  write(k: DeviceBuffer, v: DeviceBuffer, slots: DeviceBuffer, tokens: number, options?: KvRowOptions): void;
+  read(slots: DeviceBuffer, tokens: number, k: DeviceBuffer, v: DeviceBuffer, options?: KvRowOptions): void;
+  destroy(): void;
+}
+/** Sequence i has queries cuSeqlens[i] .. cuSeqlens[i + 1] - 1, the last of its keys' positions: the
+ *  prefix's prefixLength keys, then its own ownLengths[i]. */
+export interface SharedBatch {
+  cuSeqlens: Int32Array | number[]; ownLengths: Int32Array | number[];
+  prefixPages?: Int32Array | number[]; prefixLength?: number;
+  /** ceil(ownLengths[i] / pageSize) pages of each sequence in turn; without it the own keys are rows of k, v. */
+  ownPages?: Int32Array | number[];
+}
+/** Offsets in bytes. */
+export interface SharedTensors {
+  k?: DeviceBuffer; v?: DeviceBuffer; qOffset?: number; oOffset?: number; kOffset?: number; vOffset?: number;
+}
+export interface SharedOptions extends SharedTensors {
+  qHeads?: number; qStride?: number; oStride?: number; kStride?: number; vStride?: number;
+  mask?: MaskName; prefix?: number; window?: number;
+  /** Of the scores; 0: 1 / sqrt(headDim). */
+  scale?: number;
+}
+export interface SharedRun {
+  handle: unknown; batch: SharedBatch;
+  info: { tokens: number; keys: number; pairs: number; flops: number; items: number; mergedRows: number; partialRows: number };
+}
+export class SharedPrefixAttention {
+  constructor(context: DeviceContext);
+  createRun(q: DeviceBuffer, output: DeviceBuffer, cache: PagedKvCache, batch: SharedBatch, options?: SharedOptions): SharedRun;
+  /** The next batch: new lengths and pages for the same tensors. */
+  updateRun(run: SharedRun, batch: SharedBatch): void;
+  /** Other tensors of the same strides and another cache of the same geometry (the next layer's). */
+  rebindRun(run: SharedRun, q: DeviceBuffer, output: DeviceBuffer, cache: PagedKvCache, options?: SharedTensors): void;
+  encode(run: SharedRun): void;
+  destroyRun(run: SharedRun): void;
+}
+
 // ---- the whole model (the reference's Qwen3WebGPUModel / Qwen3ExecutionPlan, model.ts:49-255).
 /** Stage names of a profiled run, in order (model.ts:157-168). */
 export type ModelStage = 'embedding_norm' | 'qkv' | 'rope_attention' | 'attention_output' | 'post_attention_norm'

@@ -127,4 +127,123 @@ class CompactQ4Matmul {
   }
 }
 
-module.exports = { DeviceContext, DeviceBuffer, CausalAttentionKernel, CompactQ4Matmul, MASK };
+// ---- requests behind one shared prefix (no counterpart in the reference, which recomputes an
+// instruction's tokens with every request): a prefix's keys and values are kept in a PagedKvCache, a batch
+// is rotated to the positions that follow them, and attends to both.
+
+const DTYPE = { f16: 0, bf16: 1 };
+const KV_FORMAT = { '16bit': 0, e4m3: 1, int8: 2 };
+const ROPE_LAYOUT = { half: 0, interleaved: 1 };
+const ROPE_SCALING = { plain: 0, linear: 1, yarn: 2 };
+
+function codeOf(table, name, what) {
+  if (!Object.prototype.hasOwnProperty.call(table, name)) {
+    throw new Error(`unknown ${what} ${name}; expected ${Object.keys(table).map((k) => `'${k}'`).join(', ')}`);
+  }
+  return table[name];
+}
+const handleOf = (buffer) => (buffer ? buffer.handle : undefined);
+
+// Rotary positions: run({ q, k, positions, tokens, ... }) turns the head vectors of q and k
+// ({ x, heads, out, xStride, outStride, xOffset, outOffset }; without `out` in place) by their token's
+// position (Int32 on the device).
+class RotaryPositions {
+  constructor(context) {
+    this.context = context;
+  }
+
+  run(options) {
+    const block = (b) => b && Object.assign({}, b, { x: handleOf(b.x), out: handleOf(b.out) });
+    this.context.addon.rope(this.context.handle, Object.assign({}, options, {
+      q: block(options.q), k: block(options.k), positions: handleOf(options.positions),
+      dtype: codeOf(DTYPE, options.dtype || 'f16', 'dtype'),
+      layout: codeOf(ROPE_LAYOUT, options.layout || 'half', 'layout'),
+      scaling: codeOf(ROPE_SCALING, options.scaling || 'plain', 'scaling'),
+      inverse: options.inverse ? 1 : 0,
+    }));
+  }
+}
+
+// A paged cache of K and V and its device memory: slot s is row s % pageSize of page
+// floor(s / pageSize).
+class PagedKvCache {
+  constructor(context, { pages, pageSize, kvHeads = 8, headDim = 128, dtype = 'f16', format = '16bit' }) {
+    this.context = context;
+    Object.assign(this, { pages, pageSize, kvHeads, headDim, dtype, format });
+    const codes = codeOf(KV_FORMAT, format, 'cache format');
+    const vectors = pages * pageSize * kvHeads;
+    this.buffers = {
+      k: context.alloc(vectors * headDim * (codes ? 1 : 2)),
+      v: context.alloc(vectors * headDim * (codes ? 1 : 2)),
+      kScale: codes ? context.alloc(vectors * 4) : null,
+      vScale: codes ? context.alloc(vectors * 4) : null,
+    };
+    this.desc = {
+      pages, pageSize, kvHeads, headDim, dtype: codeOf(DTYPE, dtype, 'dtype'), format: codes,
+      k: this.buffers.k.handle, v: this.buffers.v.handle,
+      kScale: handleOf(this.buffers.kScale), vScale: handleOf(this.buffers.vScale),
+    };
+  }
+
+  // Rows of K and V ({ kStride, vStride, kOffset, vOffset }) into the slots of a device array of BigInt64;
+  // a slot outside the cache writes nothing.
+  write(k, v, slots, tokens, options = {}) {
+    this.context.addon.kvWrite(this.context.handle, this.desc,
+      Object.assign({}, options, { k: k.handle, v: v.handle, slots: slots.handle, tokens }));
+  }
+
+  // Slots back into rows; a slot outside the cache gives zeros.
+  read(slots, tokens, k, v, options = {}) {
+    this.context.addon.kvRead(this.context.handle, this.desc,
+      Object.assign({}, options, { k: k.handle, v: v.handle, slots: slots.handle, tokens }));
+  }
+
+  destroy() {
+    for (const b of Object.values(this.buffers)) if (b) b.destroy();
+  }
+}
+
+// Attention of a batch of sequences behind one shared prefix.
+//   batch: { cuSeqlens, ownLengths, prefixPages, prefixLength, ownPages }; without ownPages the own keys
+//   are the rows of options.k and options.v
+class SharedPrefixAttention {
+  constructor(context) {
+    this.context = context;
+  }
+
+  createRun(q, output, cache, batch, options = {}) {
+    const desc = Object.assign({}, options, batch, {
+      q: q.handle, o: output.handle, cache: cache.desc, k: handleOf(options.k), v: handleOf(options.v),
+      mask: maskCode(options.mask || 'causal'),
+    });
+    const addon = this.context.addon;
+    const handle = addon.createSharedRun(this.context.handle, desc);
+    return { handle, batch, info: addon.sharedRunInfo(handle) };
+  }
+
+  // The next batch (a step later): new lengths and pages for the same tensors.
+  updateRun(run, batch) {
+    this.context.addon.updateSharedRun(run.handle, batch);
+    run.batch = batch;
+    run.info = this.context.addon.sharedRunInfo(run.handle);
+  }
+
+  // Other tensors of the same strides and another cache of the same geometry (the next layer's).
+  rebindRun(run, q, output, cache, options = {}) {
+    this.context.addon.rebindSharedRun(run.handle, Object.assign({}, options, {
+      q: q.handle, o: output.handle, cache: cache.desc, k: handleOf(options.k), v: handleOf(options.v),
+    }), run.batch);
+  }
+
+  encode(run) { this.context.addon.encodeSharedRun(run.handle); }
+
+  destroyRun(run) {
+    if (run.handle) this.context.addon.destroySharedRun(run.handle);
+    run.handle = null;
+  }
+}
+
+module.exports = {
+  DeviceContext, DeviceBuffer, CausalAttentionKernel, CompactQ4Matmul, RotaryPositions, PagedKvCache,
+  SharedPrefixAttention, MASK,
+};
