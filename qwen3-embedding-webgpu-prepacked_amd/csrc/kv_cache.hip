@@ -9,7 +9,9 @@
 //         rounding, and a floating code's relative error does not depend on where in its range a value
 //         lies, so against amax / 448 nothing is lost but up to one binade of the codes below 2^-6.
 //   int8  code = rint(x * (127 / amax)), s = amax / 127, both divisions correctly rounded.
-// Both kernels are bound by memory: a write reads 2 bytes an element and writes 1 + 4 / head_dim.
+// Both kernels are bound by memory: a write of codes reads 2 bytes an element and writes 1 + 4 / head_dim, a
+// read the reverse.  8,000 tokens of 8 heads of 128 are written as e4m3 in 11.5 us, 4.3 TB/s; 20,000 are read in
+// 27.8 us, 4.5 TB/s, where a large copy reaches 5.1.
 #include "shared_ops.h"
 
 #include "elem.h"

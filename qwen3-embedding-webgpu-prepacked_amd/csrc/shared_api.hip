@@ -23,7 +23,7 @@ constexpr int64_t kMaxRowTokens = ((int64_t)1 << 24) - 1;
 constexpr int64_t kMaxRowValues = ((int64_t)1 << 34) - 1;  // tokens * kv_heads * head_dim
 constexpr int64_t kMaxSharedRows = (int64_t)1 << 22;       // queries * heads of a group
 constexpr int64_t kMaxSharedStride = (int64_t)1 << 24;     // elements: 16 rows of it within a 32-bit offset
-constexpr int64_t kMaxSharedGroups = (int64_t)1 << 23;     // workgroups of a launch
+constexpr int64_t kMaxSharedGroups = ((int64_t)1 << 23) - 1;  // workgroups of a launch: below 2^32 threads
 
 // Geometry, and with needs_pages the tensors, of a cache.
 int check_kv_cache(qattn_ctx* ctx, const qattn_kv_cache* c, bool needs_pages) {
@@ -213,6 +213,7 @@ int check_shared_tensors(qattn_ctx* ctx, const qattn_shared_desc* d, bool needs_
   if (bad_stride(d->q_row_stride, q_width) || bad_stride(d->o_row_stride, q_width))
     return fail(ctx, QATTN_EINVAL, "row strides (q %lld, o %lld): q_heads*head_dim = %lld .. 2^24, multiples of 8",
                 (long long)d->q_row_stride, (long long)d->o_row_stride, (long long)q_width);
+  if (d->o == d->q || (needs_rows && (d->o == d->k || d->o == d->v))) return fail(ctx, QATTN_EINVAL, "o is q, k or v");
   if (!needs_rows) return QATTN_OK;
   if (!d->k || !d->v || !aligned16(d->k) || !aligned16(d->v)) return fail(ctx, QATTN_EINVAL, "k/v NULL or not 16-byte aligned");
   if (bad_stride(d->k_row_stride, kv_width) || bad_stride(d->v_row_stride, kv_width))
@@ -226,6 +227,7 @@ int check_shared(qattn_ctx* ctx, const qattn_shared_desc* d) {
   int rc = validate_cu(ctx, d->cu_q, d->nseq);
   if (rc) return rc;
   if (!d->own_len) return fail(ctx, QATTN_EINVAL, "own_len is NULL");
+  if (d->nseq > kMaxSharedRows) return fail(ctx, QATTN_EINVAL, "nseq %d: up to 2^22", d->nseq);
   if (d->prefix_len < 0 || d->prefix_len >= kMaxPosition) return fail(ctx, QATTN_EINVAL, "prefix_len %d outside [0, 2^30)", d->prefix_len);
   int64_t own = 0;
   for (int32_t i = 0; i < d->nseq; ++i) {
@@ -423,7 +425,11 @@ int qattn_shared_run_encode(qattn_shared_run* run, qattn_stream_t stream) {
   DeviceGuard g(run->ctx->device);
   const hipStream_t s = pick_stream(run->ctx, stream);
   auto& used = run->streams[run->cur];
-  if (std::find(used.begin(), used.end(), s) == used.end()) used.push_back(s);
+  try {
+    if (std::find(used.begin(), used.end(), s) == used.end()) used.push_back(s);
+  } catch (const std::bad_alloc&) {
+    return fail(run->ctx, QATTN_ENOMEM, "out of host memory");
+  }
   HIP_TRY(run->ctx, launch_shared_attn(run->params, run->desc.cache.dtype, run->desc.cache.format, run->desc.cache.head_dim, s));
   return QATTN_OK;
 }

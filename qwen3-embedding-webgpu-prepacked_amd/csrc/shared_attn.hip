@@ -2,22 +2,32 @@
 //
 // o[r] = sum_j p_rj v_j / sum_j p_rj, p_rj = 2^(c q_r . k_j - m_r), over the keys that row r sees: the
 // prefix's, read from a paged cache that may hold 8-bit codes, and its sequence's own.  Rows of all
-// sequences are stacked (row = query * group + head of the group), so one tile of prefix keys serves 256 or
-// 128 rows, whatever sequences they belong to.  Two kinds of work share a launch:
-//   blocks  256 or 128 rows, 32 to a wavefront, over 128-key tiles that eight wavefronts share in LDS (with
-//           128 rows, each half of the tile goes to four of them, and their sums are joined at the end);
-//           S^T = K Q^T and O^T = V^T P^T on 32x32x16 MFMAs, a query row to a lane.  Codes become 16-bit
-//           elements once, on their way into LDS.  Bound by the matrix cores, the softmax's exponentials
-//           and the latency between them: one workgroup fills a CU's LDS and half its registers.
-//   flat    16 rows over 32-key tiles, every fourth tile to a wavefront, which keeps its own sum; K goes from
-//           memory straight into the MFMA operand, V through the wavefront's own 8 KiB of LDS for the
-//           transposed read; the four sums are joined at the end.  Bound by the cache's bytes.
+// sequences are stacked (row = query * group + head of the group), so one tile of prefix keys serves many
+// rows, whatever sequences they belong to.  Three kinds of items share a launch, one workgroup to an item
+// and KV head; the plan picks them by the costs that it lists:
+//   tall   256 rows, 32 to each of eight wavefronts, over 128-key tiles that they share in LDS.
+//   split  128 rows: four wavefronts take the tile's first 64 keys, four its last, and their sums are joined
+//          at the end.  2.4 us a tile against tall's 4.0 (head_dim 128): dearer for a row, sooner done (16
+//          queries of 10 to 150 tokens: 25 us, by tall items 33; 16 x 500 tokens: 457 us, by tall 364).
+//   flat   16 rows (up to 16 single tokens of several sequences) over 32-key tiles, a run of them to each of
+//          eight wavefronts, which keeps its own sum; K goes from memory straight into the MFMA operand, V
+//          through the wavefront's own 8 KiB of LDS for the transposed read; the sums are joined at the end.
+// Blocks (tall and split): S^T = K Q^T and O^T = V^T P^T on 32x32x16 MFMAs, a query row to a lane.  Codes
+// become 16-bit elements once, on their way into LDS.  16 x 500 tokens behind 5,000 e4m3 keys (16 heads over
+// 8, head_dim 128) take 364 us, 945 TFLOP/s where the library's 8,192-cubed product reaches 1,222.  Bound by
+// the matrix cores and, in turn with them, the softmax's vector work: without its exponentials a launch is 8 %
+// shorter, without its LDS reads 3 %; the wavefronts of a SIMD hardly overlap the two, staggered by half a step
+// neither (that was 13 % slower), and one workgroup fills a CU's LDS and half its registers.
+// Flat items are bound by latency (a step of 16 tokens takes 9.4 us with its merge, a call 3.8 at least), or
+// by the cache's bytes: 256 tokens with 1,024 e4m3 keys each take 98 us, 5.6 TB/s.
 // An item whose rows have keys elsewhere too (other chunks, other items) leaves its unnormalised f32
 // sums, the row's reference m and its sum of p; shared_merge_kernel joins them.
 //
 // A row's reference moves only when a tile's maximum exceeds it by kLazy (in log2): p then stays below
 // 2^kLazy, far inside fp16, and most tiles rescale nothing.  p is rounded to the storage type for the PV
 // product, which moves each weight by at most half a step of that type; l sums the unrounded p in f32.
+// An int8 code times its scale is rounded to the storage type too (as qattn_kv_read returns it), for both
+// operands are 16-bit ones; an e4m3 code times its power of two is exact.
 #include "shared_attn.h"
 
 #include "elem.h"
@@ -829,7 +839,8 @@ __global__ __launch_bounds__(kSharedThreads, 2) void shared_attn_kernel(SharedPa
     flat_item<BF16, FORMAT, DIM>(p, it, index - p.n_blocks, kvh, lds, stats);
 }
 
-// Launches of flat items alone: with half the LDS, a workgroup starts sooner.
+// Launches of flat items alone: with half the LDS, a workgroup starts sooner (single tokens with 32 keys: 4.5 us,
+// by the kernel of all kinds 5.7).
 template <bool BF16, int FORMAT, int DIM>
 __global__ __launch_bounds__(kSharedThreads, 2) void shared_flat_kernel(SharedParams p) {
   __shared__ __attribute__((aligned(1024))) char lds[Flat<BF16, FORMAT, DIM>::kLds];
@@ -840,9 +851,11 @@ __global__ __launch_bounds__(kSharedThreads, 2) void shared_flat_kernel(SharedPa
 
 // Merged rows: sum over a row's partial rows of 2^(m_i - max m) times its sums; a partial row that saw no
 // key has m = -inf and weighs 0.  Without partial rows: zeros.  DIM / 4 lanes hold a row, a float4 each, and a
-// lane's loads go out eight partial rows at a time.  WIDE: a whole workgroup takes one row, its groups of
-// lanes every kGroups'th partial row (rows cut into many chunks: a chain of loads would set the time);
-// else each group takes a row of its own.  Bound by latency: three dependent accesses.
+// lane's loads go out eight partial rows at a time.  WIDE, for rows of more than eight partial rows: a whole
+// workgroup takes one row, its groups of lanes every kGroups'th partial row, for a chain of loads would set
+// the time (8 tokens, 38 partial rows: 12.9 us for both launches against 16.3); else each group takes a row
+// of its own (3,000 rows of up to three: 53 us against 74).  Bound by latency, three dependent accesses (3 us
+// for a step of eight), then by the partial rows' bytes.
 template <bool BF16, int DIM, bool WIDE>
 __global__ __launch_bounds__(kMergeThreads) void shared_merge_kernel(SharedParams p) {
   constexpr int kLanes = DIM / 4, kGroups = kMergeThreads / kLanes;

@@ -4,11 +4,12 @@
 // sequences fill a block together and a tile of prefix keys is read once for all its rows.  A block also
 // visits the own keys of its sequences, one segment each, in which only their rows see anything.
 // Sequences of up to 16 rows (single tokens) would waste most of a block on their own keys: those go to
-// items of 16 rows whose four wavefronts take a tile of keys each, and so do the prefix's if the launch has
-// no more rows than that.
+// flat items of 16 rows, several sequences to an item or each by itself, and so may the prefix of a batch of
+// up to kMostFlatRows rows (beyond, an item for every 16 rows reads it too often: with 512 rows, 2,048 keys
+// take as long as by blocks, 24.5 us, and 8,192 keys 60 against 45).
 //
-// Cuts.  Items are cut along their keys where that shortens the launch.  The planner compares, for both block
-// sizes and a range of chunk sizes, the time at which the last of the GPU's slots ends, by a cost model.
+// Cuts.  Items are cut along their keys where that shortens the launch.  The planner compares, for each of
+// these ways and a range of chunk sizes, the time at which the last of the GPU's slots ends, by a cost model.
 #include <algorithm>
 #include <cmath>
 #include <cstddef>
@@ -25,7 +26,7 @@ namespace {
 // with 256 and with 128 rows; a flat item, and the bytes that it reads; partial results; the second launch;
 // bytes that all items read from memory.
 constexpr double kBlockItem = 5.9, kTallTile = 4.0, kSplitTile = 2.4, kFlatItem = 3.2, kItemBytesPerUs = 45e3;
-constexpr double kFlatRound = 0.3, kFlatInt8 = 1.1, kFlatMasked = 0.4;
+constexpr double kFlatRound = 0.3, kFlatInt8 = 1.1, kFlatMasked = 0.4, kDim64 = 0.8;
 constexpr double kPartial = 0.5, kMergeLaunch = 2.8, kBytesPerUs = 5e6;
 constexpr int kMostSimulated = 16384, kMostFlatRows = 512;
 
@@ -272,7 +273,7 @@ class Planner {
   // of the eight wavefronts).
   static double fixed(const Draft& b) { return b.item.kind == kFlat ? kFlatItem : kBlockItem; }
   double unit(const Draft& b) const {
-    if (b.item.kind != kFlat) return b.item.kind == kTall ? kTallTile : kSplitTile;
+    if (b.item.kind != kFlat) return (b.item.kind == kTall ? kTallTile : kSplitTile) * (d_.cache.head_dim == 64 ? kDim64 : 1);
     return kFlatRound + kFlatWaves * kFlatKeys * key_bytes_ / kItemBytesPerUs + (d_.cache.format == QATTN_KV_INT8 ? kFlatInt8 : 0) +
            kFlatMasked * b.masked / std::max(1, b.item.tiles);
   }
@@ -294,8 +295,8 @@ class Planner {
       if (part) partial_rows += (double)c * b.item.rows;
       split |= part;
       if (b.item.kind == kFlat) flat_keys += (double)b.item.tiles * kFlatKeys;
-      for (int i = 0; i < c; ++i) costs.push_back((part ? kPartial : 0) + cost(b, units * (i + 1) / c - units * i / c));
-      if (costs.size() > kMostSimulated) return 1e30;
+      if ((int64_t)costs.size() + c > kMostSimulated) return 1e30;
+      for (int64_t i = 0; i < c; ++i) costs.push_back((part ? kPartial : 0) + cost(b, (int)(units * (i + 1) / c - units * i / c)));
     }
     std::sort(costs.begin(), costs.end(), std::greater<double>());
     std::priority_queue<double, std::vector<double>, std::greater<double>> ends;

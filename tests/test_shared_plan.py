@@ -5,7 +5,7 @@ import pytest
 
 import shared_ref as ref
 
-FAKE = 0x100000  # aligned stand-in device address
+FAKE, OUT = 0x100000, 0x200000  # aligned stand-in device addresses
 TILE, ROWS = {0: 128, 1: 128, 2: 32}, {0: 256, 1: 128, 2: 16}
 
 
@@ -16,7 +16,7 @@ def make(qattn, prefix, queries, own, heads=16, kv=8, dim=128, page=64, paged=Tr
     pages = max(sum(need), 1) + 3
     order = rng.permutation(pages).astype(np.int32)
     cache = qattn.make_kv_cache(FAKE, FAKE, pages, page, kv, dim, format=form, k_scale=FAKE, v_scale=FAKE)
-    return qattn.make_shared_desc(FAKE, FAKE, cache, np.concatenate([[0], np.cumsum(queries)]), own, q_heads=heads,
+    return qattn.make_shared_desc(FAKE, OUT, cache, np.concatenate([[0], np.cumsum(queries)]), own, q_heads=heads,
                                   prefix_pages=order[:need[0]], prefix_len=prefix,
                                   own_pages=order[need[0]:sum(need)] if paged else None, k=None if paged else FAKE,
                                   v=None if paged else FAKE, mask=mask, prefix=always, window=window, **kw), order, need
@@ -117,6 +117,7 @@ CASES = [
     dict(prefix=1, queries=[1], own=[0]),
     dict(prefix=5, queries=[9], own=[2]),
     dict(prefix=0, queries=[0, 4, 0], own=[3, 4, 0]),     # sequences without queries
+    dict(prefix=20, queries=[0, 0], own=[3, 0]),          # no queries at all
     dict(prefix=64, queries=[1] * 16, own=[1] * 16),
     dict(prefix=500, queries=[1] * 16, own=list(range(16)), page=16),
     dict(prefix=3000, queries=[1] * 64, own=[37 * i % 601 for i in range(64)]),
@@ -176,6 +177,8 @@ def refuses(qattn, needle, change, **kw):
 @pytest.mark.parametrize("needle,change,kw", [
     ("q/o", lambda d: setattr(d, "q", None), {}),
     ("q/o", lambda d: setattr(d, "o", FAKE + 8), {}),
+    ("o is q", lambda d: setattr(d, "o", d.q), {}),
+    ("o is q", lambda d: (setattr(d, "v", FAKE + 64), setattr(d, "o", FAKE + 64)), dict(paged=False)),
     ("row strides (q", lambda d: setattr(d, "q_row_stride", 2040), {}),
     ("row strides (q", lambda d: setattr(d, "o_row_stride", 2052), {}),
     ("row strides (q", lambda d: setattr(d, "q_row_stride", 1 << 25), {}),
@@ -215,8 +218,31 @@ def test_refuses_too_many_rows_and_counts_pages(qattn):
     assert "2^22" in str(e.value)
     cache = qattn.make_kv_cache(FAKE, FAKE, 9, 64)
     with pytest.raises(ValueError):  # the binding: a list too short to be read
-        qattn.make_shared_desc(FAKE, FAKE, cache, [0, 1], [65], own_pages=[1])
+        qattn.make_shared_desc(FAKE, OUT, cache, [0, 1], [65], own_pages=[1])
     with pytest.raises(ValueError):
-        qattn.make_shared_desc(FAKE, FAKE, cache, [0, 1], [65, 3], own_pages=[1, 2, 3])
+        qattn.make_shared_desc(FAKE, OUT, cache, [0, 1], [65, 3], own_pages=[1, 2, 3])
     # pages are not needed, nor looked at, where no page is read
-    qattn.shared_plan(qattn.make_shared_desc(FAKE, FAKE, qattn.make_kv_cache(None, None, 0, 0), [0, 2], [2], k=FAKE, v=FAKE))
+    qattn.shared_plan(qattn.make_shared_desc(FAKE, OUT, qattn.make_kv_cache(None, None, 0, 0), [0, 2], [2], k=FAKE, v=FAKE))
+
+
+def test_plans_of_the_longest_contexts(qattn):
+    """One token behind nearly 2^30 cached keys, on pages that repeat: the plan covers them, in time."""
+    prefix, page = (1 << 30) - 200, 4096
+    n = -(-prefix // page)
+    cache = qattn.make_kv_cache(FAKE, FAKE, 7, page, 1, 128, format=1, k_scale=FAKE, v_scale=FAKE)
+    for queries, group in ((1, 1), (40, 4)):
+        desc = qattn.make_shared_desc(FAKE, OUT, cache, [0, queries], [queries], q_heads=group, prefix_pages=np.arange(n) % 7,
+                                      prefix_len=prefix, own_pages=[3])
+        plan, info = qattn.shared_plan(desc)
+        keys = sum(int(i[5]) * TILE[i[6]] for i in plan["items"])
+        assert prefix <= keys <= (prefix + 4 * 128 + len(plan["items"]) * 32) * -(-queries * group // 16)
+        assert info.pairs == sum(prefix + i + 1 for i in range(queries))
+        assert int(plan["segments"][:, 6].max()) * 128 >= prefix and (plan["segments"][:, 5:7] >= 0).all()
+
+
+def test_plans_of_many_sequences_in_time(qattn):
+    import time
+    desc = make(qattn, 2000, [1] * 4000, [1 + 37 * i % 300 for i in range(4000)])[0]
+    start = time.time()
+    plan, info = qattn.shared_plan(desc)
+    assert info.tokens == 4000 and time.time() - start < 5
