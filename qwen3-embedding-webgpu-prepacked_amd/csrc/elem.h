@@ -59,20 +59,25 @@ __device__ inline u32x2 e4m3_elems(uint32_t codes, float scale) {
                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, scale, true))};
   }
 }
-// Four int8 codes of a dword times `scale`, each product rounded to f32 and then to 16 bits.  0x6400 | u is
-// 1024 + u in fp16, so a byte permute and an exact packed subtraction give the codes as fp16, which the
-// multiplications widen for free: an integer conversion for each code takes the cache four times the issue
-// slots.
-template <bool BF16>
-__device__ inline u32x2 int8_elems(uint32_t codes, float scale) {
+// Four int8 codes of a dword as fp16, which is exact: 0x6400 | u is 1024 + u, so a byte permute and a packed
+// subtraction do it (an integer conversion for each code takes the cache four times the issue slots).
+__device__ inline u32x2 int8_halves(uint32_t codes) {
   typedef Elem<false>::T2 H2;
   const uint32_t u = codes ^ 0x80808080u;
   const auto pair = [&](uint32_t select) {
     const H2 raw = __builtin_bit_cast(H2, __builtin_amdgcn_perm(0x64646464u, u, select));
-    const uint32_t h = __builtin_bit_cast(uint32_t, raw - H2{(_Float16)1152.f, (_Float16)1152.f});
-    return narrow2<BF16>(fmaf(widen<false, 0>(h), scale, 0.f), fmaf(widen<false, 1>(h), scale, 0.f));
+    return __builtin_bit_cast(uint32_t, raw - H2{(_Float16)1152.f, (_Float16)1152.f});
   };
   return u32x2{pair(0x04010400u), pair(0x04030402u)};
+}
+// The codes times `scale`, each product rounded to f32 and then to 16 bits.
+template <bool BF16>
+__device__ inline u32x2 int8_elems(uint32_t codes, float scale) {
+  const u32x2 h = int8_halves(codes);
+  const auto pair = [&](uint32_t x) {
+    return narrow2<BF16>(fmaf(widen<false, 0>(x), scale, 0.f), fmaf(widen<false, 1>(x), scale, 0.f));
+  };
+  return u32x2{pair(h[0]), pair(h[1])};
 }
 
 }  // namespace qattn

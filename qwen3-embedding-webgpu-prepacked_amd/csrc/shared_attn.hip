@@ -26,9 +26,9 @@
 // A row's reference moves only when a tile's maximum exceeds it by kLazy (in log2): p then stays below
 // 2^kLazy, far inside fp16, and most tiles rescale nothing.  p is rounded to the storage type for the PV
 // product, which moves each weight by at most half a step of that type; l sums the unrounded p in f32.
-// An int8 code times its scale is rounded to the storage type too (as qattn_kv_read returns it), for both
-// operands are 16-bit ones; an e4m3 code times its power of two is exact.
 #include "shared_attn.h"
+
+#include <utility>
 
 #include "elem.h"
 
@@ -79,6 +79,15 @@ __device__ inline float rows_max(float x) {
 __device__ inline float rows_sum(float x) {
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return half_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+// Lane I of each 16-lane row, in all its lanes: an operand modifier.
+template <int I>
+__device__ inline float row_lane(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x150 + I, 0xf, 0xf, true));
+}
+template <class F, int... I>
+__device__ inline void each_index(std::integer_sequence<int, I...>, F f) {
+  (f(std::integral_constant<int, I>{}), ...);
 }
 __device__ inline int wave_max(int x) {
   for (int d = 32; d; d >>= 1) x = max(x, __shfl_xor(x, d));
@@ -140,6 +149,9 @@ struct Keys {
   __device__ float scale_of(int i, uint32_t group, uint32_t row) const {
     return *reinterpret_cast<const float*>(scale[i] + ((uint64_t)group * 64 | 4 * row));
   }
+  __device__ f4 scales_of(int i, uint32_t group, uint32_t row) const {
+    return *reinterpret_cast<const f4*>(scale[i] + ((uint64_t)group * 64 | 4 * row));
+  }
   __device__ const char* row(int i, uint32_t row, uint32_t offset) const {
     return rows[i] + ((uint64_t)row * stride[i] + offset);
   }
@@ -149,14 +161,48 @@ __device__ inline uint32_t group_of(const SharedParams& p, const SharedSeg& s, i
   return s.source == kOwnRows ? 0 : (uint32_t)p.groups[zero + s.base + (first >> 4)];
 }
 
-// 16 codes as two 16-byte chunks of 16-bit elements.
-template <bool BF16, int FORMAT>
+// ---- int8 caches -----------------------------------------------------------------------------------
+// A code times its scale would have to be rounded to a 16-bit element, K's and V's, which doubles the result's
+// error.  Instead the products take the codes, which are exact: K's scale goes to the key's scores in f32, and
+// V's to its weights.  A weight is rounded to 16 bits after that, so V's elements are the codes times a power
+// of two 2^e near the scale (exact too, and finite for any code), and the weight's factor is scale / 2^e: 1 to
+// 2.02 for the scales that kv_write gives, but fp16 ones under 2^-24.
+template <bool BF16>
+__device__ inline float near_power(float scale) {
+  const int e = min(max((int)(__float_as_uint(scale) >> 23 & 255u) - 127, BF16 ? -110 : -24), BF16 ? 119 : 8);
+  return copysignf(ldexpf(1.f, e), scale);
+}
+// Not below 2^-8: a scale of 0 gives values that vanish in rounding.
+template <bool BF16>
+__device__ inline float value_factor(float scale) {
+  const float f = scale / near_power<BF16>(scale);
+  return f < 0x1p-8f ? 0x1p-8f : f;
+}
+
+// 16 codes of K (I = 0) or V (1) as two 16-byte chunks of 16-bit elements, exactly: an e4m3 code times its
+// power of two; of an int8 code the factor of its key (below) is left out.
+template <bool BF16, int FORMAT, int I>
 __device__ inline void expand(u32x4 codes, float scale, u32x4 (&out)[2]) {
+  typedef Elem<false>::T2 H2;
+  if constexpr (FORMAT == QATTN_KV_E4M3) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const u32x2 y = FORMAT == QATTN_KV_E4M3 ? e4m3_elems<BF16>(codes[e], scale) : int8_elems<BF16>(codes[e], scale);
-    out[e >> 1][2 * (e & 1)] = y[0];
-    out[e >> 1][2 * (e & 1) + 1] = y[1];
+    for (int e = 0; e < 4; ++e) {
+      const u32x2 y = e4m3_elems<BF16>(codes[e], scale);
+      out[e >> 1][2 * (e & 1)] = y[0];
+      out[e >> 1][2 * (e & 1) + 1] = y[1];
+    }
+  } else {
+    const float two = I ? near_power<BF16>(scale) : 1.f;
+    const H2 two2 = {(_Float16)two, (_Float16)two};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      uint32_t h = int8_halves(codes[e >> 1])[e & 1];
+      if constexpr (BF16)
+        h = narrow2<true>(fmaf(widen<false, 0>(h), two, 0.f), fmaf(widen<false, 1>(h), two, 0.f));
+      else if constexpr (I == 1)
+        h = __builtin_bit_cast(uint32_t, __builtin_bit_cast(H2, h) * two2);
+      out[e >> 2][e & 3] = h;
+    }
   }
 }
 
@@ -164,7 +210,7 @@ __device__ inline void expand(u32x4 codes, float scale, u32x4 (&out)[2]) {
 // A masked key's p is 0, but 0 times an infinity or NaN is NaN.  In tiles that some row of the item sees
 // only part of, such elements of V are replaced by 0 on their way into LDS, and if there were any, the
 // rows that do see the key get them added at the end (p times an infinity is that infinity, whatever the
-// reference).
+// reference).  (An int8 code's infinity or NaN is its key's factor's.)
 template <bool BF16>
 __device__ inline void drop_nonfinite(u32x4& chunk) {
   constexpr uint32_t kExp = Elem<BF16>::kExponent;
@@ -197,20 +243,24 @@ __device__ inline f4 value_at(const SharedParams& p, const Keys<FORMAT, DIM>& ke
     } else {
       const uint32_t codes = *reinterpret_cast<const uint32_t*>(at);
       const float scale = keys.scale_of(1, group, row);
-      x = FORMAT == QATTN_KV_E4M3 ? e4m3_elems<BF16>(codes, scale) : int8_elems<BF16>(codes, scale);
+      if constexpr (FORMAT == QATTN_KV_INT8) {
+        const u32x2 h = int8_halves(codes);
+        return f4{widen<false, 0>(h[0]), widen<false, 1>(h[0]), widen<false, 0>(h[1]), widen<false, 1>(h[1])} * scale;
+      }
+      x = e4m3_elems<BF16>(codes, scale);
     }
   }
   return f4{widen<BF16, 0>(x[0]), widen<BF16, 1>(x[0]), widen<BF16, 0>(x[1]), widen<BF16, 1>(x[1])};
 }
 __device__ inline float nonfinite(float v, bool seen) { return seen && !(fabsf(v) < INFINITY) ? v : 0.f; }
-// Calls add(value, seen) for every key of the item's tiles first, first + step, ... (of `size` keys) that not
-// all rows see: value(d) is elements d .. d + 3 of its V, seen whether row `row` at position `at` sees it.
+// Calls add(value, seen) for every key of `tiles` tiles (of `size` keys) from c on that not all rows see (int8: for
+// every key): value(d) is elements d .. d + 3 of its V, seen whether row `row` at position `at` sees it.
 template <bool BF16, int FORMAT, int DIM, class Add>
 __device__ inline void each_nonfinite(const SharedParams& p, const Keys<FORMAT, DIM>& keys, Cursor c, int tiles, int row,
                                       int at, int size, Add add) {
   for (int t = 0;;) {
     const SharedSeg s = c.seg;
-    if (!s.whole) {
+    if (!s.whole || FORMAT == QATTN_KV_INT8) {
       const int mine = row >= s.row_begin && row < s.row_end ? at : -1;
       for (int key = c.tile * size; key < min(s.keys, (c.tile + 1) * size); ++key) {
         const int pos = s.position + key;
@@ -271,10 +321,12 @@ struct Tall {
     }
   }
 
-  // The loaded K (I = 0) or V (1) into LDS as 16-bit elements.  partly: infinities and NaN are
-  // taken out (of V, in tiles that some row sees only part of); returns whether there were any.
+  // The loaded K (I = 0) or V (1) into LDS as 16-bit elements, and in runs with an int8 cache its keys' factors: of
+  // scores (K; scale_log2 included) and of weights (V).  partly: infinities and NaN are taken
+  // out (of V, in tiles that some row sees only part of); returns whether there were any.
   template <int I>
-  __device__ bool store(char* lds, bool rows, int wave, int lane, bool partly) {
+  __device__ bool store(char* lds, float* factors, float scale_log2, bool rows, int wave, int lane, bool partly) {
+    const bool fold = FORMAT == QATTN_KV_INT8 && !rows;
     const auto each = [&](auto put) {
       if (!kCodes || rows) {
 #pragma unroll
@@ -285,7 +337,7 @@ struct Tall {
         for (int j = 0; j < kLoads8; ++j) {
           const int r = 16 * wave + j * kRows8 + lane / kChunks8, c = 2 * (lane % kChunks8);
           u32x4 x[2];
-          expand<BF16, FORMAT>(raw[I][j], scale[I][kCodes ? j : 0], x);
+          expand<BF16, FORMAT, I>(raw[I][j], scale[I][kCodes ? j : 0], x);
           put(r, c, x[0]);
           put(r, c + 1, x[1]);
         }
@@ -293,9 +345,23 @@ struct Tall {
     };
     uint32_t seen = 0;
     each([&](int r, int c, u32x4 x) {
-      if (I && partly) seen = see_nonfinite<BF16>(seen, x);
+      if (I && partly && !fold) seen = see_nonfinite<BF16>(seen, x);
       *reinterpret_cast<u32x4*>(lds + (I ? v_at(r, c) : k_at(r, c))) = x;
     });
+    if constexpr (FORMAT == QATTN_KV_INT8) {
+      bool any = false;
+#pragma unroll
+      for (int j = 0; j < kLoads8; ++j) {
+        float f = !fold ? 1.f : I ? value_factor<BF16>(scale[I][j]) : scale[I][j];
+        if (I && !(f < INFINITY)) {
+          any = true;
+          f = 1.f;
+        }
+        float* at = factors + 16 * wave + j * kRows8 + lane / kChunks8;
+        if (lane % kChunks8 == 0) at[I * kTallKeys] = I ? f : f * scale_log2;
+      }
+      if (fold) return I && __any(any);
+    }
     if (!I || !partly || !__any(seen & 0x80008000u)) return false;
     each([&](int r, int c, u32x4 x) {
       drop_nonfinite<BF16>(x);
@@ -311,8 +377,8 @@ __device__ constexpr int key_off(int r) { return 32 * (r >> 4) + 8 * ((r & 15) >
 // Tile t is in LDS while tile t + 1 is in registers or on its way there: at the end of an iteration those go
 // into the other buffers and tile t + 2 is asked for.
 template <bool BF16, int FORMAT, int DIM>
-__device__ inline void tall_item(const SharedParams& p, const SharedItem& it, int index, int kvh, char* lds, float2* stats,
-                                 uint32_t* dropped) {
+__device__ inline void tall_item(const SharedParams& p, const SharedItem& it, int index, int kvh, char* lds, float* factors,
+                                 float2* stats, uint32_t* dropped) {
   typedef Tall<BF16, FORMAT, DIM> T;
   constexpr int kBlocks = DIM / 32, kSteps = DIM / 16;
   const int lane = threadIdx.x & 63, lq = lane & 31, hl = lane >> 5;
@@ -360,8 +426,9 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
   };
   const auto keep = [&](int t) {
     char* buf = lds + (t & 1) * 2 * T::kTile;
-    tile.template store<0>(buf, spot.rows, wave, lane, false);
-    found |= tile.template store<1>(buf + T::kTile, spot.rows, wave, lane, !next.whole);
+    float* f = factors + (t & 1) * 2 * kTallKeys;
+    tile.template store<0>(buf, f, p.scale_log2, spot.rows, wave, lane, false);
+    found |= tile.template store<1>(buf + T::kTile, f, p.scale_log2, spot.rows, wave, lane, !next.whole);
   };
 
   ask();
@@ -394,7 +461,7 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
   // Scores, weights and sums of the 64 keys at k, v, of which the first stands at position `from`.  Operands
   // are read ahead; the scheduling barriers keep the compiler from reading them all at once, for which there
   // are no registers.
-  const auto add_part = [&](const Info& cur, int from, const char* k, const char* v) {
+  const auto add_part = [&](const Info& cur, int from, const char* k, const char* v, const float* f) {
     f16x sc[2];
     {
       // Rows lq and lq + 32, chunk 2 st + hl: its swizzled place is 2 st xor'ed onto chunk hl's.  (Formed here:
@@ -418,6 +485,24 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
       __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_s_setprio(0);
     }
+    // int8: this lane's row of 16 holds the factors of its half's keys, elements 0 .. 15 and 16 .. 31; the scores get
+    // theirs, with scale_log2, here, else that comes in with the exponential.  (A read of LDS for each lane's
+    // operands would take twice the bandwidth that K and V do at head_dim 64.)
+    constexpr bool kFold = FORMAT == QATTN_KV_INT8;
+    const float unit = kFold ? 1.f : p.scale_log2;
+    float kf[2] = {}, vf[2] = {};
+    if constexpr (kFold) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const float* mine = f + 32 * b + 8 * ((lane & 15) >> 2) + 4 * hl + (lane & 3);
+        kf[b] = mine[0];
+        vf[b] = mine[kTallKeys];
+      }
+      each_index(std::make_integer_sequence<int, 32>{}, [&](auto r) {
+        constexpr int R = decltype(r)::value;
+        sc[R >> 4][R & 15] *= row_lane<R & 15>(kf[R >> 4]);
+      });
+    }
     if (!cur.whole) {
       // Offsets from this lane's first key: the last one seen, and where the prefix and the window leave a gap.
       const int mine = row >= cur.row_begin && row < cur.row_end ? at : -1;
@@ -436,7 +521,7 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
     float top = fmaxf(fmaxf(sc[0][0], sc[0][1]), sc[0][2]);
 #pragma unroll
     for (int r = 3; r < 31; r += 2) top = fmaxf(fmaxf(top, sc[r >> 4][r & 15]), sc[(r + 1) >> 4][(r + 1) & 15]);
-    top = half_max(fmaxf(top, sc[1][15])) * p.scale_log2;
+    top = half_max(fmaxf(top, sc[1][15])) * unit;
     if (__any(top > m + kLazy)) {  // from -inf too: any score exceeds it
       const float moved = top > m + kLazy ? top : m;
       const float shrink = m == moved ? 1.f : __builtin_amdgcn_exp2f(m - moved);
@@ -449,14 +534,18 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
     // Slot j of half hl at step st is key 16 st + 8 (j >> 2) + 4 hl + (j & 3): element 8 st + j of the scores.
     u32x4 pf[4];
     float sum[2] = {};
-#pragma unroll
-    for (int r = 0; r < 32; r += 2) {
-      const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[r >> 4][r & 15], p.scale_log2, -ref));
-      const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[r >> 4][(r & 15) + 1], p.scale_log2, -ref));
+    each_index(std::make_integer_sequence<int, 16>{}, [&](auto i) {
+      constexpr int R = 2 * decltype(i)::value, B = R >> 4, E = R & 15;
+      float p0 = __builtin_amdgcn_exp2f(kFold ? sc[B][E] - ref : fmaf(sc[B][E], unit, -ref));
+      float p1 = __builtin_amdgcn_exp2f(kFold ? sc[B][E + 1] - ref : fmaf(sc[B][E + 1], unit, -ref));
       sum[0] += p0;
       sum[1] += p1;
-      pf[r >> 3][(r & 7) >> 1] = narrow2<BF16>(p0, p1);
-    }
+      if constexpr (kFold) {
+        p0 *= row_lane<E>(vf[B]);
+        p1 *= row_lane<E + 1>(vf[B]);
+      }
+      pf[R >> 3][(R & 7) >> 1] = narrow2<BF16>(p0, p1);
+    });
     l += sum[0] + sum[1];
     const auto v_frag = [&](int i) {
       const char* src = v + v_read[i % kBlocks] + i / kBlocks * 16 * T::kRow;
@@ -490,7 +579,8 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
       for (int part = part_begin; part < part_end; ++part) {
         const int from = now.from + 64 * part;
         if (now.whole || from <= min(greatest, now.last))
-          add_part(now, from, buf + part * 64 * T::kRow, buf + T::kTile + part * 64 * T::kRow);
+          add_part(now, from, buf + part * 64 * T::kRow, buf + T::kTile + part * 64 * T::kRow,
+                   factors + (t & 1) * 2 * kTallKeys + 64 * part);
       }
     }
     if (t + 1 < it.tiles) {
@@ -584,6 +674,7 @@ struct Flat {
   // half) and V's rows as they lie.
   u32x4 k[2][kSteps], v[2][kLoads16];
   float ks[2], vs[2][kCodes ? kLoads8 : 1];
+  f4 kf[2], vf[2];  // int8: the scales of keys 4 (lane >> 4) + 0 .. 3 of each group
 
   // Tile `tile` of segment s, whose two groups are `group`.  (Rows past the last key: as in Tall.)
   __device__ void load(const Keys<FORMAT, DIM>& keys, const SharedSeg& s, int tile, const uint32_t (&group)[2], int lane) {
@@ -605,7 +696,12 @@ struct Flat {
         if constexpr (kCodes) {
 #pragma unroll
           for (int h = 0; h < DIM / 64; ++h) k[b][h] = *reinterpret_cast<const u32x4*>(src + 64 * h);
-          ks[b] = keys.scale_of(0, group[b], key);
+          if constexpr (FORMAT == QATTN_KV_INT8) {
+            kf[b] = keys.scales_of(0, group[b], 4 * c);
+            vf[b] = keys.scales_of(1, group[b], 4 * c);
+          } else {
+            ks[b] = keys.scale_of(0, group[b], key);
+          }
         } else {
 #pragma unroll
           for (int st = 0; st < kSteps; ++st) k[b][st] = *reinterpret_cast<const u32x4*>(src + 128 * (st >> 1) + 16 * (st & 1));
@@ -627,7 +723,7 @@ struct Flat {
 #pragma unroll
       for (int h = 0; h < DIM / 64; ++h) {
         u32x4 x[2];
-        expand<BF16, FORMAT>(k[b][h], ks[b], x);
+        expand<BF16, FORMAT, 0>(k[b][h], ks[b], x);
         out[2 * h] = x[0];
         out[2 * h + 1] = x[1];
       }
@@ -645,19 +741,20 @@ struct Flat {
           for (int j = 0; j < kLoads8; ++j) {
             const int r = 16 * b + j * kRows8 + lane / kChunks8, c = 2 * (lane % kChunks8);
             u32x4 x[2];
-            expand<BF16, FORMAT>(v[b][j], vs[b][kCodes ? j : 0], x);
+            expand<BF16, FORMAT, 1>(v[b][j], vs[b][kCodes ? j : 0], x);
             put(r, c, x[0]);
             put(r, c + 1, x[1]);
           }
         }
       }
     };
+    const bool fold = FORMAT == QATTN_KV_INT8 && s.source != kOwnRows;
     uint32_t seen = 0;
     each([&](int r, int c, u32x4 x) {
-      if (partly) seen = see_nonfinite<BF16>(seen, x);
+      if (partly && !fold) seen = see_nonfinite<BF16>(seen, x);
       *reinterpret_cast<u32x4*>(lds + v_at(r, c)) = x;
     });
-    if (!partly || !__any(seen & 0x80008000u)) return false;
+    if (!partly || fold || !__any(seen & 0x80008000u)) return false;
     each([&](int r, int c, u32x4 x) {
       drop_nonfinite<BF16>(x);
       *reinterpret_cast<u32x4*>(lds + v_at(r, c)) = x;
@@ -725,6 +822,22 @@ __device__ inline void flat_item(const SharedParams& p, const SharedItem& it, in
         for (int st = 0; st < T::kSteps; ++st) sc[b] = mfma16<BF16>(a[st], q[st], sc[b]);
       }
       const bool part = !s.whole;
+      f4 factor[2] = {{1.f, 1.f, 1.f, 1.f}, {1.f, 1.f, 1.f, 1.f}};
+      if constexpr (FORMAT == QATTN_KV_INT8)
+        if (s.source != kOwnRows) {
+          bool any = false;
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            sc[r >> 2][r & 3] *= tile.kf[r >> 2][r & 3];
+            float f = value_factor<BF16>(tile.vf[r >> 2][r & 3]);
+            if (!(f < INFINITY)) {
+              any = true;
+              f = 1.f;
+            }
+            factor[r >> 2][r & 3] = f;
+          }
+          found |= __any(any);
+        }
       found |= tile.store(lds, s, lane, part);
       if (t + 1 < tiles) {
         now = ahead;
@@ -760,7 +873,8 @@ __device__ inline void flat_item(const SharedParams& p, const SharedItem& it, in
         const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[r >> 2][r & 3], p.scale_log2, -ref));
         const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[r >> 2][(r & 3) + 1], p.scale_log2, -ref));
         l += p0 + p1;
-        pf[r >> 1] = narrow2<BF16>(p0, p1);
+        pf[r >> 1] = FORMAT == QATTN_KV_INT8 ? narrow2<BF16>(p0 * factor[r >> 2][r & 3], p1 * factor[r >> 2][(r & 3) + 1])
+                                             : narrow2<BF16>(p0, p1);
       }
 #pragma unroll
       for (int db = 0; db < kBlocks; ++db) {
@@ -828,13 +942,14 @@ __global__ __launch_bounds__(kSharedThreads, 2) void shared_attn_kernel(SharedPa
   static_assert(kTallLds >= kFlatLds && kTallLds >= 4 * 32 * DIM * 4, "O of four wavefronts");
   __shared__ __attribute__((aligned(1024))) char lds[kTallLds];
   __shared__ __attribute__((aligned(16))) float2 stats[128];
+  __shared__ __attribute__((aligned(16))) float factors[FORMAT == QATTN_KV_INT8 ? 4 * kTallKeys : 1];  // of two tiles' keys
   __shared__ uint32_t dropped;
   const int kvh = (int)(blockIdx.x % (uint32_t)p.kv_heads);
   const int unit = (int)(blockIdx.x / (uint32_t)p.kv_heads);
   const int index = !p.flat_first ? unit : unit < p.n_flat ? p.n_blocks + unit : unit - p.n_flat;
   const SharedItem it = item_at(p, index);
   if (index < p.n_blocks)
-    tall_item<BF16, FORMAT, DIM>(p, it, index, kvh, lds, stats, &dropped);
+    tall_item<BF16, FORMAT, DIM>(p, it, index, kvh, lds, factors, stats, &dropped);
   else
     flat_item<BF16, FORMAT, DIM>(p, it, index - p.n_blocks, kvh, lds, stats);
 }

@@ -1,10 +1,10 @@
 """Attention behind one shared prefix (qattn_shared_run_*) against its definition in 64 bits, on the GPU.
 
 The bound on a row's error, from the roundings the kernel makes (u: half a step of the 16-bit type, D the
-head dim, n the keys): a score is off by at most d = scale sum |q k| (u_k + (D + 2) 2^-24), u_k being u for
-int8 codes (whose product with the scale is rounded to the type) and 0 otherwise; a weight then by a
-factor within exp(2 d), plus its own rounding u, plus f32's exp2 and sums (2^-20 + n 2^-24); fp16 weights
-below the normal range by at most 2^-25 of the largest; V by u if int8; the result by u."""
+head dim, n the keys): a score is off by at most d = scale sum |q k| (D + 2) 2^-24; a weight then by a factor
+within exp(2 d), plus its own rounding u (an int8 key's weight times its scale's factor, in f32, is rounded
+once), plus f32's exp2 and sums (2^-20 + n 2^-24); fp16 weights below the normal range by at most 2^-25 of the
+largest; the result by u.  Codes are exact."""
 import ctypes
 
 import numpy as np
@@ -19,14 +19,13 @@ GARBAGE = 0x7E11  # a NaN in fp16, a large number in bf16
 def error_bound(q, keys, vals, keep, scale, bf16, form, out):
     """Per (head, dim) of one query: q [group, dim], keys / vals [n, dim] of one KV head."""
     u, n = (2.0 ** -8 if bf16 else 2.0 ** -11), int(keep.sum())
-    rounded = u if form == "int8" else 0.0
     k, v = keys[keep], np.abs(vals[keep])
     s = q @ k.T * scale
-    d = (np.abs(q) @ np.abs(k).T * scale).max(-1, keepdims=True) * (rounded + (q.shape[1] + 2) * 2.0 ** -24)
+    d = (np.abs(q) @ np.abs(k).T * scale).max(-1, keepdims=True) * (q.shape[1] + 2) * 2.0 ** -24
     p = np.exp(s - s.max(-1, keepdims=True))
     p /= p.sum(-1, keepdims=True)
     small = 0.0 if bf16 else n * 2.0 ** -25
-    size = p @ v * (np.expm1(2 * d) + u + rounded + 2.0 ** -20 + n * 2.0 ** -24) + small * v.max(0)
+    size = p @ v * (np.expm1(2 * d) + u + 2.0 ** -20 + n * 2.0 ** -24) + small * v.max(0)
     return size + ref.half_step(np.abs(out) + size, bf16)
 
 
