@@ -8,8 +8,9 @@
 // up to kMostFlatRows rows (beyond, an item for every 16 rows reads it too often: with 512 rows, 2,048 keys
 // take as long as by blocks, 24.5 us, and 8,192 keys 60 against 45).
 //
-// Cuts.  Items are cut along their keys where that shortens the launch.  The planner compares, for each of
-// these ways and a range of chunk sizes, the time at which the last of the GPU's slots ends, by a cost model.
+// Cuts.  Items are cut along their keys where that shortens the launch: into equal chunks of a range of sizes, or
+// one after another wherever a slot's share of the work ends.  The planner compares, for each of these ways,
+// the time at which the last of the GPU's slots ends, by a cost model.
 #include <algorithm>
 #include <cmath>
 #include <cstddef>
@@ -28,7 +29,7 @@ namespace {
 constexpr double kBlockItem = 5.9, kTallTile = 4.0, kSplitTile = 2.4, kFlatItem = 3.2, kItemBytesPerUs = 45e3;
 constexpr double kFlatRound = 0.3, kFlatInt8 = 1.1, kFlatMasked = 0.4, kDim64 = 0.8;
 constexpr double kPartial = 0.5, kMergeLaunch = 2.8, kBytesPerUs = 5e6;
-constexpr int kMostSimulated = 16384, kMostFlatRows = 512;
+constexpr int kMostSimulated = 16384, kMostInTurn = 1024, kMostFlatRows = 512;
 
 struct Sequence {
   int32_t first, queries, keys;  // first query; own keys
@@ -40,7 +41,9 @@ struct Draft {
   std::vector<SharedSeg> segs;
   int masked = 0;       // tiles that not every row sees whole
   bool merged = false;  // its rows have partial results elsewhere too
-  int chunks = 1, first_part = 0;
+  std::vector<int> cuts;  // its chunks: 0, .., units()
+  int first_part = 0;
+  int chunks() const { return (int)cuts.size() - 1; }
   int units() const { return item.kind == kFlat ? (item.tiles + kFlatWaves - 1) / kFlatWaves : item.tiles; }
 };
 
@@ -279,24 +282,51 @@ class Planner {
   }
   double cost(const Draft& b, int units) const { return fixed(b) + unit(b) * units; }
 
-  int chunks_for(const Draft& b, double target) const {
-    const int n = b.units(), fit = std::max(1, (int)std::floor((target - fixed(b)) / unit(b)));
-    return (n + fit - 1) / fit;
+  // Every draft in equal chunks that take `target` at most, if they can; false if they are too many.
+  bool cut_equally(std::vector<Draft>* drafts, double target) const {
+    int64_t all = 0;
+    for (Draft& b : *drafts) {
+      const int64_t n = b.units(), fit = std::max(1, (int)std::floor((target - fixed(b)) / unit(b)));
+      const int64_t chunks = (n + fit - 1) / fit;
+      if ((all += chunks) > kMostSimulated) return false;
+      b.cuts.resize(chunks + 1);
+      for (int64_t i = 0; i <= chunks; ++i) b.cuts[i] = (int)(n * i / chunks);
+    }
+    return true;
+  }
+  // The drafts one after another, cut wherever a slot has had `target`; returns the slots it takes.
+  int cut_in_turn(std::vector<Draft>* drafts, double target) const {
+    int used = 1;
+    double room = target;
+    for (Draft& b : *drafts) {
+      const int n = b.units();
+      b.cuts.assign(1, 0);
+      while (b.cuts.back() < n) {
+        const int fit = (int)std::floor((room - fixed(b)) / unit(b));
+        if (fit < std::min(2, n - b.cuts.back()) && room < target) {
+          ++used;
+          room = target;
+          continue;
+        }
+        const int take = std::min(std::max(1, fit), n - b.cuts.back());
+        b.cuts.push_back(b.cuts.back() + take);
+        room -= cost(b, take) + kPartial;
+      }
+    }
+    return used;
   }
 
   // The time at which the last slot ends, longest item first, or the flat items' bytes have been read.
-  double span(const std::vector<Draft>& drafts, double target) const {
+  double span(const std::vector<Draft>& drafts) const {
     std::vector<double> costs;
     double partial_rows = 0, flat_keys = 0;
     bool split = false;
     for (const Draft& b : drafts) {
-      const int c = chunks_for(b, target), units = b.units();
-      const bool part = c > 1 || b.merged;
-      if (part) partial_rows += (double)c * b.item.rows;
+      const bool part = b.chunks() > 1 || b.merged;
+      if (part) partial_rows += (double)b.chunks() * b.item.rows;
       split |= part;
       if (b.item.kind == kFlat) flat_keys += (double)b.item.tiles * kFlatKeys;
-      if ((int64_t)costs.size() + c > kMostSimulated) return 1e30;
-      for (int64_t i = 0; i < c; ++i) costs.push_back((part ? kPartial : 0) + cost(b, (int)(units * (i + 1) / c - units * i / c)));
+      for (int i = 0; i < b.chunks(); ++i) costs.push_back((part ? kPartial : 0) + cost(b, b.cuts[i + 1] - b.cuts[i]));
     }
     std::sort(costs.begin(), costs.end(), std::greater<double>());
     std::priority_queue<double, std::vector<double>, std::greater<double>> ends;
@@ -316,37 +346,49 @@ class Planner {
 
   // Chooses every draft's chunks; returns the launch's time.
   double cut(std::vector<Draft>* drafts) const {
-    double longest = 0;
-    for (const Draft& b : *drafts) longest = std::max(longest, cost(b, b.units()));
-    double best_span = span(*drafts, longest), best = longest;
-    for (double target = longest * 0.85; target > kFlatItem; target *= target > longest / 2 ? 0.85 : 0.7) {
-      const double s = span(*drafts, target);
-      if (s < best_span * 0.98) {
-        best_span = s;
-        best = target;
-      }
-    }
-    double total = 0;
-    for (Draft& b : *drafts) {
-      b.chunks = best > 0 ? chunks_for(b, best) : 1;
+    double longest = 0, total = 0;
+    for (const Draft& b : *drafts) {
+      longest = std::max(longest, cost(b, b.units()));
       total += cost(b, b.units());
     }
-    return best_span < 1e30 ? best_span : total / slots_;  // too many to simulate: the slots are full
+    if (!cut_equally(drafts, longest)) {
+      for (Draft& b : *drafts) b.cuts = {0, b.units()};
+      return total / slots_;  // the slots are full
+    }
+    double best = span(*drafts);
+    std::vector<Draft> tried = *drafts;
+    const auto keep_better = [&]() {
+      const double s = span(tried);
+      if (s >= best * 0.98) return;
+      best = s;
+      for (size_t i = 0; i < tried.size(); ++i) (*drafts)[i].cuts = tried[i].cuts;
+    };
+    const double step = drafts->size() <= 256 ? 0.93 : 0.85;
+    for (double target = longest * step; target > kFlatItem; target *= target > longest / 2 ? step : 0.8) {
+      if (!cut_equally(&tried, target)) break;
+      keep_better();
+    }
+    if (tried.size() <= kMostInTurn) {
+      double target = std::max(total / slots_, kFlatItem + 1);
+      while (target < longest && cut_in_turn(&tried, target) > slots_) target *= 1.02;
+      if (target < longest) keep_better();
+    }
+    return best;
   }
 
   void emit() {
     std::vector<std::pair<double, SharedItem>> items;
     for (Draft& b : drafts_) {
       const int rows = b.item.rows;
-      const bool part = b.chunks > 1 || b.merged;
+      const bool part = b.chunks() > 1 || b.merged;
       if (part) {
         b.first_part = (int32_t)plan_->partial_rows;
-        plan_->partial_rows += (int64_t)b.chunks * rows;
+        plan_->partial_rows += (int64_t)b.chunks() * rows;
       }
-      const int round = b.item.kind == kFlat ? kFlatWaves : 1, units = b.units();
-      for (int c = 0; c < b.chunks; ++c) {
-        int begin = std::min(b.item.tiles, (int)((int64_t)units * c / b.chunks) * round);
-        int end = std::min(b.item.tiles, (int)((int64_t)units * (c + 1) / b.chunks) * round);
+      const int round = b.item.kind == kFlat ? kFlatWaves : 1;
+      for (int c = 0; c < b.chunks(); ++c) {
+        int begin = std::min(b.item.tiles, b.cuts[c] * round);
+        int end = std::min(b.item.tiles, b.cuts[c + 1] * round);
         SharedItem it = b.item;
         it.seg_begin = (int32_t)plan_->segs.size();
         it.tiles = end - begin;
@@ -423,12 +465,12 @@ class Planner {
     for (const Draft& b : drafts_)
       for (int32_t r = 0; r < b.item.rows; ++r) {
         const int64_t row = (int64_t)b.item.row0 + r;
-        if (b.chunks == 1 && !b.merged) {
+        if (b.chunks() == 1 && !b.merged) {
           direct[row] = 1;
           continue;
         }
         SharedMerge& m = all[row];
-        m.group[m.group[0].count ? 1 : 0] = {b.first_part + r, b.chunks, b.item.rows};
+        m.group[m.group[0].count ? 1 : 0] = {b.first_part + r, b.chunks(), b.item.rows};
       }
     for (int64_t row = 0; row < rows; ++row)
       if (!direct[row]) {
