@@ -2,7 +2,7 @@
 //
 // A vector is one token's head of K or V, held by head_dim / 16 lanes when it is written, by head_dim / 8
 // when it is read, and a reading thread has two vectors in flight (measured at the sizes below: writes
-// of eight elements to a lane take 13.9, of sixteen 11.5, of two vectors 11.9 us; reads 30.8 with one vector
+// of eight elements to a lane take 13.9, of sixteen 11.5, of two vectors 11.9 us, all before the codes' arithmetic was shortened to 10.1; reads 30.8 with one vector
 // of eight elements, 29.3 with one of sixteen, 27.8 with two of eight).  The largest magnitude is reduced
 // over the lanes by DPP.
 //   e4m3  code = e4m3(x / s), s = 2^(least e with amax <= 448 2^e).  A power of two costs the division no
@@ -10,7 +10,7 @@
 //         lies, so against amax / 448 nothing is lost but up to one binade of the codes below 2^-6.
 //   int8  code = rint(x * (127 / amax)), s = amax / 127, both divisions correctly rounded.
 // Both kernels are bound by memory: a write of codes reads 2 bytes an element and writes 1 + 4 / head_dim, a
-// read the reverse.  8,000 tokens of 8 heads of 128 are written as e4m3 in 11.5 us, 4.3 TB/s; 20,000 are read in
+// read the reverse.  8,000 tokens of 8 heads of 128 are written as e4m3 in 10.1 us, 4.9 TB/s; 20,000 are read in
 // 27.8 us, 4.5 TB/s, where a large copy reaches 5.1.
 #include "shared_ops.h"
 
@@ -67,25 +67,40 @@ __device__ inline int64_t vector_of(const qattn_kv_cache& c, int64_t slot, int h
   return (((slot >> shift) * c.kv_heads + head) << shift) + (slot & (c.page_size - 1));
 }
 
-// A lane's elements of a vector as 8-bit codes, and the vector's scale.
+// A lane's elements of a vector as 8-bit codes, and the vector's scale.  Wavefronts whose vectors have finite
+// elements, none of them all but zero, and no code to avoid take the short way: without it the codes'
+// arithmetic, not memory, sets the time.
 template <bool BF16, int FORMAT, int DIM>
 __device__ inline u32x4 encode(const u32x4 (&x)[2], float* scale_out) {
+#pragma clang fp contract(off)  // a code is the rounded product rounded
   constexpr int kElems = kWriteElems;
-  u32x4 out;
-  float f[kElems], amax = 0.f;
+  constexpr uint32_t kExp = Elem<BF16>::kExponent;
+  typedef uint16_t Pair __attribute__((ext_vector_type(2)));
+  // Magnitudes compare as integers.
+  Pair most2 = {0, 0};
+#pragma unroll
+  for (int e = 0; e < kElems / 2; ++e)
+    most2 = __builtin_elementwise_max(most2, __builtin_bit_cast(Pair, x[e >> 2][e & 3] & 0x7FFF7FFFu));
+  const uint32_t top = max((uint32_t)most2[0], (uint32_t)most2[1]);
+  const bool finite = top < kExp;
+  float f[kElems], amax = widen<BF16, 0>(finite ? top : 0);
 #pragma unroll
   for (int e = 0; e < kElems / 2; ++e) {
     f[2 * e] = widen<BF16, 0>(x[e >> 2][e & 3]);
     f[2 * e + 1] = widen<BF16, 1>(x[e >> 2][e & 3]);
   }
+  if (__any(!finite)) {
+    amax = 0.f;
 #pragma unroll
-  for (int e = 0; e < kElems; ++e) {
-    const float m = fabsf(f[e]);
-    amax = fmaxf(amax, m < __builtin_inff() ? m : 0.f);  // a NaN compares false too
+    for (int e = 0; e < kElems; ++e) {
+      const float m = fabsf(f[e]);
+      amax = fmaxf(amax, m < __builtin_inff() ? m : 0.f);  // a NaN compares false too
+    }
   }
   amax = lanes_max<DIM / kElems>(amax);
   const bool zeros = amax < kLeastAmax;
   float scale = 1.f, inv = 0.f;
+  u32x4 out;
   if constexpr (FORMAT == QATTN_KV_E4M3) {
     // amax = 1.m 2^e <= 1.75 2^(8 + s)
     const uint32_t bits = __float_as_uint(amax);
@@ -95,17 +110,22 @@ __device__ inline u32x4 encode(const u32x4 (&x)[2], float* scale_out) {
       inv = __uint_as_float((uint32_t)(127 - s) << 23);
     }
     // 256 * 2^8 and 256 * 2^120 are past the largest fp16 and bf16 value: there 240 is the largest code.
-    const float most = s >= (BF16 ? 120 : 8) ? 240.f : kE4m3Max;
-    float y[kElems];
+    const bool short_codes = s >= (BF16 ? 120 : 8);
+    if (__any(!finite || zeros || short_codes)) {
+      const float most = short_codes ? 240.f : kE4m3Max;
 #pragma unroll
-    for (int e = 0; e < kElems; ++e) {
-      const float v = zeros ? (f[e] - f[e] == 0.f ? 0.f : f[e]) : f[e] * inv;  // infinities and NaN stay
-      y[e] = v != v ? v : fminf(fmaxf(v, -most), most);
+      for (int e = 0; e < kElems; ++e) {
+        const float v = zeros ? (f[e] - f[e] == 0.f ? 0.f : f[e]) : f[e] * inv;  // infinities and NaN stay
+        f[e] = v != v ? v : fminf(fmaxf(v, -most), most);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) f[e] *= inv;
     }
 #pragma unroll
     for (int e = 0; e < kElems / 4; ++e) {
-      int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * e], y[4 * e + 1], 0, false);
-      w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * e + 2], y[4 * e + 3], w, true);
+      int w = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * e], f[4 * e + 1], 0, false);
+      w = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * e + 2], f[4 * e + 3], w, true);
       out[e] = (uint32_t)w;
     }
   } else {
@@ -113,17 +133,24 @@ __device__ inline u32x4 encode(const u32x4 (&x)[2], float* scale_out) {
       scale = amax / 127.f;
       inv = 127.f / amax;
     }
+    if (__any(!finite || zeros)) {
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) {
+        const float v = zeros && f[e] - f[e] == 0.f ? 0.f : f[e] * (zeros ? 1.f : inv);
+        f[e] = v != v ? 0.f : fminf(fmaxf(v, -127.f), 127.f);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) f[e] *= inv;
+    }
+    // The low byte of 3 * 2^22 + f is f rounded to an integer.
 #pragma unroll
     for (int e = 0; e < kElems / 4; ++e) {
-      uint32_t w = 0;
+      uint32_t w[4];
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const float x1 = f[4 * e + b];
-        float v = zeros && x1 - x1 == 0.f ? 0.f : x1 * (zeros ? 1.f : inv);
-        v = v != v ? 0.f : fminf(fmaxf(rintf(v), -127.f), 127.f);
-        w |= ((uint32_t)(int)v & 255u) << (8 * b);
-      }
-      out[e] = w;
+      for (int b = 0; b < 4; ++b) w[b] = __float_as_uint(f[4 * e + b] + 12582912.f);
+      const uint32_t low = __builtin_amdgcn_perm(w[1], w[0], 0x0C0C0400u), high = __builtin_amdgcn_perm(w[3], w[2], 0x04000C0Cu);
+      out[e] = low | high;
     }
   }
   *scale_out = scale;
