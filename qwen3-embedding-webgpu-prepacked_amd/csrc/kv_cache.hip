@@ -1,10 +1,10 @@
 // kv_cache.hip -- the paged K/V cache: rows quantised as they are written, slots read back into rows.
 //
 // A vector is one token's head of K or V, held by head_dim / 16 lanes when it is written, by head_dim / 8
-// when it is read, and a reading thread has two vectors in flight (measured at the sizes below: writes
-// of eight elements to a lane take 13.9, of sixteen 11.5, of two vectors 11.9 us, all before the codes' arithmetic was shortened to 10.1; reads 30.8 with one vector
-// of eight elements, 29.3 with one of sixteen, 27.8 with two of eight).  The largest magnitude is reduced
-// over the lanes by DPP.
+// when it is read, and a reading thread has two vectors in flight.  At the sizes below, writes of eight
+// elements to a lane took 13.9 us, of sixteen 11.5, of sixteen of two vectors 11.9 (and 10.1 since the codes'
+// arithmetic got shorter); reads of eight elements 30.8, of sixteen 29.3, of eight of two vectors 27.8.  The
+// largest magnitude is reduced over the lanes by DPP.
 //   e4m3  code = e4m3(x / s), s = 2^(least e with amax <= 448 2^e).  A power of two costs the division no
 //         rounding, and a floating code's relative error does not depend on where in its range a value
 //         lies, so against amax / 448 nothing is lost but up to one binade of the codes below 2^-6.
