@@ -282,13 +282,13 @@ class Planner {
   }
   double cost(const Draft& b, int units) const { return fixed(b) + unit(b) * units; }
 
-  // Every draft in equal chunks that take `target` at most, if they can; false if they are too many.
-  bool cut_equally(std::vector<Draft>* drafts, double target) const {
+  // Every draft in equal chunks that take `target` at most, if they can; false if they are more than `most`.
+  bool cut_equally(std::vector<Draft>* drafts, double target, int64_t most) const {
     int64_t all = 0;
     for (Draft& b : *drafts) {
       const int64_t n = b.units(), fit = std::max(1, (int)std::floor((target - fixed(b)) / unit(b)));
       const int64_t chunks = (n + fit - 1) / fit;
-      if ((all += chunks) > kMostSimulated) return false;
+      if ((all += chunks) > most) return false;
       b.cuts.resize(chunks + 1);
       for (int64_t i = 0; i <= chunks; ++i) b.cuts[i] = (int)(n * i / chunks);
     }
@@ -351,28 +351,35 @@ class Planner {
       longest = std::max(longest, cost(b, b.units()));
       total += cost(b, b.units());
     }
-    if (!cut_equally(drafts, longest)) {
+    if (!cut_equally(drafts, longest, kMostSimulated)) {
       for (Draft& b : *drafts) b.cuts = {0, b.units()};
       return total / slots_;  // the slots are full
     }
     double best = span(*drafts);
-    std::vector<Draft> tried = *drafts;
+    std::vector<std::vector<int>> best_cuts(drafts->size());
+    const auto keep = [&]() {
+      for (size_t i = 0; i < best_cuts.size(); ++i) best_cuts[i] = (*drafts)[i].cuts;
+    };
     const auto keep_better = [&]() {
-      const double s = span(tried);
+      const double s = span(*drafts);
       if (s >= best * 0.98) return;
       best = s;
-      for (size_t i = 0; i < tried.size(); ++i) (*drafts)[i].cuts = tried[i].cuts;
+      keep();
     };
+    keep();
+    // More chunks than a few to a slot only add to the merge.
+    const int64_t most = std::min<int64_t>(kMostSimulated, std::max<int64_t>(2 * drafts->size(), 4 * slots_));
     const double step = drafts->size() <= 256 ? 0.93 : 0.85;
     for (double target = longest * step; target > kFlatItem; target *= target > longest / 2 ? step : 0.8) {
-      if (!cut_equally(&tried, target)) break;
+      if (!cut_equally(drafts, target, most)) break;
       keep_better();
     }
-    if (tried.size() <= kMostInTurn) {
+    if (drafts->size() <= kMostInTurn) {
       double target = std::max(total / slots_, kFlatItem + 1);
-      while (target < longest && cut_in_turn(&tried, target) > slots_) target *= 1.02;
+      while (target < longest && cut_in_turn(drafts, target) > slots_) target *= 1.02;
       if (target < longest) keep_better();
     }
+    for (size_t i = 0; i < best_cuts.size(); ++i) (*drafts)[i].cuts.swap(best_cuts[i]);
     return best;
   }
 
