@@ -150,6 +150,8 @@ int qattn_rope(qattn_ctx* ctx, const qattn_rope_desc* d, qattn_stream_t stream) 
   a.magnitude = (float)(d->magnitude != 0.0 ? d->magnitude
                         : d->scaling == QATTN_ROPE_YARN ? 0.1 * std::log(d->factor) + 1.0 : 1.0);
   rope_turns(*d, a.turns);
+  for (int32_t i = 0; i < a.pairs; ++i)
+    if (!std::isfinite(a.turns[i])) return fail(ctx, QATTN_EINVAL, "theta/factor: pair %d turns past f64's range", i);
   const bool interleaved = d->layout == QATTN_ROPE_INTERLEAVED;
   const bool wide = wide_block(d->q) && (!d->k.heads || wide_block(d->k)) && d->head_dim % 8 == 0 &&
                     d->rotary_dim % (interleaved ? 8 : 16) == 0;

@@ -1533,12 +1533,16 @@ napi_value KvRows(napi_env env, napi_callback_info info, bool write) {
 napi_value KvWrite(napi_env env, napi_callback_info info) { return KvRows(env, info, true); }
 napi_value KvRead(napi_env env, napi_callback_info info) { return KvRows(env, info, false); }
 
+// What a batch asks of the tensors.
+struct BatchRows {
+  int64_t tokens = 0, own = 0;
+  bool paged = false;
+};
 // The batch of a shared run: host arrays, copied by the library.
 struct SharedBatch {
   std::vector<int32_t> prefix_pages, cu, own, own_pages;
   int32_t prefix_len = 0;
-  int64_t own_rows = 0;
-  bool paged = false;
+  BatchRows rows;
 };
 bool read_batch(napi_env env, napi_value obj, int32_t page_size, SharedBatch* b) {
   napi_value v;
@@ -1554,8 +1558,8 @@ bool read_batch(napi_env env, napi_value obj, int32_t page_size, SharedBatch* b)
     napi_throw_type_error(env, nullptr, "prefixPages must be an Int32Array");
     return false;
   }
-  b->paged = prop(env, obj, "ownPages", &v);
-  if (b->paged && !get_i32_array(env, v, &b->own_pages)) {
+  b->rows.paged = prop(env, obj, "ownPages", &v);
+  if (b->rows.paged && !get_i32_array(env, v, &b->own_pages)) {
     napi_throw_type_error(env, nullptr, "ownPages must be an Int32Array");
     return false;
   }
@@ -1565,37 +1569,40 @@ bool read_batch(napi_env env, napi_value obj, int32_t page_size, SharedBatch* b)
   int64_t own = 0;
   for (int32_t x : b->own) {
     own += pages(x);
-    b->own_rows += std::max(x, 0);
+    b->rows.own += std::max(x, 0);
   }
-  if ((int64_t)b->prefix_pages.size() < pages(b->prefix_len) || (b->paged && (int64_t)b->own_pages.size() < own)) {
+  b->rows.tokens = b->cu.back();
+  if ((int64_t)b->prefix_pages.size() < pages(b->prefix_len) || (b->rows.paged && (int64_t)b->own_pages.size() < own)) {
     napi_throw_range_error(env, nullptr, "prefixPages/ownPages: fewer pages than the lengths need");
     return false;
   }
   return true;
 }
 
-// A run holds a reference on each buffer bound to it, and the tensors that its batches have to fit.
+// A run holds a reference on each buffer bound to it, the tensors that its batches have to fit, and the
+// installed batch's rows, which tensors bound later have to hold.
 struct SharedRun {
   Ctx* owner = nullptr;
   qattn_shared_run* run = nullptr;
   qattn_shared_desc desc{};  // geometry and strides
   Tensor q, o, k, v;
+  BatchRows rows;
   std::vector<napi_ref> bound_refs;
   std::vector<const Buf*> bound;
 };
-bool batch_fits(napi_env env, const SharedRun& r, const SharedBatch& b) {
+bool batch_fits(napi_env env, const SharedRun& r, const BatchRows& b) {
   const qattn_shared_desc& d = r.desc;
   const int64_t width = (int64_t)d.q_heads * d.cache.head_dim, kv_width = (int64_t)d.cache.kv_heads * d.cache.head_dim;
-  if (!r.q.holds(b.cu.back(), d.q_row_stride, width, 2)) return past_buffer(env, "q");
-  if (!r.o.holds(b.cu.back(), d.o_row_stride, width, 2)) return past_buffer(env, "o");
+  if (!r.q.holds(b.tokens, d.q_row_stride, width, 2)) return past_buffer(env, "q");
+  if (!r.o.holds(b.tokens, d.o_row_stride, width, 2)) return past_buffer(env, "o");
   if (b.paged) return true;
   if (!r.k.buf || !r.v.buf) {
-    if (b.own_rows == 0) return true;
+    if (b.own == 0) return true;
     napi_throw_type_error(env, nullptr, "own keys need ownPages, or k and v rows");
     return false;
   }
-  if (!r.k.holds(b.own_rows, d.k_row_stride, kv_width, 2)) return past_buffer(env, "k");
-  if (!r.v.holds(b.own_rows, d.v_row_stride, kv_width, 2)) return past_buffer(env, "v");
+  if (!r.k.holds(b.own, d.k_row_stride, kv_width, 2)) return past_buffer(env, "k");
+  if (!r.v.holds(b.own, d.v_row_stride, kv_width, 2)) return past_buffer(env, "v");
   return true;
 }
 bool shared_tensors(napi_env env, napi_value obj, const Ctx* c, SharedRun* r, std::vector<Tensor>* all) {
@@ -1677,7 +1684,7 @@ napi_value CreateSharedRun(napi_env env, napi_callback_info info) {
   d.window = n.i32("window", 432);
   d.scale = n.real("scale", 0);
   SharedBatch b;
-  if (!n.ok || !read_batch(env, argv[1], d.cache.page_size, &b) || !batch_fits(env, made, b)) return nullptr;
+  if (!n.ok || !read_batch(env, argv[1], d.cache.page_size, &b) || !batch_fits(env, made, b.rows)) return nullptr;
   d.q = made.q.ptr();
   d.o = made.o.ptr();
   d.k = made.k.ptr();
@@ -1688,11 +1695,12 @@ napi_value CreateSharedRun(napi_env env, napi_callback_info info) {
   d.nseq = (int32_t)b.own.size();
   d.own_len = b.own.data();
   static const int32_t no_pages[1] = {0};
-  d.own_pages = !b.paged ? nullptr : b.own_pages.empty() ? no_pages : b.own_pages.data();
+  d.own_pages = !b.rows.paged ? nullptr : b.own_pages.empty() ? no_pages : b.own_pages.data();
   if (!d.prefix_pages) d.prefix_pages = no_pages;
   int rc = qattn_shared_run_create(c->ctx, &d, &made.run);
   if (rc) return throw_qattn(env, rc, c->ctx);
   made.owner = c;
+  made.rows = b.rows;
   auto* r = new SharedRun(made);
   c->shared_runs.insert(r);
   ++c->refs;
@@ -1709,29 +1717,27 @@ napi_value UpdateSharedRun(napi_env env, napi_callback_info info) {
   SharedRun* r = live_shared_run(env, argv[0]);
   if (!r) return nullptr;
   SharedBatch b;
-  if (!read_batch(env, argv[1], r->desc.cache.page_size, &b) || !batch_fits(env, *r, b)) return nullptr;
+  if (!read_batch(env, argv[1], r->desc.cache.page_size, &b) || !batch_fits(env, *r, b.rows)) return nullptr;
   static const int32_t no_pages[1] = {0};
   int rc = qattn_shared_run_update(r->run, b.prefix_pages.empty() ? no_pages : b.prefix_pages.data(), b.prefix_len, b.cu.data(),
                                    (int32_t)b.own.size(), b.own.data(),
-                                   !b.paged ? nullptr : b.own_pages.empty() ? no_pages : b.own_pages.data());
+                                   !b.rows.paged ? nullptr : b.own_pages.empty() ? no_pages : b.own_pages.data());
   if (rc) return throw_qattn(env, rc, r->owner->ctx);
+  r->rows = b.rows;
   return undefined(env);
 }
 
-// rebindSharedRun(run, {q, o, cache, k, v}, batch): other tensors of the same strides, a cache of the same
-// geometry (qattn_shared_run_rebind); batch: the one that the run holds, whose rows the tensors have to fit
+// rebindSharedRun(run, {q, o, cache, k, v}): other tensors of the same strides, a cache of the same geometry
+// (qattn_shared_run_rebind)
 napi_value RebindSharedRun(napi_env env, napi_callback_info info) {
-  napi_value argv[3];
-  if (!args_of(env, info, 3, argv)) return nullptr;
+  napi_value argv[2];
+  if (!args_of(env, info, 2, argv)) return nullptr;
   SharedRun* r = live_shared_run(env, argv[0]);
   if (!r) return nullptr;
   SharedRun next;
   std::vector<Tensor> all;
   next.desc = r->desc;
-  SharedBatch b;
-  if (!shared_tensors(env, argv[1], r->owner, &next, &all) || !read_batch(env, argv[2], r->desc.cache.page_size, &b) ||
-      !batch_fits(env, next, b))
-    return nullptr;
+  if (!shared_tensors(env, argv[1], r->owner, &next, &all) || !batch_fits(env, next, r->rows)) return nullptr;
   int rc = qattn_shared_run_rebind(r->run, next.q.ptr(), next.o.ptr(), &next.desc.cache, next.k.ptr(), next.v.ptr());
   if (rc) return throw_qattn(env, rc, r->owner->ctx);
   r->q = next.q;

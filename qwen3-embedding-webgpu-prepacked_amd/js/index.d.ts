@@ -200,7 +200,7 @@ export interface SharedOptions extends SharedTensors {
   scale?: number;
 }
 export interface SharedRun {
-  handle: unknown; batch: SharedBatch;
+  handle: unknown;
   info: { tokens: number; keys: number; pairs: number; flops: number; items: number; mergedRows: number; partialRows: number };
 }
 export class SharedPrefixAttention {

@@ -218,13 +218,12 @@ class SharedPrefixAttention {
     });
     const addon = this.context.addon;
     const handle = addon.createSharedRun(this.context.handle, desc);
-    return { handle, batch, info: addon.sharedRunInfo(handle) };
+    return { handle, info: addon.sharedRunInfo(handle) };
   }
 
   // The next batch (a step later): new lengths and pages for the same tensors.
   updateRun(run, batch) {
     this.context.addon.updateSharedRun(run.handle, batch);
-    run.batch = batch;
     run.info = this.context.addon.sharedRunInfo(run.handle);
   }
 
@@ -232,7 +231,7 @@ class SharedPrefixAttention {
   rebindRun(run, q, output, cache, options = {}) {
     this.context.addon.rebindSharedRun(run.handle, Object.assign({}, options, {
       q: q.handle, o: output.handle, cache: cache.desc, k: handleOf(options.k), v: handleOf(options.v),
-    }), run.batch);
+    }));
   }
 
   encode(run) { this.context.addon.encodeSharedRun(run.handle); }

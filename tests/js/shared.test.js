@@ -104,6 +104,12 @@ test('shared attention: batches and tensors are held to the buffers', () => {
   attention.rebindRun(run, q, o, other, { k: rows, v: rows });
   attention.encode(run);
   assert.throws(() => attention.rebindRun(run, small, o, other, { k: rows, v: rows }), TOO_FAR);
+  // the run remembers its batch, whatever becomes of the arrays
+  const cu = Int32Array.from(batch.cuSeqlens);
+  attention.updateRun(run, Object.assign({}, batch, { cuSeqlens: cu }));
+  cu.fill(0);
+  assert.throws(() => attention.rebindRun(run, small, o, other, { k: rows, v: rows }), TOO_FAR);
+  assert.throws(() => attention.rebindRun(run, q, o, other, { k: small, v: rows }), TOO_FAR);
   assert.throws(() => attention.rebindRun(run, q, o, wider, { k: rows, v: rows }), /qattn error -1/);
   // the cache of before the rebinding may go, the bound one may not
   cache.destroy();

@@ -410,7 +410,7 @@ def test_prefix_kept_once_equals_whole_prompts(ctx, qattn, oracle, form, bound):
     bw, T = up(whole), len(whole)
     bq, bk, bo = ctx.alloc(T * 4096), ctx.alloc(T * 2048), ctx.alloc(T * 4096)
     ctx.qk_norm_rope_qkv(bw.ptr, bq.ptr, bk.ptr, cu)
-    ctx.prefill(qattn.make_desc(bq.ptr, bk.ptr, bw.ptr, bo.ptr, cu, 0, v_row_stride=4096, v_offset=3072))
+    ctx.prefill(qattn.make_desc(bq.ptr, bk.ptr, bw.ptr, bo.ptr, cu, 0, v_row_stride=4096, v_offset=2048 + 1024))
     want = bo.read(np.uint16, (T, 2048)).view(np.float16).astype(np.float64)
     want = np.concatenate([want[a + P:b] for a, b in zip(cu[:-1], cu[1:])])
     # the instruction once, at positions 0 .. P - 1
@@ -427,7 +427,7 @@ def test_prefix_kept_once_equals_whole_prompts(ctx, qattn, oracle, form, bound):
     bi = up(instruction)
     iq, ik = ctx.alloc(P * 4096), ctx.alloc(P * 2048)
     ctx.qk_norm_rope_qkv(bi.ptr, iq.ptr, ik.ptr, np.array([0, P], np.int32))
-    ctx.kv_write(cache, ik.ptr, bi.ptr + 2 * 3072, slots.ptr, P, v_row_stride=4096)
+    ctx.kv_write(cache, ik.ptr, bi.ptr + 2 * (2048 + 1024), slots.ptr, P, v_row_stride=4096)
     # the requests: normalised and rotated to positions that restart, then P further: rotations add
     br = up(own)
     rq, rk, ro = ctx.alloc(n * 4096), ctx.alloc(n * 2048), ctx.alloc(n * 4096)
@@ -435,7 +435,7 @@ def test_prefix_kept_once_equals_whole_prompts(ctx, qattn, oracle, form, bound):
     shift = ctx.upload(np.full(n, P, np.int32))
     ctx.rope(qattn.make_rope_desc(shift.ptr, n, (rq.ptr, rq.ptr, 16), (rk.ptr, rk.ptr, 8)))
     run = ctx.shared_run(qattn.make_shared_desc(rq.ptr, ro.ptr, cache, np.concatenate([[0], np.cumsum(lengths)]), lengths,
-                                                prefix_pages=table, prefix_len=P, k=rk.ptr, v=br.ptr + 2 * 3072,
+                                                prefix_pages=table, prefix_len=P, k=rk.ptr, v=br.ptr + 2 * (2048 + 1024),
                                                 v_row_stride=4096))
     run.encode()
     ctx.synchronize()

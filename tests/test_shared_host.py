@@ -39,7 +39,7 @@ def rope_refusals():
     bad = [("", dict(dtype=2)), ("", dict(head_dim=514)), ("", dict(head_dim=64)), ("", dict(rotary_dim=3)),
            ("", dict(rotary_dim=0)), ("", dict(rotary_dim=130)), ("", dict(layout=2)), ("", dict(scaling=3)),
            ("", dict(theta=0.0)), ("", dict(theta=float("nan"))), ("", dict(theta=float("inf"))),
-           ("", dict(magnitude=float("inf"))), ("", dict(scaling=1, factor=0.0)), ("", dict(scaling=2, factor=float("nan"))),
+           ("", dict(theta=5e-324)), ("", dict(scaling=1, factor=1e-320)), ("", dict(magnitude=float("inf"))), ("", dict(scaling=1, factor=0.0)), ("", dict(scaling=2, factor=float("nan"))),
            ("", dict(scaling=2, factor=4.0, beta_slow=64.0)), ("", dict(scaling=2, factor=4.0, original_context=0.0)),
            ("", dict(scaling=2, factor=4.0, theta=1.0)), ("", dict(tokens=-1)), ("", dict(tokens=1 << 24)),
            ("", dict(positions=None)), ("", dict(positions=P + 2)), ("q", dict(heads=0)), ("k", dict(heads=-1)),
