@@ -475,7 +475,7 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
       u32x4 a[kAhead];
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) a[i] = k_frag(i);
-      __builtin_amdgcn_s_setprio(1);  // before the other wavefront's vector work
+      __builtin_amdgcn_s_setprio(1);  // before the other wavefront's vector work: 2 %
 #pragma unroll
       for (int i = 0; i < 2 * kSteps; ++i) {
         __builtin_amdgcn_sched_barrier(0);
