@@ -140,3 +140,27 @@ def test_values_near_the_type_s_least(ctx, qattn, make, bf16, form):
     c = make(ctx, qattn, bf16=bf16, form=form, spread=1e-25 if bf16 else 2.0 ** -18)
     c.run()
     c.free()
+
+
+def test_two_runs_at_once(ctx, qattn):
+    """Runs on two streams, in flight together: each has a workspace of its own."""
+    a, b = steps(ctx, qattn, form="e4m3"), blocks(ctx, qattn, form="int8", bf16=True)
+    with qattn.Context(0) as other:
+        runs = [ctx.shared_run(a.desc()), ctx.shared_run(b.desc())]
+        streams = [ctx.stream, other.stream]
+        for _ in range(20):
+            for run, stream in zip(runs, streams):
+                run.encode(stream)
+        ctx.synchronize()
+        other.synchronize()
+        a.check()
+        b.check()
+        # one run after itself on another stream, with an update between
+        runs[0].update(**a.lists())
+        runs[0].encode(other.stream)
+        other.synchronize()
+        a.check()
+        for run in runs:
+            run.destroy()
+    a.free()
+    b.free()
