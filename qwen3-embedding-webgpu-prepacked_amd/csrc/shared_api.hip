@@ -25,14 +25,14 @@ constexpr int64_t kMaxSharedRows = (int64_t)1 << 22;       // queries * heads of
 constexpr int64_t kMaxSharedStride = (int64_t)1 << 24;     // elements: 16 rows of it within a 32-bit offset
 constexpr int64_t kMaxSharedGroups = ((int64_t)1 << 23) - 1;  // workgroups of a launch: below 2^32 threads
 
-// Geometry, and with needs_pages the tensors, of a cache.
+// The geometry of a cache's vectors, and with needs_pages everything else of it.
 int check_kv_cache(qattn_ctx* ctx, const qattn_kv_cache* c, bool needs_pages) {
   if (!c) return fail(ctx, QATTN_EINVAL, "cache is NULL");
   if (c->dtype != QATTN_DTYPE_F16 && c->dtype != QATTN_DTYPE_BF16) return fail(ctx, QATTN_EINVAL, "unknown dtype %d", c->dtype);
   if (c->head_dim != 64 && c->head_dim != 128) return fail(ctx, QATTN_EINVAL, "head_dim %d: 64 or 128", c->head_dim);
   if (c->kv_heads < 1 || c->kv_heads > kMaxKvHeads) return fail(ctx, QATTN_EINVAL, "kv_heads %d outside [1, %d]", c->kv_heads, kMaxKvHeads);
-  if (c->format < QATTN_KV_16BIT || c->format > QATTN_KV_INT8) return fail(ctx, QATTN_EINVAL, "unknown cache format %d", c->format);
   if (!needs_pages) return QATTN_OK;
+  if (c->format < QATTN_KV_16BIT || c->format > QATTN_KV_INT8) return fail(ctx, QATTN_EINVAL, "unknown cache format %d", c->format);
   if (c->page_size < 16 || c->page_size > 4096 || (c->page_size & (c->page_size - 1)))
     return fail(ctx, QATTN_EINVAL, "page_size %d: a power of two in [16, 4096]", c->page_size);
   if (c->pages < 1 || (int64_t)c->pages * c->page_size * c->kv_heads >= (int64_t)1 << 35)
@@ -190,6 +190,8 @@ int qattn_kv_read(qattn_ctx* ctx, const qattn_kv_cache* cache, const int64_t* sl
 struct qattn_shared_run {
   qattn_ctx* ctx = nullptr;
   qattn_shared_desc desc{};  // without its host arrays
+  bool reads_pages = false, reads_rows = false;  // the installed plan
+  int32_t format = QATTN_KV_16BIT;               // of its pages
   SharedParams params{};
   void* image[2] = {nullptr, nullptr};
   size_t image_bytes[2] = {0, 0};
@@ -224,6 +226,11 @@ int check_shared_tensors(qattn_ctx* ctx, const qattn_shared_desc* d, bool needs_
   return QATTN_OK;
 }
 
+bool own_keys(const qattn_shared_desc& d) {
+  return std::any_of(d.own_len, d.own_len + d.nseq, [](int32_t n) { return n > 0; });
+}
+bool reads_pages(const qattn_shared_desc& d) { return d.prefix_len > 0 || (d.own_pages && own_keys(d)); }
+
 int check_shared(qattn_ctx* ctx, const qattn_shared_desc* d) {
   if (!d) return fail(ctx, QATTN_EINVAL, "desc is NULL");
   int rc = validate_cu(ctx, d->cu_q, d->nseq);
@@ -238,7 +245,7 @@ int check_shared(qattn_ctx* ctx, const qattn_shared_desc* d) {
     own += d->own_len[i];
   }
   if (own >= ((int64_t)1 << 31)) return fail(ctx, QATTN_EINVAL, "too many own keys (%lld)", (long long)own);
-  rc = check_shared_tensors(ctx, d, d->prefix_len > 0 || (d->own_pages && own), !d->own_pages && own);
+  rc = check_shared_tensors(ctx, d, reads_pages(*d), !d->own_pages && own);
   if (rc) return rc;
   if (d->mask != QATTN_MASK_CAUSAL && d->mask != QATTN_MASK_PREFIX_LOCAL) return fail(ctx, QATTN_EINVAL, "unknown mask kind %d", d->mask);
   if (d->mask == QATTN_MASK_PREFIX_LOCAL && (d->prefix < 0 || d->window < 0))
@@ -261,7 +268,20 @@ int check_shared(qattn_ctx* ctx, const qattn_shared_desc* d) {
   return check_pages("own_pages", d->own_pages, n);
 }
 
-// Plans a checked description; refuses what no launch could hold.
+// A checked description as it is planned and launched: where no page is read, the fields of the cache that
+// nothing has looked at may hold anything.
+qattn_shared_desc as_planned(qattn_shared_desc d) {
+  if (!reads_pages(d)) {
+    d.cache.pages = 0;
+    d.cache.page_size = 16;
+    d.cache.format = QATTN_KV_16BIT;
+    d.cache.k = d.cache.v = nullptr;
+    d.cache.k_scale = d.cache.v_scale = nullptr;
+  }
+  return d;
+}
+
+// Plans a checked description (as_planned); refuses what no launch could hold.
 int make_shared_plan(qattn_ctx* ctx, const qattn_shared_desc& d, int compute_units, SharedPlan* plan) {
   plan_shared(d, compute_units, plan);
   const int64_t heads = d.cache.kv_heads;
@@ -309,8 +329,9 @@ int wait_shared(qattn_shared_run* run, int i) {
 }
 
 // Plans `d` into the run's other image and switches to it; on failure the installed plan stays.
-int install_shared_plan(qattn_shared_run* run, const qattn_shared_desc& d) {
+int install_shared_plan(qattn_shared_run* run, const qattn_shared_desc& desc) {
   qattn_ctx* ctx = run->ctx;
+  const qattn_shared_desc d = as_planned(desc);
   SharedPlan plan;
   int rc = make_shared_plan(ctx, d, std::max(1, ctx->cu_count), &plan);
   if (rc) return rc;
@@ -379,14 +400,17 @@ int install_shared_plan(qattn_shared_run* run, const qattn_shared_desc& d) {
   p.most_parts = plan.most_parts;
   p.kv_heads = d.cache.kv_heads;
   p.group = d.q_heads / d.cache.kv_heads;
-  while ((1 << p.page_shift) < d.cache.page_size) ++p.page_shift;
+  p.page_shift = __builtin_ctz(d.cache.page_size);  // a power of two
   p.mask = d.mask;
   p.prefix = d.prefix;
   p.window = std::min(d.window, kMaxPosition);
   p.scale_log2 = (float)((d.scale > 0.0 ? d.scale : 1.0 / std::sqrt((double)d.cache.head_dim)) * 1.4426950408889634);
   run->params = p;
   run->info = plan.info;
-  run->desc = d;
+  run->reads_pages = reads_pages(d);
+  run->reads_rows = !d.own_pages && own_keys(d);
+  run->format = d.cache.format;
+  run->desc = desc;
   run->desc.prefix_pages = run->desc.cu_q = run->desc.own_len = nullptr;
   if (d.own_pages) run->desc.own_pages = reinterpret_cast<const int32_t*>(run);  // only whether there are any
   run->cur = next;
@@ -432,7 +456,7 @@ int qattn_shared_run_encode(qattn_shared_run* run, qattn_stream_t stream) {
   } catch (const std::bad_alloc&) {
     return fail(run->ctx, QATTN_ENOMEM, "out of host memory");
   }
-  HIP_TRY(run->ctx, launch_shared_attn(run->params, run->desc.cache.dtype, run->desc.cache.format, run->desc.cache.head_dim, s));
+  HIP_TRY(run->ctx, launch_shared_attn(run->params, run->desc.cache.dtype, run->format, run->desc.cache.head_dim, s));
   return QATTN_OK;
 }
 
@@ -466,7 +490,7 @@ int qattn_shared_run_rebind(qattn_shared_run* run, const void* q, void* o, const
   d.cache = *cache;
   d.k = k;
   d.v = v;
-  const int rc = check_shared_tensors(run->ctx, &d, run->desc.cache.k != nullptr, run->desc.k != nullptr);
+  const int rc = check_shared_tensors(run->ctx, &d, run->reads_pages, run->reads_rows);
   if (rc) return rc;
   bind_shared(&run->params, d);
   run->desc = d;
@@ -500,7 +524,7 @@ int qattn_shared_plan_describe(const qattn_shared_desc* desc, int32_t* words, in
   if (rc) return rc;
   SharedPlan plan;
   try {
-    rc = make_shared_plan(nullptr, *desc, 256, &plan);
+    rc = make_shared_plan(nullptr, as_planned(*desc), 256, &plan);
   } catch (const std::bad_alloc&) {
     rc = fail(nullptr, QATTN_ENOMEM, "out of host memory for the plan");
   }

@@ -1,0 +1,87 @@
+"""Runs of the attention behind one shared prefix on the CPU: what their host side does with fields that nothing
+reads.  The library runs over a stand-in for the HIP runtime (fake_hip.cc, preloaded into a child process)."""
+import json
+import os
+import shutil
+import subprocess
+import sys
+
+import pytest
+
+from test_host_launches import HERE, ROCM, Launches
+
+Q, O, K, V = 1 << 20, 1 << 30, 1 << 31, 1 << 32  # stand-in device addresses
+LEAST, MOST = -(1 << 31), (1 << 31) - 1
+
+
+def failure(h, call):
+    """The error's message, or None."""
+    try:
+        call()
+    except h.qattn.QattnError as e:
+        return [e.code, str(e)]
+    return None
+
+
+def unread_cache_fields():
+    """[[fields, failure of create, kernels launched, failure of a second batch, of a rebind, of a batch that
+    reads pages]] of runs whose own keys are rows, with no prefix."""
+    h, out = Launches(), []
+    q = h.qattn
+    for fields in (dict(), dict(page_size=-7), dict(page_size=48), dict(page_size=1 << 30), dict(page_size=(1 << 30) + 1),
+                   dict(page_size=MOST), dict(page_size=LEAST), dict(pages=LEAST, page_size=MOST), dict(format=2),
+                   dict(format=3), dict(format=LEAST), dict(format=MOST, page_size=MOST, pages=MOST),
+                   dict(k=3, v=5, k_scale=7, v_scale=9)):
+        cache = q.make_kv_cache(None, None, 0, 0)
+        for name, value in fields.items():
+            setattr(cache, name, value)
+        names, run = [], []
+        h.on = lambda name, *rest: names.append(name)
+        made = failure(h, lambda: run.append(h.ctx.shared_run(q.make_shared_desc(Q, O, cache, [0, 40, 41], [40, 9], k=K, v=V))))
+        row = [str(fields), made]
+        if not made:
+            run[0].encode()
+            row += [names[:], failure(h, lambda: run[0].update([0, 3], [3])),
+                    failure(h, lambda: run[0].rebind(Q + 64, O, cache, K, V)),
+                    failure(h, lambda: run[0].update([0, 3], [3], prefix_pages=[0], prefix_len=1))]
+            run[0].encode()
+            run[0].destroy()
+        out.append(row)
+    return out
+
+
+CASES = {f.__name__: f for f in (unread_cache_fields,)}
+
+
+@pytest.fixture(scope="module")
+def run_child(tmp_path_factory):
+    compiler = shutil.which("g++")
+    if not compiler or not os.path.isdir(os.path.join(ROCM, "include", "hip")):
+        pytest.skip("no g++ or HIP headers")
+    lib = str(tmp_path_factory.mktemp("fake") / "libfake_hip.so")
+    subprocess.run([compiler, "-std=c++17", "-O1", "-shared", "-fPIC", "-w", "-I" + os.path.join(ROCM, "include"), "-o", lib,
+                    os.path.join(HERE, "fake_hip.cc")], check=True)
+
+    def run(case):
+        preload = " ".join(v for v in (os.environ.get("LD_PRELOAD"), lib) if v)
+        out = subprocess.run([sys.executable, os.path.abspath(__file__), case], check=True, capture_output=True, text=True,
+                             env=dict(os.environ, LD_PRELOAD=preload, FAKE_HIP=lib), timeout=60)
+        return json.loads(out.stdout)
+
+    return run
+
+
+def test_cache_fields_that_nothing_reads_may_hold_anything(run_child):
+    """Runs that read no page need the cache's kv_heads, head_dim and dtype only: whatever the other fields hold, the
+    run is planned, launched (by the kernel of 16-bit keys), updated and rebound; a batch that reads pages is
+    refused for them."""
+    seen = run_child("unread_cache_fields")
+    assert len(seen) == 13
+    for fields, made, kernels, updated, rebound, paged in seen:
+        assert made is None and updated is None and rebound is None, (fields, made, updated, rebound)
+        assert kernels and all("shared_" in k for k in kernels) and "ILb0ELi0ELi128E" in kernels[0], (fields, kernels)
+        assert paged is not None and paged[0] == -1, fields
+
+
+if __name__ == "__main__":
+    print(json.dumps(CASES[sys.argv[1]]()))
