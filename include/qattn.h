@@ -428,7 +428,8 @@ typedef struct qattn_shared_desc {
   const void* v;
   int64_t k_row_stride, v_row_stride;
   int32_t mask, prefix, window; /* enum qattn_mask_kind; PREFIX_LOCAL: >= 0, both may be 0 */
-  double scale;             /* of the scores; 0: 1/sqrt(head_dim) */
+  double scale;             /* of the scores, below 1e30; 0: 1/sqrt(head_dim).  One that times log2 e is 0 in
+                             * f32 (up to about 4.8e-46) is refused */
 } qattn_shared_desc;
 /* Tensors 16-byte aligned, strides multiples of 8 elements up to 2^24 and at least the heads' width;
  * page numbers in [0, pages); positions below 2^30; fewer than 2^31 own keys, at most 2^22 sequences and

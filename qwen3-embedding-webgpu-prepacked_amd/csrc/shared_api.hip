@@ -226,6 +226,11 @@ int check_shared_tensors(qattn_ctx* ctx, const qattn_shared_desc* d, bool needs_
   return QATTN_OK;
 }
 
+// Of the scores, for exponentials of 2.  (A masked score is -inf: times 0 it would be NaN.)
+float scale_log2_of(const qattn_shared_desc& d) {
+  return (float)((d.scale > 0.0 ? d.scale : 1.0 / std::sqrt((double)d.cache.head_dim)) * 1.4426950408889634);
+}
+
 bool own_keys(const qattn_shared_desc& d) {
   return std::any_of(d.own_len, d.own_len + d.nseq, [](int32_t n) { return n > 0; });
 }
@@ -250,7 +255,8 @@ int check_shared(qattn_ctx* ctx, const qattn_shared_desc* d) {
   if (d->mask != QATTN_MASK_CAUSAL && d->mask != QATTN_MASK_PREFIX_LOCAL) return fail(ctx, QATTN_EINVAL, "unknown mask kind %d", d->mask);
   if (d->mask == QATTN_MASK_PREFIX_LOCAL && (d->prefix < 0 || d->window < 0))
     return fail(ctx, QATTN_EINVAL, "prefix (%d) and window (%d) must be >= 0", d->prefix, d->window);
-  if (!(d->scale >= 0.0) || !(d->scale < 1e30)) return fail(ctx, QATTN_EINVAL, "scale must be >= 0 and finite");
+  if (!(d->scale >= 0.0) || !(d->scale < 1e30)) return fail(ctx, QATTN_EINVAL, "scale must be >= 0 and below 1e30");
+  if (scale_log2_of(*d) == 0.f) return fail(ctx, QATTN_EINVAL, "scale %g vanishes in f32", d->scale);
   if (d->cu_q[d->nseq] * (int64_t)(d->q_heads / d->cache.kv_heads) > kMaxSharedRows)
     return fail(ctx, QATTN_EINVAL, "%d queries: queries * q_heads / kv_heads up to 2^22", d->cu_q[d->nseq]);
   const int32_t size = d->cache.page_size;
@@ -404,7 +410,7 @@ int install_shared_plan(qattn_shared_run* run, const qattn_shared_desc& desc) {
   p.mask = d.mask;
   p.prefix = d.prefix;
   p.window = std::min(d.window, kMaxPosition);
-  p.scale_log2 = (float)((d.scale > 0.0 ? d.scale : 1.0 / std::sqrt((double)d.cache.head_dim)) * 1.4426950408889634);
+  p.scale_log2 = scale_log2_of(d);
   run->params = p;
   run->info = plan.info;
   run->reads_pages = reads_pages(d);

@@ -1,0 +1,62 @@
+"""Attention behind one shared prefix on the GPU: the edges of scales, infinities and unused slots, against the
+definition in 64 bits.  Bounds: as in test_gpu_shared.py."""
+import numpy as np
+import pytest
+
+import shared_ref as ref
+from test_gpu_shared import error_bound
+from test_gpu_shared_blocks import FORMS, Sampled, blocks, steps, tall
+
+pytestmark = pytest.mark.gpu
+
+
+def outputs(c):
+    """(outputs, queries, the prefix's K and V, the sequences') of the checked heads in 64 bits."""
+    if isinstance(c, Sampled):
+        return c.outputs()
+    T, width = len(c.q), c.heads * c.dim
+    got, q = (ref.from_bits(x[:T, :width], c.bf16).reshape(T, c.heads, c.dim) for x in (c.output(), c.q))
+    return got, q, c.shared, c.mine
+
+
+def launched(ctx, c):
+    r = ctx.shared_run(c.desc())
+    r.encode()
+    ctx.synchronize()
+    r.destroy()
+    return outputs(c)
+
+
+def check(c, seen, scale=None):
+    """Outputs against the definition: infinities and NaN where it has them, else within the bound.  Returns the
+    definition's."""
+    got, q, shared, mine = seen
+    scale = c.dim ** -0.5 if scale is None else scale
+    with np.errstate(invalid="ignore"):
+        want = ref.attend(q, shared, mine, c.queries, *c.args, scale)
+    group, t = c.heads // c.kv, 0
+    for m, (k, v) in zip(c.queries, mine):
+        keys, vals = np.concatenate([shared[0], k]), np.concatenate([shared[1], v])
+        for j in range(m):
+            keep = ref.visible(len(keys) - m + j, len(keys), *c.args)
+            assert keep.any(), t
+            for g in range(keys.shape[1]):
+                h = slice(g * group, (g + 1) * group)
+                x, y = got[t, h], want[t, h]
+                fine = np.isfinite(y)
+                assert np.array_equal(x[~fine], y[~fine], equal_nan=True) and np.isfinite(x[fine]).all(), (t, g, x[~fine], y[~fine])
+                bound = error_bound(q[t, h], keys[:, g], vals[:, g], keep, scale, c.bf16, c.form, np.where(fine, y, 0))
+                assert (np.abs(x[fine] - y[fine]) <= bound[fine]).all(), (t, g)
+            t += 1
+    return want
+
+
+@pytest.mark.parametrize("make", [tall, blocks, steps])
+@pytest.mark.parametrize("dim,bf16,form", FORMS)
+@pytest.mark.parametrize("mask,always,window", [(0, 0, 0), (1, 70, 50)])
+def test_least_scale_averages(ctx, qattn, make, dim, bf16, form, mask, always, window):
+    """The least scale that f32 holds: every seen key weighs the same, a masked one nothing."""
+    c = make(ctx, qattn, dim=dim, bf16=bf16, form=form, mask=mask, always=always, window=window, scale=4.9e-46)
+    print("least scale", make.__name__, dim, bf16, form, mask, flush=True)
+    assert np.isfinite(check(c, launched(ctx, c), 4.9e-46)).all()
+    c.free()
