@@ -591,17 +591,6 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
   }
   if (found) *dropped = 1;
   __syncthreads();
-  if (*dropped && part_begin == 0)
-    each_nonfinite<BF16, FORMAT, DIM>(p, keys, Cursor(p, it), it.tiles, row, at, kTallKeys, [&](auto value, bool seen) {
-#pragma unroll
-      for (int db = 0; db < kBlocks; ++db)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const f4 x = value(32 * db + 8 * g + 4 * hl);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[db][4 * g + e] += nonfinite(x[e], seen);
-        }
-    });
 
   l = half_sum(l);
   if (split) {
@@ -627,6 +616,18 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
       for (int e = 0; e < 4; ++e) o[i >> 2][4 * (i & 3) + e] = f0 * o[i >> 2][4 * (i & 3) + e] + f1 * x[e];
     }
   }
+  // After the join, where a half that sees no key weighs 0, and 0 times an infinity is NaN.
+  if (*dropped)
+    each_nonfinite<BF16, FORMAT, DIM>(p, keys, Cursor(p, it), it.tiles, row, at, kTallKeys, [&](auto value, bool seen) {
+#pragma unroll
+      for (int db = 0; db < kBlocks; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f4 x = value(32 * db + 8 * g + 4 * hl);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[db][4 * g + e] += nonfinite(x[e], seen);
+        }
+    });
   // O^T: this lane holds dims 32 db + 8 g + 4 hl .. + 3 of its row.
   if (it.part < 0) {
     const float inv = l == 0.f ? 0.f : 1.f / l;  // a NaN stays one

@@ -45,7 +45,8 @@ def check(c, seen, scale=None):
                 x, y = got[t, h], want[t, h]
                 fine = np.isfinite(y)
                 assert np.array_equal(x[~fine], y[~fine], equal_nan=True) and np.isfinite(x[fine]).all(), (t, g, x[~fine], y[~fine])
-                bound = error_bound(q[t, h], keys[:, g], vals[:, g], keep, scale, c.bf16, c.form, np.where(fine, y, 0))
+                finite = np.where(np.isfinite(vals[:, g]), vals[:, g], 0)  # an infinity's dim is not in `fine`
+                bound = error_bound(q[t, h], keys[:, g], finite, keep, scale, c.bf16, c.form, np.where(fine, y, 0))
                 assert (np.abs(x[fine] - y[fine]) <= bound[fine]).all(), (t, g)
             t += 1
     return want
@@ -59,4 +60,29 @@ def test_least_scale_averages(ctx, qattn, make, dim, bf16, form, mask, always, w
     c = make(ctx, qattn, dim=dim, bf16=bf16, form=form, mask=mask, always=always, window=window, scale=4.9e-46)
     print("least scale", make.__name__, dim, bf16, form, mask, flush=True)
     assert np.isfinite(check(c, launched(ctx, c), 4.9e-46)).all()
+    c.free()
+
+
+@pytest.mark.parametrize("make", [tall, blocks, steps])
+@pytest.mark.parametrize("dim,bf16,form", [(128, False, "16bit"), (128, False, "int8"), (64, True, "16bit"), (64, True, "int8")])
+@pytest.mark.parametrize("always,window", [(0, 40), (8, 24)])
+@pytest.mark.parametrize("key", [100, 45])
+def test_an_infinity_among_few_keys_of_a_tile(ctx, qattn, make, dim, bf16, form, always, window, key):
+    """Rows whose window covers only one half of a tile see the infinity in it: the half that sees nothing must
+    not turn it into NaN."""
+    c = make(ctx, qattn, dim=dim, bf16=bf16, form=form, mask=1, always=always, window=window)
+    key, i = (key % 64, next(i for i, n in enumerate(c.own) if key % 64 < n <= key % 64 + window)) if make is steps else (key, 0)
+    at = (c.tables[1 + i][key // c.page], slice(None), key % c.page)
+    c.pool[1][at][:, ::5] = 77 if form == "int8" else 0x7F80 if bf16 else 0x7C00
+    if form == "int8":
+        c.pool[1][at] |= 1  # no code of 0, which would give NaN
+        c.scales[1][at] = np.inf
+        c.mine[i][1][key] = c.pool[1][at].view(np.int8) * np.inf
+    else:
+        c.mine[i][1][key] = ref.from_bits(c.pool[1][at], bf16)
+    c.free()
+    c.upload()
+    print("few keys", make.__name__, dim, bf16, form, always, window, key, flush=True)
+    want = check(c, launched(ctx, c))
+    assert np.isposinf(want).any() and not np.isnan(want).any() and np.isfinite(want).sum() > want.size // 2
     c.free()
