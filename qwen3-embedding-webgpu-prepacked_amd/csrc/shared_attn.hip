@@ -156,6 +156,12 @@ struct Keys {
     return rows[i] + ((uint64_t)row * stride[i] + offset);
   }
 };
+// The rows behind a source's last key, in the last group of its last page, may hold anything.  Their scores are
+// masked, but an infinity or NaN among their V must not start the repair that such values of keys need: it takes
+// many times a launch (64 tokens behind 8,190 int8 keys 2,006 us in place of 29; 16-bit ones 317 in place of 26).
+// So V is read from no row behind last_row, the last key's in the groups that end a source (its list is filled up
+// with its last group), but of int8 caches: there any code is finite, and such rows' scales are passed over.
+__device__ inline uint32_t last_row(int keys, int first) { return first + 16 <= keys ? 15 : (keys - 1) & 15; }
 // The group of key `first` of a segment, loaded as a vector: it is waited for with the tile's other loads.
 __device__ inline uint32_t group_of(const SharedParams& p, const SharedSeg& s, int first, int zero) {
   return s.source == kOwnRows ? 0 : (uint32_t)p.groups[zero + s.base + (first >> 4)];
@@ -291,11 +297,12 @@ struct Tall {
   __device__ static uint32_t v_at(int r, int c) { return r * kRow + ((c ^ (DIM == 128 ? (r & 3) << 2 : (r & 2) << 1)) << 4); }
 
   // Where the 16 rows of a tile that this wavefront loads lie.  Rows of keys past the last are read as they
-  // are, if a page holds them (their tile is not whole: their scores are masked, and infinities and NaN of
-  // their V taken out), or as the last key's.
+  // are (K and int8 codes of pages: their scores are masked) or as the last key's.
   struct Spot {
     uint32_t group;  // of pages
+    uint32_t last;   // last_row
     int row, left;   // of p.rows: the first, and how many further there are
+    int held;        // how many hold keys: 16 or more, all; 0 or less, none
     bool rows;
   };
 
@@ -311,6 +318,16 @@ struct Tall {
         raw[I][j] = *reinterpret_cast<const u32x4*>(
             keys.row(I, at.row + min(j * kRows16 + lane / kChunks16, at.left), lane % kChunks16 * 16));
     } else {
+      if constexpr (I && FORMAT != QATTN_KV_INT8) {
+        constexpr int kRows = kCodes ? kRows8 : kRows16, kChunks = kCodes ? kChunks8 : kChunks16;
+#pragma unroll
+        for (int j = 0; j < (kCodes ? kLoads8 : kLoads16); ++j) {
+          const uint32_t r = min((uint32_t)(j * kRows + lane / kChunks), at.last);
+          raw[I][j] = *reinterpret_cast<const u32x4*>(keys.in_group(I, at.group, r * keys.kBytes + lane % kChunks * 16));
+          if constexpr (kCodes) scale[I][j] = keys.scale_of(I, at.group, r);
+        }
+        return;
+      }
       const char* src = keys.in_group(I, at.group, lane * 16);
 #pragma unroll
       for (int j = 0; j < (kCodes ? kLoads8 : kLoads16); ++j) raw[I][j] = *reinterpret_cast<const u32x4*>(src + j * 1024);
@@ -325,8 +342,8 @@ struct Tall {
   // scores (K; scale_log2 included) and of weights (V).  partly: infinities and NaN are taken
   // out (of V, in tiles that some row sees only part of); returns whether there were any.
   template <int I>
-  __device__ bool store(char* lds, float* factors, float scale_log2, bool rows, int wave, int lane, bool partly) {
-    const bool fold = FORMAT == QATTN_KV_INT8 && !rows;
+  __device__ bool store(char* lds, float* factors, float scale_log2, const Spot& spot, int wave, int lane, bool partly) {
+    const bool rows = spot.rows, fold = FORMAT == QATTN_KV_INT8 && !rows;
     const auto each = [&](auto put) {
       if (!kCodes || rows) {
 #pragma unroll
@@ -354,7 +371,7 @@ struct Tall {
       for (int j = 0; j < kLoads8; ++j) {
         float f = !fold ? 1.f : I ? value_factor<BF16>(scale[I][j]) : scale[I][j];
         if (I && !(f < INFINITY)) {
-          any = true;
+          any |= j * kRows8 + lane / kChunks8 < spot.held;
           f = 1.f;
         }
         float* at = factors + 16 * wave + j * kRows8 + lane / kChunks8;
@@ -416,6 +433,8 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
     spot.group = group;
     spot.row = s.base + min(first, s.keys - 1);
     spot.left = max(s.keys - 1 - first, 0);
+    spot.held = s.keys - first;
+    spot.last = last_row(s.keys, first);
     tile.template load<0>(keys, spot, lane);
     tile.template load<1>(keys, spot, lane);
     next = Info{s.whole, s.position + ahead.tile * kTallKeys, s.position + s.keys - 1, s.row_begin, s.row_end};
@@ -427,8 +446,8 @@ __device__ inline void tall_item(const SharedParams& p, const SharedItem& it, in
   const auto keep = [&](int t) {
     char* buf = lds + (t & 1) * 2 * T::kTile;
     float* f = factors + (t & 1) * 2 * kTallKeys;
-    tile.template store<0>(buf, f, p.scale_log2, spot.rows, wave, lane, false);
-    found |= tile.template store<1>(buf + T::kTile, f, p.scale_log2, spot.rows, wave, lane, !next.whole);
+    tile.template store<0>(buf, f, p.scale_log2, spot, wave, lane, false);
+    found |= tile.template store<1>(buf + T::kTile, f, p.scale_log2, spot, wave, lane, !next.whole);
   };
 
   ask();
@@ -693,7 +712,10 @@ struct Flat {
               keys.row(1, s.base + min(first + j * kRows16 + lane / kChunks16, last), lane % kChunks16 * 16));
       } else {
         const char* src = keys.in_group(0, group[b], key * keys.kBytes + (kCodes ? 16 : 32) * c);
-        const char* rows = keys.in_group(1, group[b], lane * 16);
+        // V's row at load j.
+        const uint32_t last = FORMAT == QATTN_KV_INT8 ? 15 : last_row(s.keys, tile * kFlatKeys + 16 * b);
+        constexpr int kRows = kCodes ? kRows8 : kRows16, kChunks = kCodes ? kChunks8 : kChunks16;
+        const auto row_of = [&](int j) { return min((uint32_t)(j * kRows + lane / kChunks), last); };
         if constexpr (kCodes) {
 #pragma unroll
           for (int h = 0; h < DIM / 64; ++h) k[b][h] = *reinterpret_cast<const u32x4*>(src + 64 * h);
@@ -709,8 +731,8 @@ struct Flat {
         }
 #pragma unroll
         for (int j = 0; j < (kCodes ? kLoads8 : kLoads16); ++j) {
-          v[b][j] = *reinterpret_cast<const u32x4*>(rows + j * 1024);
-          if constexpr (kCodes) vs[b][j] = keys.scale_of(1, group[b], j * kRows8 + lane / kChunks8);
+          v[b][j] = *reinterpret_cast<const u32x4*>(keys.in_group(1, group[b], row_of(j) * keys.kBytes + lane % kChunks * 16));
+          if constexpr (kCodes) vs[b][j] = keys.scale_of(1, group[b], row_of(j));
         }
       }
     }
@@ -832,7 +854,7 @@ __device__ inline void flat_item(const SharedParams& p, const SharedItem& it, in
             sc[r >> 2][r & 3] *= tile.kf[r >> 2][r & 3];
             float f = value_factor<BF16>(tile.vf[r >> 2][r & 3]);
             if (!(f < INFINITY)) {
-              any = true;
+              any |= 16 * (r >> 2) + 4 * c + (r & 3) < s.keys - first;
               f = 1.f;
             }
             factor[r >> 2][r & 3] = f;

@@ -1,10 +1,12 @@
 """Attention behind one shared prefix on the GPU: the edges of scales, infinities and unused slots, against the
 definition in 64 bits.  Bounds: as in test_gpu_shared.py."""
+import time
+
 import numpy as np
 import pytest
 
 import shared_ref as ref
-from test_gpu_shared import error_bound
+from test_gpu_shared import Case, error_bound
 from test_gpu_shared_blocks import FORMS, Sampled, blocks, steps, tall
 
 pytestmark = pytest.mark.gpu
@@ -86,3 +88,40 @@ def test_an_infinity_among_few_keys_of_a_tile(ctx, qattn, make, dim, bf16, form,
     want = check(c, launched(ctx, c))
     assert np.isposinf(want).any() and not np.isnan(want).any() and np.isfinite(want).sum() > want.size // 2
     c.free()
+
+
+LONG = dict(prefix=8190, queries=[1] * 64, own=[1 + 37 * i % 300 for i in range(64)])  # flat items, and blocks for the prefix
+CHUNK = dict(prefix=4999, queries=[200] * 4, own=[203] * 4)
+
+
+@pytest.mark.parametrize("case", [LONG, CHUNK], ids=["steps", "prompts"])
+@pytest.mark.parametrize("bf16,form", [(False, "16bit"), (True, "e4m3"), (False, "int8")])
+def test_unused_slots_cost_nothing(ctx, qattn, case, bf16, form):
+    """What lies in slots that hold no key (a page's end that nothing has written) changes neither the results nor
+    the time: NaN codes and scales against zeros, launches in turn.  The repair that infinities of seen keys
+    need takes many times a launch, so half as much again is between the two."""
+    c = Case(ctx, qattn, bf16=bf16, form=form, **case)  # its unused slots hold NaN
+    clean = Case(ctx, qattn, bf16=bf16, form=form, **case)
+    for which in range(2):
+        unused = clean.pool[which] == 0x7FC1 if form == "16bit" else np.isnan(clean.scales[which])
+        assert unused.any()
+        clean.pool[which][unused] = 0
+        clean.scales[which][np.isnan(clean.scales[which])] = 1
+    clean.free()
+    clean.upload()
+    runs, least = [ctx.shared_run(x.desc()) for x in (c, clean)], [np.inf, np.inf]
+    for _ in range(12):
+        for i, run in enumerate(runs):
+            ctx.synchronize()
+            start = time.perf_counter()
+            for _ in range(20):
+                run.encode()
+            ctx.synchronize()
+            least[i] = min(least[i], (time.perf_counter() - start) / 20 * 1e6)
+    print(f"unused {len(c.q)} {form}: {least[0]:.1f} us, clean {least[1]:.1f}", flush=True)
+    assert np.array_equal(c.output(), clean.output())
+    assert least[0] < 1.5 * least[1], least
+    for run in runs:
+        run.destroy()
+    for x in (c, clean):
+        x.free()
