@@ -281,13 +281,14 @@ class Planner {
            kFlatMasked * b.masked / std::max(1, b.item.tiles);
   }
   double cost(const Draft& b, int units) const { return fixed(b) + unit(b) * units; }
+  // The units that `time` is enough for.  (The quotient of cost(b, n) may fall just below n.)
+  int fit(const Draft& b, double time) const { return (int)std::floor((time - fixed(b)) / unit(b) * (1 + 1e-9)); }
 
   // Every draft in equal chunks that take `target` at most, if they can; false if they are more than `most`.
   bool cut_equally(std::vector<Draft>* drafts, double target, int64_t most) const {
     int64_t all = 0;
     for (Draft& b : *drafts) {
-      const int64_t n = b.units(), fit = std::max(1, (int)std::floor((target - fixed(b)) / unit(b)));
-      const int64_t chunks = (n + fit - 1) / fit;
+      const int64_t n = b.units(), each = std::max(1, fit(b, target)), chunks = (n + each - 1) / each;
       if ((all += chunks) > most) return false;
       b.cuts.resize(chunks + 1);
       for (int64_t i = 0; i <= chunks; ++i) b.cuts[i] = (int)(n * i / chunks);
@@ -302,13 +303,13 @@ class Planner {
       const int n = b.units();
       b.cuts.assign(1, 0);
       while (b.cuts.back() < n) {
-        const int fit = (int)std::floor((room - fixed(b)) / unit(b));
-        if (fit < std::min(2, n - b.cuts.back()) && room < target) {
+        const int most = fit(b, room);
+        if (most < std::min(2, n - b.cuts.back()) && room < target) {
           ++used;
           room = target;
           continue;
         }
-        const int take = std::min(std::max(1, fit), n - b.cuts.back());
+        const int take = std::min(std::max(1, most), n - b.cuts.back());
         b.cuts.push_back(b.cuts.back() + take);
         room -= cost(b, take) + kPartial;
       }
@@ -351,10 +352,8 @@ class Planner {
       longest = std::max(longest, cost(b, b.units()));
       total += cost(b, b.units());
     }
-    if (!cut_equally(drafts, longest, kMostSimulated)) {
-      for (Draft& b : *drafts) b.cuts = {0, b.units()};
-      return total / slots_;  // the slots are full
-    }
+    for (Draft& b : *drafts) b.cuts = {0, b.units()};
+    if (drafts->size() > kMostSimulated) return total / slots_;  // the slots are full
     double best = span(*drafts);
     std::vector<std::vector<int>> best_cuts(drafts->size());
     const auto keep = [&]() {

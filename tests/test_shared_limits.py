@@ -1,4 +1,6 @@
 """Limits of the descriptions of attention behind one shared prefix, on the CPU: the values next to them."""
+import ctypes
+
 import pytest
 
 from test_shared_plan import make
@@ -22,3 +24,29 @@ def test_scales_that_vanish_in_f32_are_refused(qattn, scale, fine):
     message = refused(qattn, make(qattn, 100, [3, 1], [5, 70], scale=scale)[0])
     assert (message is None) == fine, message
     assert fine or "scale" in message
+
+
+def planned(qattn, prefix, queries, own, **kw):
+    n, info = ctypes.c_int64(0), qattn.SharedInfo()
+    desc = make(qattn, prefix, queries, own, **kw)[0]
+    qattn._check(qattn.lib().qattn_shared_plan_describe(ctypes.byref(desc), None, 0, ctypes.byref(n), ctypes.byref(info)))
+    return info
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("form", [0, 1, 2])
+@pytest.mark.parametrize("queries", [1, 16, 128, 256])
+def test_what_has_one_place_is_not_cut(qattn, dim, form, queries):
+    """With 256 KV heads each has one of the chip's 256 places, so cutting an item gains nothing and costs a merge:
+    one item of 16, 128 or 256 rows, however many tiles it has."""
+    for tiles in range(1, 401):
+        info = planned(qattn, 128 * tiles, [queries], [queries], heads=256, kv=256, dim=dim, form=form, paged=False)
+        assert (info.items, info.merged_rows, info.partial_rows) == (1, 0, 0), (tiles, info.as_dict())
+
+
+@pytest.mark.parametrize("form", [0, 1, 2])
+def test_blocks_that_fill_the_chip_are_not_cut(qattn, form):
+    """64 prompts of 64 tokens: 32 blocks of 256 rows a KV head, for 32 places, behind any prefix."""
+    for prefix in (50, 100, 128, 200, 256, 300, 900, 1500, 2500, 5000):
+        info = planned(qattn, prefix, [64] * 64, [64] * 64, form=form, paged=False)
+        assert (info.items, info.merged_rows) == (32, 0), (prefix, info.as_dict())
