@@ -236,9 +236,9 @@ int qattn_debug_mask(qattn_ctx* ctx, int32_t L, int32_t mask, int32_t prefix, in
                      uint32_t* host_bits);
 
 /* Failure injection, no counterpart in the reference: the next n device allocations that
- * qattn_run_create / qattn_run_update make for a work list or split workspace fail as if the
- * device were out of memory (QATTN_ENOMEM).  n = 0 cancels.  Lets tests drive the error paths
- * of a re-plan; process-wide, not for production use. */
+ * qattn_run_create / _update and qattn_shared_run_create / _update make for a work list or a
+ * workspace fail as if the device were out of memory (QATTN_ENOMEM).  n = 0 cancels.  Lets tests
+ * drive the error paths of a re-plan; process-wide, not for production use. */
 void qattn_debug_fail_allocs(int32_t n);
 
 /* Host evaluation of the same iteration code (attn_common.h is compiled for host and device):

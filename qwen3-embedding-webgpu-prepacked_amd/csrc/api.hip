@@ -352,16 +352,18 @@ int qattn_plan_slots(const qattn_run_desc* desc, int32_t max_slots, int32_t* slo
 
 }  // extern "C"
 
+// qattn_debug_fail_allocs: device allocations of runs still to fail.
 namespace {
-
-// qattn_debug_fail_allocs: device allocations of install_plan still to fail.
 std::atomic<int32_t> g_fail_allocs{0};
-hipError_t plan_malloc(void** p, size_t bytes) {
+}  // namespace
+hipError_t qattn::plan_malloc(void** p, size_t bytes) {
   int32_t n = g_fail_allocs.load();
   while (n > 0)
     if (g_fail_allocs.compare_exchange_weak(n, n - 1)) return hipErrorOutOfMemory;
   return hipMalloc(p, bytes);
 }
+
+namespace {
 
 // Records, on every stream that launched image i since it was installed, an event after those
 // launches (fences[i]), and forgets the streams: image i's launches are then covered by its fences.

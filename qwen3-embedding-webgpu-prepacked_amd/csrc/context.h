@@ -61,6 +61,9 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 // Host cu_seqlens: nseq in [1, QATTN_MAX_SEQS], cu[0] = 0, non-decreasing.
 int validate_cu(qattn_ctx* ctx, const int32_t* cu, int32_t nseq);
 
+// Device memory of a run's plan or workspace, or a failure asked for by qattn_debug_fail_allocs (api.hip).
+hipError_t plan_malloc(void** p, size_t bytes);
+
 // The context's RoPE table, held: another thread's call can free it (for a longer one) only after
 // `lock` is released.  Release it when the launch that reads the table is enqueued.
 struct RopeTable {

@@ -361,7 +361,7 @@ int install_shared_plan(qattn_shared_run* run, const qattn_shared_desc& desc) {
   if (host.size() > run->image_bytes[next]) {
     void* grown = nullptr;
     const size_t bytes = host.size() + host.size() / 4;  // room for a few steps
-    const hipError_t e = hipMalloc(&grown, bytes);
+    const hipError_t e = plan_malloc(&grown, bytes);
     if (e != hipSuccess) return fail(ctx, QATTN_ENOMEM, "hipMalloc(plan, %zu): %s", bytes, hipGetErrorString(e));
     if (run->image[next]) (void)hipFree(run->image[next]);
     run->image[next] = grown;
@@ -374,7 +374,7 @@ int install_shared_plan(qattn_shared_run* run, const qattn_shared_desc& desc) {
     if (run->cur >= 0 && (rc = wait_shared(run, run->cur))) return rc;
     void* grown = nullptr;
     const size_t bytes = part_bytes + part_bytes / 4;
-    const hipError_t e = hipMalloc(&grown, bytes);
+    const hipError_t e = plan_malloc(&grown, bytes);
     if (e != hipSuccess) return fail(ctx, QATTN_ENOMEM, "hipMalloc(workspace, %zu): %s", bytes, hipGetErrorString(e));
     if (run->partials) (void)hipFree(run->partials);
     run->partials = grown;

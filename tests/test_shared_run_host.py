@@ -1,5 +1,6 @@
 """Runs of the attention behind one shared prefix on the CPU: what their host side does with fields that nothing
 reads.  The library runs over a stand-in for the HIP runtime (fake_hip.cc, preloaded into a child process)."""
+import ctypes
 import json
 import os
 import shutil
@@ -50,7 +51,51 @@ def unread_cache_fields():
     return out
 
 
-CASES = {f.__name__: f for f in (unread_cache_fields,)}
+MANY = dict(cu_q=list(range(601)), own_len=[1] * 600, prefix_pages=[], prefix_len=0)  # a long plan, no partial results
+LONG = dict(cu_q=[0, 1], own_len=[1], prefix_pages=[0] * 4000, prefix_len=64000)      # a short one, cut into many
+BOTH = dict(cu_q=[0, 900, 901], own_len=[900, 1], prefix_pages=[0] * 10000, prefix_len=160000)
+POINTERS = {name: 8 * i for i, name in enumerate(("items", "segs", "starts", "merges", "positions", "groups", "part_o", "part_ml"), 12)}
+
+
+def failed_allocations():
+    """[[step, failure, the run's info, launches: [kernel, grid, pointers, whether any points into freed memory]]] of
+    a run whose device allocations fail now and then."""
+    h, out = Launches(), []
+    q, lib = h.qattn, h.qattn.lib()
+    cache = q.make_kv_cache(K, V, 8, 16)
+
+    def step(name, call, fails=0):
+        lib.qattn_debug_fail_allocs(fails)
+        error = failure(h, call)
+        lib.qattn_debug_fail_allocs(0)
+        launches = []
+
+        def on(kernel, grid, block, args):
+            at = {n: h.word(args, 0, ctypes.c_uint64, o) for n, o in POINTERS.items()}
+            launches.append([kernel, grid, list(at.values()), any(h.fake.fake_hip_freed(x) for x in at.values())])
+
+        h.on = on
+        if run:
+            run[0].encode()
+        out.append([name, error, run[0].info().as_dict() if run else None, launches])
+
+    run = []
+    desc = lambda b: q.make_shared_desc(Q, O, cache, k=K, v=V, **b)  # noqa: E731
+    step("create fails", lambda: run.append(h.ctx.shared_run(desc(LONG))), 1)
+    step("create fails", lambda: run.append(h.ctx.shared_run(desc(LONG))), 2)
+    step("create", lambda: run.append(h.ctx.shared_run(desc(MANY))))
+    step("update", lambda: run[0].update(**MANY))  # both images hold a long plan now
+    step("workspace fails", lambda: run[0].update(**LONG), 1)
+    step("update", lambda: run[0].update(**LONG))
+    step("image fails", lambda: run[0].update(**BOTH), 1)
+    step("both fail", lambda: run[0].update(**BOTH), 2)
+    step("update", lambda: run[0].update(**BOTH))
+    step("update", lambda: run[0].update(**MANY))
+    run[0].destroy()
+    return out
+
+
+CASES = {f.__name__: f for f in (unread_cache_fields, failed_allocations)}
 
 
 @pytest.fixture(scope="module")
@@ -81,6 +126,23 @@ def test_cache_fields_that_nothing_reads_may_hold_anything(run_child):
         assert made is None and updated is None and rebound is None, (fields, made, updated, rebound)
         assert kernels and all("shared_" in k for k in kernels) and "ILb0ELi0ELi128E" in kernels[0], (fields, kernels)
         assert paged is not None and paged[0] == -1, fields
+
+
+def test_a_failed_allocation_leaves_the_run_its_plan(run_child):
+    """Device memory that runs out in a create or an update is an error of its own; the run goes on with the plan that
+    it had, in memory that is still its own."""
+    steps = run_child("failed_allocations")
+    before = None
+    for name, error, info, launches in steps:
+        assert (error is not None) == ("fail" in name), (name, error)
+        assert error is None or (error[0] == -3 and "hipMalloc" in error[1]), error
+        assert not any(freed for *_, freed in launches), name
+        if "fail" in name:
+            assert before is None or [info, launches] == before, name
+        elif before:
+            assert [info, launches] != before
+        before = info and [info, launches]
+    assert [len(launches) for *_, launches in steps] == [0, 0, 1, 1, 1, 2, 2, 2, 2, 1]
 
 
 if __name__ == "__main__":
