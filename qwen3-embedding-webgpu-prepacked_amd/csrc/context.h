@@ -40,10 +40,13 @@ void set_last_error(qattn_ctx* ctx, const std::string& message);
       return ::qattn::fail((ctx), QATTN_EHIP, "%s failed: %s", #expr, hipGetErrorString(e_)); \
   } while (0)
 
-// Makes `dev` current for the scope and restores the caller's device afterwards.
+// Makes `dev` current for the scope and restores the caller's device afterwards.  Drops the error that an earlier
+// call on this thread may have left (memory that ran out, here or in the caller's code): a launch is checked by the
+// runtime's last error, and would report that one as its own.
 struct DeviceGuard {
   int prev = -1;
   explicit DeviceGuard(int dev) {
+    (void)hipGetLastError();
     if (hipGetDevice(&prev) != hipSuccess) prev = -1;
     if (prev != dev) (void)hipSetDevice(dev);
   }
