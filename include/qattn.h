@@ -432,8 +432,9 @@ typedef struct qattn_shared_desc {
                              * f32 (up to about 4.8e-46) is refused */
 } qattn_shared_desc;
 /* Tensors 16-byte aligned, strides multiples of 8 elements up to 2^24 and at least the heads' width;
- * page numbers in [0, pages); positions below 2^30; fewer than 2^31 own keys, at most 2^22 sequences and
- * 2^22 rows (queries * q_heads / kv_heads).  o must not overlap what the launch reads.
+ * page numbers in [0, pages); positions below 2^30; fewer than 2^31 own keys, at most QATTN_MAX_SEQS
+ * sequences and 2^22 rows (queries * q_heads / kv_heads); over all KV heads fewer than 2^23 workgroups
+ * and merged rows, or the plan is refused.  o must not overlap what the launch reads.
  * The run plans the launch on the host, as qattn_run_create does: rows (query, head of the group) of
  * all sequences are stacked, so that a tile of prefix keys is read once for up to 256 rows; long key
  * ranges of few rows are spread over workgroups and their partial results merged by a second launch. */

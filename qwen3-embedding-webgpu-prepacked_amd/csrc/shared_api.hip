@@ -241,7 +241,6 @@ int check_shared(qattn_ctx* ctx, const qattn_shared_desc* d) {
   int rc = validate_cu(ctx, d->cu_q, d->nseq);
   if (rc) return rc;
   if (!d->own_len) return fail(ctx, QATTN_EINVAL, "own_len is NULL");
-  if (d->nseq > kMaxSharedRows) return fail(ctx, QATTN_EINVAL, "nseq %d: up to 2^22", d->nseq);
   if (d->prefix_len < 0 || d->prefix_len >= kMaxPosition) return fail(ctx, QATTN_EINVAL, "prefix_len %d outside [0, 2^30)", d->prefix_len);
   int64_t own = 0;
   for (int32_t i = 0; i < d->nseq; ++i) {

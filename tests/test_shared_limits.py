@@ -50,3 +50,18 @@ def test_blocks_that_fill_the_chip_are_not_cut(qattn, form):
     for prefix in (50, 100, 128, 200, 256, 300, 900, 1500, 2500, 5000):
         info = planned(qattn, prefix, [64] * 64, [64] * 64, form=form, paged=False)
         assert (info.items, info.merged_rows) == (32, 0), (prefix, info.as_dict())
+
+
+def test_as_many_sequences_as_elsewhere(qattn):
+    """65,536 sequences, as for the other launches; one more is refused."""
+    assert planned(qattn, 20, [1] * 65536, [1] * 65536).tokens == 65536
+    message = refused(qattn, make(qattn, 20, [1] * 65537, [1] * 65537)[0])
+    assert message and "nseq=65537" in message and "65536" in message
+
+
+def test_limits_that_the_header_states(qattn):
+    """A launch has fewer than 2^23 workgroups, and merges fewer than 2^23 rows, over all KV heads."""
+    queries = [1] * 65536
+    assert planned(qattn, 100, queries, queries, heads=63 * 2, kv=63, page=16).merged_rows == 1 << 17
+    message = refused(qattn, make(qattn, 100, queries, queries, heads=64 * 2, kv=64, page=16)[0])
+    assert message and "too many rows for one launch" in message
