@@ -373,9 +373,11 @@ enum qattn_kv_format {
   QATTN_KV_E4M3 = 1,  /* OCP e4m3 code of x / scale, scale the least power of two with amax <= 448 scale;
                        * infinities become +-448 scale, NaN the NaN code; no code whose value is past
                        * the largest of `dtype` (240 takes the place of 256 and more at scale 2^8 for
-                       * fp16, 2^120 for bf16) */
+                       * fp16, 2^120 for bf16).  Scales are positive normal powers of two, whoever
+                       * writes them: of any other scale the readers here take the exponent only, so
+                       * that values come out wrong by up to 2 times */
   QATTN_KV_INT8 = 2   /* rint(x * (127 / amax)) in [-127, 127], scale = amax / 127; infinities become
-                       * +-127, NaN 0 */
+                       * +-127, NaN 0.  Readers take any scale */
 };
 /* A paged cache in the caller's device memory: slot s is row s % page_size of page s / page_size;
  * codes [pages][kv_heads][page_size][head_dim], scales [pages][kv_heads][page_size].  Device
@@ -398,8 +400,9 @@ typedef struct qattn_kv_cache {
 int qattn_kv_write(qattn_ctx* ctx, const qattn_kv_cache* cache, const void* k, int64_t k_row_stride,
                    const void* v, int64_t v_row_stride, const int64_t* slots, int64_t tokens,
                    qattn_stream_t stream);
-/* Reads slots back into rows: element = code * scale rounded to `dtype`; a slot outside the cache
- * gives a row of zeros.  Otherwise as qattn_kv_write (slots may repeat). */
+/* Reads slots back into rows: element = code * scale rounded to `dtype` (an e4m3 scale being a power
+ * of two, see above); a slot outside the cache gives a row of zeros.  Otherwise as qattn_kv_write
+ * (slots may repeat). */
 int qattn_kv_read(qattn_ctx* ctx, const qattn_kv_cache* cache, const int64_t* slots, int64_t tokens,
                   void* k, int64_t k_row_stride, void* v, int64_t v_row_stride, qattn_stream_t stream);
 
@@ -410,13 +413,16 @@ typedef struct qattn_shared_run qattn_shared_run;
  * head h reads KV head h / (q_heads / kv_heads).  A query sees the keys at its position and before it,
  * under QATTN_MASK_PREFIX_LOCAL those of positions < prefix or > its own - window.  One that sees none
  * (at a position below 0: m beyond the keys; an empty mask) gives zeros, and a key that a query does
- * not see adds nothing to it, whatever it holds. */
+ * not see adds nothing to it, whatever it holds; nor does a cache row that holds no key.  A seen
+ * key's infinite value gives that infinity, or NaN where its weight is next to none: below 2^-25 of
+ * the largest for fp16, or below 2^-126. */
 typedef struct qattn_shared_desc {
   const void* q; /* head h of packed query t at element t*q_row_stride + h*head_dim; o likewise */
   void* o;
   int64_t q_row_stride, o_row_stride;
   int32_t q_heads;          /* a multiple of cache.kv_heads, up to 64 of them to a KV head */
-  qattn_kv_cache cache;     /* kv_heads, head_dim and dtype always; the rest if pages are read */
+  qattn_kv_cache cache;     /* kv_heads, head_dim and dtype always; the rest if pages are read.  e4m3
+                             * scales have to be powers of two (enum qattn_kv_format) */
   const int32_t* prefix_pages; /* host: ceil(prefix_len / page_size) page numbers; copied */
   int32_t prefix_len;       /* may be 0 */
   const int32_t* cu_q;      /* host: nseq+1 non-decreasing offsets of the packed queries, from 0; copied */
@@ -445,7 +451,8 @@ int qattn_shared_run_create(qattn_ctx* ctx, const qattn_shared_desc* desc, qattn
 int qattn_shared_run_encode(qattn_shared_run* run, qattn_stream_t stream);
 /* New lengths and pages (a step later, the next batch); the tensors hold as many rows as it names.
  * Works as qattn_run_update: two plan images, waits only for this run's launches that read the older
- * one, and on failure the run keeps its plan. */
+ * one, and on failure the run keeps its plan.  It plans anew and copies the plan to the device, both
+ * before it returns: 50 to 270 us for steps of 16 to 256 tokens. */
 int qattn_shared_run_update(qattn_shared_run* run, const int32_t* prefix_pages, int32_t prefix_len,
                             const int32_t* cu_q, int32_t nseq, const int32_t* own_len, const int32_t* own_pages);
 /* Other tensors of the same strides, and another cache of the same geometry (the layers of a model):

@@ -8,18 +8,21 @@
 //   tall   256 rows, 32 to each of eight wavefronts, over 128-key tiles that they share in LDS.
 //   split  128 rows: four wavefronts take the tile's first 64 keys, four its last, and their sums are joined
 //          at the end.  2.4 us a tile against tall's 4.0 (head_dim 128): dearer for a row, sooner done (16
-//          queries of 10 to 150 tokens: 25 us, by tall items 33; 16 x 500 tokens: 457 us, by tall 364).
+//          queries of 10 to 150 tokens: 25 us, by tall items 33; 16 x 500 tokens: 457 us, by tall 366).
 //   flat   16 rows (up to 16 single tokens of several sequences) over 32-key tiles, a run of them to each of
 //          eight wavefronts, which keeps its own sum; K goes from memory straight into the MFMA operand, V
 //          through the wavefront's own 8 KiB of LDS for the transposed read; the sums are joined at the end.
 // Blocks (tall and split): S^T = K Q^T and O^T = V^T P^T on 32x32x16 MFMAs, a query row to a lane.  Codes
 // become 16-bit elements once, on their way into LDS.  16 x 500 tokens behind 5,000 e4m3 keys (16 heads over
-// 8, head_dim 128) take 364 us, 945 TFLOP/s where the library's 8,192-cubed product reaches 1,222.  Bound by
+// 8, head_dim 128) take 366 us, 939 TFLOP/s where the library's 8,192-cubed product reaches 1,222.  Bound by
 // the matrix cores and, in turn with them, the softmax's vector work: without its exponentials a launch is 8 %
 // shorter, without its LDS reads 3 %; the wavefronts of a SIMD hardly overlap the two, staggered by half a step
-// neither (that was 13 % slower), and one workgroup fills a CU's LDS and half its registers.
+// neither (that was 13 % slower), and one workgroup fills a CU's LDS and half its registers.  (At head_dim 128
+// codes take all 256 of a lane's, int8 ones spill five; scalar registers are spilled by every kernel of blocks, 9
+// to 78 of them.)
 // Flat items are bound by latency (a step of 16 tokens takes 9.4 us with its merge, a call 3.8 at least), or
-// by the cache's bytes: 256 tokens with 1,024 e4m3 keys each take 98 us, 5.6 TB/s.
+// by the cache's bytes: 256 tokens with 1,024 e4m3 keys each take 98 us, 5.6 TB/s of reads (a copy, which writes
+// half of its bytes, moves 5.2).
 // An item whose rows have keys elsewhere too (other chunks, other items) leaves its unnormalised f32
 // sums, the row's reference m and its sum of p; shared_merge_kernel joins them.
 //
@@ -171,8 +174,8 @@ __device__ inline uint32_t group_of(const SharedParams& p, const SharedSeg& s, i
 // A code times its scale would have to be rounded to a 16-bit element, K's and V's, which doubles the result's
 // error.  Instead the products take the codes, which are exact: K's scale goes to the key's scores in f32, and
 // V's to its weights.  A weight is rounded to 16 bits after that, so V's elements are the codes times a power
-// of two 2^e near the scale (exact too, and finite for any code), and the weight's factor is scale / 2^e: 1 to
-// 2.02 for the scales that kv_write gives, but fp16 ones under 2^-24.
+// of two 2^e near the scale (exact too, and finite for any code), and the weight's factor is scale / 2^e: for the
+// scales that kv_write gives 1 to 2.02 (bf16, whose greatest scale is 2^121: 4.03), less for fp16 ones under 2^-24.
 template <bool BF16>
 __device__ inline float near_power(float scale) {
   const int e = min(max((int)(__float_as_uint(scale) >> 23 & 255u) - 127, BF16 ? -110 : -24), BF16 ? 119 : 8);
@@ -185,8 +188,8 @@ __device__ inline float value_factor(float scale) {
   return f < 0x1p-8f ? 0x1p-8f : f;
 }
 
-// 16 codes of K (I = 0) or V (1) as two 16-byte chunks of 16-bit elements, exactly: an e4m3 code times its
-// power of two; of an int8 code the factor of its key (below) is left out.
+// 16 codes of K (I = 0) or V (1) as two 16-byte chunks of 16-bit elements: an e4m3 code times its power of
+// two, exactly but below the type's normal range; of an int8 code, exactly, the factor of its key is left out.
 template <bool BF16, int FORMAT, int I>
 __device__ inline void expand(u32x4 codes, float scale, u32x4 (&out)[2]) {
   typedef Elem<false>::T2 H2;
@@ -215,8 +218,9 @@ __device__ inline void expand(u32x4 codes, float scale, u32x4 (&out)[2]) {
 // ---- values that a row must not see ----------------------------------------------------------------
 // A masked key's p is 0, but 0 times an infinity or NaN is NaN.  In tiles that some row of the item sees
 // only part of, such elements of V are replaced by 0 on their way into LDS, and if there were any, the
-// rows that do see the key get them added at the end (p times an infinity is that infinity, whatever the
-// reference).  (An int8 code's infinity or NaN is its key's factor's.)
+// rows that do see the key get them added at the end: p times an infinity is that infinity.  (An int8 code's
+// infinity or NaN is its key's factor's.)  Elsewhere it meets p as it was rounded, and sums that are scaled down:
+// an infinity whose weight underflows there becomes NaN.
 template <bool BF16>
 __device__ inline void drop_nonfinite(u32x4& chunk) {
   constexpr uint32_t kExp = Elem<BF16>::kExponent;
