@@ -13,6 +13,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -90,7 +91,15 @@ int fail(qattn_ctx* ctx, int code, const char* fmt, ...) {
   va_start(ap, fmt);
   vsnprintf(buf, sizeof(buf), fmt, ap);
   va_end(ap);
-  set_last_error(ctx, buf);
+  try {
+    set_last_error(ctx, buf);
+  } catch (const std::bad_alloc&) {  // no message, rather than an exception or an earlier call's
+    g_last_error.clear();
+    if (ctx) {
+      std::lock_guard<std::mutex> lock(ctx->mu);
+      ctx->last_error.clear();
+    }
+  }
   return code;
 }
 

@@ -317,7 +317,12 @@ int retire_shared(qattn_shared_run* run, int i) {
       (void)hipEventDestroy(ev);
       return fail(run->ctx, QATTN_EHIP, "hipEventRecord: %s", hipGetErrorString(e));
     }
-    run->fences[i].push_back(ev);
+    try {
+      run->fences[i].push_back(ev);
+    } catch (const std::bad_alloc&) {
+      (void)hipEventDestroy(ev);
+      return fail(run->ctx, QATTN_ENOMEM, "out of host memory");
+    }
   }
   run->streams[i].clear();
   return QATTN_OK;

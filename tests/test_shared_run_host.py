@@ -95,7 +95,54 @@ def failed_allocations():
     return out
 
 
-CASES = {f.__name__: f for f in (unread_cache_fields, failed_allocations)}
+def host_memory():
+    """{call: how often it returned what}, each call again and again with its first, second, .. allocation on the host
+    failing, until it makes no more."""
+    h, new, out = Launches(), ctypes.CDLL(os.environ["FAIL_NEW"]), {}
+    new.fail_new_at.argtypes = [ctypes.c_long]
+    q, lib, ctx = h.qattn, h.qattn.lib(), h.ctx.handle
+    cache = q.make_kv_cache(K, V, 8, 16)
+    desc = lambda b: q.make_shared_desc(Q, O, cache, k=K, v=V, **b)  # noqa: E731
+    first, second, refused, handle, words = desc(LONG), desc(BOTH), desc(LONG), ctypes.c_void_p(), ctypes.c_int64()
+    refused.q_heads = 7
+
+    def sweep(name, call, prepare=lambda: None, after=lambda: None):
+        counts, n, more = {}, 0, True
+        while more:
+            n += 1
+            prepare()
+            new.fail_new_at(n)
+            code = call()
+            more = bool(new.fail_new_did())
+            new.fail_new_at(0)
+            if more and name != "destroy":
+                counts[code] = counts.get(code, 0) + 1
+            after()
+        out[name] = [n, counts, code]
+
+    def create():
+        return lib.qattn_shared_run_create(ctx, ctypes.byref(first), ctypes.byref(handle))
+
+    def destroy():
+        lib.qattn_shared_run_destroy(handle)
+        handle.value = None
+
+    def used():  # a run with launches on two streams
+        create()
+        lib.qattn_shared_run_encode(handle, None)
+        lib.qattn_shared_run_encode(handle, 0x5000)
+
+    d = second
+    sweep("create", create, after=destroy)
+    sweep("update", lambda: lib.qattn_shared_run_update(handle, d.prefix_pages, d.prefix_len, d.cu_q, d.nseq, d.own_len, None), used, destroy)
+    sweep("encode", lambda: lib.qattn_shared_run_encode(handle, 0x6000), used, destroy)
+    sweep("describe", lambda: lib.qattn_shared_plan_describe(ctypes.byref(first), None, 0, ctypes.byref(words), None))
+    sweep("refused", lambda: lib.qattn_shared_run_create(ctx, ctypes.byref(refused), ctypes.byref(handle)))
+    sweep("destroy", destroy, used)
+    return out
+
+
+CASES = {f.__name__: f for f in (unread_cache_fields, failed_allocations, host_memory)}
 
 
 @pytest.fixture(scope="module")
@@ -106,11 +153,13 @@ def run_child(tmp_path_factory):
     lib = str(tmp_path_factory.mktemp("fake") / "libfake_hip.so")
     subprocess.run([compiler, "-std=c++17", "-O1", "-shared", "-fPIC", "-w", "-I" + os.path.join(ROCM, "include"), "-o", lib,
                     os.path.join(HERE, "fake_hip.cc")], check=True)
+    new = os.path.join(os.path.dirname(lib), "libfail_new.so")
+    subprocess.run([compiler, "-std=c++17", "-O1", "-shared", "-fPIC", "-o", new, os.path.join(HERE, "fail_new.cc"), "-ldl"], check=True)
 
-    def run(case):
-        preload = " ".join(v for v in (os.environ.get("LD_PRELOAD"), lib) if v)
+    def run(case, failing_new=False):
+        preload = " ".join(v for v in (os.environ.get("LD_PRELOAD"), new if failing_new else None, lib) if v)
         out = subprocess.run([sys.executable, os.path.abspath(__file__), case], check=True, capture_output=True, text=True,
-                             env=dict(os.environ, LD_PRELOAD=preload, FAKE_HIP=lib), timeout=60)
+                             env=dict(os.environ, LD_PRELOAD=preload, FAKE_HIP=lib, FAIL_NEW=new), timeout=60)
         return json.loads(out.stdout)
 
     return run
@@ -143,6 +192,20 @@ def test_a_failed_allocation_leaves_the_run_its_plan(run_child):
             assert [info, launches] != before
         before = info and [info, launches]
     assert [len(launches) for *_, launches in steps] == [0, 0, 1, 1, 1, 2, 2, 2, 2, 1]
+
+
+def test_host_memory_that_runs_out_is_an_error_code(run_child):
+    """No exception leaves a call, whichever of its allocations fails: planning and encoding report it, a refusal stays
+    one, and a run is destroyed all the same."""
+    if "QATTN_LIB" in os.environ:
+        pytest.skip("an instrumented library brings its own operator new")
+    seen = run_child("host_memory", failing_new=True)
+    for name in ("create", "update", "encode", "describe"):
+        n, counts, last = seen[name]
+        assert last == 0 and set(counts) <= {"-3", "0"} and counts["-3"] >= (1 if name == "encode" else 20), (name, seen[name])
+    n, counts, last = seen["refused"]
+    assert last == -1 and set(counts) == {"-1"} and n > 1
+    assert seen["destroy"][0] > 1
 
 
 if __name__ == "__main__":
