@@ -54,7 +54,7 @@ extern "C" {
  *    qattn_debug_fail_allocs
  * 8: qattn_debug_run_timeline
  * 9: qattn_buffer_read_after, qattn_event_synchronize; added since without a change to what was
- *    there: qattn_rope, qattn_kv_*, qattn_shared_* */
+ *    there: qattn_rope, qattn_kv_*, qattn_shared_*, qattn_rmsnorm_q8, qattn_quantize_q8, qattn_w4_* */
 #define QATTN_ABI_VERSION 9
 
 #define QATTN_Q_HEADS 16
@@ -486,6 +486,64 @@ int qattn_shared_run_get_info(const qattn_shared_run* run, qattn_shared_info* in
  * words NULL: only *count. */
 int qattn_shared_plan_describe(const qattn_shared_desc* desc, int32_t* words, int64_t capacity, int64_t* count,
                                qattn_shared_info* info);
+
+/* ---- a forward with 8-bit activations: rows into 8 bits, products with 4-bit weights ------------------ */
+/* No counterpart in the reference, whose activations are f16 throughout.  A stage hands the next one rows of
+ * 8-bit codes with one f32 scale each (value = code * scale), and the products of such rows with 4-bit weights run
+ * in whole numbers on the matrix cores.  16-bit tensors are fp16 or bf16 (enum qattn_dtype), arithmetic f32.
+ * Rows: 16-byte aligned (codes 8), strides in elements, at least the width, multiples of 8, at most 2^22; what a
+ * call writes may not overlap anything else that it touches, where nothing else is said.  All calls here enqueue
+ * on `stream` (NULL: the context stream), allocate nothing, wait for nothing and keep nothing between calls, so
+ * that they can be captured and may overlap. */
+
+/* codes[r][c] = rint(x[r][c] * (127 / amax)), scales[r] = amax / 127, amax the row's largest magnitude; each
+ * operation rounded to f32.  A row with an infinity or a NaN gets codes of 0 and a scale of NaN, one whose amax is
+ * below 2^-100 codes of 0 and a scale of 0.  width a multiple of 8 in [8, 32768]; rows below 2^24. */
+int qattn_quantize_q8(qattn_ctx* ctx, const void* x, int64_t x_row_stride, int8_t* codes, int64_t codes_row_stride,
+                      float* scales, int64_t rows, int32_t width, int32_t dtype, qattn_stream_t stream);
+/* Residual add + RMSNorm (qattn_rmsnorm's formula) with an 8-bit result: v = f32(x) + f32(residual), sum <- v in
+ * `dtype` (without a residual v = f32(x), and sum is NULL too); t = f32(sum) * weight[c] (without a residual of x),
+ * codes = rint(t * (127 / amax)) with amax the row's largest |t|, scales = amax / 127 * inv, inv = 1 / sqrt(sum(v^2) /
+ * width + eps).  The norm's factor cancels in the codes, which therefore depend on no order of a sum.  A row with
+ * an infinity or a NaN among its t, or whose sum of squares passes f32's range, gets codes of 0 and a scale of NaN;
+ * amax below 2^-100 gives codes and a scale of 0.  weight: device f32 [width], 16-byte aligned.  sum may be x or
+ * residual (with its stride). */
+int qattn_rmsnorm_q8(qattn_ctx* ctx, const void* x, int64_t x_row_stride, const void* residual, int64_t residual_row_stride,
+                     void* sum, int64_t sum_row_stride, const float* weight, int8_t* codes, int64_t codes_row_stride,
+                     float* scales, int64_t rows, int32_t width, int32_t dtype, double eps, qattn_stream_t stream);
+
+/* 4-bit weights with group scales: W(n, k) = (code - zero) * multiplier * scale[n], code, zero and multiplier of 4
+ * bits, zero and multiplier one pair for every 32 columns of a row (a group), with zero * multiplier <= 128 and
+ * (15 - zero) * multiplier <= 127, so that (code - zero) * multiplier is a whole number of 8 bits.  The image that
+ * the products read is written on the host, once, by one of the functions below, and copied to the device by the
+ * caller; K a multiple of 32 up to 65536, N up to 2^22, 17/32 of a byte for each weight (K padded to 128, N to 16).
+ * None of these needs a device or a context; messages are in qattn_last_error(NULL). */
+int64_t qattn_w4_bytes(int32_t K, int32_t N); /* -1 for a shape that is none */
+/* codes: [N][K / 2], column 2 i in the low nibble of byte i, column 2 i + 1 in its high nibble; groups: [N][K / 32],
+ * multiplier | zero << 4; scales: [N], finite. */
+int qattn_w4_pack(const uint8_t* codes, const uint8_t* groups, const float* scales, int32_t K, int32_t N, void* image,
+                  int64_t image_bytes);
+/* Quantises finite f32 rows.  scale[n] = f32(largest magnitude of the row / 120); a group whose value of the largest
+ * magnitude (the first) is a has zero 8 if a < 0, else 7, and the multiplier m of floor(|a| / 8 / scale) and one
+ * more, within [1, 15], that leaves the smaller sum of squared differences (the lower at a tie), with codes
+ * rint(w / (scale * m)) + zero clamped to 4 bits.  A group of zeros has multiplier 0, a row below 2^-100 is zeros. */
+int qattn_w4_quantize(const float* w, int64_t row_stride, int32_t K, int32_t N, void* image, int64_t image_bytes);
+/* The same for the values f32(scale) * (q - 8) of a q4_0-tile32-compact tensor (qattn_q4_matmul): group scales of
+ * 11 bits become multiples of the row's, so the weights change: by about 3 % of their size where a model's groups
+ * differ as normal values do, beside the 8.6 % that Q4_0 has left out. */
+int qattn_w4_from_q4(const void* q4, int64_t q4_bytes, int32_t K, int32_t N, void* image, int64_t image_bytes);
+
+/* y[m][n] = x_scale[m] * scale[n] * sum over k of x[m][k] * (code - zero) * multiplier, for m < M, n < N, rounded to
+ * `dtype` once; the sum is exact (32-bit whole numbers), so a row's result does not depend on its batch.  x: 8-bit rows,
+ * ldx a multiple of 16; w: the image on the device, 16-byte aligned; M below 2^24, and fewer than 2^22 blocks of 32
+ * rows and 16 columns.  One to 16 rows (a step's tokens) are matrix-vector products, bound by the weights. */
+int qattn_w4_matmul(qattn_ctx* ctx, const int8_t* x, int64_t ldx, const float* x_scale, int32_t M, int32_t K, const void* w,
+                    int64_t w_bytes, int32_t N, void* y, int64_t ldy, int32_t dtype, qattn_stream_t stream);
+/* The FFN's gate/up projection and SwiGLU: y[m][j] = g / (1 + exp(-g)) * u with g and u the f32 results of rows j and
+ * n_inter + j of a weight of 2 n_inter rows, rounded once.  n_inter a multiple of 32. */
+int qattn_w4_matmul_swiglu(qattn_ctx* ctx, const int8_t* x, int64_t ldx, const float* x_scale, int32_t M, int32_t K,
+                           const void* w, int64_t w_bytes, int32_t n_inter, void* y, int64_t ldy, int32_t dtype,
+                           qattn_stream_t stream);
 
 /* ---- consumer: last-token pool + L2 norm  (replaces LastTokenPoolKernel, ops.ts:347-379) --- */
 /* For each sequence i < nseq: out[i*out_row_stride + d] = f32(x[r*row_stride + d]) * s for

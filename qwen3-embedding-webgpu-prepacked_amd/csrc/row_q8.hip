@@ -1,0 +1,165 @@
+// row_q8.hip -- rows of 16-bit elements into 8-bit codes with one scale each: as they are, or as the RMSNorm of a
+// residual sum.
+//
+//   v = x + r (f32), x' = v rounded to the type, inv = 1 / sqrt(sum(v^2) / width + eps)
+//   t = x' * weight, amax = max |t|, code = rint(t * (127 / amax)), scale = amax / 127 * inv
+//
+// The norm's factor inv is one number for a row, so it cancels in the codes and stands in the scale alone.  The
+// sum of squares and the largest value then take one reduction between them, the row is read once and stays in
+// registers, and the codes do not depend on the order in which a sum is formed.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "elem.h"
+#include "w4_ops.h"
+
+namespace qattn {
+namespace {
+
+// Codes of 8 values, four to a dword.  Adding 1.5 * 2^23 rounds a value to a whole number, ties to even, in the
+// low byte; the product is rounded to f32 before (contraction would round once).
+__device__ inline u32x2 codes8(const float* t, float factor) {
+#pragma clang fp contract(off)
+  uint32_t c[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) c[e] = __float_as_uint(t[e] * factor + 12582912.f);
+  const auto pack = [](uint32_t a, uint32_t b, uint32_t p, uint32_t q) {
+    const uint32_t lo = __builtin_amdgcn_perm(b, a, 0x0C0C0400u), hi = __builtin_amdgcn_perm(q, p, 0x04000C0Cu);
+    return lo | hi;
+  };
+  return u32x2{pack(c[0], c[1], c[2], c[3]), pack(c[4], c[5], c[6], c[7])};
+}
+
+// T threads to a row, C pieces of 8 elements to a thread.
+template <bool BF16, bool NORM, bool SUM, int T, int C>
+__global__ __launch_bounds__(T < 256 ? 256 : T) void row_q8_kernel(RowQ8 p) {
+  constexpr int kRows = T < 256 ? 256 / T : 1, kWaves = T / 64;
+  const int tid = threadIdx.x % T;
+  const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / T;
+  if (row >= p.rows) return;  // T > 64: one row to a workgroup, so this is uniform
+  const uint16_t* const x = static_cast<const uint16_t*>(p.x) + row * p.x_stride;
+  u32x4 a[C], r[C];
+#pragma unroll
+  for (int j = 0; j < C; ++j) {
+    const int c = 8 * (tid + T * j);
+    a[j] = c < p.width ? *reinterpret_cast<const u32x4*>(x + c) : u32x4{};
+    if constexpr (SUM)
+      r[j] = c < p.width ? *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p.residual) + row * p.residual_stride + c)
+                         : u32x4{};
+  }
+  float t[8 * C];
+  float squares = 0.f;
+  uint32_t most = 0;  // the largest magnitude's bits: NaN above infinity above every number
+#pragma unroll
+  for (int j = 0; j < C; ++j) {
+    const int c = 8 * (tid + T * j);
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = widen<BF16, 0>(a[j][i]);
+      v[2 * i + 1] = widen<BF16, 1>(a[j][i]);
+      if constexpr (SUM) {
+        v[2 * i] += widen<BF16, 0>(r[j][i]);
+        v[2 * i + 1] += widen<BF16, 1>(r[j][i]);
+      }
+    }
+    if constexpr (NORM)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) squares = fmaf(v[e], v[e], squares);
+    if constexpr (SUM) {
+      u32x4 s;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[i] = narrow2<BF16>(v[2 * i], v[2 * i + 1]);
+      if (c < p.width) *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.sum) + row * p.sum_stride + c) = s;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = widen<BF16, 0>(s[i]);
+        v[2 * i + 1] = widen<BF16, 1>(s[i]);
+      }
+    }
+    if constexpr (NORM) {
+      float4 w[2] = {};
+      if (c < p.width) {
+        w[0] = *reinterpret_cast<const float4*>(p.weight + c);
+        w[1] = *reinterpret_cast<const float4*>(p.weight + c + 4);
+      }
+      const float g[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= g[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      t[8 * j + e] = v[e];
+      most = max(most, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+    }
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    if constexpr (NORM) squares += __shfl_xor(squares, d, 64);
+    most = max(most, (uint32_t)__shfl_xor((int)most, d, 64));
+  }
+  if constexpr (kWaves > 1) {
+    __shared__ float part_squares[kWaves];
+    __shared__ uint32_t part_most[kWaves];
+    if ((tid & 63) == 0) {
+      part_squares[tid >> 6] = squares;
+      part_most[tid >> 6] = most;
+    }
+    __syncthreads();
+    squares = part_squares[0];
+    most = part_most[0];
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i) {
+      squares += part_squares[i];
+      most = max(most, part_most[i]);
+    }
+  }
+  // A row with an infinity or a NaN, or whose squares pass f32's range: codes of zero, a scale of NaN.  A row of
+  // next to nothing: zeros, with a scale of zero.
+  const float amax = __uint_as_float(most);
+  const bool lost = most >= 0x7F800000u || (NORM && !(squares < INFINITY)), none = amax < kLeastAmax;
+  const float factor = lost || none ? 0.f : 127.f / amax;
+  if (tid == 0) {
+    const float inv = NORM ? 1.f / sqrtf(squares / (float)p.width + p.eps) : 1.f;
+    p.scales[row] = lost ? __builtin_nanf("") : none ? 0.f : amax / 127.f * inv;
+  }
+  int8_t* const out = p.codes + row * p.codes_stride;
+#pragma unroll
+  for (int j = 0; j < C; ++j) {
+    const int c = 8 * (tid + T * j);
+    if (c < p.width) *reinterpret_cast<u32x2*>(out + c) = lost ? u32x2{} : codes8(t + 8 * j, factor);
+  }
+}
+
+template <bool BF16, bool NORM, bool SUM>
+void launch(const RowQ8& p, hipStream_t stream) {
+#define ROW_Q8(T, C)                                                                                               \
+  hipLaunchKernelGGL((row_q8_kernel<BF16, NORM, SUM, T, C>),                                                       \
+                     dim3((unsigned)((p.rows + (T < 256 ? 256 / T : 1) - 1) / (T < 256 ? 256 / T : 1))),          \
+                     dim3(T < 256 ? 256 : T), 0, stream, p)
+  if (p.width <= 512)
+    ROW_Q8(64, 1);
+  else if (p.width <= 1024)
+    ROW_Q8(64, 2);
+  else if (p.width <= 2048)
+    ROW_Q8(64, 4);
+  else if (p.width <= 8192)
+    ROW_Q8(256, 4);
+  else
+    ROW_Q8(1024, 4);
+#undef ROW_Q8
+}
+
+}  // namespace
+
+hipError_t launch_row_q8(const RowQ8& p, bool bf16, hipStream_t stream) {
+  if (p.rows <= 0) return hipSuccess;
+  const int kind = p.weight ? (p.residual ? 2 : 1) : 0;
+  if (bf16)
+    kind == 2 ? launch<true, true, true>(p, stream) : kind == 1 ? launch<true, true, false>(p, stream) : launch<true, false, false>(p, stream);
+  else
+    kind == 2 ? launch<false, true, true>(p, stream) : kind == 1 ? launch<false, true, false>(p, stream) : launch<false, false, false>(p, stream);
+  return hipGetLastError();
+}
+
+}  // namespace qattn

@@ -229,6 +229,15 @@ def lib():
         "qattn_shared_run_get_info": (ctypes.c_int, [vp, ctypes.POINTER(SharedInfo)]),
         "qattn_shared_plan_describe": (ctypes.c_int, [ctypes.POINTER(SharedDesc), vp, i64, ctypes.POINTER(i64),
                                                       ctypes.POINTER(SharedInfo)]),
+        "qattn_quantize_q8": (ctypes.c_int, [vp, vp, i64, vp, i64, vp, i64, i32, i32, vp]),
+        "qattn_rmsnorm_q8": (ctypes.c_int, [vp, vp, i64, vp, i64, vp, i64, vp, vp, i64, vp, i64, i32, i32, ctypes.c_double,
+                                            vp]),
+        "qattn_w4_bytes": (i64, [i32, i32]),
+        "qattn_w4_pack": (ctypes.c_int, [vp, vp, vp, i32, i32, vp, i64]),
+        "qattn_w4_quantize": (ctypes.c_int, [vp, i64, i32, i32, vp, i64]),
+        "qattn_w4_from_q4": (ctypes.c_int, [vp, i64, i32, i32, vp, i64]),
+        "qattn_w4_matmul": (ctypes.c_int, [vp, vp, i64, vp, i32, i32, vp, i64, i32, vp, i64, i32, vp]),
+        "qattn_w4_matmul_swiglu": (ctypes.c_int, [vp, vp, i64, vp, i32, i32, vp, i64, i32, vp, i64, i32, vp]),
         "qattn_model_create": (ctypes.c_int, [vp, ctypes.POINTER(ModelDesc), pvp]),
         "qattn_model_destroy": (None, [vp]),
         "qattn_model_plan_create": (ctypes.c_int, [vp, i32, i32, pvp]),
@@ -342,6 +351,43 @@ def shared_plan(desc):
         out[name] = part if width == 1 else part.reshape(count, width)
         at += count * width
     return out, info
+
+
+def _w4_image(K, N):
+    size = lib().qattn_w4_bytes(K, N)
+    if size < 0:
+        raise QattnError(EINVAL, f"no 4-bit weight has K={K}, N={N}")
+    return np.zeros(size, np.uint8)
+
+
+def w4_pack(codes, groups, scales):
+    """The image of 4-bit weights from codes uint8 [N, K / 2] (even columns low), groups uint8 [N, K / 32]
+    (multiplier | zero << 4) and row scales f32 [N] (qattn_w4_pack)."""
+    codes, groups = np.ascontiguousarray(codes, np.uint8), np.ascontiguousarray(groups, np.uint8)
+    scales = np.ascontiguousarray(scales, np.float32)
+    N, K = codes.shape[0], 2 * codes.shape[1]
+    if groups.shape != (N, K // 32) or scales.shape != (N,):
+        raise ValueError(f"codes of {N} rows and {K} columns need groups {(N, K // 32)} and scales {(N,)}")
+    image = _w4_image(K, N)
+    _check(lib().qattn_w4_pack(_np_ptr(codes), _np_ptr(groups), _np_ptr(scales), K, N, _np_ptr(image), image.nbytes))
+    return image
+
+
+def w4_quantize(w):
+    """The image of float rows w [N, K] (qattn_w4_quantize)."""
+    w = np.ascontiguousarray(w, np.float32)
+    N, K = w.shape
+    image = _w4_image(K, N)
+    _check(lib().qattn_w4_quantize(_np_ptr(w), K, K, N, _np_ptr(image), image.nbytes))
+    return image
+
+
+def w4_from_q4(q4, K, N):
+    """The image of a q4_0-tile32-compact tensor, as bytes or an array (qattn_w4_from_q4)."""
+    q4 = np.frombuffer(q4, np.uint8) if isinstance(q4, (bytes, bytearray, memoryview)) else np.ascontiguousarray(q4)
+    image = _w4_image(K, N)
+    _check(lib().qattn_w4_from_q4(_np_ptr(q4), q4.nbytes, K, N, _np_ptr(image), image.nbytes))
+    return image
 
 
 def plan_slots(desc, max_slots=0):
@@ -681,6 +727,34 @@ class Context:
 
     def shared_run(self, desc):
         return SharedRun(self, desc)
+
+    def quantize_q8(self, x_ptr, codes_ptr, scales_ptr, rows, width, dtype=F16, x_row_stride=None, codes_row_stride=None,
+                    stream=None):
+        """Rows into 8-bit codes and a scale each (qattn_quantize_q8)."""
+        _check(lib().qattn_quantize_q8(self.handle, x_ptr, width if x_row_stride is None else x_row_stride, codes_ptr,
+                                       width if codes_row_stride is None else codes_row_stride, scales_ptr, rows, width,
+                                       dtype, stream), self.handle)
+
+    def rmsnorm_q8(self, x_ptr, weight_ptr, codes_ptr, scales_ptr, rows, width=HIDDEN, residual_ptr=None, sum_ptr=None,
+                   eps=1e-6, dtype=F16, x_row_stride=None, residual_row_stride=None, sum_row_stride=None,
+                   codes_row_stride=None, stream=None):
+        """Residual add (into sum) + RMSNorm as 8-bit codes and a scale for each row (qattn_rmsnorm_q8)."""
+        strides = [width if s is None else s for s in (x_row_stride, residual_row_stride, sum_row_stride, codes_row_stride)]
+        _check(lib().qattn_rmsnorm_q8(self.handle, x_ptr, strides[0], residual_ptr, strides[1], sum_ptr, strides[2],
+                                      weight_ptr, codes_ptr, strides[3], scales_ptr, rows, width, dtype, eps, stream),
+               self.handle)
+
+    def w4_matmul(self, x_ptr, x_scale_ptr, M, K, w_ptr, w_bytes, N, y_ptr, dtype=F16, ldx=None, ldy=None, stream=None):
+        """y = x W^T for 8-bit rows x [M, K] and a 4-bit weight image (qattn_w4_matmul)."""
+        _check(lib().qattn_w4_matmul(self.handle, x_ptr, K if ldx is None else ldx, x_scale_ptr, M, K, w_ptr, w_bytes, N,
+                                     y_ptr, N if ldy is None else ldy, dtype, stream), self.handle)
+
+    def w4_matmul_swiglu(self, x_ptr, x_scale_ptr, M, K, w_ptr, w_bytes, n_inter, y_ptr, dtype=F16, ldx=None, ldy=None,
+                         stream=None):
+        """y = swiglu(x W^T) for a [gate | up] weight image (qattn_w4_matmul_swiglu)."""
+        _check(lib().qattn_w4_matmul_swiglu(self.handle, x_ptr, K if ldx is None else ldx, x_scale_ptr, M, K, w_ptr,
+                                            w_bytes, n_inter, y_ptr, n_inter if ldy is None else ldy, dtype, stream),
+               self.handle)
 
     def model(self, token_embd, output_norm, layers, eps=1e-6, rope_theta=1e6, mask=MASK_PREFIX_LOCAL,
               prefix=176, window=432, flags=0):
