@@ -169,9 +169,317 @@ void launch_small(const W4Product& p, hipStream_t stream) {
                      stream, p, (int)blocks_m);
 }
 
+// ---- many rows: workgroup tiles of 32 MF rows and 64 NWN columns, 2 x NWN wavefronts of 16 MF x 64, K in steps of 64.
+// X comes by LDS-DMA, three steps ahead; every weight is taken apart once for the workgroup, into an LDS tile of
+// 8-bit weights.  G > 1: so many such groups of wavefronts share K and add up in LDS.
+//
+// LDS tiles have rows of 64 bytes; the four 16-byte pieces of row r lie at c ^ ((r >> 2) & 3), so that 16 rows
+// reading one piece cover all banks.
+//
+// Step kb (X tile and weight tile kb in LDS, the first half's fragments in registers): half 1 reads the other row
+// fragments, takes weights kb + 1 apart into the free weight tile and runs the first half's products; the barrier
+// publishes that tile and X tile kb + 1; half 2 reads the next step's fragments under the other half's products.
+// X tile kb + 3 goes into the buffer that tile kb - 1 left at the previous barrier.
+__device__ inline uint32_t lds_off(int row, int piece) { return row * 64 + ((piece ^ ((row >> 2) & 3)) << 4); }
+
+typedef __attribute__((address_space(3))) void lds_void_t;
+__device__ inline void dma16(__amdgpu_buffer_rsrc_t rs, char* dst, uint32_t off) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t*)dst, 16, off, 0, 0, 0);
+}
+__device__ inline i32x4 load16s(__amdgpu_buffer_rsrc_t rs, uint32_t off, uint32_t soff) {
+  return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, off, soff, 0));
+}
+__device__ inline uint32_t load1s(__amdgpu_buffer_rsrc_t rs, uint32_t off, uint32_t soff) {
+  return __builtin_amdgcn_raw_buffer_load_b8(rs, off, soff, 0);
+}
+__device__ inline void store16(u32x4 v, __amdgpu_buffer_rsrc_t rs, uint32_t off) {
+  __builtin_amdgcn_raw_buffer_store_b128(v, rs, off, 0, 0);
+}
+__device__ inline void store2(uint16_t v, __amdgpu_buffer_rsrc_t rs, uint32_t off) {
+  __builtin_amdgcn_raw_buffer_store_b16(v, rs, off, 0, 0);
+}
+// Waits for all but the newest V vector-memory operations and for all LDS operations of this wavefront, then meets
+// the workgroup.  One block of its own: the compiler's barrier would wait for every LDS-DMA load in flight.
+template <int V>
+__device__ inline void barrier_but() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(V) : "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+template <bool BF16, bool SWIGLU, int MF, int NWN, int G>
+__global__ __launch_bounds__(128 * NWN * G, 2) void w4_tile_kernel(W4Product p, int tiles_n, int tiles_total, int per_xcd) {
+  constexpr int kWaves = 2 * NWN;  // per group
+  constexpr int kTileM = 32 * MF, kTileN = 64 * NWN;
+  constexpr int kBytesA = kTileM * 64, kBytesB = kTileN * 64;
+  constexpr int AJ = MF / NWN;                  // X loads per wavefront and step
+  constexpr int A1 = AJ / 2, A2 = AJ - A1;      // ... in the first / second half step
+  constexpr int H = MF / 2;                     // row fragments per half step
+  __shared__ __attribute__((aligned(1024))) char sA0[G * kBytesA];
+  __shared__ __attribute__((aligned(1024))) char sA1[G * kBytesA];
+  __shared__ __attribute__((aligned(1024))) char sA2[G * kBytesA];
+  __shared__ __attribute__((aligned(1024))) char sA3[G * kBytesA];
+  __shared__ __attribute__((aligned(1024))) char sB0[G * kBytesB];
+  __shared__ __attribute__((aligned(1024))) char sB1[G * kBytesB];
+
+  // Consecutive workgroups of an XCD (workgroup b runs on XCD b % 8) walk the column tiles of one row tile: its X
+  // rows stay in that XCD's L2.
+  const int u = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+  if (u >= tiles_total) return;
+  const int64_t m0 = (int64_t)(u / tiles_n) * kTileM;
+  const int n0 = (u % tiles_n) * kTileN;
+  const int gwave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int grp = G == 1 ? 0 : gwave / kWaves, wave = G == 1 ? gwave : gwave % kWaves;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, kq = lane >> 4;
+  const int wr = 16 * MF * (wave & 1), wc = 64 * (wave >> 1);
+  const W4Layout at(p.K, p.N);
+  const int blocks = (int)at.blocks;
+  // Steps of this group; K is padded to whole blocks of two steps.
+  const int steps_all = 2 * blocks, share = (steps_all + G - 1) / G;
+  const int step0 = grp * share;
+  const int steps = G == 1 ? steps_all : __builtin_amdgcn_readfirstlane(max(0, min(share, steps_all - step0)));
+
+  // X rows of the tile.  A range starts at its step's first column and ends with the last row's K columns, so that
+  // a load past either reads zeros; what it reads past a row's end inside the tensor meets zero weights.
+  const int rows = (int)(p.M - m0 < kTileM ? p.M - m0 : kTileM);
+  const int8_t* const x0 = p.x + m0 * p.ldx;
+  const int x_bytes = (rows - 1) * (int)p.ldx + p.K;  // below 2^30
+  uint32_t a_src[AJ];
+#pragma unroll
+  for (int j = 0; j < AJ; ++j) {
+    const int row = 16 * (AJ * wave + j) + (lane >> 2);
+    a_src[j] = (uint32_t)row * (uint32_t)p.ldx + 16u * ((lane & 3) ^ ((row >> 2) & 3));
+  }
+  const uint32_t a_dst = grp * kBytesA + 1024 * AJ * wave;
+  auto load_a = [&](char* dst, int kb, int j0, int n) W4_INLINE {
+    const int first = 64 * (step0 + kb);
+    // In a scalar register (the compiler's saturating difference is a vector one, and would be looped over).
+    const int left = __builtin_amdgcn_readfirstlane(kb < steps ? max(x_bytes - first, 0) : 0);
+    const auto rs = rsrc(x0 + first, (uint32_t)left);
+#pragma unroll
+    for (int j = j0; j < j0 + n; ++j) dma16(rs, dst + a_dst + 1024 * j, a_src[j]);
+  };
+  // Thread (row = tid / 2, half = tid & 1) takes the record of group 2 kb + half of its weight row apart: columns 0-15
+  // (piece 2 half) and 16-31 (piece 2 half + 1) of 32 half.  A wavefront's 32 rows are two tiles of the image.
+  // SWIGLU: of each 64 rows 32 are the gate's of 32 features, then the up projection's.
+  const int first_tile = (SWIGLU ? (wave & 1 ? p.N >> 5 : 0) + ((n0 + 32 * (wave & ~1)) >> 5) : (n0 + 32 * wave) >> 4);
+  const int my_tiles = __builtin_amdgcn_readfirstlane(max(0, min(2, (int)at.tiles - first_tile)));
+  const uint8_t* const codes = p.w + (int64_t)first_tile * blocks * 1024;
+  const uint8_t* const groups = p.w + at.groups_at() + (int64_t)first_tile * blocks * 64;
+  const int brow = 32 * wave + (lane >> 1), half = lane & 1;
+  const uint32_t w_rec = (uint32_t)(lane >> 5) * (uint32_t)blocks * 1024u + 256u * half + 16u * ((lane >> 1) & 15);
+  const uint32_t w_grp = (uint32_t)(lane >> 5) * (uint32_t)blocks * 64u + 4u * ((lane >> 1) & 15) + half;
+  const uint32_t b_lo = grp * kBytesB + lds_off(brow, 2 * half), b_hi = grp * kBytesB + lds_off(brow, 2 * half + 1);
+  struct WRegs {
+    i32x4 record;
+    uint32_t group;
+  };
+  auto load_wg = [&](WRegs& r, int kb) W4_INLINE {
+    const uint32_t k = (uint32_t)(step0 + kb);
+    r.group = load1s(rsrc(groups, kb < steps ? (uint32_t)my_tiles * (uint32_t)blocks * 64u : 0u), w_grp, (k >> 1) * 64u + 2u * (k & 1u));
+  };
+  auto load_wr = [&](WRegs& r, int kb) W4_INLINE {
+    r.record = load16s(rsrc(codes, kb < steps ? (uint32_t)my_tiles * (uint32_t)blocks * 1024u : 0u), w_rec, (uint32_t)(step0 + kb) * 512u);
+  };
+  auto store_b = [&](char* dst, const WRegs& r) W4_INLINE {
+    const Group g = group_of(r.group);
+    *reinterpret_cast<i32x4*>(dst + b_lo) = weights16<0>(r.record, g);
+    *reinterpret_cast<i32x4*>(dst + b_hi) = weights16<1>(r.record, g);
+  };
+  i32x4 acc[MF][4];
+#pragma unroll
+  for (int mb = 0; mb < MF; ++mb)
+#pragma unroll
+    for (int nb = 0; nb < 4; ++nb) acc[mb][nb] = i32x4{};
+  const uint32_t a_rd = grp * kBytesA + lds_off(wr + l16, kq), b_rd = grp * kBytesB + lds_off(wc + l16, kq);
+
+  WRegs wreg[4];
+  i32x4 a_lo[H], a_hi[H], b0[4], b1[4];
+  auto read_a = [&](i32x4 (&f)[H], const char* q) W4_INLINE {
+#pragma unroll
+    for (int i = 0; i < H; ++i) f[i] = *reinterpret_cast<const i32x4*>(q + 1024 * i);
+  };
+  auto read_b = [&](i32x4 (&f)[4], const char* q) W4_INLINE {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = *reinterpret_cast<const i32x4*>(q + 1024 * i);
+  };
+  auto mma = [&](const i32x4 (&b)[4], const i32x4 (&a)[H], int m8) W4_INLINE {
+#pragma unroll
+    for (int mb = 0; mb < H; ++mb)
+#pragma unroll
+      for (int nb = 0; nb < 4; ++nb) acc[m8 + mb][nb] = mfma(b[nb], a[mb], acc[m8 + mb][nb]);
+  };
+  // The tile's scales, the oldest loads of all: a row's and a column's to a thread, shared out at the end.
+  const int tid = threadIdx.x;
+  float my_xs = 0.f, my_ws = 0.f;
+  if (tid < rows) my_xs = p.x_scale[m0 + tid];
+  if (tid < kTileN) {
+    const int64_t n = SWIGLU ? (tid >> 5 & 1 ? p.N >> 1 : 0) + (n0 >> 1) + 32 * (tid >> 6) + (tid & 31) : n0 + tid;
+    if (n < 16 * at.tiles) my_ws = reinterpret_cast<const float*>(p.w + at.scales_at())[n];
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  load_wg(wreg[0], 0);
+  load_wr(wreg[0], 0);
+  load_a(sA0, 0, 0, AJ);
+  __builtin_amdgcn_sched_barrier(0);
+  load_wg(wreg[1], 1);
+  load_a(sA1, 1, 0, AJ);
+  __builtin_amdgcn_sched_barrier(0);
+  load_wr(wreg[1], 1);
+  load_wg(wreg[2], 2);
+  load_a(sA2, 2, 0, AJ);
+  __builtin_amdgcn_sched_barrier(0);
+  load_wr(wreg[2], 2);
+  store_b(sB0, wreg[0]);
+  barrier_but<4 + 2 * AJ>();  // X tile 0: newer are the weights and X of 1 and 2
+  read_b(b0, sB0 + b_rd);
+  read_a(a_lo, sA0 + a_rd);
+  auto step = [&](const char* a_cur, const char* a_nxt, char* a_new, char* b_nxt, i32x4 (&b_cur)[4], i32x4 (&b_new)[4],
+                  const WRegs& w_use, WRegs& w_new, int kb) W4_INLINE {
+    read_a(a_hi, a_cur + a_rd + 1024 * H);
+    load_wg(w_new, kb + 3);
+    load_a(a_new, kb + 3, 0, A1);
+    store_b(b_nxt, w_use);
+    mma(b_cur, a_lo, 0);
+    // X tile kb + 1: newer are at least step kb - 1's AJ + 2 loads and this half's 1 + A1.
+    barrier_but<3 + AJ + A1>();
+    read_b(b_new, b_nxt + b_rd);
+    read_a(a_lo, a_nxt + a_rd);
+    load_a(a_new, kb + 3, A1, A2);
+    load_wr(w_new, kb + 3);
+    mma(b_cur, a_hi, H);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+#pragma unroll 1
+  for (int kb = 0; kb < (G == 1 ? steps_all : share); kb += 4) {  // steps past the end add zero products
+    step(sA0, sA1, sA3, sB1, b0, b1, wreg[1], wreg[3], kb);
+    step(sA1, sA2, sA0, sB0, b1, b0, wreg[2], wreg[0], kb + 1);
+    step(sA2, sA3, sA1, sB1, b0, b1, wreg[3], wreg[1], kb + 2);
+    step(sA3, sA0, sA2, sB0, b1, b0, wreg[0], wreg[2], kb + 3);
+  }
+  barrier_but<0>();
+
+  // G = 2: group g finishes the rows of half g of every wavefront's tile.
+  if constexpr (G == 2) {
+    char* const ex = (wave == 0 ? sA0 : wave == 1 ? sA1 : wave == 2 ? sA2 : sA3) + 16 * lane;
+    auto send = [&](int m8, char* q) W4_INLINE {
+#pragma unroll
+      for (int mb = 0; mb < H; ++mb)
+#pragma unroll
+        for (int nb = 0; nb < 4; ++nb) *reinterpret_cast<i32x4*>(q + 1024 * (4 * mb + nb)) = acc[m8 + mb][nb];
+    };
+    auto take = [&](int m8, const char* q) W4_INLINE {
+#pragma unroll
+      for (int mb = 0; mb < H; ++mb)
+#pragma unroll
+        for (int nb = 0; nb < 4; ++nb) acc[mb][nb] = acc[m8 + mb][nb] + *reinterpret_cast<const i32x4*>(q + 1024 * (4 * mb + nb));
+    };
+    static_assert(G != 2 || (kWaves == 4 && 2 * kBytesA >= 2 * 4096 * H), "a wavefront's two halves fill an X buffer");
+    if (grp == 0)
+      send(H, ex);
+    else
+      send(0, ex + 4096 * H);
+    __syncthreads();
+    if (grp == 0)
+      take(0, ex + 4096 * H);
+    else
+      take(H, ex);
+    __syncthreads();
+  }
+
+  // Output through LDS, kRows rows of a wavefront at a time: stores of 16 bytes in whole 128-byte lines.  Lane (l16,
+  // kq) holds row 16 mb + l16, columns 16 nb + 4 kq .. + 3.
+  constexpr int kMine = G > 1 ? H : MF;  // row fragments this wavefront finishes
+  constexpr int kHold = 4 * G * kBytesA / 128 / (kWaves * G);
+  constexpr int kMost = kHold < 64 ? kHold : 64;
+  constexpr int kRows = 16 * kMine < kMost ? 16 * kMine : kMost;
+  constexpr int kPer = G * kBytesA / (128 * kRows);  // wavefronts per X buffer
+  static_assert(4 * kPer >= kWaves * G && 16 * kMine % kRows == 0 && kRows % 16 == 0, "a stage per writer, whole fragments");
+  const int slot = gwave / kPer;
+  char* const stage = (slot == 0 ? sA0 : slot == 1 ? sA1 : slot == 2 ? sA2 : sA3) + 128 * kRows * (gwave % kPer);
+  const int n_out = SWIGLU ? p.N >> 1 : p.N;
+  const int row0 = wr + 16 * kMine * grp, col0 = SWIGLU ? (n0 + wc) >> 1 : n0 + wc;
+  const auto yrs = rsrc(static_cast<uint16_t*>(p.y) + m0 * p.ldy, ((uint32_t)(rows - 1) * (uint32_t)p.ldy + (uint32_t)n_out) * 2u);
+  constexpr uint32_t kNowhere = 0x80000000u;  // past every range: 256 rows of at most 2^22 elements
+  constexpr int kPieces = SWIGLU ? 4 : 8;     // 16-byte pieces of a row
+  auto place = [&](int row, int c) W4_INLINE {
+    return stage + row * (16 * kPieces) + ((SWIGLU ? c ^ ((row >> 2) & 3) : c ^ ((row >> 1) & 7)) << 4);
+  };
+  // The weight tiles are free: the scales' place.
+  float *const sXs = reinterpret_cast<float*>(sB0), *const sWs = reinterpret_cast<float*>(sB1);
+  static_assert(128 * NWN * G >= kTileM && 128 * NWN * G >= kTileN && G * kBytesB >= 4 * kTileM, "a thread and a place for every scale");
+  if (tid < kTileM) sXs[tid] = my_xs;
+  if (tid < kTileN) sWs[tid] = my_ws;
+  __syncthreads();
+  float4 ws[4];
+#pragma unroll
+  for (int nb = 0; nb < 4; ++nb) ws[nb] = *reinterpret_cast<const float4*>(sWs + wc + 16 * nb + 4 * kq);
+#pragma unroll
+  for (int pass = 0; pass < 16 * kMine / kRows; ++pass) {
+#pragma unroll
+    for (int mb = 0; mb < kRows / 16; ++mb) {
+      const i32x4(&v)[4] = acc[pass * (kRows / 16) + mb];
+      const int row = 16 * mb + l16;
+      const float xs = sXs[row0 + kRows * pass + row];
+      auto scaled = [&](int nb, float (&f)[4]) W4_INLINE {
+        const float s[4] = {ws[nb].x, ws[nb].y, ws[nb].z, ws[nb].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = (float)v[nb][e] * s[e] * xs;
+      };
+#pragma unroll
+      for (int nb = 0; nb < (SWIGLU ? 2 : 4); ++nb) {
+        float f[4];
+        scaled(nb, f);
+        if constexpr (SWIGLU) {  // columns 0-31: gate, 32-63: up, of the same 32 features
+          float t[4];
+          scaled(nb + 2, t);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) f[e] = swiglu(f[e], t[e]);
+        }
+        *reinterpret_cast<u32x2*>(place(row, 2 * nb + (kq >> 1)) + 8 * (kq & 1)) = u32x2{narrow2<BF16>(f[0], f[1]), narrow2<BF16>(f[2], f[3])};
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    constexpr int kRowsPer = 64 / kPieces;  // rows per store instruction
+#pragma unroll
+    for (int i = 0; i < kRows / kRowsPer; ++i) {
+      const int row = kRowsPer * i + lane / kPieces, c = lane % kPieces;
+      const u32x4 v = *reinterpret_cast<const u32x4*>(place(row, c));
+      const int m = row0 + kRows * pass + row, n = col0 + 8 * c;
+      store16(v, yrs, m < rows && n + 8 <= n_out ? ((uint32_t)m * (uint32_t)p.ldy + (uint32_t)n) * 2u : kNowhere);
+    }
+    // A last piece of fewer than 8 columns goes element by element.
+    const int part = (n_out - col0) >> 3;
+    if ((n_out & 7) && n_out > col0 && part < kPieces) {
+#pragma unroll 1
+      for (int i = 0; i < kRows / 8; ++i) {
+        const int row = 8 * i + (lane >> 3), m = row0 + kRows * pass + row, n = col0 + 8 * part + (lane & 7);
+        const uint16_t v = *reinterpret_cast<const uint16_t*>(place(row, part) + 2 * (lane & 7));
+        store2(v, yrs, m < rows && n < n_out ? ((uint32_t)m * (uint32_t)p.ldy + (uint32_t)n) * 2u : kNowhere);
+      }
+    }
+  }
+}
+
+template <bool BF16, bool SWIGLU, int MF, int NWN, int G>
+void launch_tile(const W4Product& p, hipStream_t stream) {
+  const int64_t tiles_m = ((int64_t)p.M + 32 * MF - 1) / (32 * MF), tiles_n = ((int64_t)p.N + 64 * NWN - 1) / (64 * NWN);
+  const int64_t tiles = tiles_m * tiles_n, per_xcd = (tiles + 7) / 8;
+  hipLaunchKernelGGL((w4_tile_kernel<BF16, SWIGLU, MF, NWN, G>), dim3((unsigned)(8 * per_xcd)), dim3(128 * NWN * G), 0, stream, p,
+                     (int)tiles_n, (int)tiles, (int)per_xcd);
+}
+
 template <bool BF16, bool SWIGLU>
 hipError_t launch(const W4Product& p, hipStream_t stream) {
-  launch_small<BF16, SWIGLU, 2, 2, 4>(p, stream);
+  const auto tiles = [&](int tm, int tn) { return (((int64_t)p.M + tm - 1) / tm) * (((int64_t)p.N + tn - 1) / tn); };
+  if (tiles(128, 128) <= 64 || p.M <= 128)
+    launch_small<BF16, SWIGLU, 2, 2, 4>(p, stream);
+  else if (tiles(128, 128) <= 256)
+    launch_tile<BF16, SWIGLU, 4, 2, 2>(p, stream);
+  else if (tiles(256, 256) <= 256)
+    launch_tile<BF16, SWIGLU, 8, 2, 1>(p, stream);
+  else
+    launch_tile<BF16, SWIGLU, 8, 4, 1>(p, stream);
   return hipGetLastError();
 }
 
