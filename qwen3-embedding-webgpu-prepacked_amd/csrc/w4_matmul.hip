@@ -32,6 +32,7 @@ __device__ inline __amdgpu_buffer_rsrc_t rsrc(const void* base, uint32_t bytes) 
 __device__ inline i32x4 load16(__amdgpu_buffer_rsrc_t rs, uint32_t off) {
   return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, off, 0, 0));
 }
+__device__ inline uint32_t load1(__amdgpu_buffer_rsrc_t rs, uint32_t off) { return __builtin_amdgcn_raw_buffer_load_b8(rs, off, 0, 0); }
 __device__ inline i32x4 mfma(i32x4 a, i32x4 b, i32x4 c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
 
 // A group's multiplier in both halves of a dword, and 128 - zero * multiplier in its four bytes.
@@ -40,7 +41,7 @@ struct Group {
 };
 __device__ inline Group group_of(uint32_t byte) {
   const uint32_t m = byte & 15u, z = byte >> 4 & 15u;
-  return {m * 0x00010001u, (128u - m * z) * 0x01010101u};
+  return {__builtin_amdgcn_perm(0, m, 0x0C000C00u), __builtin_amdgcn_perm(0, 128u - m * z, 0u)};
 }
 __device__ inline uint32_t weights4(uint32_t nibbles, Group g) {
   const u16x2 v = __builtin_bit_cast(u16x2, nibbles) * __builtin_bit_cast(u16x2, g.mult) + __builtin_bit_cast(u16x2, g.bias);
@@ -60,11 +61,12 @@ __device__ inline float swiglu(float g, float u) {
   return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.44269504f)) * u;
 }
 
-// ---- few rows: a workgroup to 16 MB rows and 16 NB columns (SwiGLU: 8 NB features), its W wavefronts take the
-// blocks of 128 columns of K in turn and add up in LDS.  No operand is staged: a lane's 16 bytes of codes are two
-// fragments, and its 32 bytes of x the two that meet them.
-template <bool BF16, bool SWIGLU, int MB, int NB, int W>
+// ---- few rows: a workgroup to 16 MB rows and 16 NB columns (SwiGLU: 8 NB features), whose W wavefronts take the
+// blocks of 128 columns of K in turn, U of them in flight, and add up in LDS.  No operand is staged: a lane's 16
+// bytes of codes are two fragments, and its 32 bytes of x the two that meet them.
+template <bool BF16, bool SWIGLU, int MB, int NB, int W, int U>
 __global__ __launch_bounds__(64 * W) void w4_small_kernel(W4Product p, int blocks_m) {
+  static_assert(!SWIGLU || NB % 2 == 0, "as many gate tiles as up tiles");
   __shared__ i32x4 part[W > 1 ? W - 1 : 1][MB * NB][64];
   const int lane = threadIdx.x & 63, l16 = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -72,17 +74,17 @@ __global__ __launch_bounds__(64 * W) void w4_small_kernel(W4Product p, int block
   const int nblk = (int)(blockIdx.x / (unsigned)blocks_m);
   const W4Layout at(p.K, p.N);
   const int blocks = (int)at.blocks;
-  // Tiles of 16 weight rows: the gate's, then the up projection's.
+  // Tiles of 16 weight rows (SwiGLU: the gate's, then the up projection's); those past the last read as zeros, and so
+  // do blocks past K: a group byte of zero makes weights of zero.
   const int tile0 = SWIGLU ? NB / 2 * nblk : NB * nblk;
-  const int last = (int)at.tiles - 1;
-  const uint8_t *codes[NB], *groups[NB];
+  __amdgpu_buffer_rsrc_t codes[NB], groups[NB];
   int tile[NB];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     tile[nb] = SWIGLU ? tile0 + nb % (NB / 2) + (nb < NB / 2 ? 0 : p.N >> 5) : tile0 + nb;
-    const int t = tile[nb] < last ? tile[nb] : last;  // past the last tile: read it again, store nothing
-    codes[nb] = p.w + (int64_t)t * blocks * 1024;
-    groups[nb] = p.w + at.groups_at() + (int64_t)t * blocks * 64;
+    const bool here = tile[nb] < at.tiles;
+    codes[nb] = rsrc(p.w + (int64_t)tile[nb] * blocks * 1024, here ? (uint32_t)blocks * 1024u : 0u);
+    groups[nb] = rsrc(p.w + at.groups_at() + (int64_t)tile[nb] * blocks * 64, here ? (uint32_t)blocks * 64u : 0u);
   }
   // Rows past M and what lies behind the last row's K columns read as zeros; columns of K's padding meet zero weights.
   const int rows = (int)(p.M - m0 < 16 * MB ? p.M - m0 : 16 * MB);
@@ -91,27 +93,53 @@ __global__ __launch_bounds__(64 * W) void w4_small_kernel(W4Product p, int block
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) x_off[mb] = (uint32_t)(16 * mb + l16) * (uint32_t)p.ldx + 32u * q;
 
+  struct Stage {
+    i32x4 x[MB][2], record[NB];
+    uint32_t group[NB];
+  };
+  auto load = [&](Stage& st, int kb) W4_INLINE {
+    const uint32_t k = (uint32_t)kb;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      st.record[nb] = load16(codes[nb], 1024u * k + 16u * lane);
+      st.group[nb] = load1(groups[nb], 64u * k + 4u * l16 + q);
+    }
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+      st.x[mb][0] = load16(xs, x_off[mb] + 128u * k);
+      st.x[mb][1] = load16(xs, x_off[mb] + 128u * k + 16u);
+    }
+  };
   i32x4 acc[NB][MB];
 #pragma unroll
   for (int i = 0; i < NB * MB; ++i) acc[i / MB][i % MB] = i32x4{};
-  for (int kb = wave; kb < blocks; kb += W) {
-    i32x4 x[MB][2];
-#pragma unroll
-    for (int mb = 0; mb < MB; ++mb) {
-      x[mb][0] = load16(xs, x_off[mb] + 128u * kb);
-      x[mb][1] = load16(xs, x_off[mb] + 128u * kb + 16u);
-    }
+  auto multiply = [&](const Stage& st) W4_INLINE {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const i32x4 record = *reinterpret_cast<const i32x4*>(codes[nb] + (int64_t)kb * 1024 + 16 * lane);
-      const uint32_t four = *reinterpret_cast<const uint32_t*>(groups[nb] + (int64_t)kb * 64 + 4 * l16);
-      const Group g = group_of(four >> (8 * q));
-      const i32x4 lo = weights16<0>(record, g), hi = weights16<1>(record, g);
+      const Group g = group_of(st.group[nb]);
+      const i32x4 lo = weights16<0>(st.record[nb], g), hi = weights16<1>(st.record[nb], g);
 #pragma unroll
-      for (int mb = 0; mb < MB; ++mb) {
-        acc[nb][mb] = mfma(lo, x[mb][0], acc[nb][mb]);
-        acc[nb][mb] = mfma(hi, x[mb][1], acc[nb][mb]);
-      }
+      for (int mb = 0; mb < MB; ++mb) acc[nb][mb] = mfma(lo, st.x[mb][0], acc[nb][mb]);
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) acc[nb][mb] = mfma(hi, st.x[mb][1], acc[nb][mb]);
+    }
+  };
+  Stage ring[U];
+#pragma unroll
+  for (int i = 0; i < U; ++i) load(ring[i], wave + W * i);
+  // The scales of lane (l16, q): row l16, columns 4 q .. 4 q + 3 of a 16 x 16 block.
+  float x_scale[MB];
+  float4 w_scale[NB];
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) x_scale[mb] = 16 * mb + l16 < rows ? p.x_scale[m0 + 16 * mb + l16] : 0.f;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+    w_scale[nb] = tile[nb] < at.tiles ? reinterpret_cast<const float4*>(p.w + at.scales_at())[4 * tile[nb] + q] : float4{};
+  for (int kb = wave; kb < blocks; kb += W * U) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      multiply(ring[i]);
+      if (kb + W * U < blocks) load(ring[i], kb + W * (U + i));
     }
   }
   if constexpr (W > 1) {
@@ -125,29 +153,27 @@ __global__ __launch_bounds__(64 * W) void w4_small_kernel(W4Product p, int block
 #pragma unroll
       for (int i = 0; i < NB * MB; ++i) acc[i / MB][i % MB] += part[w][i][lane];
   }
-  // Lane (l16, q) holds row l16 and columns 4 q .. 4 q + 3 of a 16 x 16 block.
-  const float* const w_scale = reinterpret_cast<const float*>(p.w + at.scales_at());
   const int n_out = SWIGLU ? p.N >> 1 : p.N;
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) {
-    const int64_t m = m0 + 16 * mb + l16;
-    if (m >= p.M) continue;
-    const float xscale = p.x_scale[m];
-    uint16_t* const y = static_cast<uint16_t*>(p.y) + m * p.ldy;
+    if (16 * mb + l16 >= rows) continue;
+    uint16_t* const y = static_cast<uint16_t*>(p.y) + (m0 + 16 * mb + l16) * p.ldy;
 #pragma unroll
     for (int nb = 0; nb < (SWIGLU ? NB / 2 : NB); ++nb) {
       const int n = 16 * (tile0 + nb) + 4 * q;
       if (n >= n_out) continue;
-      const float4 s = *reinterpret_cast<const float4*>(w_scale + 16 * tile[nb] + 4 * q);
-      const float sn[4] = {s.x, s.y, s.z, s.w};
+      auto scaled = [&](int b, float (&f)[4]) W4_INLINE {
+        const float s[4] = {w_scale[b].x, w_scale[b].y, w_scale[b].z, w_scale[b].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = (float)acc[b][mb][e] * s[e] * x_scale[mb];
+      };
       float v[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = (float)acc[nb][mb][e] * sn[e] * xscale;
+      scaled(nb, v);
       if constexpr (SWIGLU) {
-        const float4 t = *reinterpret_cast<const float4*>(w_scale + 16 * tile[nb + NB / 2] + 4 * q);
-        const float tn[4] = {t.x, t.y, t.z, t.w};
+        float t[4];
+        scaled(nb + NB / 2, t);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = swiglu(v[e], (float)acc[nb + NB / 2][mb][e] * tn[e] * xscale);
+        for (int e = 0; e < 4; ++e) v[e] = swiglu(v[e], t[e]);
       }
       const u32x2 d = {narrow2<BF16>(v[0], v[1]), narrow2<BF16>(v[2], v[3])};
       if (n + 4 <= n_out) {
@@ -161,26 +187,16 @@ __global__ __launch_bounds__(64 * W) void w4_small_kernel(W4Product p, int block
   }
 }
 
-template <bool BF16, bool SWIGLU, int MB, int NB, int W>
+template <bool BF16, bool SWIGLU, int MB, int NB, int W, int U>
 void launch_small(const W4Product& p, hipStream_t stream) {
-  const int64_t blocks_m = (p.M + 16 * MB - 1) / (16 * MB), tiles = W4Layout(p.K, SWIGLU ? p.N / 2 : p.N).tiles;
+  static_assert(!SWIGLU || NB % 2 == 0, "as many gate tiles as up tiles");
+  const int64_t blocks_m = ((int64_t)p.M + 16 * MB - 1) / (16 * MB), tiles = W4Layout(p.K, SWIGLU ? p.N / 2 : p.N).tiles;
   const int64_t per = SWIGLU ? NB / 2 : NB, blocks_n = (tiles + per - 1) / per;
-  hipLaunchKernelGGL((w4_small_kernel<BF16, SWIGLU, MB, NB, W>), dim3((unsigned)(blocks_m * blocks_n)), dim3(64 * W), 0,
+  hipLaunchKernelGGL((w4_small_kernel<BF16, SWIGLU, MB, NB, W, U>), dim3((unsigned)(blocks_m * blocks_n)), dim3(64 * W), 0,
                      stream, p, (int)blocks_m);
 }
 
-// ---- many rows: workgroup tiles of 32 MF rows and 64 NWN columns, 2 x NWN wavefronts of 16 MF x 64, K in steps of 64.
-// X comes by LDS-DMA, three steps ahead; every weight is taken apart once for the workgroup, into an LDS tile of
-// 8-bit weights.  G > 1: so many such groups of wavefronts share K and add up in LDS.
-//
-// LDS tiles have rows of 64 bytes; the four 16-byte pieces of row r lie at c ^ ((r >> 2) & 3), so that 16 rows
-// reading one piece cover all banks.
-//
-// Step kb (X tile and weight tile kb in LDS, the first half's fragments in registers): half 1 reads the other row
-// fragments, takes weights kb + 1 apart into the free weight tile and runs the first half's products; the barrier
-// publishes that tile and X tile kb + 1; half 2 reads the next step's fragments under the other half's products.
-// X tile kb + 3 goes into the buffer that tile kb - 1 left at the previous barrier.
-__device__ inline uint32_t lds_off(int row, int piece) { return row * 64 + ((piece ^ ((row >> 2) & 3)) << 4); }
+constexpr uint32_t kNowhere = 0x80000000u;  // past every range of a tile: 256 rows of at most 2^22 elements
 
 typedef __attribute__((address_space(3))) void lds_void_t;
 __device__ inline void dma16(__amdgpu_buffer_rsrc_t rs, char* dst, uint32_t off) {
@@ -207,20 +223,244 @@ __device__ inline void barrier_but() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-template <bool BF16, bool SWIGLU, int MF, int NWN, int G>
-__global__ __launch_bounds__(128 * NWN * G, 2) void w4_tile_kernel(W4Product p, int tiles_n, int tiles_total, int per_xcd) {
-  constexpr int kWaves = 2 * NWN;  // per group
+
+// ---- in between: workgroup tiles of 16 MF rows and 128 columns, groups of four wavefronts of 16 MF x 32, K in blocks
+// of 128.  X comes by LDS-DMA, three blocks ahead; each wavefront takes its own weights apart, straight into
+// fragments.  G groups share K and add up in LDS.
+//
+// LDS rows of X have 128 bytes; the eight 16-byte pieces of row r lie at c ^ ((r >> 1) & 7), so that 16 rows reading
+// one piece cover all banks.
+template <bool BF16, bool SWIGLU, int MF, int G>
+__global__ __launch_bounds__(256 * G, 2) void w4_mid_kernel(W4Product p, int tiles_n, int tiles_total, int per_xcd) {
+  constexpr int kTileM = 16 * MF, kStage = kTileM * 128, XJ = MF / 2;  // X loads per wavefront and block
+  __shared__ __attribute__((aligned(1024))) char sX0[G * kStage];
+  __shared__ __attribute__((aligned(1024))) char sX1[G * kStage];
+  __shared__ __attribute__((aligned(1024))) char sX2[G * kStage];
+  __shared__ __attribute__((aligned(1024))) char sX3[G * kStage];
+
+  const int u = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+  if (u >= tiles_total) return;
+  const int64_t m0 = (int64_t)(u / tiles_n) * kTileM;
+  const int n0 = (u % tiles_n) * 128;
+  const int gwave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int grp = gwave >> 2, wave = gwave & 3;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, q = lane >> 4;
+  const W4Layout at(p.K, p.N);
+  const int blocks = (int)at.blocks, share = (blocks + G - 1) / G;
+  const int block0 = grp * share;
+  const int mine = G == 1 ? blocks : __builtin_amdgcn_readfirstlane(max(0, min(share, blocks - block0)));
+
+  // A block's range starts at its first column and ends with the last row's K columns.
+  const int rows = (int)(p.M - m0 < kTileM ? p.M - m0 : kTileM);
+  const int8_t* const x0 = p.x + m0 * p.ldx;
+  const int x_bytes = (rows - 1) * (int)p.ldx + p.K;
+  uint32_t x_src[XJ];
+#pragma unroll
+  for (int j = 0; j < XJ; ++j) {
+    const int row = 8 * (XJ * wave + j) + (lane >> 3);
+    x_src[j] = (uint32_t)row * (uint32_t)p.ldx + 16u * ((lane & 7) ^ ((row >> 1) & 7));
+  }
+  const uint32_t x_dst = grp * kStage + 1024 * XJ * wave;
+  auto load_x = [&](char* dst, int kb) W4_INLINE {
+    const int first = 128 * (block0 + kb);
+    const int left = __builtin_amdgcn_readfirstlane(kb < mine ? max(x_bytes - first, 0) : 0);
+    const auto rs = rsrc(x0 + first, (uint32_t)left);
+#pragma unroll
+    for (int j = 0; j < XJ; ++j) dma16(rs, dst + x_dst + 1024 * j, x_src[j]);
+  };
+  // The wavefront's two tiles of 16 weight rows (SwiGLU: of the gate and the up projection).
+  const int tile0 = SWIGLU ? (n0 >> 5) + wave : (n0 >> 4) + 2 * wave, tile1 = SWIGLU ? tile0 + (p.N >> 5) : tile0 + 1;
+  const uint8_t *const codes0 = p.w + (int64_t)tile0 * blocks * 1024, *const codes1 = p.w + (int64_t)tile1 * blocks * 1024;
+  const uint8_t *const groups0 = p.w + at.groups_at() + (int64_t)tile0 * blocks * 64, *const groups1 = p.w + at.groups_at() + (int64_t)tile1 * blocks * 64;
+  const uint32_t here0 = tile0 < at.tiles, here1 = tile1 < at.tiles;
+  struct WRegs {
+    i32x4 r0, r1;
+    uint32_t g0, g1;
+  };
+  auto load_w = [&](WRegs& r, int kb) W4_INLINE {
+    const uint32_t k = (uint32_t)(block0 + kb), some = kb < mine ? (uint32_t)blocks : 0u;
+    r.g0 = load1s(rsrc(groups0, here0 * some * 64u), 4u * l16 + q, k * 64u);
+    r.r0 = load16s(rsrc(codes0, here0 * some * 1024u), 16u * lane, k * 1024u);
+    r.g1 = load1s(rsrc(groups1, here1 * some * 64u), 4u * l16 + q, k * 64u);
+    r.r1 = load16s(rsrc(codes1, here1 * some * 1024u), 16u * lane, k * 1024u);
+  };
+  i32x4 acc[MF][2];
+#pragma unroll
+  for (int mb = 0; mb < MF; ++mb) acc[mb][0] = acc[mb][1] = i32x4{};
+  const uint32_t x_rd = grp * kStage + l16 * 128 + (((2 * q) ^ ((l16 >> 1) & 7)) << 4);
+  WRegs wreg[4];
+  load_x(sX0, 0);
+  __builtin_amdgcn_sched_barrier(0);
+  load_w(wreg[0], 0);
+  __builtin_amdgcn_sched_barrier(0);
+  load_x(sX1, 1);
+  __builtin_amdgcn_sched_barrier(0);
+  load_w(wreg[1], 1);
+  __builtin_amdgcn_sched_barrier(0);
+  load_x(sX2, 2);
+  __builtin_amdgcn_sched_barrier(0);
+  load_w(wreg[2], 2);
+  // The scales: a row's to a thread of the first group, a column's to one.
+  const int tid = threadIdx.x;
+  float my_xs = 0.f, my_ws = 0.f;
+  if (tid < rows) my_xs = p.x_scale[m0 + tid];
+  if (tid < 128) {  // SwiGLU: 16 gate columns, then 16 of the up projection, for each wavefront
+    const int64_t n = SWIGLU ? (tid >> 4 & 1 ? p.N >> 1 : 0) + (n0 >> 1) + 16 * (tid >> 5) + (tid & 15) : n0 + tid;
+    if (n < 16 * at.tiles) my_ws = reinterpret_cast<const float*>(p.w + at.scales_at())[n];
+  }
+  // Block kb: its X has landed by the barrier, which also frees the buffer of kb - 1 for kb + 3.  Newer at the barrier
+  // than its X loads are those of two blocks, X and weights: 2 (XJ + 4).
+  auto step = [&](const char* cur, char* next, const WRegs& w, WRegs& w_next, int kb) W4_INLINE {
+    barrier_but<2 * (XJ + 4)>();
+    load_x(next, kb + 3);
+    __builtin_amdgcn_sched_barrier(0);
+    load_w(w_next, kb + 3);
+    i32x4 x[MF][2];
+#pragma unroll
+    for (int mb = 0; mb < MF; ++mb) {
+      x[mb][0] = *reinterpret_cast<const i32x4*>(cur + x_rd + 2048 * mb);
+      x[mb][1] = *reinterpret_cast<const i32x4*>(cur + (x_rd ^ 16) + 2048 * mb);
+    }
+    const Group g0 = group_of(w.g0), g1 = group_of(w.g1);
+    i32x4 b0 = weights16<0>(w.r0, g0), b1 = weights16<0>(w.r1, g1);
+#pragma unroll
+    for (int mb = 0; mb < MF; ++mb) {
+      acc[mb][0] = mfma(b0, x[mb][0], acc[mb][0]);
+      acc[mb][1] = mfma(b1, x[mb][0], acc[mb][1]);
+    }
+    b0 = weights16<1>(w.r0, g0), b1 = weights16<1>(w.r1, g1);
+#pragma unroll
+    for (int mb = 0; mb < MF; ++mb) {
+      acc[mb][0] = mfma(b0, x[mb][1], acc[mb][0]);
+      acc[mb][1] = mfma(b1, x[mb][1], acc[mb][1]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+#pragma unroll 1
+  for (int kb = 0; kb < share; kb += 4) {  // blocks past the end add zero products
+    step(sX0, sX3, wreg[0], wreg[3], kb);
+    step(sX1, sX0, wreg[1], wreg[0], kb + 1);
+    step(sX2, sX1, wreg[2], wreg[1], kb + 2);
+    step(sX3, sX2, wreg[3], wreg[2], kb + 3);
+  }
+  barrier_but<0>();
+
+  // G > 1: group g finishes row fragments g MF / G and on of every wavefront's tile; the others' sums of them lie at
+  // [wavefront][g][sender] in the X buffers.
+  constexpr int kMine = MF / G;
+  if constexpr (G > 1) {
+    constexpr int kPart = 2 * kMine * 1024, kWave = G * (G - 1) * kPart;
+    static_assert(kWave <= G * kStage, "a wavefront's parts fit an X buffer");
+    char* const ex = (wave == 0 ? sX0 : wave == 1 ? sX1 : wave == 2 ? sX2 : sX3) + 16 * lane;
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+      if (g != grp)
+#pragma unroll
+        for (int i = 0; i < 2 * kMine; ++i)
+          *reinterpret_cast<i32x4*>(ex + (g * (G - 1) + (grp < g ? grp : grp - 1)) * kPart + 1024 * i) = acc[g * kMine + i / 2][i % 2];
+    __syncthreads();
+#pragma unroll
+    for (int g = 0; g < G; ++g)  // (a constant index for the registers)
+      if (g == grp)
+#pragma unroll
+        for (int i = 0; i < 2 * kMine; ++i) {
+          i32x4 t = acc[g * kMine + i / 2][i % 2];
+#pragma unroll
+          for (int from = 0; from < G - 1; ++from) t += *reinterpret_cast<const i32x4*>(ex + (g * (G - 1) + from) * kPart + 1024 * i);
+          acc[i / 2][i % 2] = t;
+        }
+    __syncthreads();
+  }
+  // Output through LDS, stored as whole rows of the tile.  Lane (l16, q) holds row 16 mb + l16, columns 4 q .. + 3 of
+  // the wavefront's two 16.
+  constexpr int kPieces = SWIGLU ? 8 : 16;  // 16-byte pieces of a row
+  static_assert(kTileM * 256 <= G * kStage * 2, "the tile's rows fit two X buffers");
+  float *const sXs = reinterpret_cast<float*>(sX2), *const sWs = reinterpret_cast<float*>(sX3);
+  if (tid < kTileM) sXs[tid] = my_xs;
+  if (tid < 128) sWs[tid] = my_ws;
+  __syncthreads();
+  auto place = [&](int row, int c) W4_INLINE {
+    return (row < kTileM / 2 ? sX0 : sX1) + row % (kTileM / 2) * (16 * kPieces) + ((SWIGLU ? c ^ ((row >> 1) & 7) : c ^ (row & 15)) << 4);
+  };
+  const float4 w0 = *reinterpret_cast<const float4*>(sWs + 32 * wave + 4 * q), w1 = *reinterpret_cast<const float4*>(sWs + 32 * wave + 16 + 4 * q);
+  const float s0[4] = {w0.x, w0.y, w0.z, w0.w}, s1[4] = {w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int row = 16 * (kMine * grp + i) + l16;
+    const float xs = sXs[row];
+    float f[4], t[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f[e] = (float)acc[i][0][e] * s0[e] * xs;
+      t[e] = (float)acc[i][1][e] * s1[e] * xs;
+    }
+    if constexpr (SWIGLU) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] = swiglu(f[e], t[e]);
+      *reinterpret_cast<u32x2*>(place(row, 2 * wave + (q >> 1)) + 8 * (q & 1)) = u32x2{narrow2<BF16>(f[0], f[1]), narrow2<BF16>(f[2], f[3])};
+    } else {
+      *reinterpret_cast<u32x2*>(place(row, 4 * wave + (q >> 1)) + 8 * (q & 1)) = u32x2{narrow2<BF16>(f[0], f[1]), narrow2<BF16>(f[2], f[3])};
+      *reinterpret_cast<u32x2*>(place(row, 4 * wave + 2 + (q >> 1)) + 8 * (q & 1)) = u32x2{narrow2<BF16>(t[0], t[1]), narrow2<BF16>(t[2], t[3])};
+    }
+  }
+  __syncthreads();
+  const int n_out = SWIGLU ? p.N >> 1 : p.N, col0 = SWIGLU ? n0 >> 1 : n0;
+  const auto yrs = rsrc(static_cast<uint16_t*>(p.y) + m0 * p.ldy, ((uint32_t)(rows - 1) * (uint32_t)p.ldy + (uint32_t)n_out) * 2u);
+  constexpr int kRowsPer = 256 * G / kPieces;  // rows per store of the workgroup
+#pragma unroll
+  for (int i = 0; i < (kTileM + kRowsPer - 1) / kRowsPer; ++i) {
+    const int row = kRowsPer * i + tid / kPieces, c = tid % kPieces, n = col0 + 8 * c;
+    if (kTileM % kRowsPer && row >= kTileM) break;
+    store16(*reinterpret_cast<const u32x4*>(place(row, c)), yrs,
+            row < rows && n + 8 <= n_out ? ((uint32_t)row * (uint32_t)p.ldy + (uint32_t)n) * 2u : kNowhere);
+  }
+  // A last piece of fewer than 8 columns goes element by element.
+  const int part = (n_out - col0) >> 3;
+  if ((n_out & 7) && part < kPieces) {
+#pragma unroll 1
+    for (int i = tid; i < kTileM * 8; i += 256 * G) {
+      const int row = i >> 3, n = col0 + 8 * part + (i & 7);
+      const uint16_t v = *reinterpret_cast<const uint16_t*>(place(row, part) + 2 * (i & 7));
+      store2(v, yrs, row < rows && n < n_out ? ((uint32_t)row * (uint32_t)p.ldy + (uint32_t)n) * 2u : kNowhere);
+    }
+  }
+}
+
+template <bool BF16, bool SWIGLU, int MF, int G>
+void launch_mid(const W4Product& p, hipStream_t stream) {
+  const int64_t tiles_m = ((int64_t)p.M + 16 * MF - 1) / (16 * MF), tiles_n = ((int64_t)p.N + 127) / 128;
+  const int64_t tiles = tiles_m * tiles_n, per_xcd = (tiles + 7) / 8;
+  hipLaunchKernelGGL((w4_mid_kernel<BF16, SWIGLU, MF, G>), dim3((unsigned)(8 * per_xcd)), dim3(256 * G), 0, stream, p, (int)tiles_n,
+                     (int)tiles, (int)per_xcd);
+}
+
+// ---- many rows: workgroup tiles of 32 MF rows and 64 NWN columns, 2 x NWN wavefronts of 16 MF x 64, K in steps of 64.
+// X comes by LDS-DMA, three steps ahead; every weight is taken apart once for the workgroup, into an LDS tile of
+// 8-bit weights.
+//
+// LDS tiles have rows of 64 bytes; the four 16-byte pieces of row r lie at c ^ ((r >> 2) & 3), so that 16 rows
+// reading one piece cover all banks.
+//
+// Step kb (X tile and weight tile kb in LDS, the first half's fragments in registers): half 1 reads the other row
+// fragments, takes weights kb + 1 apart into the free weight tile and runs the first half's products; the barrier
+// publishes that tile and X tile kb + 1; half 2 reads the next step's fragments under the other half's products.
+// X tile kb + 3 goes into the buffer that tile kb - 1 left at the previous barrier.
+__device__ inline uint32_t lds_off(int row, int piece) { return row * 64 + ((piece ^ ((row >> 2) & 3)) << 4); }
+
+template <bool BF16, bool SWIGLU, int MF, int NWN>
+__global__ __launch_bounds__(128 * NWN, 2) void w4_tile_kernel(W4Product p, int tiles_n, int tiles_total, int per_xcd) {
+  constexpr int kWaves = 2 * NWN;
   constexpr int kTileM = 32 * MF, kTileN = 64 * NWN;
   constexpr int kBytesA = kTileM * 64, kBytesB = kTileN * 64;
   constexpr int AJ = MF / NWN;                  // X loads per wavefront and step
   constexpr int A1 = AJ / 2, A2 = AJ - A1;      // ... in the first / second half step
   constexpr int H = MF / 2;                     // row fragments per half step
-  __shared__ __attribute__((aligned(1024))) char sA0[G * kBytesA];
-  __shared__ __attribute__((aligned(1024))) char sA1[G * kBytesA];
-  __shared__ __attribute__((aligned(1024))) char sA2[G * kBytesA];
-  __shared__ __attribute__((aligned(1024))) char sA3[G * kBytesA];
-  __shared__ __attribute__((aligned(1024))) char sB0[G * kBytesB];
-  __shared__ __attribute__((aligned(1024))) char sB1[G * kBytesB];
+  __shared__ __attribute__((aligned(1024))) char sA0[kBytesA];
+  __shared__ __attribute__((aligned(1024))) char sA1[kBytesA];
+  __shared__ __attribute__((aligned(1024))) char sA2[kBytesA];
+  __shared__ __attribute__((aligned(1024))) char sA3[kBytesA];
+  __shared__ __attribute__((aligned(1024))) char sB0[kBytesB];
+  __shared__ __attribute__((aligned(1024))) char sB1[kBytesB];
 
   // Consecutive workgroups of an XCD (workgroup b runs on XCD b % 8) walk the column tiles of one row tile: its X
   // rows stay in that XCD's L2.
@@ -228,16 +468,12 @@ __global__ __launch_bounds__(128 * NWN * G, 2) void w4_tile_kernel(W4Product p, 
   if (u >= tiles_total) return;
   const int64_t m0 = (int64_t)(u / tiles_n) * kTileM;
   const int n0 = (u % tiles_n) * kTileN;
-  const int gwave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int grp = G == 1 ? 0 : gwave / kWaves, wave = G == 1 ? gwave : gwave % kWaves;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, l16 = lane & 15, kq = lane >> 4;
   const int wr = 16 * MF * (wave & 1), wc = 64 * (wave >> 1);
   const W4Layout at(p.K, p.N);
   const int blocks = (int)at.blocks;
-  // Steps of this group; K is padded to whole blocks of two steps.
-  const int steps_all = 2 * blocks, share = (steps_all + G - 1) / G;
-  const int step0 = grp * share;
-  const int steps = G == 1 ? steps_all : __builtin_amdgcn_readfirstlane(max(0, min(share, steps_all - step0)));
+  const int steps = 2 * blocks;  // K is padded to whole blocks of two steps
 
   // X rows of the tile.  A range starts at its step's first column and ends with the last row's K columns, so that
   // a load past either reads zeros; what it reads past a row's end inside the tensor meets zero weights.
@@ -250,9 +486,9 @@ __global__ __launch_bounds__(128 * NWN * G, 2) void w4_tile_kernel(W4Product p, 
     const int row = 16 * (AJ * wave + j) + (lane >> 2);
     a_src[j] = (uint32_t)row * (uint32_t)p.ldx + 16u * ((lane & 3) ^ ((row >> 2) & 3));
   }
-  const uint32_t a_dst = grp * kBytesA + 1024 * AJ * wave;
+  const uint32_t a_dst = 1024 * AJ * wave;
   auto load_a = [&](char* dst, int kb, int j0, int n) W4_INLINE {
-    const int first = 64 * (step0 + kb);
+    const int first = 64 * kb;
     // In a scalar register (the compiler's saturating difference is a vector one, and would be looped over).
     const int left = __builtin_amdgcn_readfirstlane(kb < steps ? max(x_bytes - first, 0) : 0);
     const auto rs = rsrc(x0 + first, (uint32_t)left);
@@ -269,17 +505,17 @@ __global__ __launch_bounds__(128 * NWN * G, 2) void w4_tile_kernel(W4Product p, 
   const int brow = 32 * wave + (lane >> 1), half = lane & 1;
   const uint32_t w_rec = (uint32_t)(lane >> 5) * (uint32_t)blocks * 1024u + 256u * half + 16u * ((lane >> 1) & 15);
   const uint32_t w_grp = (uint32_t)(lane >> 5) * (uint32_t)blocks * 64u + 4u * ((lane >> 1) & 15) + half;
-  const uint32_t b_lo = grp * kBytesB + lds_off(brow, 2 * half), b_hi = grp * kBytesB + lds_off(brow, 2 * half + 1);
+  const uint32_t b_lo = lds_off(brow, 2 * half), b_hi = lds_off(brow, 2 * half + 1);
   struct WRegs {
     i32x4 record;
     uint32_t group;
   };
   auto load_wg = [&](WRegs& r, int kb) W4_INLINE {
-    const uint32_t k = (uint32_t)(step0 + kb);
+    const uint32_t k = (uint32_t)kb;
     r.group = load1s(rsrc(groups, kb < steps ? (uint32_t)my_tiles * (uint32_t)blocks * 64u : 0u), w_grp, (k >> 1) * 64u + 2u * (k & 1u));
   };
   auto load_wr = [&](WRegs& r, int kb) W4_INLINE {
-    r.record = load16s(rsrc(codes, kb < steps ? (uint32_t)my_tiles * (uint32_t)blocks * 1024u : 0u), w_rec, (uint32_t)(step0 + kb) * 512u);
+    r.record = load16s(rsrc(codes, kb < steps ? (uint32_t)my_tiles * (uint32_t)blocks * 1024u : 0u), w_rec, (uint32_t)kb * 512u);
   };
   auto store_b = [&](char* dst, const WRegs& r) W4_INLINE {
     const Group g = group_of(r.group);
@@ -291,7 +527,7 @@ __global__ __launch_bounds__(128 * NWN * G, 2) void w4_tile_kernel(W4Product p, 
   for (int mb = 0; mb < MF; ++mb)
 #pragma unroll
     for (int nb = 0; nb < 4; ++nb) acc[mb][nb] = i32x4{};
-  const uint32_t a_rd = grp * kBytesA + lds_off(wr + l16, kq), b_rd = grp * kBytesB + lds_off(wc + l16, kq);
+  const uint32_t a_rd = lds_off(wr + l16, kq), b_rd = lds_off(wc + l16, kq);
 
   WRegs wreg[4];
   i32x4 a_lo[H], a_hi[H], b0[4], b1[4];
@@ -351,7 +587,7 @@ __global__ __launch_bounds__(128 * NWN * G, 2) void w4_tile_kernel(W4Product p, 
     __builtin_amdgcn_sched_barrier(0);
   };
 #pragma unroll 1
-  for (int kb = 0; kb < (G == 1 ? steps_all : share); kb += 4) {  // steps past the end add zero products
+  for (int kb = 0; kb < steps; kb += 4) {  // steps past the end add zero products
     step(sA0, sA1, sA3, sB1, b0, b1, wreg[1], wreg[3], kb);
     step(sA1, sA2, sA0, sB0, b1, b0, wreg[2], wreg[0], kb + 1);
     step(sA2, sA3, sA1, sB1, b0, b1, wreg[3], wreg[1], kb + 2);
@@ -359,55 +595,25 @@ __global__ __launch_bounds__(128 * NWN * G, 2) void w4_tile_kernel(W4Product p, 
   }
   barrier_but<0>();
 
-  // G = 2: group g finishes the rows of half g of every wavefront's tile.
-  if constexpr (G == 2) {
-    char* const ex = (wave == 0 ? sA0 : wave == 1 ? sA1 : wave == 2 ? sA2 : sA3) + 16 * lane;
-    auto send = [&](int m8, char* q) W4_INLINE {
-#pragma unroll
-      for (int mb = 0; mb < H; ++mb)
-#pragma unroll
-        for (int nb = 0; nb < 4; ++nb) *reinterpret_cast<i32x4*>(q + 1024 * (4 * mb + nb)) = acc[m8 + mb][nb];
-    };
-    auto take = [&](int m8, const char* q) W4_INLINE {
-#pragma unroll
-      for (int mb = 0; mb < H; ++mb)
-#pragma unroll
-        for (int nb = 0; nb < 4; ++nb) acc[mb][nb] = acc[m8 + mb][nb] + *reinterpret_cast<const i32x4*>(q + 1024 * (4 * mb + nb));
-    };
-    static_assert(G != 2 || (kWaves == 4 && 2 * kBytesA >= 2 * 4096 * H), "a wavefront's two halves fill an X buffer");
-    if (grp == 0)
-      send(H, ex);
-    else
-      send(0, ex + 4096 * H);
-    __syncthreads();
-    if (grp == 0)
-      take(0, ex + 4096 * H);
-    else
-      take(H, ex);
-    __syncthreads();
-  }
-
   // Output through LDS, kRows rows of a wavefront at a time: stores of 16 bytes in whole 128-byte lines.  Lane (l16,
   // kq) holds row 16 mb + l16, columns 16 nb + 4 kq .. + 3.
-  constexpr int kMine = G > 1 ? H : MF;  // row fragments this wavefront finishes
-  constexpr int kHold = 4 * G * kBytesA / 128 / (kWaves * G);
+  constexpr int kHold = 4 * kBytesA / 128 / kWaves;
   constexpr int kMost = kHold < 64 ? kHold : 64;
-  constexpr int kRows = 16 * kMine < kMost ? 16 * kMine : kMost;
-  constexpr int kPer = G * kBytesA / (128 * kRows);  // wavefronts per X buffer
-  static_assert(4 * kPer >= kWaves * G && 16 * kMine % kRows == 0 && kRows % 16 == 0, "a stage per writer, whole fragments");
-  const int slot = gwave / kPer;
-  char* const stage = (slot == 0 ? sA0 : slot == 1 ? sA1 : slot == 2 ? sA2 : sA3) + 128 * kRows * (gwave % kPer);
+  constexpr int kRows = 16 * MF < kMost ? 16 * MF : kMost;
+  constexpr int kPer = kBytesA / (128 * kRows);  // wavefronts per X buffer
+  static_assert(4 * kPer >= kWaves && 16 * MF % kRows == 0 && kRows % 16 == 0, "a stage per wavefront, whole fragments");
+  const int slot = wave / kPer;
+  char* const stage = (slot == 0 ? sA0 : slot == 1 ? sA1 : slot == 2 ? sA2 : sA3) + 128 * kRows * (wave % kPer);
   const int n_out = SWIGLU ? p.N >> 1 : p.N;
-  const int row0 = wr + 16 * kMine * grp, col0 = SWIGLU ? (n0 + wc) >> 1 : n0 + wc;
+  const int row0 = wr, col0 = SWIGLU ? (n0 + wc) >> 1 : n0 + wc;
   const auto yrs = rsrc(static_cast<uint16_t*>(p.y) + m0 * p.ldy, ((uint32_t)(rows - 1) * (uint32_t)p.ldy + (uint32_t)n_out) * 2u);
-  constexpr uint32_t kNowhere = 0x80000000u;  // past every range: 256 rows of at most 2^22 elements
   constexpr int kPieces = SWIGLU ? 4 : 8;     // 16-byte pieces of a row
   auto place = [&](int row, int c) W4_INLINE {
     return stage + row * (16 * kPieces) + ((SWIGLU ? c ^ ((row >> 2) & 3) : c ^ ((row >> 1) & 7)) << 4);
   };
   // The weight tiles are free: the scales' place.
   float *const sXs = reinterpret_cast<float*>(sB0), *const sWs = reinterpret_cast<float*>(sB1);
-  static_assert(128 * NWN * G >= kTileM && 128 * NWN * G >= kTileN && G * kBytesB >= 4 * kTileM, "a thread and a place for every scale");
+  static_assert(128 * NWN >= kTileM && 128 * NWN >= kTileN && kBytesB >= 4 * kTileM, "a thread and a place for every scale");
   if (tid < kTileM) sXs[tid] = my_xs;
   if (tid < kTileN) sWs[tid] = my_ws;
   __syncthreads();
@@ -415,7 +621,7 @@ __global__ __launch_bounds__(128 * NWN * G, 2) void w4_tile_kernel(W4Product p, 
 #pragma unroll
   for (int nb = 0; nb < 4; ++nb) ws[nb] = *reinterpret_cast<const float4*>(sWs + wc + 16 * nb + 4 * kq);
 #pragma unroll
-  for (int pass = 0; pass < 16 * kMine / kRows; ++pass) {
+  for (int pass = 0; pass < 16 * MF / kRows; ++pass) {
 #pragma unroll
     for (int mb = 0; mb < kRows / 16; ++mb) {
       const i32x4(&v)[4] = acc[pass * (kRows / 16) + mb];
@@ -461,25 +667,41 @@ __global__ __launch_bounds__(128 * NWN * G, 2) void w4_tile_kernel(W4Product p, 
   }
 }
 
-template <bool BF16, bool SWIGLU, int MF, int NWN, int G>
+template <bool BF16, bool SWIGLU, int MF, int NWN>
 void launch_tile(const W4Product& p, hipStream_t stream) {
   const int64_t tiles_m = ((int64_t)p.M + 32 * MF - 1) / (32 * MF), tiles_n = ((int64_t)p.N + 64 * NWN - 1) / (64 * NWN);
   const int64_t tiles = tiles_m * tiles_n, per_xcd = (tiles + 7) / 8;
-  hipLaunchKernelGGL((w4_tile_kernel<BF16, SWIGLU, MF, NWN, G>), dim3((unsigned)(8 * per_xcd)), dim3(128 * NWN * G), 0, stream, p,
+  hipLaunchKernelGGL((w4_tile_kernel<BF16, SWIGLU, MF, NWN>), dim3((unsigned)(8 * per_xcd)), dim3(128 * NWN), 0, stream, p,
                      (int)tiles_n, (int)tiles, (int)per_xcd);
 }
 
 template <bool BF16, bool SWIGLU>
 hipError_t launch(const W4Product& p, hipStream_t stream) {
   const auto tiles = [&](int tm, int tn) { return (((int64_t)p.M + tm - 1) / tm) * (((int64_t)p.N + tn - 1) / tn); };
-  if (tiles(128, 128) <= 64 || p.M <= 128)
-    launch_small<BF16, SWIGLU, 2, 2, 4>(p, stream);
-  else if (tiles(128, 128) <= 256)
-    launch_tile<BF16, SWIGLU, 4, 2, 2>(p, stream);
-  else if (tiles(256, 256) <= 256)
-    launch_tile<BF16, SWIGLU, 8, 2, 1>(p, stream);
-  else
-    launch_tile<BF16, SWIGLU, 8, 4, 1>(p, stream);
+  // Workgroups that fit the card less those of the last round of a launch.
+  const auto idle = [](int64_t groups, int at_once) { return (at_once - groups % at_once) % at_once; };
+  const int64_t small = tiles(32, 32), whole = tiles(256, 256), half = tiles(256, 128);
+  if (p.M <= 16 || small <= 96) {
+    if (p.K > 8192)
+      launch_small<BF16, SWIGLU, 1, 2, 8, 2>(p, stream);
+    else
+      launch_small<BF16, SWIGLU, 1, 2, 8, 1>(p, stream);
+  } else if (p.M <= 32 || small <= 640) {
+    if (small <= 256 && p.K >= 2048)
+      launch_small<BF16, SWIGLU, 2, 2, 8, 1>(p, stream);
+    else
+      launch_small<BF16, SWIGLU, 2, 2, 4, 1>(p, stream);
+  } else if (p.K > 128 && (idle(whole, 256) <= 80 || idle(whole, 256) <= whole / 8)) {
+    launch_tile<BF16, SWIGLU, 8, 4>(p, stream);
+  } else if (half >= 700 || (half >= 160 && p.K <= 256)) {
+    launch_tile<BF16, SWIGLU, 8, 2>(p, stream);
+  } else if (idle(tiles(128, 128), 512) <= 300) {
+    launch_mid<BF16, SWIGLU, 8, 1>(p, stream);
+  } else if (tiles(64, 128) <= 256 && p.K >= 2048) {
+    launch_mid<BF16, SWIGLU, 4, 2>(p, stream);
+  } else {
+    launch_mid<BF16, SWIGLU, 4, 1>(p, stream);
+  }
   return hipGetLastError();
 }
 

@@ -1,4 +1,4 @@
-"""The hand-counted waits of the tiled kernel for 8-bit rows and 4-bit weights, followed through the gfx950 assembly
+"""The hand-counted waits of the tiled kernels for 8-bit rows and 4-bit weights, followed through the gfx950 assembly
 on the CPU, as test_q4_waits.py does for the Q4_0 kernels: by barrier b every load of the b-th X tile must have
 landed on the strength of the explicit waits alone."""
 import os
@@ -21,7 +21,7 @@ def kernels(tmp_path_factory):
                     "-packed-fp32-ops", "--cuda-device-only", "-S", "-o", out, SOURCE], check=True, capture_output=True)
     found, name = {}, None
     for line in open(out):
-        start = re.match(r"(_ZN5qattn\w*w4_tile_kernel\w+):", line)
+        start = re.match(r"(_ZN5qattn\w*w4_(?:tile|mid)_kernel\w+):", line)
         if start:
             name = start.group(1)
             found[name] = []
@@ -55,12 +55,14 @@ def events(lines):
 
 
 def test_every_published_x_tile_has_landed(kernels):
-    assert len(kernels) >= 8
+    assert sum("w4_tile" in name for name in kernels) == 8 and sum("w4_mid" in name for name in kernels) == 12
     for name, lines in kernels.items():
         prologue, loop = events(lines)
-        assert sum(e[0] == "wait" for e in prologue) == 1 and sum(e[0] == "wait" for e in loop) == 4, name
-        mf, nwn = [int(v) for v in re.findall(r"Li(\d+)E", name)][:2]
-        group = mf // nwn  # LDS-DMA loads of an X tile, per wavefront
+        mf, second = [int(v) for v in re.findall(r"Li(\d+)E", name)][:2]
+        # LDS-DMA loads of an X tile, per wavefront, and the barriers ahead of the loop: the first kernel reads X tile 0
+        # before its loop, the other in it.
+        group, ahead = (mf // second, 1) if "w4_tile" in name else (mf // 2, 0)
+        assert sum(e[0] == "wait" for e in prologue) == ahead and sum(e[0] == "wait" for e in loop) == 4, name
         issued, dma, barrier = 0, [], 0  # dma: issue numbers of the LDS-DMA loads
         for event in prologue + PASSES * loop:
             if event[0] == "wait":
