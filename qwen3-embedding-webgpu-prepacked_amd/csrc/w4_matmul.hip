@@ -35,6 +35,22 @@ __device__ inline i32x4 load16(__amdgpu_buffer_rsrc_t rs, uint32_t off) {
 __device__ inline uint32_t load1(__amdgpu_buffer_rsrc_t rs, uint32_t off) { return __builtin_amdgcn_raw_buffer_load_b8(rs, off, 0, 0); }
 __device__ inline i32x4 mfma(i32x4 a, i32x4 b, i32x4 c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
 
+typedef __attribute__((address_space(3))) void lds_void_t;
+__device__ inline void dma16(__amdgpu_buffer_rsrc_t rs, char* dst, uint32_t off) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t*)dst, 16, off, 0, 0, 0);
+}
+// Waits for all but the newest V vector-memory operations, or for all LDS reads, of this wavefront.
+template <int V>
+__device__ inline void wait_but() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(V) : "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+__device__ inline void wait_lds() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 // A group's multiplier in both halves of a dword, and 128 - zero * multiplier in its four bytes.
 struct Group {
   uint32_t mult, bias;
@@ -56,18 +72,31 @@ __device__ inline i32x4 weights16(i32x4 record, Group g) {
   return w;
 }
 
+// Results rounded to f32 before they are to 16 bits: otherwise some are by one instruction that multiplies and rounds
+// once, and a row's result would depend on the kernel that its batch takes.
+template <bool BF16>
+__device__ inline u32x2 narrow4(const float (&f)[4]) {
+  float a = f[0], b = f[1], c = f[2], d = f[3];
+  asm("" : "+v"(a), "+v"(b), "+v"(c), "+v"(d));
+  return u32x2{narrow2<BF16>(a, b), narrow2<BF16>(c, d)};
+}
+
 // silu(g) * u.  The hardware's exp2 and reciprocal are within about an f32 ulp, far inside the result's rounding.
 __device__ inline float swiglu(float g, float u) {
   return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.44269504f)) * u;
 }
 
 // ---- few rows: a workgroup to 16 MB rows and 16 NB columns (SwiGLU: 8 NB features), whose W wavefronts take the
-// blocks of 128 columns of K in turn, U of them in flight, and add up in LDS.  No operand is staged: a lane's 16
-// bytes of codes are two fragments, and its 32 bytes of x the two that meet them.
+// blocks of 128 columns of K in turn, U of them in flight, and add up in LDS.  A lane's 16 bytes of codes are two
+// fragments as they come.  X goes through LDS, a region to each wavefront: the 16 rows of a fragment are as many cache
+// lines to a load of its own, which the address unit takes one by one (64 clocks; 16 by rows, as here).
 template <bool BF16, bool SWIGLU, int MB, int NB, int W, int U>
 __global__ __launch_bounds__(64 * W) void w4_small_kernel(W4Product p, int blocks_m) {
   static_assert(!SWIGLU || NB % 2 == 0, "as many gate tiles as up tiles");
-  __shared__ i32x4 part[W > 1 ? W - 1 : 1][MB * NB][64];
+  static_assert(U >= 1 && U <= 2 && NB <= 2 * U, "two buffers, which take a wavefront's sums in the end");
+  constexpr int kRegion = 2048 * MB;
+  __shared__ __attribute__((aligned(1024))) char sX0[W * kRegion];
+  __shared__ __attribute__((aligned(1024))) char sX1[U > 1 ? W * kRegion : 16];
   const int lane = threadIdx.x & 63, l16 = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t m0 = (int64_t)(blockIdx.x % (unsigned)blocks_m) * (16 * MB);
@@ -87,109 +116,126 @@ __global__ __launch_bounds__(64 * W) void w4_small_kernel(W4Product p, int block
     groups[nb] = rsrc(p.w + at.groups_at() + (int64_t)tile[nb] * blocks * 64, here ? (uint32_t)blocks * 64u : 0u);
   }
   // Rows past M and what lies behind the last row's K columns read as zeros; columns of K's padding meet zero weights.
+  // Rows of 128 bytes in LDS, piece c of row r at c ^ ((r >> 1) & 7).
   const int rows = (int)(p.M - m0 < 16 * MB ? p.M - m0 : 16 * MB);
-  const auto xs = rsrc(p.x + m0 * p.ldx, (uint32_t)(rows - 1) * (uint32_t)p.ldx + (uint32_t)p.K);
-  uint32_t x_off[MB];
+  const uint32_t x_bytes = (uint32_t)(rows - 1) * (uint32_t)p.ldx + (uint32_t)p.K;
+  uint32_t x_src[2 * MB];
 #pragma unroll
-  for (int mb = 0; mb < MB; ++mb) x_off[mb] = (uint32_t)(16 * mb + l16) * (uint32_t)p.ldx + 32u * q;
+  for (int j = 0; j < 2 * MB; ++j) {
+    const int row = 8 * j + (lane >> 3);
+    x_src[j] = (uint32_t)row * (uint32_t)p.ldx + 16u * ((lane & 7) ^ ((row >> 1) & 7));
+  }
+  const uint32_t x_rd = l16 * 128 + (((2 * q) ^ ((l16 >> 1) & 7)) << 4);
+  auto region = [&](int i) W4_INLINE { return (i ? sX1 : sX0) + wave * kRegion; };
 
-  struct Stage {
-    i32x4 x[MB][2], record[NB];
+  struct Weights {
+    i32x4 record[NB];
     uint32_t group[NB];
   };
-  auto load = [&](Stage& st, int kb) W4_INLINE {
-    const uint32_t k = (uint32_t)kb;
+  auto load_x = [&](char* dst, int kb) W4_INLINE {
+    const auto xs = rsrc(p.x + m0 * p.ldx, kb < blocks ? x_bytes : 0u);  // nothing past the last block
+#pragma unroll
+    for (int j = 0; j < 2 * MB; ++j) dma16(xs, dst + 1024 * j, x_src[j] + 128u * (uint32_t)kb);
+  };
+  auto load_w = [&](Weights& w, int kb) W4_INLINE {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      st.record[nb] = load16(codes[nb], 1024u * k + 16u * lane);
-      st.group[nb] = load1(groups[nb], 64u * k + 4u * l16 + q);
-    }
-#pragma unroll
-    for (int mb = 0; mb < MB; ++mb) {
-      st.x[mb][0] = load16(xs, x_off[mb] + 128u * k);
-      st.x[mb][1] = load16(xs, x_off[mb] + 128u * k + 16u);
+      w.record[nb] = load16(codes[nb], 1024u * (uint32_t)kb + 16u * lane);
+      w.group[nb] = load1(groups[nb], 64u * (uint32_t)kb + 4u * l16 + q);
     }
   };
   i32x4 acc[NB][MB];
 #pragma unroll
   for (int i = 0; i < NB * MB; ++i) acc[i / MB][i % MB] = i32x4{};
-  auto multiply = [&](const Stage& st) W4_INLINE {
+  // Of the 16 x 16 sums (SwiGLU: pairs of them) each of the first wavefronts finishes one; its scales.
+  constexpr int kUnits = SWIGLU ? MB * NB / 2 : MB * NB;
+  static_assert(kUnits <= W, "a wavefront for each");
+  const int my_nb = wave / MB, my_row = 16 * (wave % MB) + l16;
+  float x_scale = 0.f;
+  float4 w_scale = {}, up_scale = {};
+  if (wave < kUnits) {
+    const float4* const scales = reinterpret_cast<const float4*>(p.w + at.scales_at());
+    if (my_row < rows) x_scale = p.x_scale[m0 + my_row];
+    if (tile0 + my_nb < at.tiles) w_scale = scales[4 * (tile0 + my_nb) + q];
+    if (SWIGLU && tile0 + my_nb + (p.N >> 5) < at.tiles) up_scale = scales[4 * (tile0 + my_nb + (p.N >> 5)) + q];
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  Weights ring[U];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      const Group g = group_of(st.group[nb]);
-      const i32x4 lo = weights16<0>(st.record[nb], g), hi = weights16<1>(st.record[nb], g);
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb) acc[nb][mb] = mfma(lo, st.x[mb][0], acc[nb][mb]);
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb) acc[nb][mb] = mfma(hi, st.x[mb][1], acc[nb][mb]);
-    }
-  };
-  Stage ring[U];
-#pragma unroll
-  for (int i = 0; i < U; ++i) load(ring[i], wave + W * i);
-  // The scales of lane (l16, q): row l16, columns 4 q .. 4 q + 3 of a 16 x 16 block.
-  float x_scale[MB];
-  float4 w_scale[NB];
-#pragma unroll
-  for (int mb = 0; mb < MB; ++mb) x_scale[mb] = 16 * mb + l16 < rows ? p.x_scale[m0 + 16 * mb + l16] : 0.f;
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb)
-    w_scale[nb] = tile[nb] < at.tiles ? reinterpret_cast<const float4*>(p.w + at.scales_at())[4 * tile[nb] + q] : float4{};
+  for (int i = 0; i < U; ++i) {
+    load_x(region(i), wave + W * i);
+    load_w(ring[i], wave + W * i);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  // Blocks past the end are loads of zeros: as many loads are in flight at each wait.
   for (int kb = wave; kb < blocks; kb += W * U) {
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      multiply(ring[i]);
-      if (kb + W * U < blocks) load(ring[i], kb + W * (U + i));
+      // X of this block has landed: newer are the U - 1 blocks behind it.
+      wait_but<(U - 1) * (2 * MB + 2 * NB)>();
+      i32x4 x[MB][2];
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) {
+        x[mb][0] = *reinterpret_cast<const i32x4*>(region(i) + x_rd + 2048 * mb);
+        x[mb][1] = *reinterpret_cast<const i32x4*>(region(i) + (x_rd ^ 16) + 2048 * mb);
+      }
+      wait_lds();
+      load_x(region(i), kb + W * (U + i));
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const Group g = group_of(ring[i].group[nb]);
+        const i32x4 lo = weights16<0>(ring[i].record[nb], g), hi = weights16<1>(ring[i].record[nb], g);
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) acc[nb][mb] = mfma(lo, x[mb][0], acc[nb][mb]);
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) acc[nb][mb] = mfma(hi, x[mb][1], acc[nb][mb]);
+      }
+      load_w(ring[i], kb + W * (U + i));
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
-  if constexpr (W > 1) {
-    if (wave > 0)
+  // A wavefront's sums take the place of its X, once the last of that has landed.
+  wait_but<0>();
+  auto part = [&](int w, int i) W4_INLINE {
+    return reinterpret_cast<i32x4*>((i < 2 * MB ? sX0 : sX1) + w * kRegion + 1024 * (i % (2 * MB)) + 16 * lane);
+  };
 #pragma unroll
-      for (int i = 0; i < NB * MB; ++i) part[wave - 1][i][lane] = acc[i / MB][i % MB];
-    __syncthreads();
-    if (wave > 0) return;
+  for (int i = 0; i < NB * MB; ++i) *part(wave, i) = acc[i / MB][i % MB];
+  __syncthreads();
+  if (wave >= kUnits) return;
+  // Lane (l16, q) holds row l16, columns 4 q .. 4 q + 3 of its 16 x 16.
+  auto sum = [&](int i, float4 scale, float (&f)[4]) W4_INLINE {
+    i32x4 t = *part(0, i);
 #pragma unroll
-    for (int w = 0; w < W - 1; ++w)
+    for (int w = 1; w < W; ++w) t += *part(w, i);
+    const float s[4] = {scale.x, scale.y, scale.z, scale.w};
 #pragma unroll
-      for (int i = 0; i < NB * MB; ++i) acc[i / MB][i % MB] += part[w][i][lane];
+    for (int e = 0; e < 4; ++e) f[e] = (float)t[e] * s[e] * x_scale;
+  };
+  float v[4];
+  sum(wave, w_scale, v);
+  if constexpr (SWIGLU) {
+    float t[4];
+    sum(wave + kUnits, up_scale, t);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = swiglu(v[e], t[e]);
   }
-  const int n_out = SWIGLU ? p.N >> 1 : p.N;
+  const int n_out = SWIGLU ? p.N >> 1 : p.N, n = 16 * (tile0 + my_nb) + 4 * q;
+  if (my_row >= rows || n >= n_out) return;
+  uint16_t* const y = static_cast<uint16_t*>(p.y) + (m0 + my_row) * p.ldy + n;
+  const u32x2 d = narrow4<BF16>(v);
+  if (n + 4 <= n_out) {
+    *reinterpret_cast<u32x2*>(y) = d;
+  } else {
 #pragma unroll
-  for (int mb = 0; mb < MB; ++mb) {
-    if (16 * mb + l16 >= rows) continue;
-    uint16_t* const y = static_cast<uint16_t*>(p.y) + (m0 + 16 * mb + l16) * p.ldy;
-#pragma unroll
-    for (int nb = 0; nb < (SWIGLU ? NB / 2 : NB); ++nb) {
-      const int n = 16 * (tile0 + nb) + 4 * q;
-      if (n >= n_out) continue;
-      auto scaled = [&](int b, float (&f)[4]) W4_INLINE {
-        const float s[4] = {w_scale[b].x, w_scale[b].y, w_scale[b].z, w_scale[b].w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] = (float)acc[b][mb][e] * s[e] * x_scale[mb];
-      };
-      float v[4];
-      scaled(nb, v);
-      if constexpr (SWIGLU) {
-        float t[4];
-        scaled(nb + NB / 2, t);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = swiglu(v[e], t[e]);
-      }
-      const u32x2 d = {narrow2<BF16>(v[0], v[1]), narrow2<BF16>(v[2], v[3])};
-      if (n + 4 <= n_out) {
-        *reinterpret_cast<u32x2*>(y + n) = d;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 3; ++e)
-          if (n + e < n_out) y[n + e] = (uint16_t)(d[e >> 1] >> (16 * (e & 1)));
-      }
-    }
+    for (int e = 0; e < 3; ++e)
+      if (n + e < n_out) y[e] = (uint16_t)(d[e >> 1] >> (16 * (e & 1)));
   }
 }
 
 template <bool BF16, bool SWIGLU, int MB, int NB, int W, int U>
 void launch_small(const W4Product& p, hipStream_t stream) {
-  static_assert(!SWIGLU || NB % 2 == 0, "as many gate tiles as up tiles");
   const int64_t blocks_m = ((int64_t)p.M + 16 * MB - 1) / (16 * MB), tiles = W4Layout(p.K, SWIGLU ? p.N / 2 : p.N).tiles;
   const int64_t per = SWIGLU ? NB / 2 : NB, blocks_n = (tiles + per - 1) / per;
   hipLaunchKernelGGL((w4_small_kernel<BF16, SWIGLU, MB, NB, W, U>), dim3((unsigned)(blocks_m * blocks_n)), dim3(64 * W), 0,
@@ -198,10 +244,6 @@ void launch_small(const W4Product& p, hipStream_t stream) {
 
 constexpr uint32_t kNowhere = 0x80000000u;  // past every range of a tile: 256 rows of at most 2^22 elements
 
-typedef __attribute__((address_space(3))) void lds_void_t;
-__device__ inline void dma16(__amdgpu_buffer_rsrc_t rs, char* dst, uint32_t off) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t*)dst, 16, off, 0, 0, 0);
-}
 __device__ inline i32x4 load16s(__amdgpu_buffer_rsrc_t rs, uint32_t off, uint32_t soff) {
   return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, off, soff, 0));
 }
@@ -226,7 +268,8 @@ __device__ inline void barrier_but() {
 
 // ---- in between: workgroup tiles of 16 MF rows and 128 columns, groups of four wavefronts of 16 MF x 32, K in blocks
 // of 128.  X comes by LDS-DMA, three blocks ahead; each wavefront takes its own weights apart, straight into
-// fragments.  G groups share K and add up in LDS.
+// fragments: no store to LDS and one barrier a block, for which the taking apart, done once for each tile of rows, is
+// most of the vector work and the bound.  G groups share K and add up in LDS.
 //
 // LDS rows of X have 128 bytes; the eight 16-byte pieces of row r lie at c ^ ((r >> 1) & 7), so that 16 rows reading
 // one piece cover all banks.
@@ -397,10 +440,10 @@ __global__ __launch_bounds__(256 * G, 2) void w4_mid_kernel(W4Product p, int til
     if constexpr (SWIGLU) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) f[e] = swiglu(f[e], t[e]);
-      *reinterpret_cast<u32x2*>(place(row, 2 * wave + (q >> 1)) + 8 * (q & 1)) = u32x2{narrow2<BF16>(f[0], f[1]), narrow2<BF16>(f[2], f[3])};
+      *reinterpret_cast<u32x2*>(place(row, 2 * wave + (q >> 1)) + 8 * (q & 1)) = narrow4<BF16>(f);
     } else {
-      *reinterpret_cast<u32x2*>(place(row, 4 * wave + (q >> 1)) + 8 * (q & 1)) = u32x2{narrow2<BF16>(f[0], f[1]), narrow2<BF16>(f[2], f[3])};
-      *reinterpret_cast<u32x2*>(place(row, 4 * wave + 2 + (q >> 1)) + 8 * (q & 1)) = u32x2{narrow2<BF16>(t[0], t[1]), narrow2<BF16>(t[2], t[3])};
+      *reinterpret_cast<u32x2*>(place(row, 4 * wave + (q >> 1)) + 8 * (q & 1)) = narrow4<BF16>(f);
+      *reinterpret_cast<u32x2*>(place(row, 4 * wave + 2 + (q >> 1)) + 8 * (q & 1)) = narrow4<BF16>(t);
     }
   }
   __syncthreads();
@@ -642,7 +685,7 @@ __global__ __launch_bounds__(128 * NWN, 2) void w4_tile_kernel(W4Product p, int 
 #pragma unroll
           for (int e = 0; e < 4; ++e) f[e] = swiglu(f[e], t[e]);
         }
-        *reinterpret_cast<u32x2*>(place(row, 2 * nb + (kq >> 1)) + 8 * (kq & 1)) = u32x2{narrow2<BF16>(f[0], f[1]), narrow2<BF16>(f[2], f[3])};
+        *reinterpret_cast<u32x2*>(place(row, 2 * nb + (kq >> 1)) + 8 * (kq & 1)) = narrow4<BF16>(f);
       }
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -678,23 +721,39 @@ void launch_tile(const W4Product& p, hipStream_t stream) {
 template <bool BF16, bool SWIGLU>
 hipError_t launch(const W4Product& p, hipStream_t stream) {
   const auto tiles = [&](int tm, int tn) { return (((int64_t)p.M + tm - 1) / tm) * (((int64_t)p.N + tn - 1) / tn); };
-  // Workgroups that fit the card less those of the last round of a launch.
+  // Workgroups that fit the card at once less those of a launch's last round.
   const auto idle = [](int64_t groups, int at_once) { return (at_once - groups % at_once) % at_once; };
   const int64_t small = tiles(32, 32), whole = tiles(256, 256), half = tiles(256, 128);
+  // Microseconds on one MI355X, M x K -> N: the variant taken against the next best one's.  Launches that the card
+  // holds at once go to the few-rows kernel, whose wavefronts share K (700 x 256 -> 1,024 3.9 against 4.9 of the next
+  // kernel, 200 x 1,024 -> 4,096 7.1 against 6.4); short sums let more of them through (20,000 x 128 -> 40 4.5 against
+  // 6.1).  Within it, 16 rows a workgroup where they are all there are or workgroups are few (50 x 4,096 -> 96 3.8
+  // against 4.4), and long sums in flight twice (1 x 65,536 -> 4,096 36 against 41; 1 x 4,096 -> 8,192 5.2 both); long
+  // sums of few workgroups too (64 x 4,096 -> 4,096 5.6 against 7.1; 100 x 1,024 -> 4,096 4.7 against 4.3), and 64
+  // rows where that still fits at once (333 x 8,192 -> 1,000 10.6 against 13.1; 100 x 1,024 -> 2 x 2,816 5.9 against 5.7).
   if (p.M <= 16 || small <= 96) {
     if (p.K > 8192)
       launch_small<BF16, SWIGLU, 1, 2, 8, 2>(p, stream);
     else
       launch_small<BF16, SWIGLU, 1, 2, 8, 1>(p, stream);
-  } else if (p.M <= 32 || small <= 640) {
-    if (small <= 256 && p.K >= 2048)
-      launch_small<BF16, SWIGLU, 2, 2, 8, 1>(p, stream);
+  } else if (p.M <= 32 || small <= (p.K <= 256 ? 1280 : 704)) {
+    if (p.K >= 2048 && small <= 256)
+      launch_small<BF16, SWIGLU, 2, 2, 4, 2>(p, stream);
+    else if (p.K >= 2048 && tiles(64, 32) <= 256)
+      launch_small<BF16, SWIGLU, 4, 2, 8, 1>(p, stream);
     else
       launch_small<BF16, SWIGLU, 2, 2, 4, 1>(p, stream);
+    // The largest tiles where their last round leaves few places (8,000 x 4,096 -> 4,096 117 against 127 of half of
+    // them, 4,000 x 1,024 -> 4,096 22.3 against 23.5; 5,000 x 1,024 -> 4,096, a second round of 64, 35 against 29).
   } else if (p.K > 128 && (idle(whole, 256) <= 80 || idle(whole, 256) <= whole / 8)) {
     launch_tile<BF16, SWIGLU, 8, 4>(p, stream);
+    // Half of them for the rest of the long launches, and for short sums, most of whose time is the result's
+    // (6,000 x 1,024 -> 4,096 33.6 against 36.1; 3,000 x 256 -> 2 x 1,024 7.8 against 8.4).
   } else if (half >= 700 || (half >= 160 && p.K <= 256)) {
     launch_tile<BF16, SWIGLU, 8, 2>(p, stream);
+    // In between two workgroups to a compute unit, of 128 rows unless a round would be mostly empty (4,000 x 2,048 ->
+    // 1,024 14.5 against 14.9; 1,500 x 1,024 -> 2 x 2,816 17.8 against 19.8), and two groups that share a long sum
+    // where there is one workgroup to a unit (1,419 x 2,048 -> 1,024 8.9 against 9.7; 500 x 1,024 -> 4,096 7.4 against 7.0).
   } else if (idle(tiles(128, 128), 512) <= 300) {
     launch_mid<BF16, SWIGLU, 8, 1>(p, stream);
   } else if (tiles(64, 128) <= 256 && p.K >= 2048) {

@@ -78,7 +78,8 @@ def test_product(ctx, qattn, M, K, N, bf16):
 
 
 GATE_CASES = [(1, 32, 32), (1, 4096, 96), (5, 160, 64), (16, 1024, 2816), (17, 96, 32), (50, 1024, 1024), (64, 256, 96),
-              (130, 1056, 160), (257, 128, 2816), (700, 512, 416), (1500, 1024, 1024), (3000, 64, 288)]
+              (130, 1056, 160), (257, 128, 2816), (700, 512, 416), (1500, 1024, 1024), (3000, 64, 288), (3900, 192, 1952), (5001, 288, 2080),
+              (40, 4096, 2048), (90, 4096, 1056), (9, 8224, 64)]
 
 
 @pytest.mark.parametrize("bf16", [False, True])
@@ -158,4 +159,47 @@ def test_a_row_does_not_depend_on_its_batch(ctx, qattn, K, N, swiglu):
         ctx.synchronize()
         assert np.array_equal(y.read(np.uint16, (count, N)), whole[first:first + count]), (first, count)
     for b in (bx, bs, y, w):
+        b.free()
+
+
+def halves(M):
+    """(t, scale) whose f32 products lie next to a border of fp16: rounded to f32 first they go one way, at once the other."""
+    rng = rng_of(11)
+    t, scale = np.zeros(0, np.int64), np.zeros(0, np.float32)
+    while len(t) < M:
+        a, b = rng.integers(1, 128, 1 << 20), (1 + rng.random(1 << 20)).astype(np.float32)
+        exact = a.astype(np.float64) * b.astype(np.float64)
+        twice = exact.astype(np.float32).astype(np.float16)
+        hit = twice != exact.astype(np.float16)
+        t, scale = np.concatenate([t, a[hit]]), np.concatenate([scale, b[hit]])
+    return t[:M], scale[:M]
+
+
+@pytest.mark.parametrize("swiglu", [False, True])
+def test_a_rounding_does_not_depend_on_the_kernel(ctx, qattn, swiglu):
+    """Products are rounded to f32, then to 16 bits, in every kernel and at every place of a column in it."""
+    M, K, N = 6000, 32, 800 if swiglu else 795
+    t, scale = halves(M)
+    x = np.zeros((M, K), np.int8)
+    x[:, 0], x[:, 1] = t, 1
+    codes = np.full((2 * N if swiglu else N, K), 8, np.uint8)
+    codes[:, 0] += 1                                   # weights of 1 in the first column
+    if swiglu:
+        codes[N:, 0], codes[N:, 1] = 8, 9              # the up product is the row's scale
+    groups, scales = np.full((len(codes), 1), 1 | 8 << 4, np.uint8), np.ones(len(codes), np.float32)
+    image = qattn.w4_pack(w4_ref.nibbles(codes), groups, scales)
+    ldy = -(-N // 8) * 8
+    w, bx, bs, y = ctx.upload(image), ctx.upload(x), ctx.upload(scale), ctx.alloc(M * ldy * 2)
+    call = ctx.w4_matmul_swiglu if swiglu else ctx.w4_matmul
+    seen = []
+    for count in (M, 3000, 1200, 300, 40, 9):
+        call(bx.ptr, bs.ptr, count, K, w.ptr, image.nbytes, N, y.ptr, ldy=ldy)
+        ctx.synchronize()
+        seen.append(y.read(np.uint16, (M, ldy))[:count, :N])
+        assert np.array_equal(seen[-1], seen[0][:count]), count
+    assert (seen[0] == seen[0][:, :1]).all()           # a row's columns are all alike
+    if not swiglu:
+        want = (t.astype(np.float32) * scale).astype(np.float16)
+        assert np.array_equal(seen[0][:, 0], want.view(np.uint16))
+    for b in (w, bx, bs, y):
         b.free()

@@ -21,7 +21,7 @@ def kernels(tmp_path_factory):
                     "-packed-fp32-ops", "--cuda-device-only", "-S", "-o", out, SOURCE], check=True, capture_output=True)
     found, name = {}, None
     for line in open(out):
-        start = re.match(r"(_ZN5qattn\w*w4_(?:tile|mid)_kernel\w+):", line)
+        start = re.match(r"(_ZN5qattn\w*w4_(?:tile|mid|small)_kernel\w+):", line)
         if start:
             name = start.group(1)
             found[name] = []
@@ -55,14 +55,19 @@ def events(lines):
 
 
 def test_every_published_x_tile_has_landed(kernels):
-    assert sum("w4_tile" in name for name in kernels) == 8 and sum("w4_mid" in name for name in kernels) == 12
+    assert [sum("w4_" + kind in name for name in kernels) for kind in ("tile", "mid", "small")] == [8, 12, 20]
     for name, lines in kernels.items():
         prologue, loop = events(lines)
-        mf, second = [int(v) for v in re.findall(r"Li(\d+)E", name)][:2]
-        # LDS-DMA loads of an X tile, per wavefront, and the barriers ahead of the loop: the first kernel reads X tile 0
-        # before its loop, the other in it.
-        group, ahead = (mf // second, 1) if "w4_tile" in name else (mf // 2, 0)
-        assert sum(e[0] == "wait" for e in prologue) == ahead and sum(e[0] == "wait" for e in loop) == 4, name
+        sizes = [int(v) for v in re.findall(r"Li(\d+)E", name)]
+        # LDS-DMA loads of an X tile, per wavefront, and the waits ahead of the loop and in it: the first kernel reads X
+        # tile 0 before its loop, the others in it; a wavefront of the last waits for its own X alone.
+        if "w4_tile" in name:
+            group, ahead, waits = sizes[0] // sizes[1], 1, 4
+        elif "w4_mid" in name:
+            group, ahead, waits = sizes[0] // 2, 0, 4
+        else:
+            group, ahead, waits = 2 * sizes[0], 0, sizes[3]
+        assert sum(e[0] == "wait" for e in prologue) == ahead and sum(e[0] == "wait" for e in loop) == waits, name
         issued, dma, barrier = 0, [], 0  # dma: issue numbers of the LDS-DMA loads
         for event in prologue + PASSES * loop:
             if event[0] == "wait":
