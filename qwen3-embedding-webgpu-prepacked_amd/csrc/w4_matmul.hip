@@ -253,6 +253,11 @@ __device__ inline uint32_t load1s(__amdgpu_buffer_rsrc_t rs, uint32_t off, uint3
 __device__ inline void store16(u32x4 v, __amdgpu_buffer_rsrc_t rs, uint32_t off) {
   __builtin_amdgcn_raw_buffer_store_b128(v, rs, off, 0, 0);
 }
+// Past the L2, which a large result would only sweep: the tiles of many rows take 4 to 9 % less, and what reads the
+// result next takes at most as much longer (8,000 x 4,096: 60.8 us for both against 60.4; 20,000 x 2,816: 165 against 171).
+__device__ inline void store16_far(u32x4 v, __amdgpu_buffer_rsrc_t rs, uint32_t off) {
+  __builtin_amdgcn_raw_buffer_store_b128(v, rs, off, 0, 2);
+}
 __device__ inline void store2(uint16_t v, __amdgpu_buffer_rsrc_t rs, uint32_t off) {
   __builtin_amdgcn_raw_buffer_store_b16(v, rs, off, 0, 0);
 }
@@ -695,7 +700,7 @@ __global__ __launch_bounds__(128 * NWN, 2) void w4_tile_kernel(W4Product p, int 
       const int row = kRowsPer * i + lane / kPieces, c = lane % kPieces;
       const u32x4 v = *reinterpret_cast<const u32x4*>(place(row, c));
       const int m = row0 + kRows * pass + row, n = col0 + 8 * c;
-      store16(v, yrs, m < rows && n + 8 <= n_out ? ((uint32_t)m * (uint32_t)p.ldy + (uint32_t)n) * 2u : kNowhere);
+      store16_far(v, yrs, m < rows && n + 8 <= n_out ? ((uint32_t)m * (uint32_t)p.ldy + (uint32_t)n) * 2u : kNowhere);
     }
     // A last piece of fewer than 8 columns goes element by element.
     const int part = (n_out - col0) >> 3;
@@ -724,13 +729,16 @@ hipError_t launch(const W4Product& p, hipStream_t stream) {
   // Workgroups that fit the card at once less those of a launch's last round.
   const auto idle = [](int64_t groups, int at_once) { return (at_once - groups % at_once) % at_once; };
   const int64_t small = tiles(32, 32), whole = tiles(256, 256), half = tiles(256, 128);
-  // Microseconds on one MI355X, M x K -> N: the variant taken against the next best one's.  Launches that the card
-  // holds at once go to the few-rows kernel, whose wavefronts share K (700 x 256 -> 1,024 3.9 against 4.9 of the next
-  // kernel, 200 x 1,024 -> 4,096 7.1 against 6.4); short sums let more of them through (20,000 x 128 -> 40 4.5 against
-  // 6.1).  Within it, 16 rows a workgroup where they are all there are or workgroups are few (50 x 4,096 -> 96 3.8
-  // against 4.4), and long sums in flight twice (1 x 65,536 -> 4,096 36 against 41; 1 x 4,096 -> 8,192 5.2 both); long
-  // sums of few workgroups too (64 x 4,096 -> 4,096 5.6 against 7.1; 100 x 1,024 -> 4,096 4.7 against 4.3), and 64
-  // rows where that still fits at once (333 x 8,192 -> 1,000 10.6 against 13.1; 100 x 1,024 -> 2 x 2,816 5.9 against 5.7).
+  // Figures: microseconds on one MI355X, M x K -> N, the variant taken and the next best one.
+  //
+  // Few rows, or few tiles: wavefronts that share K fill the card (700 x 256 -> 1,024 3.9 and 4.9 in tiles of 64;
+  // 700 x 2,048 -> 1,024 7.4 and 8.9; but 250 x 1,024 -> 4,096, 1,024 tiles, 7.5 and 6.4).  Sums of one or two blocks let
+  // more tiles through (20,000 x 128 -> 40 4.5 and 6.1).  Of these kernels
+  // - 16 rows where there are no more or tiles are few (50 x 4,096 -> 96 3.8, of 32 rows 4.4), long sums two blocks
+  //   ahead (1 x 65,536 -> 4,096 36 and 41; 1 x 4,096 -> 8,192 5.2 either way);
+  // - 32 rows two blocks ahead for long sums of few tiles (64 x 4,096 -> 4,096 5.6 and 7.1), 64 rows for long sums of
+  //   more (333 x 8,192 -> 1,000 10.6 and 13.1), else 32 rows one block ahead (100 x 1,024 -> 4,096 4.3, two ahead 4.7;
+  //   50 x 1,024 -> 2 x 2,816 4.1, of 64 rows 4.2).
   if (p.M <= 16 || small <= 96) {
     if (p.K > 8192)
       launch_small<BF16, SWIGLU, 1, 2, 8, 2>(p, stream);
@@ -743,17 +751,17 @@ hipError_t launch(const W4Product& p, hipStream_t stream) {
       launch_small<BF16, SWIGLU, 4, 2, 8, 1>(p, stream);
     else
       launch_small<BF16, SWIGLU, 2, 2, 4, 1>(p, stream);
-    // The largest tiles where their last round leaves few places (8,000 x 4,096 -> 4,096 117 against 127 of half of
-    // them, 4,000 x 1,024 -> 4,096 22.3 against 23.5; 5,000 x 1,024 -> 4,096, a second round of 64, 35 against 29).
+    // The largest tiles where their last round leaves few places (8,000 x 4,096 -> 4,096 117, in halves of them 127;
+    // 4,000 x 1,024 -> 4,096 22 and 23.5; but 5,000 x 1,024 -> 4,096, a second round of 64 tiles, 35 and 29).
   } else if (p.K > 128 && (idle(whole, 256) <= 80 || idle(whole, 256) <= whole / 8)) {
     launch_tile<BF16, SWIGLU, 8, 4>(p, stream);
     // Half of them for the rest of the long launches, and for short sums, most of whose time is the result's
-    // (6,000 x 1,024 -> 4,096 33.6 against 36.1; 3,000 x 256 -> 2 x 1,024 7.8 against 8.4).
+    // (6,000 x 1,024 -> 4,096 33.6 and 36.1; 3,000 x 256 -> 2 x 1,024 7.8 and 8.4).
   } else if (half >= 700 || (half >= 160 && p.K <= 256)) {
     launch_tile<BF16, SWIGLU, 8, 2>(p, stream);
-    // In between two workgroups to a compute unit, of 128 rows unless a round would be mostly empty (4,000 x 2,048 ->
-    // 1,024 14.5 against 14.9; 1,500 x 1,024 -> 2 x 2,816 17.8 against 19.8), and two groups that share a long sum
-    // where there is one workgroup to a unit (1,419 x 2,048 -> 1,024 8.9 against 9.7; 500 x 1,024 -> 4,096 7.4 against 7.0).
+    // In between two workgroups to a compute unit, of 128 rows unless a round would be mostly empty (2,000 x 4,096 ->
+    // 4,096 38 and, of 64 rows, 47; but 1,500 x 1,024 -> 2 x 2,816 19.8 and 17.8), and two groups that share a long sum
+    // where there is one workgroup to a unit (1,419 x 2,048 -> 1,024 8.9 and 9.7; 500 x 1,024 -> 4,096 7.4 and 7.0).
   } else if (idle(tiles(128, 128), 512) <= 300) {
     launch_mid<BF16, SWIGLU, 8, 1>(p, stream);
   } else if (tiles(64, 128) <= 256 && p.K >= 2048) {
