@@ -1788,6 +1788,136 @@ napi_value SharedRunInfo(napi_env env, napi_callback_info info) {
   return out;
 }
 
+// ---- a forward with 8-bit activations: rows into 8 bits, products with 4-bit weights ----------------------
+
+// quantizeQ8(ctx, {x, codes, scales, rows, width, xStride, codesStride, dtype})  (qattn_quantize_q8)
+// rmsnormQ8(ctx, the same and {weight, eps, residual, residualStride, sum, sumStride})  (qattn_rmsnorm_q8)
+napi_value RowsQ8(napi_env env, napi_callback_info info, bool norm) {
+  napi_value argv[2];
+  if (!args_of(env, info, 2, argv)) return nullptr;
+  Ctx* c = live_ctx(env, argv[0]);
+  if (!c) return nullptr;
+  Tensor x, codes, scales, weight, residual, sum;
+  if (!tensor_of(env, argv[1], "x", c, true, &x) || !tensor_of(env, argv[1], "codes", c, true, &codes) ||
+      !tensor_of(env, argv[1], "scales", c, true, &scales))
+    return nullptr;
+  if (norm && (!tensor_of(env, argv[1], "weight", c, true, &weight) || !tensor_of(env, argv[1], "residual", c, false, &residual) ||
+               !tensor_of(env, argv[1], "sum", c, false, &sum)))
+    return nullptr;
+  Numbers n{env, argv[1]};
+  const int64_t rows = n.wide("rows", 0);
+  const int32_t width = n.i32("width", 0), dtype = n.i32("dtype", QATTN_DTYPE_F16);
+  const int64_t xs = n.wide("xStride", width), cs = n.wide("codesStride", width);
+  const int64_t rs = n.wide("residualStride", width);
+  const int64_t ss = n.wide("sumStride", !sum.buf ? width : sum.ptr() == x.ptr() ? xs : sum.ptr() == residual.ptr() ? rs : width);
+  const double eps = n.real("eps", 1e-6);
+  if (!n.ok) return nullptr;
+  const char* past = !x.holds(rows, xs, width, 2)                                ? "x"
+                     : !codes.holds(rows, cs, width, 1)                          ? "codes"
+                     : !scales.holds(rows, 1, 1, 4)                              ? "scales"
+                     : weight.buf && !weight.holds(1, width, width, 4)           ? "weight"
+                     : residual.buf && !residual.holds(rows, rs, width, 2)       ? "residual"
+                     : sum.buf && !sum.holds(rows, ss, width, 2)                 ? "sum"
+                                                                                 : nullptr;
+  if (past) {
+    past_buffer(env, past);
+    return nullptr;
+  }
+  int8_t* const out = static_cast<int8_t*>(codes.ptr());
+  float* const scale = static_cast<float*>(scales.ptr());
+  const int rc = norm ? qattn_rmsnorm_q8(c->ctx, x.ptr(), xs, residual.ptr(), rs, sum.ptr(), ss, static_cast<const float*>(weight.ptr()),
+                                         out, cs, scale, rows, width, dtype, eps, nullptr)
+                      : qattn_quantize_q8(c->ctx, x.ptr(), xs, out, cs, scale, rows, width, dtype, nullptr);
+  if (rc) return throw_qattn(env, rc, c->ctx);
+  return undefined(env);
+}
+napi_value QuantizeQ8(napi_env env, napi_callback_info info) { return RowsQ8(env, info, false); }
+napi_value RmsnormQ8(napi_env env, napi_callback_info info) { return RowsQ8(env, info, true); }
+
+// w4Matmul(ctx, {x, xScale, rows, k, w, wBytes, n, y, xStride, yStride, dtype, swiglu}): with swiglu n is the
+// count of features (qattn_w4_matmul, qattn_w4_matmul_swiglu)
+napi_value W4Matmul(napi_env env, napi_callback_info info) {
+  napi_value argv[2];
+  if (!args_of(env, info, 2, argv)) return nullptr;
+  Ctx* c = live_ctx(env, argv[0]);
+  if (!c) return nullptr;
+  Tensor x, scale, w, y;
+  if (!tensor_of(env, argv[1], "x", c, true, &x) || !tensor_of(env, argv[1], "xScale", c, true, &scale) ||
+      !tensor_of(env, argv[1], "w", c, true, &w) || !tensor_of(env, argv[1], "y", c, true, &y))
+    return nullptr;
+  Numbers n{env, argv[1]};
+  const int32_t rows = n.i32("rows", 0), k = n.i32("k", 0), cols = n.i32("n", 0), dtype = n.i32("dtype", QATTN_DTYPE_F16);
+  const bool swiglu = n.i32("swiglu", 0) != 0;
+  const int64_t size = n.wide("wBytes", (int64_t)w.buf->bytes - w.off), ldx = n.wide("xStride", k), ldy = n.wide("yStride", cols);
+  if (!n.ok) return nullptr;
+  const char* past = !x.holds(rows, ldx, k, 1)                             ? "x"
+                     : !scale.holds(rows, 1, 1, 4)                         ? "xScale"
+                     : size > (int64_t)w.buf->bytes - w.off                ? "w"
+                     : !y.holds(rows, ldy, cols, 2)                        ? "y"
+                                                                           : nullptr;
+  if (past) {
+    past_buffer(env, past);
+    return nullptr;
+  }
+  const int rc = (swiglu ? qattn_w4_matmul_swiglu : qattn_w4_matmul)(c->ctx, static_cast<const int8_t*>(x.ptr()), ldx,
+                                                                     static_cast<const float*>(scale.ptr()), rows, k, w.ptr(), size,
+                                                                     cols, y.ptr(), ldy, dtype, nullptr);
+  if (rc) return throw_qattn(env, rc, c->ctx);
+  return undefined(env);
+}
+
+// w4Image(kind, k, n, data...) -> Uint8Array, the image of 4-bit weights on the host:
+//   'pack', codes, groups, scales (qattn_w4_pack); 'quantize', rows of f32 (qattn_w4_quantize);
+//   'q4', a tile32-compact Q4_0 tensor (qattn_w4_from_q4)
+napi_value W4Image(napi_env env, napi_callback_info info) {
+  napi_value argv[6];
+  size_t count = 6;
+  NAPI_OK(env, napi_get_cb_info(env, info, &count, argv, nullptr, nullptr));
+  char kind[16] = "";
+  size_t length = 0;
+  int64_t k, n;
+  void* data[3] = {};
+  size_t bytes[3] = {};
+  bool ok = count >= 4 && napi_get_value_string_utf8(env, argv[0], kind, sizeof kind, &length) == napi_ok && get_i64(env, argv[1], &k) &&
+            get_i64(env, argv[2], &n) && k >= 0 && k <= INT32_MAX && n >= 0 && n <= INT32_MAX;
+  const bool pack = !std::strcmp(kind, "pack"), rows = !std::strcmp(kind, "quantize");
+  ok = ok && (pack || rows || !std::strcmp(kind, "q4")) && count >= (pack ? 6u : 4u);
+  for (int i = 0; ok && i < (pack ? 3 : 1); ++i) ok = typed_bytes(env, argv[3 + i], &data[i], &bytes[i]);
+  if (!ok) {
+    napi_throw_type_error(env, nullptr, "expected ('pack' | 'quantize' | 'q4', k, n, typed arrays)");
+    return nullptr;
+  }
+  const int64_t size = qattn_w4_bytes((int32_t)k, (int32_t)n);
+  if (size < 0) {
+    napi_throw_range_error(env, nullptr, ("no 4-bit weight has k=" + std::to_string(k) + ", n=" + std::to_string(n)).c_str());
+    return nullptr;
+  }
+  const uint64_t cells = (uint64_t)k * (uint64_t)n;
+  if (pack ? bytes[0] != cells / 2 || bytes[1] != cells / 32 || bytes[2] != (uint64_t)n * 4 : rows && bytes[0] != cells * 4) {
+    napi_throw_range_error(env, nullptr, pack ? "codes [n][k / 2], groups [n][k / 32] and scales [n] are of other sizes"
+                                              : "rows of f32 [n][k] are of another size");
+    return nullptr;
+  }
+  if (!pack && !rows && (int64_t)bytes[0] < qattn_q4_compact_bytes((int32_t)k, (int32_t)n)) {
+    napi_throw_range_error(env, nullptr, "the Q4_0 tensor holds fewer weights");
+    return nullptr;
+  }
+  if ((pack && (uintptr_t)data[2] % 4) || (rows && (uintptr_t)data[0] % 4)) {
+    napi_throw_range_error(env, nullptr, "f32 values at an odd address");
+    return nullptr;
+  }
+  napi_value ab, out;
+  void* image = nullptr;
+  NAPI_OK(env, napi_create_arraybuffer(env, (size_t)size, &image, &ab));
+  const int rc = pack   ? qattn_w4_pack(static_cast<uint8_t*>(data[0]), static_cast<uint8_t*>(data[1]), static_cast<float*>(data[2]),
+                                        (int32_t)k, (int32_t)n, image, size)
+                 : rows ? qattn_w4_quantize(static_cast<float*>(data[0]), k, (int32_t)k, (int32_t)n, image, size)
+                        : qattn_w4_from_q4(data[0], (int64_t)bytes[0], (int32_t)k, (int32_t)n, image, size);
+  if (rc) return throw_qattn(env, rc, nullptr);
+  NAPI_OK(env, napi_create_typedarray(env, napi_uint8_array, (size_t)size, ab, 0, &out));
+  return out;
+}
+
 napi_value AbiVersion(napi_env env, napi_callback_info) {
   napi_value v;
   napi_create_int32(env, qattn_abi_version(), &v);
@@ -1820,7 +1950,9 @@ napi_value Init(napi_env env, napi_value exports) {
       {"kvRead", KvRead},             {"createSharedRun", CreateSharedRun},
       {"updateSharedRun", UpdateSharedRun}, {"rebindSharedRun", RebindSharedRun},
       {"encodeSharedRun", EncodeSharedRun}, {"destroySharedRun", DestroySharedRun},
-      {"sharedRunInfo", SharedRunInfo},
+      {"sharedRunInfo", SharedRunInfo}, {"quantizeQ8", QuantizeQ8},
+      {"rmsnormQ8", RmsnormQ8},       {"w4Matmul", W4Matmul},
+      {"w4Image", W4Image},
   };
   for (const Fn& f : fns) {
     napi_value fn;

@@ -214,6 +214,38 @@ export class SharedPrefixAttention {
   destroyRun(run: SharedRun): void;
 }
 
+// ---- a forward with 8-bit activations: rows into 8 bits, their products with 4-bit weights.
+/** Strides in elements (default the width), offsets in bytes. */
+export interface RowsQ8Options { dtype?: DtypeName; xStride?: number; xOffset?: number }
+export interface NormQ8Options extends RowsQ8Options {
+  /** Added to x; the sum goes to `sum`, which may be x or residual. */
+  residual?: DeviceBuffer; sum?: DeviceBuffer; eps?: number;
+  residualStride?: number; sumStride?: number; residualOffset?: number; sumOffset?: number;
+}
+/** `capacity` rows of `width` 8-bit codes and a Float32 scale each. */
+export class EightBitRows {
+  constructor(context: DeviceContext, capacity: number, width: number);
+  readonly codes: DeviceBuffer;
+  readonly scales: DeviceBuffer;
+  quantize(x: DeviceBuffer, rows: number, options?: RowsQ8Options): void;
+  /** weight: Float32 [width], on the device. */
+  rmsnorm(x: DeviceBuffer, weight: DeviceBuffer, rows: number, options?: NormQ8Options): void;
+  destroy(): void;
+}
+export interface FourBitWeight { k: number; n: number; buffer: DeviceBuffer }
+export interface FourBitOptions { dtype?: DtypeName; yStride?: number; yOffset?: number }
+/** 4-bit weights with whole-number group scales, laid out on the host, and products with them. */
+export class FourBitMatmul {
+  constructor(context: DeviceContext);
+  quantize(rows: Float32Array, k: number, n: number): FourBitWeight;
+  /** codes [n][k / 2], even columns low; groups [n][k / 32], multiplier | zero << 4; scales [n]. */
+  pack(codes: Uint8Array, groups: Uint8Array, scales: Float32Array, k: number, n: number): FourBitWeight;
+  upload(model: PrepackedModel, name: string): FourBitWeight;
+  run(x: EightBitRows, rows: number, weight: FourBitWeight, y: DeviceBuffer, options?: FourBitOptions): void;
+  /** weight: [gate | up]; y has n / 2 columns. */
+  runSwiglu(x: EightBitRows, rows: number, weight: FourBitWeight, y: DeviceBuffer, options?: FourBitOptions): void;
+}
+
 // ---- the whole model (the reference's Qwen3WebGPUModel / Qwen3ExecutionPlan, model.ts:49-255).
 /** Stage names of a profiled run, in order (model.ts:157-168). */
 export type ModelStage = 'embedding_norm' | 'qkv' | 'rope_attention' | 'attention_output' | 'post_attention_norm'

@@ -3,7 +3,8 @@
 // engine surface).
 const { Qwen3EmbeddingEngine, packPadded, packVarlen, cuSeqlensOf } = require('./embedding-engine');
 const {
-  DeviceContext, DeviceBuffer, CausalAttentionKernel, CompactQ4Matmul, RotaryPositions, PagedKvCache, SharedPrefixAttention, MASK,
+  DeviceContext, DeviceBuffer, CausalAttentionKernel, CompactQ4Matmul, RotaryPositions, PagedKvCache, SharedPrefixAttention, EightBitRows,
+  FourBitMatmul, MASK,
 } = require('./ops');
 const { HipAttentionRuntime, HipAttentionPlan } = require('./runtime');
 const { HipQwen3Model, HipQwen3Plan, HipQwen3Runtime } = require('./model');
@@ -22,6 +23,8 @@ module.exports = {
   RotaryPositions,
   PagedKvCache,
   SharedPrefixAttention,
+  EightBitRows,
+  FourBitMatmul,
   DeviceContext,
   DeviceBuffer,
   MASK,

@@ -242,7 +242,89 @@ class SharedPrefixAttention {
   }
 }
 
+// ---- a forward with 8-bit activations (no counterpart in the reference, whose activations are f16): a stage
+// hands the next one rows of 8-bit codes with a scale each, and their products with 4-bit weights run in whole
+// numbers.
+
+// Device memory for `capacity` rows of `width` 8-bit codes and their f32 scales.
+class EightBitRows {
+  constructor(context, capacity, width) {
+    this.context = context;
+    Object.assign(this, { capacity, width, codes: context.alloc(capacity * width), scales: context.alloc(capacity * 4) });
+  }
+
+  _options(x, rows, options) {
+    return Object.assign({}, options, {
+      x: x.handle, codes: this.codes.handle, scales: this.scales.handle, rows, width: this.width,
+      dtype: codeOf(DTYPE, options.dtype || 'f16', 'dtype'),
+    });
+  }
+
+  // Rows of x as they are ({ xStride, xOffset, dtype }).
+  quantize(x, rows, options = {}) {
+    this.context.addon.quantizeQ8(this.context.handle, this._options(x, rows, options));
+  }
+
+  // The RMSNorm of x, or of x + residual, which goes to `sum` ({ residual, sum, eps, strides, offsets, dtype }).
+  rmsnorm(x, weight, rows, options = {}) {
+    this.context.addon.rmsnormQ8(this.context.handle, Object.assign(this._options(x, rows, options), {
+      weight: weight.handle, residual: handleOf(options.residual), sum: handleOf(options.sum),
+    }));
+  }
+
+  destroy() {
+    this.codes.destroy();
+    this.scales.destroy();
+  }
+}
+
+// 4-bit weights [n, k] with whole-number group scales, laid out on the host and kept on the device, and products
+// of EightBitRows with them.
+class FourBitMatmul {
+  constructor(context) {
+    this.context = context;
+  }
+
+  _place(k, n, image) {
+    const buffer = this.context.alloc(image.byteLength);
+    buffer.write(image);
+    return { k, n, buffer };
+  }
+
+  // Float32 rows, rounded to 4 bits.
+  quantize(rows, k, n) { return this._place(k, n, this.context.addon.w4Image('quantize', k, n, rows)); }
+
+  // A caller's own codes [n][k / 2], groups [n][k / 32] (multiplier | zero << 4) and Float32 scales [n].
+  pack(codes, groups, scales, k, n) { return this._place(k, n, this.context.addon.w4Image('pack', k, n, codes, groups, scales)); }
+
+  // A parsed .wgpack's q4_0-tile32-compact tensor; its group scales become multiples of the row's.
+  upload(model, name) {
+    const t = model.tensors.get(name);
+    if (!t) throw new Error(`prepacked model has no tensor ${name}`);
+    if (t.storage !== 'q4_0-tile32-compact') throw new Error(`${name} is not a compact Q4_0 tensor`);
+    const [k, n] = t.dimensions;
+    return this._place(k, n, this.context.addon.w4Image('q4', k, n, new Uint8Array(model.buffer, t.byteOffset, t.byteLength)));
+  }
+
+  _run(x, rows, weight, n, y, options, swiglu) {
+    if (x.width !== weight.k) throw new Error(`rows of ${x.width} codes meet weights of ${weight.k} columns`);
+    this.context.addon.w4Matmul(this.context.handle, Object.assign({}, options, {
+      x: x.codes.handle, xScale: x.scales.handle, rows, k: weight.k, w: weight.buffer.handle, n, y: y.handle, swiglu,
+      dtype: codeOf(DTYPE, options.dtype || 'f16', 'dtype'),
+    }));
+  }
+
+  // y [rows, n] = x W^T ({ yStride, yOffset, dtype }); yStride a multiple of 8, by default n.
+  run(x, rows, weight, y, options = {}) { this._run(x, rows, weight, weight.n, y, options, 0); }
+
+  // y [rows, n / 2] = swiglu of a [gate | up] weight's products.
+  runSwiglu(x, rows, weight, y, options = {}) {
+    if (weight.n % 64) throw new Error(`${weight.n} weight rows are no [gate | up] of whole blocks of 32`);
+    this._run(x, rows, weight, weight.n / 2, y, options, 1);
+  }
+}
+
 module.exports = {
   DeviceContext, DeviceBuffer, CausalAttentionKernel, CompactQ4Matmul, RotaryPositions, PagedKvCache,
-  SharedPrefixAttention, MASK,
+  SharedPrefixAttention, EightBitRows, FourBitMatmul, MASK,
 };
