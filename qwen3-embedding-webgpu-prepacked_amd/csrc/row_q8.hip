@@ -30,13 +30,16 @@ __device__ inline u32x2 codes8(const float* t, float factor) {
   return u32x2{pack(c[0], c[1], c[2], c[3]), pack(c[4], c[5], c[6], c[7])};
 }
 
-// T threads to a row, C pieces of 8 elements to a thread.
+// T threads to a row, C pieces of 8 elements to a thread; memory is the bound.  Up to 512 elements a row takes as many
+// lanes as it fills, so that a wavefront holds several narrow ones, and up to 2048 one wavefront, which needs no
+// barrier; more take as many threads as leave two pieces to each, for more loads in flight.
 template <bool BF16, bool NORM, bool SUM, int T, int C>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void row_q8_kernel(RowQ8 p) {
   constexpr int kRows = T < 256 ? 256 / T : 1, kWaves = T / 64;
+  static_assert(T <= 64 || T >= 256, "rows that share a workgroup are within a wavefront each");
   const int tid = threadIdx.x % T;
   const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / T;
-  if (row >= p.rows) return;  // T > 64: one row to a workgroup, so this is uniform
+  if (row >= p.rows) return;  // T > 64: one row to a workgroup, so this is uniform; else the T lanes leave together
   const uint16_t* const x = static_cast<const uint16_t*>(p.x) + row * p.x_stride;
   u32x4 a[C], r[C];
 #pragma unroll
@@ -94,7 +97,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void row_q8_kernel(RowQ8 p) {
     }
   }
 #pragma unroll
-  for (int d = 32; d; d >>= 1) {
+  for (int d = T < 64 ? T / 2 : 32; d; d >>= 1) {
     if constexpr (NORM) squares += __shfl_xor(squares, d, 64);
     most = max(most, (uint32_t)__shfl_xor((int)most, d, 64));
   }
@@ -137,14 +140,28 @@ void launch(const RowQ8& p, hipStream_t stream) {
   hipLaunchKernelGGL((row_q8_kernel<BF16, NORM, SUM, T, C>),                                                       \
                      dim3((unsigned)((p.rows + (T < 256 ? 256 / T : 1) - 1) / (T < 256 ? 256 / T : 1))),          \
                      dim3(T < 256 ? 256 : T), 0, stream, p)
-  if (p.width <= 512)
+  // Microseconds on one MI355X, with a residual's sum where not said otherwise, the variant taken and others: 20,000 x 64
+  // 4.5, a wavefront to a row 9.2; 20,000 x 256 8.5 and 10.9; 20,000 x 512 16.9, half a wavefront 17.2; 8,000 x 1,024
+  // 13.9, four pieces to a lane 15.2; 8,000 x 2,048 24.7 (without the norm 10.6), 256 threads 23.9 (11.7); 1,419 x 2,560
+  // without the sum 5.2, four pieces 6.1, one 5.6; 2,000 x 5,000 17.8, four 18.7; 500 x 16,384 14.7, four 15.2.
+  if (p.width <= 64)
+    ROW_Q8(8, 1);
+  else if (p.width <= 128)
+    ROW_Q8(16, 1);
+  else if (p.width <= 256)
+    ROW_Q8(32, 1);
+  else if (p.width <= 512)
     ROW_Q8(64, 1);
   else if (p.width <= 1024)
     ROW_Q8(64, 2);
   else if (p.width <= 2048)
     ROW_Q8(64, 4);
+  else if (p.width <= 4096)
+    ROW_Q8(256, 2);
   else if (p.width <= 8192)
-    ROW_Q8(256, 4);
+    ROW_Q8(512, 2);
+  else if (p.width <= 16384)
+    ROW_Q8(1024, 2);
   else
     ROW_Q8(1024, 4);
 #undef ROW_Q8

@@ -65,11 +65,11 @@ def check_scales(got, want, width, norm):
     assert (np.abs(got - want)[fine] <= want[fine] * scale_bound(width, norm) + 2.0 ** -149).all()
 
 
-WIDTHS = [8, 64, 136, 512, 520, 1000, 1024, 1032, 2048, 2056, 4096, 5000, 8192, 8200, 16384, 32760, 32768]
+WIDTHS = [8, 64, 72, 128, 136, 256, 264, 512, 520, 1000, 1024, 1032, 2048, 2056, 4096, 5000, 8192, 8200, 16384, 32760, 32768]
 
 
 @pytest.mark.parametrize("bf16", [False, True])
-@pytest.mark.parametrize("rows,width", [(3, w) for w in WIDTHS] + [(1, 1024), (5, 1024), (2000, 1024), (777, 136), (301, 2560)])
+@pytest.mark.parametrize("rows,width", [(3, w) for w in WIDTHS] + [(1, 1024), (5, 1024), (2000, 1024), (777, 136), (301, 2560), (2001, 64), (1003, 128), (513, 256), (33, 8)])
 def test_quantize(ctx, qattn, rows, width, bf16):
     print("quantize", rows, width, bf16, flush=True)
     rng = rng_of(rows * 7 + width)
@@ -92,7 +92,7 @@ def test_quantize(ctx, qattn, rows, width, bf16):
 
 
 @pytest.mark.parametrize("bf16", [False, True])
-@pytest.mark.parametrize("rows,width", [(3, w) for w in WIDTHS] + [(1, 1024), (5, 1024), (1419, 1024), (777, 136)])
+@pytest.mark.parametrize("rows,width", [(3, w) for w in WIDTHS] + [(1, 1024), (5, 1024), (1419, 1024), (777, 136), (2001, 64), (1003, 128), (513, 256), (33, 8)])
 @pytest.mark.parametrize("sum_in", [None, "own", "x", "residual"])
 def test_rmsnorm(ctx, qattn, rows, width, bf16, sum_in):
     print("rmsnorm", rows, width, bf16, sum_in, flush=True)
