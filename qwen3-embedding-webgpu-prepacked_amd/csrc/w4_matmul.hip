@@ -734,9 +734,11 @@ void launch_tile(const W4Product& p, hipStream_t stream) {
 template <bool BF16, bool SWIGLU>
 hipError_t launch(const W4Product& p, hipStream_t stream) {
   const auto tiles = [&](int tm, int tn) { return (((int64_t)p.M + tm - 1) / tm) * (((int64_t)p.N + tn - 1) / tn); };
-  // Workgroups that fit the card at once less those of a launch's last round.
+  // Workgroups that fit the card at once less those of a launch's last round; whether so much of a launch's tiles is
+  // rows and columns that there are.
   const auto idle = [](int64_t groups, int at_once) { return (at_once - groups % at_once) % at_once; };
-  const int64_t small = tiles(32, 32), whole = tiles(256, 256), half = tiles(256, 128);
+  const auto full = [&](int tm, int tn, int percent) { return 100 * (int64_t)p.M * p.N >= percent * tiles(tm, tn) * tm * tn; };
+  const int64_t small = tiles(32, 32), whole = tiles(256, 256);
   // Figures: microseconds on one MI355X, M x K -> N, the variant taken and the next best one.
   //
   // Few rows, or few tiles: wavefronts that share K fill the card (700 x 256 -> 1,024 3.9 and 4.9 in tiles of 64;
@@ -759,18 +761,20 @@ hipError_t launch(const W4Product& p, hipStream_t stream) {
       launch_small<BF16, SWIGLU, 4, 2, 8, 1>(p, stream);
     else
       launch_small<BF16, SWIGLU, 2, 2, 4, 1>(p, stream);
-    // The largest tiles where their last round leaves few places (8,000 x 4,096 -> 4,096 117, in halves of them 127;
-    // 4,000 x 1,024 -> 4,096 22 and 23.5; but 5,000 x 1,024 -> 4,096, a second round of 64 tiles, 35 and 29).
-  } else if (p.K > 128 && (idle(whole, 256) <= 80 || idle(whole, 256) <= whole / 8)) {
+    // The largest tiles for long sums where their last round leaves few places (8,000 x 4,096 -> 4,096 112, in halves of
+    // them 122; 2,400 x 1,024 -> 4,096 16.2 and 17.4; gate/up of 20,000 x 1,024 -> 2 x 2,816 121 and 125; but 5,000 x
+    // 1,024 -> 4,096, a second round of 64 tiles, 33 and 27, and 8,000 x 512 -> 4,096 27.5 and 25.6).
+  } else if (p.K >= 1024 && full(256, 256, 80) && (idle(whole, 256) <= 96 || idle(whole, 256) <= whole / 8)) {
     launch_tile<BF16, SWIGLU, 8, 4>(p, stream);
-    // Half of them for the rest of the long launches, and for short sums, most of whose time is the result's
-    // (6,000 x 1,024 -> 4,096 33.6 and 36.1; 3,000 x 256 -> 2 x 1,024 7.8 and 8.4).
-  } else if (half >= 700 || (half >= 160 && p.K <= 256)) {
+    // Half of them where they are enough (1,500 x 1,024 -> 4,096 12.0, of 64 x 128 13.5; 6,000 x 1,024 -> 4,096 29, of 128
+    // x 128 34; 8,000 x 256 -> 4,096 20 and 31; but 20,000 x 1,024 -> 300, a fifth of whose tiles is empty, 14.1 and 13.2).
+  } else if (tiles(256, 128) >= 160 && full(256, 128, 80)) {
     launch_tile<BF16, SWIGLU, 8, 2>(p, stream);
-    // In between two workgroups to a compute unit, of 128 rows unless a round would be mostly empty (2,000 x 4,096 ->
-    // 4,096 38 and, of 64 rows, 47; but 1,500 x 1,024 -> 2 x 2,816 19.8 and 17.8), and two groups that share a long sum
-    // where there is one workgroup to a unit (1,419 x 2,048 -> 1,024 8.9 and 9.7; 500 x 1,024 -> 4,096 7.4 and 7.0).
-  } else if (idle(tiles(128, 128), 512) <= 300) {
+    // In between two workgroups to a compute unit, of 128 rows unless a round would be mostly empty (2,000 x 2,048 -> 2,048
+    // 14.8 and, of 64 rows, 15.2; 100 x 1,024 -> 40,000 12.5 and 13.2; but 3,000 x 1,024 -> 1,024 9.2 and 9.1, and 64 x
+    // 1,024 -> 70,016 18.7 and 13.3), and two groups that share a long sum where there is one workgroup to a unit
+    // (1,419 x 2,048 -> 1,024 8.9 and 9.7; 500 x 1,024 -> 4,096 7.4 and 7.0).
+  } else if (idle(tiles(128, 128), 512) <= 300 && full(128, 128, 70)) {
     launch_mid<BF16, SWIGLU, 8, 1>(p, stream);
   } else if (tiles(64, 128) <= 256 && p.K >= 2048) {
     launch_mid<BF16, SWIGLU, 4, 2>(p, stream);

@@ -79,7 +79,7 @@ def test_product(ctx, qattn, M, K, N, bf16):
 
 GATE_CASES = [(1, 32, 32), (1, 4096, 96), (5, 160, 64), (16, 1024, 2816), (17, 96, 32), (50, 1024, 1024), (64, 256, 96),
               (130, 1056, 160), (257, 128, 2816), (700, 512, 416), (1500, 1024, 1024), (3000, 64, 288), (3900, 192, 1952), (5001, 288, 2080),
-              (40, 4096, 2048), (90, 4096, 1056), (9, 8224, 64)]
+              (40, 4096, 2048), (90, 4096, 1056), (9, 8224, 64), (2401, 1056, 2048)]
 
 
 @pytest.mark.parametrize("bf16", [False, True])
