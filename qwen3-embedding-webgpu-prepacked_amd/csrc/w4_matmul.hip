@@ -93,7 +93,7 @@ __device__ inline float swiglu(float g, float u) {
 template <bool BF16, bool SWIGLU, int MB, int NB, int W, int U>
 __global__ __launch_bounds__(64 * W) void w4_small_kernel(W4Product p, int blocks_m) {
   static_assert(!SWIGLU || NB % 2 == 0, "as many gate tiles as up tiles");
-  static_assert(U >= 1 && U <= 2 && NB <= 2 * U, "two buffers, which take a wavefront's sums in the end");
+  static_assert(U >= 1 && U <= 2 && NB * MB * 1024 <= U * 2048 * MB, "two buffers, which take a wavefront's sums in the end");
   constexpr int kRegion = 2048 * MB;
   __shared__ __attribute__((aligned(1024))) char sX0[W * kRegion];
   __shared__ __attribute__((aligned(1024))) char sX1[U > 1 ? W * kRegion : 16];
@@ -147,17 +147,21 @@ __global__ __launch_bounds__(64 * W) void w4_small_kernel(W4Product p, int block
   i32x4 acc[NB][MB];
 #pragma unroll
   for (int i = 0; i < NB * MB; ++i) acc[i / MB][i % MB] = i32x4{};
-  // Of the 16 x 16 sums (SwiGLU: pairs of them) each of the first wavefronts finishes one; its scales.
-  constexpr int kUnits = SWIGLU ? MB * NB / 2 : MB * NB;
-  static_assert(kUnits <= W, "a wavefront for each");
-  const int my_nb = wave / MB, my_row = 16 * (wave % MB) + l16;
-  float x_scale = 0.f;
-  float4 w_scale = {}, up_scale = {};
-  if (wave < kUnits) {
+  // Of the 16 x 16 sums (SwiGLU: pairs of them) each of the first wavefronts finishes as many; their scales.
+  constexpr int kUnits = SWIGLU ? MB * NB / 2 : MB * NB, kEach = kUnits > W ? kUnits / W : 1;
+  static_assert(kUnits <= W || kUnits % W == 0, "as many for each wavefront");
+  float x_scale[kEach];
+  float4 w_scale[kEach], up_scale[kEach];
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const int unit = wave + W * j, nb = unit / MB, row = 16 * (unit % MB) + l16;
+    x_scale[j] = 0.f;
+    w_scale[j] = up_scale[j] = float4{};
+    if (unit >= kUnits) continue;
     const float4* const scales = reinterpret_cast<const float4*>(p.w + at.scales_at());
-    if (my_row < rows) x_scale = p.x_scale[m0 + my_row];
-    if (tile0 + my_nb < at.tiles) w_scale = scales[4 * (tile0 + my_nb) + q];
-    if (SWIGLU && tile0 + my_nb + (p.N >> 5) < at.tiles) up_scale = scales[4 * (tile0 + my_nb + (p.N >> 5)) + q];
+    if (row < rows) x_scale[j] = p.x_scale[m0 + row];
+    if (tile0 + nb < at.tiles) w_scale[j] = scales[4 * (tile0 + nb) + q];
+    if (SWIGLU && tile0 + nb + (p.N >> 5) < at.tiles) up_scale[j] = scales[4 * (tile0 + nb + (p.N >> 5)) + q];
   }
   __builtin_amdgcn_sched_barrier(0);
   Weights ring[U];
@@ -203,34 +207,39 @@ __global__ __launch_bounds__(64 * W) void w4_small_kernel(W4Product p, int block
 #pragma unroll
   for (int i = 0; i < NB * MB; ++i) *part(wave, i) = acc[i / MB][i % MB];
   __syncthreads();
-  if (wave >= kUnits) return;
-  // Lane (l16, q) holds row l16, columns 4 q .. 4 q + 3 of its 16 x 16.
-  auto sum = [&](int i, float4 scale, float (&f)[4]) W4_INLINE {
-    i32x4 t = *part(0, i);
+  const int n_out = SWIGLU ? p.N >> 1 : p.N;
 #pragma unroll
-    for (int w = 1; w < W; ++w) t += *part(w, i);
-    const float s[4] = {scale.x, scale.y, scale.z, scale.w};
+  for (int j = 0; j < kEach; ++j) {
+    const int unit = wave + W * j;
+    if (unit >= kUnits) return;
+    // Lane (l16, q) holds row l16, columns 4 q .. 4 q + 3 of its 16 x 16.
+    auto sum = [&](int i, float4 scale, float (&f)[4]) W4_INLINE {
+      i32x4 t = *part(0, i);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = (float)t[e] * s[e] * x_scale;
-  };
-  float v[4];
-  sum(wave, w_scale, v);
-  if constexpr (SWIGLU) {
-    float t[4];
-    sum(wave + kUnits, up_scale, t);
+      for (int w = 1; w < W; ++w) t += *part(w, i);
+      const float s[4] = {scale.x, scale.y, scale.z, scale.w};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = swiglu(v[e], t[e]);
-  }
-  const int n_out = SWIGLU ? p.N >> 1 : p.N, n = 16 * (tile0 + my_nb) + 4 * q;
-  if (my_row >= rows || n >= n_out) return;
-  uint16_t* const y = static_cast<uint16_t*>(p.y) + (m0 + my_row) * p.ldy + n;
-  const u32x2 d = narrow4<BF16>(v);
-  if (n + 4 <= n_out) {
-    *reinterpret_cast<u32x2*>(y) = d;
-  } else {
+      for (int e = 0; e < 4; ++e) f[e] = (float)t[e] * s[e] * x_scale[j];
+    };
+    float v[4];
+    sum(unit, w_scale[j], v);
+    if constexpr (SWIGLU) {
+      float t[4];
+      sum(unit + kUnits, up_scale[j], t);
 #pragma unroll
-    for (int e = 0; e < 3; ++e)
-      if (n + e < n_out) y[e] = (uint16_t)(d[e >> 1] >> (16 * (e & 1)));
+      for (int e = 0; e < 4; ++e) v[e] = swiglu(v[e], t[e]);
+    }
+    const int n = 16 * (tile0 + unit / MB) + 4 * q, row = 16 * (unit % MB) + l16;
+    if (row >= rows || n >= n_out) continue;
+    uint16_t* const y = static_cast<uint16_t*>(p.y) + (m0 + row) * p.ldy + n;
+    const u32x2 d = narrow4<BF16>(v);
+    if (n + 4 <= n_out) {
+      *reinterpret_cast<u32x2*>(y) = d;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 3; ++e)
+        if (n + e < n_out) y[e] = (uint16_t)(d[e >> 1] >> (16 * (e & 1)));
+    }
   }
 }
 
@@ -741,14 +750,16 @@ hipError_t launch(const W4Product& p, hipStream_t stream) {
   const int64_t small = tiles(32, 32), whole = tiles(256, 256);
   // Figures: microseconds on one MI355X, M x K -> N, the variant taken and the next best one.
   //
-  // Few rows, or few tiles: wavefronts that share K fill the card (700 x 256 -> 1,024 3.9 and 4.9 in tiles of 64;
-  // 700 x 2,048 -> 1,024 7.4 and 8.9; but 250 x 1,024 -> 4,096, 1,024 tiles, 7.5 and 6.4).  Sums of one or two blocks let
-  // more tiles through (20,000 x 128 -> 40 4.5 and 6.1).  Of these kernels
+  // Few rows, or few tiles: wavefronts that share K fill the card (700 x 256 -> 1,024 3.9 and, in tiles of 64 x 128, 4.9;
+  // 700 x 2,048 -> 1,024 7.3 and 8.8; but 300 x 1,024 -> 4,096, 1,280 tiles, 7.7 and 6.6).  Sums of one or two blocks let
+  // more tiles through (20,000 x 128 -> 40 4.4 and 6.1).  Of these kernels
   // - 16 rows where there are no more or tiles are few (50 x 4,096 -> 96 3.8, of 32 rows 4.4), long sums two blocks
   //   ahead (1 x 65,536 -> 4,096 36 and 41; 1 x 4,096 -> 8,192 5.2 either way);
   // - 32 rows two blocks ahead for long sums of few tiles (64 x 4,096 -> 4,096 5.6 and 7.1), 64 rows for long sums of
   //   more (333 x 8,192 -> 1,000 10.6 and 13.1), else 32 rows one block ahead (100 x 1,024 -> 4,096 4.3, two ahead 4.7;
-  //   50 x 1,024 -> 2 x 2,816 4.1, of 64 rows 4.2).
+  //   50 x 1,024 -> 2 x 2,816 4.1, of 64 rows 4.2);
+  // - beyond, 64 rows and four wavefronts as long as they fit at once (1,000 x 2,048 -> 1,024 7.7 and, in tiles of 64 x
+  //   128, 8.8; 200 x 1,024 -> 4,096 5.9 and 6.4; but 300 x 1,024 -> 4,096 7.7 and 6.6).
   if (p.M <= 16 || small <= 96) {
     if (p.K > 8192)
       launch_small<BF16, SWIGLU, 1, 2, 8, 2>(p, stream);
@@ -761,6 +772,8 @@ hipError_t launch(const W4Product& p, hipStream_t stream) {
       launch_small<BF16, SWIGLU, 4, 2, 8, 1>(p, stream);
     else
       launch_small<BF16, SWIGLU, 2, 2, 4, 1>(p, stream);
+  } else if (tiles(64, 32) <= 512) {
+    launch_small<BF16, SWIGLU, 4, 2, 4, 1>(p, stream);
     // The largest tiles for long sums where their last round leaves few places (8,000 x 4,096 -> 4,096 112, in halves of
     // them 122; 2,400 x 1,024 -> 4,096 16.2 and 17.4; gate/up of 20,000 x 1,024 -> 2 x 2,816 121 and 125; but 5,000 x
     // 1,024 -> 4,096, a second round of 64 tiles, 33 and 27, and 8,000 x 512 -> 4,096 27.5 and 25.6).

@@ -69,6 +69,10 @@ CASES = [(1, 32, 1), (1, 64, 17), (2, 96, 16), (15, 128, 33), (16, 160, 48), (17
          (16, 1024, 4096), (31, 1024, 100), (33, 992, 129), (50, 2048, 1024), (64, 224, 257), (65, 512, 513), (100, 1024, 1001),
          (129, 1056, 640), (255, 288, 1024), (257, 384, 250), (333, 2592, 1001), (500, 1024, 1024), (1000, 96, 77),
          (1419, 2048, 1024), (2049, 1120, 1000), (4000, 128, 4096), (8000, 64, 40)]
+# Each kernel with a last tile of few rows, and columns that end inside its last 16 or its last 8.
+CASES += [(1300, 320, 1003), (1500, 2080, 1023), (4097, 160, 2052), (3841, 288, 4085), (20000, 64, 130), (2400, 256, 2049),
+          (33, 96, 40001), (60, 4096, 1025), (100, 8192, 290), (7, 16384, 50), (2401, 1056, 4090), (1900, 96, 2003),
+          (999, 2080, 1021), (195, 288, 4090), (64, 1024, 20001), (64, 2080, 2045)]
 
 
 @pytest.mark.parametrize("bf16", [False, True])
@@ -78,8 +82,9 @@ def test_product(ctx, qattn, M, K, N, bf16):
 
 
 GATE_CASES = [(1, 32, 32), (1, 4096, 96), (5, 160, 64), (16, 1024, 2816), (17, 96, 32), (50, 1024, 1024), (64, 256, 96),
-              (130, 1056, 160), (257, 128, 2816), (700, 512, 416), (1500, 1024, 1024), (3000, 64, 288), (3900, 192, 1952), (5001, 288, 2080),
-              (40, 4096, 2048), (90, 4096, 1056), (9, 8224, 64), (2401, 1056, 2048)]
+              (130, 1056, 160), (257, 128, 2816), (700, 512, 416), (1500, 1024, 1024), (3000, 64, 288), (3900, 192, 1952),
+              (5001, 288, 2080), (40, 4096, 2048), (90, 4096, 1056), (9, 8224, 64), (2401, 1056, 2048), (199, 1056, 2048),
+              (100, 2080, 2016), (1411, 2080, 512), (1900, 96, 1024)]
 
 
 @pytest.mark.parametrize("bf16", [False, True])

@@ -29,8 +29,10 @@ def get(buf, rows, width, dtype, stride):
 
 
 # Sizes of every kernel of the products.
-@pytest.mark.parametrize("M,K,N,swiglu", [(2500, 1056, 4090, False), (2500, 1024, 2048, True), (3000, 160, 4090, False), (3000, 160, 2048, True), (3000, 128, 2040, False), (1500, 128, 1400, False), (2200, 64, 2050, False),
-                                          (1419, 2048, 1020, False), (1500, 256, 512, True), (700, 96, 1023, False), (333, 2080, 999, False)])
+@pytest.mark.parametrize("M,K,N,swiglu", [(2500, 1056, 4090, False), (2500, 1024, 2048, True), (3000, 160, 4090, False), (3000, 160, 2048, True),
+                                          (3000, 128, 2040, False), (1500, 128, 1400, False), (2200, 64, 2050, False),
+                                          (1419, 2048, 1020, False), (1500, 256, 512, True), (700, 96, 1023, False), (333, 2080, 999, False),
+                                          (1000, 288, 1000, False)])
 def test_products_of_rows_far_apart(ctx, qattn, M, K, N, swiglu):
     print("far", M, K, N, swiglu, flush=True)
     rng = rng_of(M + K + N)

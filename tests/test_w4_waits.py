@@ -55,7 +55,7 @@ def events(lines):
 
 
 def test_every_published_x_tile_has_landed(kernels):
-    assert [sum("w4_" + kind in name for name in kernels) for kind in ("tile", "mid", "small")] == [8, 12, 20]
+    assert [sum("w4_" + kind in name for name in kernels) for kind in ("tile", "mid", "small")] == [8, 12, 24]
     for name, lines in kernels.items():
         prologue, loop = events(lines)
         sizes = [int(v) for v in re.findall(r"Li(\d+)E", name)]
