@@ -39,7 +39,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void row_q8_kernel(RowQ8 p) {
   constexpr int kRows = T < 256 ? 256 / T : 1, kWaves = T / 64;
   static_assert(T <= 64 || T >= 256, "rows that share a workgroup are within a wavefront each");
   const int tid = threadIdx.x % T;
-  const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / T;
+  const int64_t row = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kRows + threadIdx.x / T;
   if (row >= p.rows) return;  // T > 64: one row to a workgroup, so this is uniform; else the T lanes leave together
   const uint16_t* const x = static_cast<const uint16_t*>(p.x) + row * p.x_stride;
   u32x4 a[C], r[C];
@@ -137,10 +137,13 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void row_q8_kernel(RowQ8 p) {
 
 template <bool BF16, bool NORM, bool SUM>
 void launch(const RowQ8& p, hipStream_t stream) {
-#define ROW_Q8(T, C)                                                                                               \
-  hipLaunchKernelGGL((row_q8_kernel<BF16, NORM, SUM, T, C>),                                                       \
-                     dim3((unsigned)((p.rows + (T < 256 ? 256 / T : 1) - 1) / (T < 256 ? 256 / T : 1))),          \
-                     dim3(T < 256 ? 256 : T), 0, stream, p)
+  // A dimension of a grid has to stay below 2^32 threads.
+  const auto grid = [&](int rows) {
+    const int64_t groups = (p.rows + rows - 1) / rows, x = groups < (1 << 20) ? groups : 1 << 20;
+    return dim3((unsigned)x, (unsigned)((groups + x - 1) / x));
+  };
+#define ROW_Q8(T, C) \
+  hipLaunchKernelGGL((row_q8_kernel<BF16, NORM, SUM, T, C>), grid(T < 256 ? 256 / T : 1), dim3(T < 256 ? 256 : T), 0, stream, p)
   // Microseconds on one MI355X, with a residual's sum where not said otherwise, the variant taken and others: 20,000 x 64
   // 4.5, a wavefront to a row 9.2; 20,000 x 256 8.5 and 10.9; 20,000 x 512 16.9, half a wavefront 17.2; 8,000 x 1,024
   // 13.9, four pieces to a lane 15.2; 8,000 x 2,048 24.7 (without the norm 10.6), 256 threads 23.9 (11.7); 1,419 x 2,560

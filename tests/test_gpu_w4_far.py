@@ -83,6 +83,23 @@ def test_rows_into_8_bits_far_apart(ctx, qattn):
         b.free()
 
 
+def test_rows_into_8_bits_beyond_a_grids_dimension(ctx, qattn):
+    """A workgroup to a row, and more rows than a launch has workgroups in one dimension."""
+    M, width = (1 << 20) + 7, 2056
+    rng = rng_of(8)
+    rows = [0, 1, (1 << 20) - 1, 1 << 20, (1 << 20) + 1, M - 1]
+    bits = some_rows(rng, len(rows), width, True)
+    x, codes, scales = ctx.alloc(M * width * 2), ctx.alloc(M * width), ctx.alloc(M * 4)
+    put(x, rows, bits, 2 * width)
+    ctx.quantize_q8(x.ptr, codes.ptr, scales.ptr, M, width, qattn.BF16)
+    ctx.synchronize()
+    want = w4_ref.quantize_q8(bits, True)
+    assert np.array_equal(get(codes, rows, width, np.int8, width), want[0])
+    check_scales(scales.read(np.float32, (M,))[rows], want[1], width, False)
+    for b in (x, codes, scales):
+        b.free()
+
+
 def test_weights_of_most_rows(ctx, qattn):
     """2^22 weight rows, whose codes take 4 GiB and more: the last columns are those of the last rows by themselves."""
     K, N, last = 2080, 1 << 22, 528
@@ -128,3 +145,26 @@ def test_weights_of_most_rows(ctx, qattn):
             b.free()
     w.free()
     b_alone.free()
+
+
+@pytest.mark.parametrize("N", [8, 112])
+def test_most_rows(ctx, qattn, N):
+    """2^24 - 1 rows: as many workgroups as a call may have, and results past 2^31 bytes."""
+    M, K = (1 << 24) - 1, 32
+    rng = rng_of(N)
+    codes, groups, scales = w4_ref.random_weights(rng, N, K)
+    image = qattn.w4_pack(w4_ref.nibbles(codes), groups, scales)
+    block, block_scale = rng.integers(-128, 128, (1 << 20, K)).astype(np.int8), (rng.random(1 << 20) / 300).astype(np.float32)
+    bx, bs, w, y = ctx.alloc(M * K), ctx.alloc(M * 4), ctx.upload(image), ctx.alloc(M * N * 2)
+    for at in range(0, M, 1 << 20):
+        bx.write(block[:M - at], at * K)
+        bs.write(block_scale[:M - at], at * 4)
+    ctx.w4_matmul(bx.ptr, bs.ptr, M, K, w.ptr, image.nbytes, N, y.ptr)
+    ctx.synchronize()
+    rows = np.concatenate([np.arange(300), np.arange(M - 300, M), rng.integers(0, M, 50)])
+    got = np.stack([y.read(np.uint16, (N,), int(r) * N * 2) for r in rows])
+    at = rows % (1 << 20)
+    want = w4_ref.product(block[at], block_scale[at], codes, groups, scales)
+    check(ref.from_bits(got, False), want, w4_ref.product_bound(want, False), block_scale[at], False)
+    for b in (bx, bs, w, y):
+        b.free()

@@ -63,7 +63,26 @@ def product_refusals():
             "bad": [[str(c), *product(**c)] for c in both + alone] + [["swiglu " + str(c), *product(**{**swiglu, **c})] for c in both + gate]}
 
 
-CASES = {f.__name__: f for f in (row_refusals, product_refusals)}
+def largest_launches():
+    """[what, workgroups, threads] of the first dimension of the largest calls there are."""
+    h, out = Launches(), []
+    now = [""]
+    h.on = lambda name, grid, block, args: out.append([now[0], grid, block])
+    most = (1 << 24) - 1
+    for width in (8, 72, 136, 264, 520, 1032, 2056, 4104, 8200, 16384):
+        now[0] = f"rows of {width}"
+        h.ctx.quantize_q8(X, C, F, most, width)
+        h.ctx.rmsnorm_q8(X, W, C, F, most, width, R, S)
+    for M, K, N in ((1, 32, 1 << 22), (16, 65536, 1 << 22), (32, 2048, 1 << 22), (most, 32, 1), (most, 32, 112), (200, 1024, 1 << 22),
+                    (480, 1024, 1 << 22), (most, 4096, 100), (1 << 19, 1024, 4080)):
+        now[0] = f"{M} x {K} -> {N}"
+        h.ctx.w4_matmul(X, S, M, K, W, 1 << 40, N, Y, ldy=-(-N // 8) * 8)
+        if N % 64 == 0:
+            h.ctx.w4_matmul_swiglu(X, S, M, K, W, 1 << 40, N // 2, Y)
+    return out
+
+
+CASES = {f.__name__: f for f in (row_refusals, product_refusals, largest_launches)}
 
 
 @pytest.fixture(scope="module")
@@ -84,7 +103,14 @@ def w4_child(tmp_path_factory):
     return run
 
 
-@pytest.mark.parametrize("case", sorted(CASES))
+def test_the_largest_launches_fit_a_grid(w4_child):
+    launches = w4_child("largest_launches")
+    assert len(launches) > 30
+    for what, grid, block in launches:
+        assert 0 < grid and grid * block < 1 << 32 and block <= 1024, what
+
+
+@pytest.mark.parametrize("case", ["row_refusals", "product_refusals"])
 def test_refusals_on_the_host(w4_child, case):
     got = w4_child(case)
     for i, (code, message, launches) in enumerate(got["fine"]):
