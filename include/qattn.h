@@ -506,8 +506,8 @@ int qattn_quantize_q8(qattn_ctx* ctx, const void* x, int64_t x_row_stride, int8_
  * codes = rint(t * (127 / amax)) with amax the row's largest |t|, scales = amax / 127 * inv, inv = 1 / sqrt(sum(v^2) /
  * width + eps).  The norm's factor cancels in the codes, which therefore depend on no order of a sum.  A row with
  * an infinity or a NaN among its t, or whose sum of squares passes f32's range, gets codes of 0 and a scale of NaN;
- * amax below 2^-100 gives codes and a scale of 0.  weight: device f32 [width], 16-byte aligned.  sum may be x or
- * residual (with its stride). */
+ * amax below 2^-100 gives codes and a scale of 0.  Squares below f32's range count as any others do, whatever eps
+ * (rounded to f32) is.  weight: device f32 [width], 16-byte aligned.  sum may be x or residual (with its stride). */
 int qattn_rmsnorm_q8(qattn_ctx* ctx, const void* x, int64_t x_row_stride, const void* residual, int64_t residual_row_stride,
                      void* sum, int64_t sum_row_stride, const float* weight, int8_t* codes, int64_t codes_row_stride,
                      float* scales, int64_t rows, int32_t width, int32_t dtype, double eps, qattn_stream_t stream);

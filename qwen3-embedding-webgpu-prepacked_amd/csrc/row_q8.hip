@@ -31,6 +31,12 @@ __device__ inline u32x2 codes8(const float* t, float factor) {
   return u32x2{pack(c[0], c[1], c[2], c[3]), pack(c[4], c[5], c[6], c[7])};
 }
 
+// A row of bf16 may be so small that its squares leave f32's range: their sum would be 0 and, with an eps of 0, the scale
+// infinite.  So below kTinyEps the squares of the values times 2^100 are summed as well, which none leaves downwards.
+// That sum counts where the plain one is below kTinySquares, and then stays in range itself; elsewhere what the plain
+// one has lost, 2^-150 for a value, is nothing beside kTinySquares or eps.
+constexpr float kTinyEps = 0x1p-100f, kTinySquares = 0x1p-80f;
+
 // T threads to a row, C pieces of 8 elements to a thread; memory is the bound.  Up to 512 elements a row takes as many
 // lanes as it fills, so that a wavefront holds several narrow ones, and up to 2048 one wavefront, which needs no
 // barrier; more take as many threads as leave two pieces to each, for more loads in flight.
@@ -52,7 +58,8 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void row_q8_kernel(RowQ8 p) {
                          : u32x4{};
   }
   float t[8 * C];
-  float squares = 0.f;
+  float squares = 0.f, raised = 0.f;
+  const bool tiny_eps = BF16 && NORM && p.eps < kTinyEps;
   uint32_t most = 0;  // the largest magnitude's bits: NaN above infinity above every number
 #pragma unroll
   for (int j = 0; j < C; ++j) {
@@ -67,9 +74,13 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void row_q8_kernel(RowQ8 p) {
         v[2 * i + 1] += widen<BF16, 1>(r[j][i]);
       }
     }
-    if constexpr (NORM)
+    if constexpr (NORM) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) squares = fmaf(v[e], v[e], squares);
+      if (tiny_eps)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) raised = fmaf(v[e] * 0x1p100f, v[e] * 0x1p100f, raised);
+    }
     if constexpr (SUM) {
       u32x4 s;
 #pragma unroll
@@ -100,21 +111,25 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void row_q8_kernel(RowQ8 p) {
 #pragma unroll
   for (int d = T < 64 ? T / 2 : 32; d; d >>= 1) {
     if constexpr (NORM) squares += __shfl_xor(squares, d, 64);
+    if (tiny_eps) raised += __shfl_xor(raised, d, 64);
     most = max(most, (uint32_t)__shfl_xor((int)most, d, 64));
   }
   if constexpr (kWaves > 1) {
-    __shared__ float part_squares[kWaves];
+    __shared__ float part_squares[kWaves], part_raised[kWaves];
     __shared__ uint32_t part_most[kWaves];
     if ((tid & 63) == 0) {
       part_squares[tid >> 6] = squares;
+      part_raised[tid >> 6] = raised;
       part_most[tid >> 6] = most;
     }
     __syncthreads();
     squares = part_squares[0];
+    raised = part_raised[0];
     most = part_most[0];
 #pragma unroll
     for (int i = 1; i < kWaves; ++i) {
       squares += part_squares[i];
+      raised += part_raised[i];
       most = max(most, part_most[i]);
     }
   }
@@ -124,8 +139,12 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void row_q8_kernel(RowQ8 p) {
   const bool lost = most >= 0x7F800000u || (NORM && !(squares < INFINITY)), none = amax < kLeastAmax;
   const float factor = lost || none ? 0.f : 127.f / amax;
   if (tid == 0) {
-    const float inv = NORM ? 1.f / sqrtf(squares / (float)p.width + p.eps) : 1.f;
-    p.scales[row] = lost ? __builtin_nanf("") : none ? 0.f : amax / 127.f * inv;
+    float scale = amax / 127.f;
+    if (tiny_eps && squares < kTinySquares)
+      scale = (float)((double)scale / sqrt((double)raised * 0x1p-200 / p.width + (double)p.eps));
+    else if constexpr (NORM)
+      scale *= 1.f / sqrtf(squares / (float)p.width + p.eps);
+    p.scales[row] = lost ? __builtin_nanf("") : none ? 0.f : scale;
   }
   int8_t* const out = p.codes + row * p.codes_stride;
 #pragma unroll
