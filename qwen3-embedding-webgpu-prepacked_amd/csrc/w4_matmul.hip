@@ -264,8 +264,14 @@ __device__ inline uint32_t load1s(__amdgpu_buffer_rsrc_t rs, uint32_t off, uint3
 __device__ inline void store16(u32x4 v, __amdgpu_buffer_rsrc_t rs, uint32_t off) {
   __builtin_amdgcn_raw_buffer_store_b128(v, rs, off, 0, 0);
 }
-// Past the L2, which a large result would only sweep: the tiles of many rows take 4 to 9 % less, and what reads the
-// result next takes at most as much longer (8,000 x 4,096: 60.8 us for both against 60.4; 20,000 x 2,816: 165 against 171).
+// Past the L2s, for tiles of many rows whose result takes up to kFarBytes: a kernel's end writes back what its L2s hold, and
+// of a small result that is all.  Of a larger one the call that reads it loses more than the product gains, so the two
+// together decide: the product and qattn_quantize_q8 of its result, microseconds on one MI355X, past the L2s and plainly:
+// 1,500 x 1,024 -> 4,096 (12 MB) 17.4 and 18.2, 2,400 rows (20 MB) 24.2 and 24.7, 3,200 (26 MB) 27.7 and 27.1, 8,000 (66 MB)
+// 62.3 and 59.9, 12,000 (98 MB) 88.1 and 85.8, 20,000 (164 MB) 141.5 either way.  SwiGLU's results, half as large for their
+// products, go past them at any size: 1,024 -> 2 x 2,816 of 3,200 rows 35.9 and 36.4, 8,000 71.3 and 74.2, 12,000 103.0 and
+// 100.9, 20,000 166 and 167.
+constexpr int64_t kFarBytes = 24 << 20;
 __device__ inline void store16_far(u32x4 v, __amdgpu_buffer_rsrc_t rs, uint32_t off) {
   __builtin_amdgcn_raw_buffer_store_b128(v, rs, off, 0, 2);
 }
@@ -510,7 +516,7 @@ void launch_mid(const W4Product& p, hipStream_t stream) {
 __device__ inline uint32_t lds_off(int row, int piece) { return row * 64 + ((piece ^ ((row >> 2) & 3)) << 4); }
 
 template <bool BF16, bool SWIGLU, int MF, int NWN>
-__global__ __launch_bounds__(128 * NWN, 2) void w4_tile_kernel(W4Product p, int tiles_n, int tiles_total, int per_xcd) {
+__global__ __launch_bounds__(128 * NWN, 2) void w4_tile_kernel(W4Product p, int tiles_n, int tiles_total, int per_xcd, int far) {
   constexpr int kWaves = 2 * NWN;
   constexpr int kTileM = 32 * MF, kTileN = 64 * NWN;
   constexpr int kBytesA = kTileM * 64, kBytesB = kTileN * 64;
@@ -722,7 +728,11 @@ __global__ __launch_bounds__(128 * NWN, 2) void w4_tile_kernel(W4Product p, int 
       const int row = kRowsPer * i + lane / kPieces, c = lane % kPieces;
       const u32x4 v = *reinterpret_cast<const u32x4*>(place(row, c));
       const int m = row0 + kRows * pass + row, n = col0 + 8 * c;
-      store16_far(v, yrs, m < rows && n + 8 <= n_out ? ((uint32_t)m * (uint32_t)p.ldy + (uint32_t)n) * 2u : kNowhere);
+      const uint32_t at_y = m < rows && n + 8 <= n_out ? ((uint32_t)m * (uint32_t)p.ldy + (uint32_t)n) * 2u : kNowhere;
+      if (SWIGLU || far)
+        store16_far(v, yrs, at_y);
+      else
+        store16(v, yrs, at_y);
     }
     // A last piece of fewer than 8 columns goes element by element.
     const int part = (n_out - col0) >> 3;
@@ -742,7 +752,7 @@ void launch_tile(const W4Product& p, hipStream_t stream) {
   const int64_t tiles_m = ((int64_t)p.M + 32 * MF - 1) / (32 * MF), tiles_n = ((int64_t)p.N + 64 * NWN - 1) / (64 * NWN);
   const int64_t tiles = tiles_m * tiles_n, per_xcd = (tiles + 7) / 8;
   hipLaunchKernelGGL((w4_tile_kernel<BF16, SWIGLU, MF, NWN>), dim3((unsigned)(8 * per_xcd)), dim3(128 * NWN), 0, stream, p,
-                     (int)tiles_n, (int)tiles, (int)per_xcd);
+                     (int)tiles_n, (int)tiles, (int)per_xcd, SWIGLU || (int64_t)p.M * p.N * 2 <= kFarBytes);
 }
 
 template <bool BF16, bool SWIGLU>

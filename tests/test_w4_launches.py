@@ -20,6 +20,24 @@ def launch(h, M, K, N, swiglu, bf16=False):
     call(X, S, M, K, W, 1 << 40, N, Y, dtype=h.qattn.BF16 if bf16 else h.qattn.F16, ldy=-(-N // 8) * 8)
 
 
+STORES = [(1500, 1024, 4096, False), (2400, 1024, 4096, False), (2900, 1024, 4096, False), (3200, 1024, 4096, False), (8000, 1024, 4096, False),
+          (20000, 1024, 4096, False), (2401, 1056, 2048, True), (20000, 1024, 2816, True), (8000, 2048, 1024, False)]
+
+
+def stores():
+    """[(M, K, N, swiglu, whether the tiles of many rows store past the L2s)]"""
+    h, out = Launches(), []
+    now = []
+
+    def on(name, grid, block, args):
+        assert "w4_tile_kernel" in name, (now, name)
+        out.append([*now, h.word(args, 4)])  # product, tiles_n, tiles_total, per_xcd, far
+    h.on = on
+    for now in STORES:
+        launch(h, *now)
+    return out
+
+
 def kernels():
     """The products' kernels that the library holds, and those that the sizes of test_gpu_w4_kernels.py take, with the
     kernel that each is compared with: [[all], [[size's index, swiglu, bf16, kernel, other]]]."""
@@ -37,7 +55,7 @@ def kernels():
     return [[k for k in held if re.search(r"w4_(small|mid|tile)_kernel", k)], out]
 
 
-CASES = {f.__name__: f for f in (kernels,)}
+CASES = {f.__name__: f for f in (stores, kernels)}
 
 
 @pytest.fixture(scope="module")
@@ -56,6 +74,16 @@ def child(tmp_path_factory):
         return json.loads(out.stdout)
 
     return run
+
+
+def test_large_results_stay_where_their_reader_finds_them(child):
+    """A product's result of more than 24 MiB is stored plainly: past the L2s the product itself gains less than the call
+    that reads the result loses.  SwiGLU's results, where both are alike, go past them."""
+    seen = child("stores")
+    assert len(seen) == len(STORES)
+    for M, K, N, swiglu, far in seen:
+        assert far == (swiglu or 2 * M * N <= 24 << 20), (M, K, N, swiglu)
+    assert {far for *_, far in seen} == {0, 1}
 
 
 def test_every_kernel_is_taken_by_the_size_that_names_it(child):
