@@ -163,10 +163,12 @@ void launch(const RowQ8& p, hipStream_t stream) {
   };
 #define ROW_Q8(T, C) \
   hipLaunchKernelGGL((row_q8_kernel<BF16, NORM, SUM, T, C>), grid(T < 256 ? 256 / T : 1), dim3(T < 256 ? 256 : T), 0, stream, p)
-  // Microseconds on one MI355X, with a residual's sum where not said otherwise, the variant taken and others: 20,000 x 64
-  // 4.5, a wavefront to a row 9.2; 20,000 x 256 8.5 and 10.9; 20,000 x 512 16.9, half a wavefront 17.2; 8,000 x 1,024
-  // 13.9, four pieces to a lane 15.2; 8,000 x 2,048 24.7 (without the norm 10.6), 256 threads 23.9 (11.7); 1,419 x 2,560
-  // without the sum 5.2, four pieces 6.1, one 5.6; 2,000 x 5,000 17.8, four 18.7; 500 x 16,384 14.7, four 15.2.
+  // Microseconds on one MI355X over four sets of rows in turn, fp16 with a residual's sum where not said otherwise, the
+  // variant taken and others: 20,000 x 64 5.5, a wavefront to a row 9.2; 20,000 x 256 8.5 and 10.7; 20,000 x 512 15.5, half
+  // a wavefront 15.0; 8,000 x 1,024 11.1, half a wavefront the same, 256 threads 13.0; 2,048 wide without the norm 9.0
+  // for 8,000, 256 threads 10.1, and with the sum, which does not decide, 7.5 and 7.6 for 2,000, 24.8 and 24.0 for 8,000, 52.2
+  // either way for 20,000; 1,419 x 2,560 without the sum 5.2, four pieces 5.7, one 5.3; 2,000 x 5,000 15.4, four 18.1, one
+  // 16.6; 500 x 16,384 11.4, four 15.2.
   if (p.width <= 64)
     ROW_Q8(8, 1);
   else if (p.width <= 128)

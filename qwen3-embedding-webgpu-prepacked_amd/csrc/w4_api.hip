@@ -68,7 +68,8 @@ int check_w4(qattn_ctx* ctx, const W4Product& p, int64_t w_bytes, int32_t out_co
   if (!rows16(p.y, p.ldy, out_cols))
     return fail(ctx, QATTN_EINVAL, "y: 16-byte aligned, ldy at least the %d columns, a multiple of 8, at most 2^22", out_cols);
   if (reinterpret_cast<uintptr_t>(p.x_scale) % 4 || !aligned16(p.w)) return fail(ctx, QATTN_EINVAL, "x_scale not 4-byte or w not 16-byte aligned");
-  // Blocks of 32 rows and 32 columns, the smallest of any kernel.
+  // Blocks of 32 rows and 16 columns, the smallest that any kernel takes of more than 16 rows (but of few blocks); those of
+  // fewer rows have at most 2^17.
   if ((((int64_t)p.M + 31) / 32) * (((int64_t)out_cols + 15) / 16) > kMaxGroups)
     return fail(ctx, QATTN_EINVAL, "M=%d by %d columns: more than 2^22 blocks of a launch", p.M, out_cols);
   const Range written[] = {range_of("y", p.y, p.M, p.ldy, out_cols, 2)};

@@ -511,8 +511,9 @@ void launch_mid(const W4Product& p, hipStream_t stream) {
 // publishes that tile and X tile kb + 1; half 2 reads the next step's fragments under the other half's products.
 // X tile kb + 3 goes into the buffer that tile kb - 1 left at the previous barrier.
 //
-// 8,000 x 4,096 -> 4,096: 112 us, 2,390 TOP/s (a loop of nothing but these instructions reaches 3,495).  Matrix cores and
-// LDS are busy half of the time each, vector units 40 %, and the clock follows their power: with zeros for X 97 us.
+// 8,000 x 4,096 -> 4,096: 117 us over four sets of buffers in turn, 2,290 TOP/s, 111 where one is used again (a loop of
+// nothing but these instructions reaches 3,495).  LDS is busy half of the time, the matrix cores a little less, vector
+// units 40 %, and the clock follows their power: with zeros for X 102 us.
 __device__ inline uint32_t lds_off(int row, int piece) { return row * 64 + ((piece ^ ((row >> 2) & 3)) << 4); }
 
 template <bool BF16, bool SWIGLU, int MF, int NWN>
@@ -789,13 +790,14 @@ hipError_t launch(const W4Product& p, hipStream_t stream) {
       launch_small<BF16, SWIGLU, 2, 2, 4, 1>(p, stream);
   } else if (tiles(64, 32) <= 512) {
     launch_small<BF16, SWIGLU, 4, 2, 4, 1>(p, stream);
-    // The largest tiles for long sums where their last round leaves few places (8,000 x 4,096 -> 4,096 112, in halves of
-    // them 122; 2,400 x 1,024 -> 4,096 16.2 and 17.4; gate/up of 20,000 x 1,024 -> 2 x 2,816 121 and 125; but 5,000 x
-    // 1,024 -> 4,096, a second round of 64 tiles, 33 and 27, and 8,000 x 512 -> 4,096 27.5 and 25.6).
+    // The largest tiles for long sums where their last round leaves few places (8,000 x 4,096 -> 4,096 120, in halves of
+    // them 132; 2,400 x 1,024 -> 4,096 16.5 and 18.4; gate/up of 20,000 x 1,024 -> 2 x 2,816 121 and 125; but 5,000 x
+    // 1,024 -> 4,096, a second round of 64 tiles, 34 and 30, and of shorter sums, with what reads the result, 20,000 x 512
+    // -> 1,024 38.1 and 34.8, 8,000 x 512 -> 4,096 45.4 and 44.7, over four sets of buffers 46.5 and 49.3).
   } else if (p.K >= 1024 && full(256, 256, 80) && (idle(whole, 256) <= 96 || idle(whole, 256) <= whole / 8)) {
     launch_tile<BF16, SWIGLU, 8, 4>(p, stream);
-    // Half of them where they are enough (1,500 x 1,024 -> 4,096 12.0, of 64 x 128 13.5; 6,000 x 1,024 -> 4,096 29, of 128
-    // x 128 34; 8,000 x 256 -> 4,096 20 and 31; but 20,000 x 1,024 -> 300, a fifth of whose tiles is empty, 14.1 and 13.2).
+    // Half of them where they are enough (1,500 x 1,024 -> 4,096 12.1, of 128 x 128 13.3; 6,000 x 1,024 -> 4,096 32.6 and
+    // 35.7; 8,000 x 256 -> 4,096 24 and 32; but 20,000 x 1,024 -> 300, a fifth of whose tiles is empty, 14.1 and 13.2).
   } else if (tiles(256, 128) >= 160 && full(256, 128, 80)) {
     launch_tile<BF16, SWIGLU, 8, 2>(p, stream);
     // In between two workgroups to a compute unit, of 128 rows unless a round would be mostly empty (2,000 x 2,048 -> 2,048
