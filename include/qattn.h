@@ -517,7 +517,8 @@ int qattn_rmsnorm_q8(qattn_ctx* ctx, const void* x, int64_t x_row_stride, const 
  * (15 - zero) * multiplier <= 127, so that (code - zero) * multiplier is a whole number of 8 bits.  The image that
  * the products read is written on the host, once, by one of the functions below, and copied to the device by the
  * caller; K a multiple of 32 up to 65536, N up to 2^22, 17/32 of a byte for each weight (K padded to 128, N to 16).
- * None of these needs a device or a context; messages are in qattn_last_error(NULL). */
+ * None of these needs a device or a context; messages are in qattn_last_error(NULL).  An image may not lie over what it
+ * is made from. */
 int64_t qattn_w4_bytes(int32_t K, int32_t N); /* -1 for a shape that is none */
 /* codes: [N][K / 2], column 2 i in the low nibble of byte i, column 2 i + 1 in its high nibble; groups: [N][K / 32],
  * multiplier | zero << 4; scales: [N], finite. */

@@ -52,6 +52,13 @@ int check(const void* from, const void* image, int64_t image_bytes, int32_t K, i
   return QATTN_OK;
 }
 
+// The image is cleared before its source is read for the last time, so it may not lie over `bytes` of it.
+int check_apart(const void* image, int64_t need, const void* from, int64_t bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(image), y = reinterpret_cast<uintptr_t>(from);
+  if (x < y ? y - x < (uintptr_t)need : x - y < (uintptr_t)bytes) return fail(nullptr, QATTN_EINVAL, "the image overlaps what it is made from");
+  return QATTN_OK;
+}
+
 // The rows of `load(n, g, w)`, which gives the 32 weights of a group.
 template <typename Load>
 int quantize(const Load& load, int32_t K, int32_t N, void* out) {
@@ -122,9 +129,12 @@ int64_t qattn_w4_bytes(int32_t K, int32_t N) {
 int qattn_w4_pack(const uint8_t* codes, const uint8_t* groups, const float* scales, int32_t K, int32_t N, void* out,
                   int64_t image_bytes) {
   if (!groups || !scales) return fail(nullptr, QATTN_EINVAL, "groups/scales is NULL");
-  const int rc = check(codes, out, image_bytes, K, N);
+  int rc = check(codes, out, image_bytes, K, N);
   if (rc) return rc;
-  const int64_t per_row = K / kGroup;
+  const int64_t per_row = K / kGroup, need = qattn_w4_bytes(K, N);
+  if ((rc = check_apart(out, need, codes, N * per_row * 16)) || (rc = check_apart(out, need, groups, N * per_row)) ||
+      (rc = check_apart(out, need, scales, 4 * (int64_t)N)))
+    return rc;
   for (int32_t n = 0; n < N; ++n) {
     if (!std::isfinite(scales[n])) return fail(nullptr, QATTN_EINVAL, "the scale of row %d is not finite", n);
     for (int64_t g = 0; g < per_row; ++g) {
@@ -152,18 +162,20 @@ int qattn_w4_pack(const uint8_t* codes, const uint8_t* groups, const float* scal
 }
 
 int qattn_w4_quantize(const float* w, int64_t row_stride, int32_t K, int32_t N, void* image, int64_t image_bytes) {
-  const int rc = check(w, image, image_bytes, K, N);
+  int rc = check(w, image, image_bytes, K, N);
   if (rc) return rc;
   if (row_stride < K) return fail(nullptr, QATTN_EINVAL, "row_stride %lld: at least K = %d", (long long)row_stride, K);
+  if ((rc = check_apart(image, qattn_w4_bytes(K, N), w, 4 * ((N - 1) * row_stride + K)))) return rc;
   return quantize([&](int64_t n, int64_t g, float* out) { std::memcpy(out, w + n * row_stride + g * kGroup, 4 * kGroup); }, K, N, image);
 }
 
 int qattn_w4_from_q4(const void* q4, int64_t q4_bytes, int32_t K, int32_t N, void* image, int64_t image_bytes) {
-  const int rc = check(q4, image, image_bytes, K, N);
+  int rc = check(q4, image, image_bytes, K, N);
   if (rc) return rc;
-  if (q4_bytes < qattn_q4_compact_bytes(K, N))
-    return fail(nullptr, QATTN_EINVAL, "q4_bytes %lld: a %d x %d tile32-compact tensor holds %lld", (long long)q4_bytes, N, K,
-                (long long)qattn_q4_compact_bytes(K, N));
+  const int64_t size = qattn_q4_compact_bytes(K, N);
+  if (q4_bytes < size)
+    return fail(nullptr, QATTN_EINVAL, "q4_bytes %lld: a %d x %d tile32-compact tensor holds %lld", (long long)q4_bytes, N, K, (long long)size);
+  if ((rc = check_apart(image, qattn_w4_bytes(K, N), q4, size))) return rc;
   const uint8_t* const from = static_cast<const uint8_t*>(q4);
   const int64_t blocks = K / kGroup;
   return quantize(
