@@ -492,8 +492,9 @@ int qattn_shared_plan_describe(const qattn_shared_desc* desc, int32_t* words, in
  * 8-bit codes with one f32 scale each (value = code * scale), and the products of such rows with 4-bit weights run
  * in whole numbers on the matrix cores.  16-bit tensors are fp16 or bf16 (enum qattn_dtype), arithmetic f32.
  * Rows: 16-byte aligned (codes 8), strides in elements, at least the width, multiples of 8, at most 2^22; what a
- * call writes may not overlap anything else that it touches, where nothing else is said.  All calls here enqueue
- * on `stream` (NULL: the context stream), allocate nothing, wait for nothing and keep nothing between calls, so
+ * call writes may not overlap anything else that it touches, where nothing else is said (a tensor reaches from its
+ * first row to the end of its last: two whose rows lie in turn overlap).  All calls here enqueue on `stream` (NULL:
+ * the context stream), allocate nothing, wait for nothing and keep nothing between calls, so
  * that they can be captured and may overlap. */
 
 /* codes[r][c] = rint(x[r][c] * (127 / amax)), scales[r] = amax / 127, amax the row's largest magnitude; each
@@ -534,14 +535,16 @@ int qattn_w4_quantize(const float* w, int64_t row_stride, int32_t K, int32_t N, 
  * differ as normal values do, beside the 8.6 % that Q4_0 has left out. */
 int qattn_w4_from_q4(const void* q4, int64_t q4_bytes, int32_t K, int32_t N, void* image, int64_t image_bytes);
 
-/* y[m][n] = x_scale[m] * scale[n] * sum over k of x[m][k] * (code - zero) * multiplier, for m < M, n < N, rounded to
- * `dtype` once; the sum is exact (32-bit whole numbers), so a row's result does not depend on its batch.  x: 8-bit rows,
- * ldx a multiple of 16; w: the image on the device, 16-byte aligned; M below 2^24, and fewer than 2^22 blocks of 32
- * rows and 16 columns.  One to 16 rows (a step's tokens) are matrix-vector products, bound by the weights. */
+/* y[m][n] = (sum * scale[n]) * x_scale[m], sum over k of x[m][k] * (code - zero) * multiplier, for m < M, n < N: the sum
+ * is exact (32-bit whole numbers), then it and each product are rounded to f32, the result to `dtype`, so a row's result
+ * does not depend on its batch.  x: 8-bit rows, ldx a multiple of 16; w: the image on the device, 16-byte aligned; M
+ * below 2^24, and fewer than 2^22 blocks of 32 rows and 16 columns.  One to 16 rows (a step's tokens) are
+ * matrix-vector products, bound by the weights. */
 int qattn_w4_matmul(qattn_ctx* ctx, const int8_t* x, int64_t ldx, const float* x_scale, int32_t M, int32_t K, const void* w,
                     int64_t w_bytes, int32_t N, void* y, int64_t ldy, int32_t dtype, qattn_stream_t stream);
 /* The FFN's gate/up projection and SwiGLU: y[m][j] = g / (1 + exp(-g)) * u with g and u the f32 results of rows j and
- * n_inter + j of a weight of 2 n_inter rows, rounded once.  n_inter a multiple of 32. */
+ * n_inter + j of a weight of 2 n_inter rows, rounded once; the sigmoid of a gate below -87 may be 0, where it is below
+ * 2^-125.  n_inter a multiple of 32. */
 int qattn_w4_matmul_swiglu(qattn_ctx* ctx, const int8_t* x, int64_t ldx, const float* x_scale, int32_t M, int32_t K,
                            const void* w, int64_t w_bytes, int32_t n_inter, void* y, int64_t ldy, int32_t dtype,
                            qattn_stream_t stream);
